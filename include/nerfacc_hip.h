@@ -446,6 +446,51 @@ int nfa_pdf_loss_fwd(const float *query_vals, const float *cdfs_query, const flo
 int nfa_pdf_loss_bwd(const float *g_loss, const int32_t *ids_left, const int32_t *ids_right, const float *coef,
                      int64_t n_rays, int64_t n_query, int64_t n_key, float *g_cdfs_key, void *stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Feature operators: what turns samples into features between sampling and rendering.  No reference counterpart (the reference
+ * leaves fields to its examples).  Element types: NFA_DTYPE_*; every sum, statistic and state is held in 32 bits, outputs are
+ * rounded once.  Row strides are in elements; rows are contiguous inside.
+ * ------------------------------------------------------------------------------------- */
+#define NFA_DTYPE_F32 0
+#define NFA_DTYPE_BF16 1
+#define NFA_DTYPE_F16 2
+
+#define NFA_ACT_NONE 0
+#define NFA_ACT_RELU 1
+#define NFA_ACT_SIGMOID 2
+#define NFA_ACT_SOFTPLUS 3
+#define NFA_ACT_SILU 4
+#define NFA_ACT_GELU 5 /* x Phi(x), the exact form */
+#define NFA_ACT_EXP 6
+
+/* outputs = act(inputs weight^T + bias) + residual.
+ * nfa_linear_fwd  inputs [rows, in_features], weight [out_features, in_features] and bias [out_features] (nullable), residual
+ *                 [rows, out_features] (nullable) -> outputs [rows, out_features] contiguous.  saved (nullable unless a backward
+ *                 pass follows): what nfa_linear_bwd differentiates the activation from, nfa_linear_saved_bytes(...) bytes; 0
+ *                 bytes = it needs none, or (relu, exp, softplus without a residual) the outputs themselves.
+ * nfa_linear_bwd  grad_outputs [rows, out_features] -> grad_inputs [rows, in_features] contiguous, grad_weight, grad_bias (each
+ *                 nullable); the residual's gradient is grad_outputs.  saved = the forward call's saved array, or its outputs where
+ *                 nfa_linear_saved_bytes says 0 and the activation is not NONE.  workspace: nfa_linear_bwd_workspace_bytes(...). */
+typedef struct nfa_linear_args {
+    int64_t rows;
+    int32_t in_features, out_features;
+    int32_t dtype, activation;
+    const void *inputs;
+    int64_t inputs_stride;
+    const void *weight;         /* contiguous */
+    const void *bias;           /* nullable */
+    const void *residual;       /* nullable, forward only */
+    int64_t residual_stride;
+    const void *grad_outputs;   /* backward only */
+    int64_t grad_outputs_stride;
+} nfa_linear_args;
+
+int64_t nfa_linear_saved_bytes(int64_t rows, int32_t out_features, int32_t dtype, int32_t activation, int32_t has_residual);
+int nfa_linear_fwd(const nfa_linear_args *args, void *outputs, void *saved, void *stream);
+int64_t nfa_linear_bwd_workspace_bytes(int64_t rows, int32_t in_features, int32_t out_features, int32_t dtype);
+int nfa_linear_bwd(const nfa_linear_args *args, const void *saved, void *grad_inputs, void *grad_weight, void *grad_bias,
+                   void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,7 @@ Native code: nerfacc_amd/libnerfacc_hip.so (hand-written HIP for gfx950, C ABI i
 include/nerfacc_hip.h), built by `python -m nerfacc_amd.build`.
 """
 from .data_specs import RayIntervals, RaySamples
+from .dense import linear
 from .estimators.occ_grid import OccGridEstimator
 from .estimators.prop_net import PropNetEstimator
 from .grid import ray_aabb_intersect, sample_positions, traverse_grids
@@ -43,3 +44,5 @@ __all__ = [
 ]
 # additions of this implementation (not in the reference's list of 24 names)
 __all__ += ["sample_positions", "set_option", "get_option", "reset_options", "list_options", "options", "release_workspace"]
+# feature operators between sampling and rendering
+__all__ += ["linear"]

@@ -1,0 +1,93 @@
+// feature.hpp — what the feature operators (dense.hip, conv.hip, selective.hip) share: the three element types, activations with
+// their derivatives, and the reduction of partial sums.
+#pragma once
+
+#include "common.hpp"
+
+namespace nfa {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+
+template <class T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
+// one rounding to nearest even (v_cvt_pk_bf16_f32 / v_cvt_f16_f32)
+template <class T> __device__ __forceinline__ T from_f(float v) { return (T)v; }
+
+inline int64_t dtype_bytes(int32_t dtype) { return dtype == NFA_DTYPE_F32 ? 4 : 2; }
+inline bool dtype_ok(int32_t dtype) { return dtype >= NFA_DTYPE_F32 && dtype <= NFA_DTYPE_F16; }
+
+// calls f(T{}) with the element type of `dtype`
+template <class F>
+inline void with_dtype(int32_t dtype, F &&f) {
+    if (dtype == NFA_DTYPE_F32) f(float{});
+    else if (dtype == NFA_DTYPE_BF16) f(bf16{});
+    else f(f16{});
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^x in one v_exp_f32: 1 ulp, results below 2^-126 become 0
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// v_rcp_f32 (1 ulp)
+__device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// sigmoid with the exponential taken of -|x|: no overflow at either end, and a relative error of a few ulp at both
+__device__ __forceinline__ float sigmoid_f(float x) {
+    const float e = fast_exp2(-fabsf(x) * kLog2e), r = fast_rcp(1.0f + e);
+    return x != x ? x : (x >= 0.0f ? r : e * r);
+}
+
+// log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1], with log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, as its odd
+// series: every term is positive, so small steps (x around -7 in a scan) keep their relative accuracy, which log(1 + e) would not.
+// The series is cut after s^15 / 15: the rest is below 3^-16 / 17 = 1.4e-9 of the first term.
+__device__ __forceinline__ float softplus_f(float x) {
+    const float e = fast_exp2(-fabsf(x) * kLog2e);
+    const float s = e * fast_rcp(2.0f + e), q = s * s;
+    float p = 1.0f / 15.0f;
+    p = fmaf(p, q, 1.0f / 13.0f);
+    p = fmaf(p, q, 1.0f / 11.0f);
+    p = fmaf(p, q, 1.0f / 9.0f);
+    p = fmaf(p, q, 1.0f / 7.0f);
+    p = fmaf(p, q, 1.0f / 5.0f);
+    p = fmaf(p, q, 1.0f / 3.0f);
+    p = fmaf(p, q, 1.0f);
+    return x != x ? x : fmaxf(x, 0.0f) + 2.0f * s * p;
+}
+
+constexpr float kInvSqrt2 = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f;
+
+// What a layer keeps for its backward pass (include/nerfacc_hip.h: nfa_linear_saved): relu, exp and softplus are differentiated from
+// their own value a = act(z), which loses nothing by its rounding (the sign; e^z itself; 1 - e^-a with the relative error of a); the
+// others from z, whose relative rounding error is the derivative's.
+inline bool act_from_value(int32_t act) { return act == NFA_ACT_RELU || act == NFA_ACT_EXP || act == NFA_ACT_SOFTPLUS; }
+
+__device__ __forceinline__ float act_fwd(int act, float z) {
+    switch (act) {
+        case NFA_ACT_RELU: return z < 0.0f ? 0.0f : z;      // (NaN stays NaN)
+        case NFA_ACT_SIGMOID: return sigmoid_f(z);
+        case NFA_ACT_SOFTPLUS: return softplus_f(z);
+        case NFA_ACT_SILU: return z * sigmoid_f(z);
+        case NFA_ACT_GELU: return 0.5f * z * erfcf(-z * kInvSqrt2);
+        case NFA_ACT_EXP: return expf(z);
+        default: return z;
+    }
+}
+// the derivative, from the saved number (act_from_value)
+__device__ __forceinline__ float act_slope(int act, float s) {
+    switch (act) {
+        case NFA_ACT_RELU: return s > 0.0f ? 1.0f : (s != s ? s : 0.0f);
+        case NFA_ACT_SIGMOID: { const float r = sigmoid_f(s); return r * sigmoid_f(-s); }
+        case NFA_ACT_SOFTPLUS: return -expm1f(-s);
+        case NFA_ACT_SILU: { const float r = sigmoid_f(s); return r * fmaf(s, sigmoid_f(-s), 1.0f); }
+        case NFA_ACT_GELU: return fmaf(s * kInvSqrt2Pi, expf(-0.5f * s * s), 0.5f * erfcf(-s * kInvSqrt2));
+        case NFA_ACT_EXP: return s;
+        default: return 1.0f;
+    }
+}
+
+inline bool act_ok(int32_t act) { return act >= NFA_ACT_NONE && act <= NFA_ACT_EXP; }
+
+// out[c] = sum over r of part[r][c] in a fixed order (no atomics: the same bits every time), rounded once
+void launch_reduce_rows(const float *part, int64_t rows, int64_t cols, int64_t ld, void *out, int32_t dtype, hipStream_t s);
+
+}  // namespace nfa

@@ -20,6 +20,7 @@
 #include <map>
 #include <mutex>
 #include <optional>
+#include <set>
 #include <string>
 #include <thread>
 #include <tuple>
@@ -1399,6 +1400,111 @@ py::tuple grid_threshold(const Tensor &occs, double occ_thre, const std::optiona
     return py::make_tuple(binaries, thre);
 }
 
+// ---------------------------------------------------------------------------------------------------
+// feature operators (dense.hip, conv.hip, selective.hip).  The shapes and dtypes are checked by the Python layer
+// (nerfacc_amd/dense.py, selective.py); what would be read out of bounds is checked here again.
+// ---------------------------------------------------------------------------------------------------
+inline int32_t dtype_of(const Tensor &t) {
+    if (t.scalar_type() == at::kFloat) return NFA_DTYPE_F32;
+    if (t.scalar_type() == at::kBFloat16) return NFA_DTYPE_BF16;
+    TORCH_CHECK(t.scalar_type() == at::kHalf, "nerfacc_amd: float32, bfloat16 or float16 expected, got ", t.scalar_type());
+    return NFA_DTYPE_F16;
+}
+
+// a [rows, cols] tensor whose rows are contiguous and do not overlap, at any row stride; copied if it is not one
+inline Tensor as_rows(const Tensor &t, const char *name, int64_t rows, int64_t cols, const Tensor &like) {
+    TORCH_CHECK(t.defined() && t.is_cuda(), name, " must be a CUDA/HIP tensor (nerfacc_amd has no CPU kernels)");
+    TORCH_CHECK(t.device() == like.device() && t.scalar_type() == like.scalar_type(), name, " differs in device or dtype");
+    TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, name, " must have shape [", rows, ", ", cols, "]");
+    if ((t.stride(1) == 1 || cols == 1) && (t.stride(0) >= cols || rows <= 1)) return t;
+    return t.contiguous();
+}
+inline int64_t row_stride(const Tensor &t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+inline Tensor dense_of(const Tensor &t, const char *name, at::ScalarType dtype, int64_t n, const Tensor &like) {
+    TORCH_CHECK(t.defined() && t.is_cuda(), name, " must be a CUDA/HIP tensor (nerfacc_amd has no CPU kernels)");
+    TORCH_CHECK(t.device() == like.device() && t.scalar_type() == dtype && t.numel() == n, name, " differs in device, dtype or size");
+    return t.contiguous();
+}
+inline OptTensor dense_of(const OptTensor &t, const char *name, at::ScalarType dtype, int64_t n, const Tensor &like) {
+    if (!t || !t->defined()) return std::nullopt;
+    return dense_of(*t, name, dtype, n, like);
+}
+inline OptTensor some(const Tensor &t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+// How many nodes of the autograd graphs behind `tensors` were recorded on another stream than the current one of their device.
+// A backward pass that is captured into a graph waits for the streams of all of them; one outside the capture (a leaf whose
+// accumulator an eager graph keeps alive) ends the capture, and on ROCm the process.
+int64_t foreign_nodes(const std::vector<OptTensor> &tensors) {
+    std::vector<torch::autograd::Node *> todo;
+    std::set<torch::autograd::Node *> seen;
+    std::vector<std::shared_ptr<torch::autograd::Node>> held;
+    auto add = [&](torch::autograd::Node *n) { if (n && seen.insert(n).second) todo.push_back(n); };
+    for (auto &t : tensors) {
+        if (!t || !t->defined() || !t->requires_grad()) continue;
+        if (auto fn = t->grad_fn()) { held.push_back(fn); add(fn.get()); }
+        else if (auto acc = torch::autograd::impl::try_get_grad_accumulator(*t)) { held.push_back(acc); add(acc.get()); }
+    }
+    int64_t n = 0;
+    while (!todo.empty()) {
+        auto *node = todo.back();
+        todo.pop_back();
+        if (auto s = node->stream())
+            n += s->device_type() != at::kCPU && s->id() != c10::hip::getCurrentHIPStream(s->device_index()).id();
+        for (auto &e : node->next_edges()) add(e.function.get());
+    }
+    return n;
+}
+
+std::tuple<Tensor, OptTensor> linear_fwd(const Tensor &x_, const Tensor &w_, const OptTensor &b_, const OptTensor &r_, int64_t act, bool save) {
+    TORCH_CHECK(x_.dim() == 2 && w_.dim() == 2, "linear: 2-D inputs and weight expected");
+    const int64_t m = x_.size(0), k = w_.size(1), n = w_.size(0);
+    const Tensor x = as_rows(x_, "inputs", m, k, x_), w = dense_of(w_, "weight", x_.scalar_type(), n * k, x_);
+    const OptTensor b = dense_of(b_, "bias", x_.scalar_type(), n, x_);
+    Tensor r;
+    if (r_ && r_->defined()) r = as_rows(*r_, "residual", m, n, x_);
+    Guard g(device_of(x_));
+    Tensor out = at::empty({m, n}, x_.options()), saved;
+    if (save && nfa_linear_saved_bytes(m, (int32_t)n, dtype_of(x), (int32_t)act, r.defined()) > 0) saved = at::empty({m, n}, x_.options());
+    nfa_linear_args a{};
+    a.rows = m; a.in_features = (int32_t)k; a.out_features = (int32_t)n;
+    a.dtype = dtype_of(x); a.activation = (int32_t)act;
+    a.inputs = x.data_ptr(); a.inputs_stride = row_stride(x);
+    a.weight = w.data_ptr(); a.bias = ptr<void>(b);
+    if (r.defined()) { a.residual = r.data_ptr(); a.residual_stride = row_stride(r); }
+    check_rc(nfa_linear_fwd(&a, out.data_ptr(), ptr<void>(saved), stream_of(x)));
+    return {out, some(saved)};
+}
+
+std::tuple<OptTensor, OptTensor, OptTensor> linear_bwd(const Tensor &g_, const Tensor &x_, const Tensor &w_, const OptTensor &saved_, int64_t act,
+                                                       bool need_x, bool need_w, bool need_b) {
+    TORCH_CHECK(x_.dim() == 2 && w_.dim() == 2, "linear: 2-D inputs and weight expected");
+    const int64_t m = x_.size(0), k = w_.size(1), n = w_.size(0);
+    const Tensor x = as_rows(x_, "inputs", m, k, x_), w = dense_of(w_, "weight", x_.scalar_type(), n * k, x_);
+    const Tensor gy = as_rows(g_, "grad_outputs", m, n, x_);
+    const OptTensor saved = dense_of(saved_, "saved", x_.scalar_type(), m * n, x_);
+    Guard g(device_of(x_));
+    Tensor gx, gw, gb;
+    if (need_x) gx = at::empty({m, k}, x_.options());
+    if (m == 0) {
+        if (need_w) gw = at::zeros({n, k}, x_.options());
+        if (need_b) gb = at::zeros({n}, x_.options());
+        return {some(gx), some(gw), some(gb)};
+    }
+    if (need_w) gw = at::empty({n, k}, x_.options());
+    if (need_b) gb = at::empty({n}, x_.options());
+    nfa_linear_args a{};
+    a.rows = m; a.in_features = (int32_t)k; a.out_features = (int32_t)n;
+    a.dtype = dtype_of(x); a.activation = (int32_t)act;
+    a.inputs = x.data_ptr(); a.inputs_stride = row_stride(x);
+    a.weight = w.data_ptr();
+    a.grad_outputs = gy.data_ptr(); a.grad_outputs_stride = row_stride(gy);
+    Tensor ws;
+    if (need_w || need_b) ws = at::empty({nfa_linear_bwd_workspace_bytes(m, (int32_t)k, (int32_t)n, a.dtype)}, opts(x, at::kByte));
+    check_rc(nfa_linear_bwd(&a, ptr<void>(saved), ptr<void>(gx), ptr<void>(gw), ptr<void>(gb), ptr<void>(ws), stream_of(x)));
+    return {some(gx), some(gw), some(gb)};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1486,4 +1592,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("grid_occupied_cells", &grid_occupied_cells);
     m.def("set_timing", &set_timing, "names"_a = py::none());
     m.def("timing_summary", &timing_summary);
+    m.def("foreign_nodes", &foreign_nodes);
+    m.def("linear_fwd", &linear_fwd);
+    m.def("linear_bwd", &linear_bwd);
 }

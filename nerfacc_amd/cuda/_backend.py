@@ -183,6 +183,28 @@ def _check_input(t: torch.Tensor, name: str, dtype=None) -> None:
         raise RuntimeError(f"{name} must have dtype {dtype}, got {t.dtype}")
 
 
+_DTYPE_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _dtype_id(t: torch.Tensor) -> int:
+    return _DTYPE_IDS[t.dtype]
+
+
+def _as_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """a 2-D tensor whose rows are contiguous and do not overlap, at any row stride; copied if it is not one"""
+    if t is None or ((t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1)):
+        return t
+    return t.contiguous()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.shape[1] if t.shape[0] <= 1 else t.stride(0)
+
+
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if t is None else t.contiguous()
+
+
 class _Guard:
     """OptionalCUDAGuard(device_of(t)) of the reference (utils_cuda.cuh:23-24)."""
 
@@ -1094,6 +1116,47 @@ class _CtypesC:
                 _ptr(g_colors), _ptr(g_opac), _ptr(g_depth), _ptr(g_w), _ptr(g_T), _ptr(g_a), _ptr(g_sig), _ptr(g_rgb),
                 _stream(sigmas)))
         return g_sig, g_rgb
+
+    # -- feature operators ---------------------------------------------------------------------------------------------
+    @staticmethod
+    def foreign_nodes(tensors) -> int:
+        """(the extension counts autograd nodes of other streams; Python cannot ask a node for its stream)"""
+        return 0
+
+    @staticmethod
+    def linear_fwd(x, w, b, r, act: int, save: bool):
+        """(outputs, saved or None): nfa_linear_fwd"""
+        m, (n, k) = x.shape[0], w.shape
+        x, w, b, r = _as_rows(x), _dense(w), _dense(b), _as_rows(r)
+        with _Guard(x):
+            out = torch.empty((m, n), dtype=x.dtype, device=x.device)
+            L = load_library()
+            kept = save and L.nfa_linear_saved_bytes(m, n, _dtype_id(x), act, int(r is not None)) > 0
+            saved = torch.empty_like(out) if kept else None
+            a = _STRUCTS["nfa_linear_args"](rows=m, in_features=k, out_features=n, dtype=_dtype_id(x), activation=act, inputs=_ptr(x),
+                                            inputs_stride=_row_stride(x), weight=_ptr(w), bias=_ptr(b), residual=_ptr(r),
+                                            residual_stride=0 if r is None else _row_stride(r))
+            _check(L.nfa_linear_fwd(ctypes.byref(a), _ptr(out), _ptr(saved), _stream(x)))
+        return out, saved
+
+    @staticmethod
+    def linear_bwd(g, x, w, saved, act: int, need_x: bool, need_w: bool, need_b: bool):
+        """(grad_inputs, grad_weight, grad_bias), None where not asked for: nfa_linear_bwd"""
+        m, (n, k) = x.shape[0], w.shape
+        g, x, w, saved = _as_rows(g), _as_rows(x), _dense(w), _dense(saved)
+        new = torch.empty if m else torch.zeros
+        with _Guard(x):
+            gx = torch.empty((m, k), dtype=x.dtype, device=x.device) if need_x else None
+            gw = new((n, k), dtype=x.dtype, device=x.device) if need_w else None
+            gb = new((n,), dtype=x.dtype, device=x.device) if need_b else None
+            if m:
+                L = load_library()
+                ws = torch.empty(L.nfa_linear_bwd_workspace_bytes(m, k, n, _dtype_id(x)), dtype=torch.uint8, device=x.device)
+                a = _STRUCTS["nfa_linear_args"](rows=m, in_features=k, out_features=n, dtype=_dtype_id(x), activation=act, inputs=_ptr(x),
+                                                inputs_stride=_row_stride(x), weight=_ptr(w), grad_outputs=_ptr(g),
+                                                grad_outputs_stride=_row_stride(g))
+                _check(L.nfa_linear_bwd(ctypes.byref(a), _ptr(saved), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), _stream(x)))
+        return gx, gw, gb
 
 
 def _select_backend():
