@@ -491,6 +491,86 @@ int64_t nfa_linear_bwd_workspace_bytes(int64_t rows, int32_t in_features, int32_
 int nfa_linear_bwd(const nfa_linear_args *args, const void *saved, void *grad_inputs, void *grad_weight, void *grad_bias,
                    void *workspace, void *stream);
 
+/* Sequences of a flat [rows, ...] array.  packed_info [n_rays, 2] int64 (start, count): rows [start, start + count) of each ray, in any
+ * order, not overlapping; parts outside [0, rows) are cut off, and rows of no sequence get zero outputs and zero gradients.  NULL =
+ * n_rays sequences of rows / n_rays rows each, one behind the other.
+ * nfa_row_map  row_ray / row_pos [rows] int32: the sequence of each row and its position there (-1: none), what the calls below take
+ *              for packed sequences (NULL for equal ones). */
+int nfa_row_map(const int64_t *packed_info, int64_t n_rays, int64_t rows, int32_t *row_ray, int32_t *row_pos, void *stream);
+
+/* Short causal convolution along each sequence, channel by channel:
+ *   z[t] = bias + sum_j weight[:, j] x[t - width + 1 + j],  outputs = act(z);  rows before the first come from initial_state (zeros
+ *   without one).  activation: NFA_ACT_NONE or NFA_ACT_SILU.  width: 2 .. 4.
+ * nfa_causal_conv_fwd   outputs [rows, channels] contiguous; final_state (nullable) [n_rays, width - 1, channels]: the last width - 1
+ *                       inputs of each sequence, its initial state in front where it is shorter.
+ * nfa_causal_conv_bwd   grad_outputs, grad_final_state (nullable) -> grad_inputs, grad_weight, grad_bias, grad_initial_state (each
+ *                       nullable).  workspace: nfa_causal_conv_bwd_workspace_bytes(...).
+ * nfa_causal_conv_step  one row per sequence: inputs [n_rays, channels] and state -> outputs and out_state (may be state itself). */
+typedef struct nfa_causal_conv_args {
+    int64_t n_rays, rows;
+    int32_t channels, width;
+    int32_t dtype, activation;
+    const void *inputs;
+    int64_t inputs_stride;
+    const void *weight;           /* [channels, width] */
+    const void *bias;             /* [channels] nullable */
+    const void *initial_state;    /* [n_rays, width - 1, channels] nullable */
+    const int64_t *packed_info;   /* nullable */
+    const int32_t *row_ray;       /* with packed_info */
+    const int32_t *row_pos;
+    const void *grad_outputs;     /* backward only */
+    int64_t grad_outputs_stride;
+    const void *grad_final_state; /* backward only, nullable */
+} nfa_causal_conv_args;
+
+int nfa_causal_conv_fwd(const nfa_causal_conv_args *args, void *outputs, void *final_state, void *stream);
+int64_t nfa_causal_conv_bwd_workspace_bytes(int64_t rows, int32_t channels, int32_t width, int32_t dtype);
+int nfa_causal_conv_bwd(const nfa_causal_conv_args *args, void *grad_inputs, void *grad_weight, void *grad_bias,
+                        void *grad_initial_state, void *workspace, void *stream);
+int nfa_causal_conv_step(const nfa_causal_conv_args *args, const void *state, void *outputs, void *out_state, void *stream);
+
+/* Selective state space scan along each sequence:
+ *   step = delta (+ delta_bias), softplus of it if delta_softplus;   h[t] = exp(step A) h[t - 1] + step B[t] u[t]    (channels x states)
+ *   y[t] = C[t] . h[t] + D u[t],   outputs = y (gate == NULL) or y silu(gate)
+ * h before the first row comes from initial_state (zeros without one).  inputs (u), delta, gate, B, C, outputs: dtype; A, D, delta_bias
+ * and states: float.  states: 1 .. NFA_SCAN_MAX_STATES.
+ * nfa_selective_scan_fwd   outputs [rows, channels] contiguous; final_state (nullable) [n_rays, channels, states]; checkpoints
+ *                          (nullable unless a backward pass follows): nfa_selective_scan_checkpoint_bytes(...).
+ *                          workspace: nfa_selective_scan_workspace_bytes(..., 0), may be 0 bytes.
+ * nfa_selective_scan_bwd   grad_outputs, grad_final_state (nullable) -> the gradients of every input (grad_D, grad_gate, grad_delta_bias,
+ *                          grad_initial_state nullable).  workspace: nfa_selective_scan_workspace_bytes(..., 1).
+ * nfa_selective_scan_step  one row per sequence: -> outputs and out_state (may be state itself). */
+#define NFA_SCAN_MAX_STATES 256
+
+typedef struct nfa_selective_scan_args {
+    int64_t n_rays, rows;
+    int32_t channels, states;
+    int32_t dtype, delta_softplus;
+    const void *inputs, *delta, *gate, *B, *C;      /* [rows, channels] x 3 (gate nullable), [rows, states] x 2 */
+    int64_t inputs_stride, delta_stride, gate_stride, B_stride, C_stride;
+    const float *A;                                 /* [channels, states] */
+    const float *D, *delta_bias;                    /* [channels], nullable */
+    const float *initial_state;                     /* [n_rays, channels, states] nullable */
+    const int64_t *packed_info;                     /* nullable */
+    const int32_t *row_ray, *row_pos;               /* with packed_info */
+    const void *grad_outputs;                       /* backward only */
+    int64_t grad_outputs_stride;
+    const float *grad_final_state;                  /* backward only, nullable */
+} nfa_selective_scan_args;
+
+typedef struct nfa_selective_scan_grads {
+    void *inputs, *delta, *gate, *B, *C;            /* contiguous, dtype; gate nullable */
+    float *A, *D, *delta_bias, *initial_state;      /* D, delta_bias, initial_state nullable */
+} nfa_selective_scan_grads;
+
+int64_t nfa_selective_scan_checkpoint_bytes(int64_t rows, int32_t channels, int32_t states);
+int64_t nfa_selective_scan_workspace_bytes(int64_t n_rays, int64_t rows, int32_t channels, int32_t states, int32_t backward);
+int nfa_selective_scan_fwd(const nfa_selective_scan_args *args, void *outputs, float *final_state, float *checkpoints,
+                           void *workspace, void *stream);
+int nfa_selective_scan_bwd(const nfa_selective_scan_args *args, const float *checkpoints, const nfa_selective_scan_grads *grads,
+                           void *workspace, void *stream);
+int nfa_selective_scan_step(const nfa_selective_scan_args *args, const float *state, void *outputs, float *out_state, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

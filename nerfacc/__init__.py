@@ -12,7 +12,7 @@ import nerfacc_amd as _impl
 from nerfacc_amd import *  # noqa: F401,F403
 from nerfacc_amd import __version__  # noqa: F401
 
-for _name in ("cuda", "data_specs", "dense", "grid", "losses", "pack", "pdf", "scan", "volrend", "version", "sharding",
+for _name in ("cuda", "data_specs", "dense", "grid", "losses", "pack", "pdf", "scan", "selective", "volrend", "version", "sharding",
               "estimators", "estimators.base", "estimators.occ_grid", "estimators.prop_net"):
     _mod = importlib.import_module("nerfacc_amd." + _name)
     sys.modules[__name__ + "." + _name] = _mod

@@ -15,6 +15,7 @@ from .losses import distortion
 from .options import get_option, list_options, options, release_workspace, reset_options, set_option
 from .pack import pack_info
 from .pdf import importance_sampling, searchsorted
+from .selective import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 from .scan import exclusive_prod, exclusive_sum, inclusive_prod, inclusive_sum
 from .version import __version__
 from .volrend import (
@@ -45,4 +46,4 @@ __all__ = [
 # additions of this implementation (not in the reference's list of 24 names)
 __all__ += ["sample_positions", "set_option", "get_option", "reset_options", "list_options", "options", "release_workspace"]
 # feature operators between sampling and rendering
-__all__ += ["linear"]
+__all__ += ["linear", "causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step"]

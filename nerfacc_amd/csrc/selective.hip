@@ -1,0 +1,811 @@
+// selective.hip — selective state space scan along each sequence (ray), forward, backward and one row at a time, for gfx950.
+//
+//   step = softplus(delta + bias),  h[t] = exp(step A) h[t-1] + step B[t] u[t],  y[t] = C[t] . h[t] + D u[t],  out = y silu(gate)
+//
+// What bounds it: per (row, channel, state) one exponential (a quarter-rate instruction) and four full-rate ones, against 2-4 bytes per
+// (row, channel) and tensor: with 16 states the vector units need two to three times as long as memory.  So a lane keeps as many of a
+// channel's states as registers allow (up to 16, P lanes per channel beyond that), everything per (row, channel) — softplus, gate,
+// loads — is shared by them, B[t] and C[t] come from LDS as broadcasts, and the loads of the next eight rows are in flight meanwhile.
+//
+// A wave owns 64 / P channels of one sequence and walks its rows: no hand-off, no atomics.  Where the sequences are too few for the
+// chip, they are cut into chunks: a first pass leaves what each chunk adds to the state and the sum of its steps (its decay is
+// exp(A sum)), a short pass chains the chunks, and the main pass starts every chunk from its state.
+//
+// Backward: h is formed again from states the forward pass left every eight rows (any place of a row grid holds the start of at most
+// one such eighth, because sequences do not overlap: slot = row / 8 needs no table).  With G = dL/dh,  G[t] = C[t] dy[t] +
+// exp(step[t+1] A) G[t+1]:
+//   dC = sum_d dy h,  dB = sum_d G step u,  du = step sum_s G B + D dy,  dstep = sum_s G (A a h[t-1] + B u),  dA = sum_t G step a h[t-1].
+// The sums over channels are exchanged across lanes (halving the values at every step: 16 values over 32 lanes cost 16 + 4 moves);
+// the sums over rows stay in registers over all rows of a wave; both are joined in a fixed order.
+#include "feature.hpp"
+
+namespace nfa {
+namespace {
+
+constexpr int kTile = 8;                // rows between kept states, and rows whose loads are in flight together
+
+struct ScanArgs {
+    const void *u, *dt, *z, *B, *C, *gy;
+    int64_t ld_u, ld_dt, ld_z, ld_B, ld_C, ld_gy;
+    const float *A, *D, *bias, *init, *gfinal;
+    const int64_t *info;
+    const int32_t *ray, *pos;
+    void *y, *gu, *gdt, *gz;
+    float *final_state, *kept, *ginit;
+    float *ends, *sums;                 // chunks: [slots][states][channels], [slots][channels]
+    float *part_bc;                     // backward: [channel blocks][rows][2][padded states]
+    float *part_w;                      // backward: [workers][channels * states + 2 * channels]
+    int64_t rows, n_rays, length, chunk, chunks, slots, tasks, workers;
+    int32_t channels, states, softplus, blocks;
+};
+
+// a task: a run of rows of one sequence
+struct Task { int64_t ray, start, count, first, n, slot; bool live; };      // sequence rows [start, start + count), the task's [first, first + n) of it
+
+__device__ __forceinline__ void sequence_rows(const ScanArgs &a, int64_t ray, int64_t &start, int64_t &count) {
+    if (!a.info) { start = ray * a.length; count = a.length; return; }
+    start = readfirstlane_i64(a.info[2 * ray]);
+    count = readfirstlane_i64(a.info[2 * ray + 1]);
+    if (start < 0) { count += start; start = 0; }
+    if (start > a.rows) start = a.rows;
+    if (count < 0) count = 0;
+    if (count > a.rows - start) count = a.rows - start;
+}
+// chunk k >= 1 of a sequence begins `chunk` rows behind the one before it, so no two of them begin in the same block of `chunk` rows
+__device__ __forceinline__ int64_t chunk_slot(const ScanArgs &a, int64_t ray, int64_t start, int64_t k) {
+    return k == 0 ? a.slots - a.n_rays + ray : (start + k * a.chunk) / a.chunk;
+}
+
+__device__ __forceinline__ Task find_task(const ScanArgs &a, int64_t id, int lane) {
+    Task t;
+    int64_t k = 0;
+    t.live = true;
+    if (a.chunk == 0) t.ray = id;
+    else if (!a.info) { t.ray = id / a.chunks; k = id - t.ray * a.chunks; }
+    else if (id < a.n_rays) t.ray = id;
+    else {                              // the chunk that begins inside block id - n_rays, if one does
+        const int64_t base = (id - a.n_rays) * a.chunk;
+        t.live = false;
+        t.ray = 0;
+        for (int64_t r = base; r < base + a.chunk && r < a.rows; r += kWave) {
+            const int64_t row = r + lane;
+            int32_t p = -1;
+            if (row < base + a.chunk && row < a.rows) p = a.pos[row];
+            const unsigned long long hit = __ballot(p > 0 && p % (int32_t)a.chunk == 0);
+            if (hit) {
+                const int src = __ffsll((long long)hit) - 1;
+                k = __builtin_amdgcn_readlane(p, src) / (int32_t)a.chunk;
+                t.ray = __builtin_amdgcn_readfirstlane(a.ray[r + src]);
+                t.live = true;
+                break;
+            }
+        }
+        if (!t.live) { t.start = t.count = t.first = t.n = t.slot = 0; return t; }
+    }
+    sequence_rows(a, t.ray, t.start, t.count);
+    t.first = k * a.chunk;
+    t.n = t.count - t.first;
+    if (a.chunk && t.n > a.chunk) t.n = a.chunk;
+    if (t.n < 0) t.n = 0;
+    t.slot = a.chunk ? chunk_slot(a, t.ray, t.start, k) : 0;
+    if (k > 0 && t.n == 0) t.live = false;
+    return t;
+}
+
+// exchanges the upper half (odd rows) of `a` with the lower half (even rows) of `b` in one instruction and adds: with a = b every lane
+// gets its pair's sum, with two values lanes without the bit get a's sum and lanes with it b's
+template <int BIT>
+__device__ __forceinline__ float swap_add(float a, float b) {
+    const unsigned i = __builtin_bit_cast(unsigned, a), j = __builtin_bit_cast(unsigned, b);
+    unsigned x, y;                                          // (elements by value: a bit cast of an element takes the first one)
+    if constexpr (BIT == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(i, j, false, false);
+        x = r[0], y = r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane16_swap(i, j, false, false);
+        x = r[0], y = r[1];
+    }
+    return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
+}
+// the value of the lane whose number differs in BIT
+template <int BIT>
+__device__ __forceinline__ float other_lane(float v) {
+    if constexpr (BIT == 8) return dpp_f<0x128>(0.0f, v);                                    // row_ror:8
+    else if constexpr (BIT == 4) return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x101f));   // xor 4
+    else if constexpr (BIT == 2) return dpp_f<0x4e>(0.0f, v);                                // quad_perm [2, 3, 0, 1]
+    else return dpp_f<0xb1>(0.0f, v);                                                        // quad_perm [1, 0, 3, 2]
+}
+template <int BIT>
+__device__ __forceinline__ float add_other(float v) {
+    if constexpr (BIT >= 16) return swap_add<BIT>(v, v);
+    else return v + other_lane<BIT>(v);
+}
+// two values summed over the lane pair that differs in BIT: lanes without the bit get v0's sum, lanes with it v1's
+template <int BIT>
+__device__ __forceinline__ float halve(float v0, float v1, int lane) {
+    if constexpr (BIT >= 16) {
+        return swap_add<BIT>(v0, v1);
+    } else {
+        const bool up = lane & BIT;
+        return (up ? v1 : v0) + other_lane<BIT>(up ? v0 : v1);
+    }
+}
+// sums v[0 .. CNT) over the lanes that differ in the bits BIT, BIT / 2, ... 1; afterwards v[0 .. left) holds the values
+// that number_of() names
+template <int CNT, int BIT>
+__device__ __forceinline__ void sum_over_lanes(float *v, int lane) {
+    if constexpr (BIT > 0) {
+        if constexpr (CNT > 1) {
+#pragma unroll
+            for (int i = 0; i < CNT / 2; ++i) v[i] = halve<BIT>(v[2 * i], v[2 * i + 1], lane);
+            sum_over_lanes<CNT / 2, BIT / 2>(v, lane);
+        } else {
+            v[0] = add_other<BIT>(v[0]);
+            sum_over_lanes<1, BIT / 2>(v, lane);
+        }
+    }
+}
+constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
+
+// sum over the P lanes of a channel (lane = part * (64 / P) + channel)
+template <int P>
+__device__ __forceinline__ float sum_parts(float v) {
+    if constexpr (P >= 2) v = add_other<32>(v);
+    if constexpr (P >= 4) v = add_other<16>(v);
+    if constexpr (P >= 8) v = add_other<8>(v);
+    if constexpr (P >= 16) v = add_other<4>(v);
+    if constexpr (P >= 32) v = add_other<2>(v);
+    return v;
+}
+
+// what a wave has in hand of the next eight rows
+template <class T, int NS, int P, bool HAS_C, bool HAS_Z, bool HAS_G>
+struct Rows {
+    static constexpr int SP = NS * P, kStates = kTile * SP / kWave > 0 ? (kTile * SP + kWave - 1) / kWave : 1;
+    T u[kTile], dt[kTile], z[HAS_Z ? kTile : 1], g[HAS_G ? kTile : 1];
+    T b[kStates], c[HAS_C ? kStates : 1];
+
+    __device__ __forceinline__ void load(const ScanArgs &a, int64_t row, int n, int64_t ch, bool on, int lane) {
+#pragma unroll
+        for (int t = 0; t < kTile; ++t) {
+            u[t] = dt[t] = T(0.0f);
+            if (HAS_Z) z[t] = T(0.0f);
+            if (HAS_G) g[t] = T(0.0f);
+            if (t < n && on) {
+                if (!HAS_G || a.u) u[t] = reinterpret_cast<const T *>(a.u)[(row + t) * a.ld_u + ch];
+                dt[t] = reinterpret_cast<const T *>(a.dt)[(row + t) * a.ld_dt + ch];
+                if (HAS_Z && a.z) z[t] = reinterpret_cast<const T *>(a.z)[(row + t) * a.ld_z + ch];
+                if (HAS_G) g[t] = reinterpret_cast<const T *>(a.gy)[(row + t) * a.ld_gy + ch];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kStates; ++k) {
+            const int e = k * kWave + lane, t = e / SP, s = e % SP;
+            b[k] = T(0.0f);
+            if (HAS_C) c[k] = T(0.0f);
+            if (t < n && s < a.states) {
+                b[k] = reinterpret_cast<const T *>(a.B)[(row + t) * a.ld_B + s];
+                if (HAS_C) c[k] = reinterpret_cast<const T *>(a.C)[(row + t) * a.ld_C + s];
+            }
+        }
+    }
+    // B and C into this wave's LDS: [2][kTile][SP]
+    __device__ __forceinline__ void stage(float *lds, int lane) const {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < kStates; ++k) {
+            const int e = k * kWave + lane;
+            if (e < kTile * SP) {
+                lds[e] = to_f(b[k]);
+                if (HAS_C) lds[kTile * SP + e] = to_f(c[k]);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+};
+
+template <int NS> __device__ __forceinline__ void read_states(const float *at, float (&v)[NS]) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) v[i] = at[i];
+}
+
+// main pass (LOCAL = false): outputs, kept states, final state; first pass over chunks (LOCAL): what a chunk adds, and its steps' sum
+template <class T, int NS, int P, bool LOCAL>
+__global__ __launch_bounds__(kBlock) void scan_fwd_kernel(ScanArgs a) {
+    constexpr int SP = NS * P, CH = kWave / P;
+    __shared__ __attribute__((aligned(16))) float shared[kWavesPerBlock][2 * kTile * SP];
+    const int lane = lane_id(), wave = wave_in_block(), part = lane / CH;
+    const int64_t id = (int64_t)blockIdx.x * kWavesPerBlock + wave;
+    const int64_t task = id / a.blocks;
+    if (task >= a.tasks) return;
+    const int64_t ch = (id - task * a.blocks) * CH + lane % CH;
+    const bool on = ch < a.channels;
+    const Task t = find_task(a, task, lane);
+    if (!t.live) return;
+    float *lds = shared[wave];
+    float A2[NS], h[NS];
+    const float D = on && a.D ? a.D[ch] : 0.0f, bias = on && a.bias ? a.bias[ch] : 0.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int s = part * NS + i;
+        const bool here = on && s < a.states;
+        A2[i] = here ? a.A[ch * a.states + s] * kLog2e : 0.0f;
+        h[i] = 0.0f;
+        if (!LOCAL && here) {
+            if (a.chunk) h[i] = a.ends[(t.slot * a.states + s) * a.channels + ch];
+            else if (a.init) h[i] = a.init[(t.ray * a.channels + ch) * a.states + s];
+        }
+    }
+    Rows<T, NS, P, !LOCAL, !LOCAL, false> next;
+    const int64_t row0 = t.start + t.first;
+    int left = (int)(t.n < kTile ? t.n : kTile);
+    next.load(a, row0, left, ch, on, lane);
+    for (int64_t k = 0; k < t.n; k += kTile) {
+        const auto rows = next;
+        const int n = left;
+        rows.stage(lds, lane);
+        const int64_t rest = t.n - k - kTile;
+        left = (int)(rest < kTile ? (rest > 0 ? rest : 0) : kTile);
+        if (left > 0) next.load(a, row0 + k + kTile, left, ch, on, lane);
+        if (!LOCAL && a.kept && t.first + k > 0) {
+            float *to = a.kept + ((row0 + k) / kTile) * a.states * a.channels;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const int s = part * NS + i;
+                if (on && s < a.states) to[(int64_t)s * a.channels + ch] = h[i];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kTile; ++j) {
+            if (j >= n) break;
+            const float u = to_f(rows.u[j]);
+            float step = to_f(rows.dt[j]) + bias;
+            if (a.softplus) step = softplus_f(step);
+            const float in = step * u;
+            float B[NS], C[NS], y = 0.0f;
+            read_states<NS>(lds + j * SP + part * NS, B);
+            if (!LOCAL) read_states<NS>(lds + (kTile + j) * SP + part * NS, C);
+            sum += step;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                h[i] = fmaf(fast_exp2(step * A2[i]), h[i], in * B[i]);
+                if (!LOCAL) y = fmaf(C[i], h[i], y);
+            }
+            if (!LOCAL) {
+                y = fmaf(D, u, sum_parts<P>(y));
+                if (a.z) {
+                    const float z = to_f(rows.z[j]);
+                    y *= z * sigmoid_f(z);
+                }
+                if (on && part == 0) reinterpret_cast<T *>(a.y)[(row0 + k + j) * a.channels + ch] = from_f<T>(y);
+            }
+        }
+    }
+    if (LOCAL) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int s = part * NS + i;
+            if (on && s < a.states) a.ends[(t.slot * a.states + s) * a.channels + ch] = h[i];
+        }
+        if (on && part == 0) a.sums[t.slot * a.channels + ch] = sum;
+    } else if (a.final_state && t.first + t.n == t.count) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int s = part * NS + i;
+            if (on && s < a.states) a.final_state[(t.ray * a.channels + ch) * a.states + s] = h[i];
+        }
+    }
+}
+
+// chunk by chunk, a lane per (channel, state): ends[slot] becomes the state that the chunk starts from (REV: the gradient that
+// reaches its last row from behind), from what each chunk adds on its own
+template <bool REV>
+__global__ __launch_bounds__(kBlock) void scan_chain_kernel(ScanArgs a) {
+    const int64_t per = (int64_t)a.channels * a.states;
+    const int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x, ray = blockIdx.y;
+    if (e >= per) return;
+    const int64_t s = e / a.channels, ch = e - s * a.channels;
+    int64_t start, count;
+    sequence_rows(a, ray, start, count);
+    const float A2 = a.A[ch * a.states + s] * kLog2e;
+    const float *from = REV ? a.gfinal : a.init;
+    float h = from ? from[(ray * a.channels + ch) * a.states + s] : 0.0f;
+    const int64_t chunks = count > 0 ? (count + a.chunk - 1) / a.chunk : 1;
+    constexpr int kAhead = 8;
+    for (int64_t k0 = 0; k0 < chunks; k0 += kAhead) {
+        float add[kAhead], decay[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t k = k0 + i < chunks ? k0 + i : chunks - 1, slot = chunk_slot(a, ray, start, REV ? chunks - 1 - k : k);
+            add[i] = a.ends[(slot * a.states + s) * a.channels + ch];
+            decay[i] = fast_exp2(a.sums[slot * a.channels + ch] * A2);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (k0 + i >= chunks) break;
+            const int64_t k = k0 + i, slot = chunk_slot(a, ray, start, REV ? chunks - 1 - k : k);
+            a.ends[(slot * a.states + s) * a.channels + ch] = h;
+            h = fmaf(decay[i], h, add[i]);
+        }
+    }
+}
+
+// the gradient that a chunk adds at its first row, and its steps' sum
+template <class T, int NS, int P>
+__global__ __launch_bounds__(kBlock) void scan_bwd_local_kernel(ScanArgs a) {
+    constexpr int SP = NS * P, CH = kWave / P;
+    __shared__ __attribute__((aligned(16))) float shared[kWavesPerBlock][2 * kTile * SP];
+    const int lane = lane_id(), wave = wave_in_block(), part = lane / CH;
+    const int64_t id = (int64_t)blockIdx.x * kWavesPerBlock + wave;
+    const int64_t task = id / a.blocks;
+    if (task >= a.tasks) return;
+    const int64_t ch = (id - task * a.blocks) * CH + lane % CH;
+    const bool on = ch < a.channels;
+    const Task t = find_task(a, task, lane);
+    if (!t.live) return;
+    float *lds = shared[wave];
+    float A2[NS], G[NS], sum = 0.0f;
+    const float bias = on && a.bias ? a.bias[ch] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int s = part * NS + i;
+        A2[i] = on && s < a.states ? a.A[ch * a.states + s] * kLog2e : 0.0f;
+        G[i] = 0.0f;
+    }
+    const int64_t row0 = t.start + t.first, tiles = (t.n + kTile - 1) / kTile;
+    Rows<T, NS, P, true, true, true> next;
+    auto rows_in = [&](int64_t k) { const int64_t r = t.n - k * kTile; return (int)(r < kTile ? r : kTile); };
+    ScanArgs b = a;
+    b.u = nullptr;                                          // not needed here
+    if (tiles > 0) next.load(b, row0 + (tiles - 1) * kTile, rows_in(tiles - 1), ch, on, lane);
+    for (int64_t k = tiles - 1; k >= 0; --k) {
+        const auto rows = next;
+        const int n = rows_in(k);
+        rows.stage(lds, lane);
+        if (k > 0) next.load(b, row0 + (k - 1) * kTile, kTile, ch, on, lane);
+#pragma unroll
+        for (int j = kTile - 1; j >= 0; --j) {
+            if (j >= n) continue;
+            float step = to_f(rows.dt[j]) + bias;
+            if (a.softplus) step = softplus_f(step);
+            float dy = to_f(rows.g[j]);
+            if (a.z) {
+                const float z = to_f(rows.z[j]);
+                dy *= z * sigmoid_f(z);
+            }
+            float C[NS];
+            read_states<NS>(lds + (kTile + j) * SP + part * NS, C);
+            sum += step;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) G[i] = fmaf(C[i], dy, G[i]) * fast_exp2(step * A2[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int s = part * NS + i;
+        if (on && s < a.states) a.ends[(t.slot * a.states + s) * a.channels + ch] = G[i];
+    }
+    if (on && part == 0) a.sums[t.slot * a.channels + ch] = sum;
+}
+
+template <class T, int NS, int P>
+__global__ __launch_bounds__(kBlock) void scan_bwd_kernel(ScanArgs a) {
+    constexpr int SP = NS * P, CH = kWave / P;
+    __shared__ __attribute__((aligned(16))) float shared[kWavesPerBlock][2 * kTile * SP];
+    const int lane = lane_id(), wave = wave_in_block(), part = lane / CH;
+    const int64_t id = (int64_t)blockIdx.x * kWavesPerBlock + wave;
+    const int64_t worker = id / a.blocks;
+    if (worker >= a.workers) return;
+    const int block = (int)(id - worker * a.blocks);
+    const int64_t ch = (int64_t)block * CH + lane % CH;
+    const bool on = ch < a.channels;
+    float *lds = shared[wave];
+    float A[NS], A2[NS], dA[NS], dD = 0.0f, dbias = 0.0f;
+    const float D = on && a.D ? a.D[ch] : 0.0f, bias = on && a.bias ? a.bias[ch] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int s = part * NS + i;
+        A[i] = on && s < a.states ? a.A[ch * a.states + s] : 0.0f;
+        A2[i] = A[i] * kLog2e;
+        dA[i] = 0.0f;
+    }
+    // after the exchange over channels: this lane's values, their places, and whether it is the one that stores them
+    constexpr int kBits = log2_of(CH), kHalvings = kBits < log2_of(2 * NS) ? kBits : log2_of(2 * NS), kLeft = 2 * NS >> kHalvings;
+    int number = 0;
+#pragma unroll
+    for (int i = 0; i < kHalvings; ++i) number |= ((lane >> (kBits - 1 - i)) & 1) << i;
+    const bool stores = (lane & ((1 << (kBits - kHalvings)) - 1)) == 0;
+
+    for (int64_t task = worker; task < a.tasks; task += a.workers) {
+        const Task t = find_task(a, task, lane);
+        if (!t.live) continue;
+        float G[NS];                                        // dL/dh of the row behind, times its decay
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int s = part * NS + i;
+            const bool here = on && s < a.states;
+            G[i] = 0.0f;
+            if (here && a.chunk) G[i] = a.ends[(t.slot * a.states + s) * a.channels + ch];
+            else if (here && a.gfinal) G[i] = a.gfinal[(t.ray * a.channels + ch) * a.states + s];
+        }
+        const int64_t row0 = t.start + t.first, tiles = (t.n + kTile - 1) / kTile;
+        Rows<T, NS, P, true, true, true> rows;
+        for (int64_t k = tiles - 1; k >= 0; --k) {
+            const int64_t row = row0 + k * kTile;
+            const int n = (int)(t.n - k * kTile < kTile ? t.n - k * kTile : kTile);
+            rows.load(a, row, n, ch, on, lane);
+            float h0[NS], h[kTile][NS], e[kTile][NS];
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const int s = part * NS + i;
+                h0[i] = 0.0f;
+                if (on && s < a.states) {
+                    if (t.first + k > 0) h0[i] = a.kept[((row / kTile) * a.states + s) * a.channels + ch];
+                    else if (a.init) h0[i] = a.init[(t.ray * a.channels + ch) * a.states + s];
+                }
+            }
+            rows.stage(lds, lane);
+#pragma unroll
+            for (int j = 0; j < kTile; ++j) {
+                float step = to_f(rows.dt[j]) + bias;
+                if (a.softplus) step = softplus_f(step);
+                const float in = step * to_f(rows.u[j]);
+                float B[NS];
+                read_states<NS>(lds + j * SP + part * NS, B);
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    e[j][i] = fast_exp2(step * A2[i]);
+                    h[j][i] = fmaf(e[j][i], j ? h[j - 1][i] : h0[i], in * B[i]);
+                }
+            }
+#pragma unroll
+            for (int j = kTile - 1; j >= 0; --j) {
+                if (j >= n) continue;
+                const float u = to_f(rows.u[j]), raw = to_f(rows.dt[j]) + bias, step = a.softplus ? softplus_f(raw) : raw;
+                const float gy = to_f(rows.g[j]), z = to_f(rows.z[j]), sig = sigmoid_f(z);
+                const float dy = a.z ? gy * z * sig : gy, in = step * u;
+                float B[NS], C[NS], v[2 * NS], y = 0.0f, sB = 0.0f, sA = 0.0f;
+                read_states<NS>(lds + j * SP + part * NS, B);
+                read_states<NS>(lds + (kTile + j) * SP + part * NS, C);
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    const float g = fmaf(C[i], dy, G[i]);
+                    y = fmaf(C[i], h[j][i], y);
+                    v[i] = g * in;
+                    v[NS + i] = dy * h[j][i];
+                    sB = fmaf(g, B[i], sB);
+                    const float w = g * (e[j][i] * (j ? h[j - 1][i] : h0[i]));
+                    sA = fmaf(w, A[i], sA);
+                    dA[i] = fmaf(w, step, dA[i]);
+                    G[i] = g * e[j][i];
+                }
+                sB = sum_parts<P>(sB);
+                sA = sum_parts<P>(sA);
+                float dstep = fmaf(u, sB, sA);
+                if (a.softplus) dstep *= sigmoid_f(raw);
+                if (a.z) y = fmaf(D, u, sum_parts<P>(y));
+                if (on && part == 0) {
+                    const int64_t at = (row + j) * a.channels + ch;
+                    reinterpret_cast<T *>(a.gu)[at] = from_f<T>(fmaf(step, sB, D * dy));
+                    reinterpret_cast<T *>(a.gdt)[at] = from_f<T>(dstep);
+                    if (a.z) reinterpret_cast<T *>(a.gz)[at] = from_f<T>(gy * y * (sig * fmaf(z, 1.0f - sig, 1.0f)));
+                    dD = fmaf(dy, u, dD);
+                    dbias += dstep;
+                }
+                sum_over_lanes<2 * NS, CH / 2>(v, lane);
+                float *to = a.part_bc + ((int64_t)block * a.rows + row + j) * (2 * SP);
+                if (stores) {
+#pragma unroll
+                    for (int i = 0; i < kLeft; ++i) {
+                        const int q = i * (1 << kHalvings) + number;
+                        to[(q / NS) * SP + part * NS + q % NS] = v[i];
+                    }
+                }
+            }
+        }
+        if (a.ginit && t.first == 0) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const int s = part * NS + i;
+                if (on && s < a.states) a.ginit[(t.ray * a.channels + ch) * a.states + s] = G[i];
+            }
+        }
+    }
+    const int64_t per = (int64_t)a.channels * (a.states + 2);
+    float *to = a.part_w + worker * per;
+    if (!on) return;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int s = part * NS + i;
+        if (s < a.states) to[ch * a.states + s] = dA[i];
+    }
+    if (part == 0) {
+        to[(int64_t)a.channels * a.states + ch] = dD;
+        to[(int64_t)a.channels * (a.states + 1) + ch] = dbias;
+    }
+}
+
+// dB and dC of a row: the channel blocks' sums in order; zeros for rows of no sequence
+template <class T>
+__global__ __launch_bounds__(kBlock) void scan_join_bc_kernel(ScanArgs a, int sp, T *gB, T *gC) {
+    const int64_t n = a.rows * 2 * a.states;
+    for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < n; e += (int64_t)gridDim.x * kBlock) {
+        const int64_t row = e / (2 * a.states);
+        const int q = (int)(e - row * 2 * a.states), which = q / a.states, s = q - which * a.states;
+        float v = 0.0f;
+        if (!a.info || a.pos[row] >= 0)
+            for (int b = 0; b < a.blocks; ++b) v += a.part_bc[((int64_t)b * a.rows + row) * (2 * sp) + which * sp + s];
+        (which ? gC : gB)[row * a.states + s] = from_f<T>(v);
+    }
+}
+
+// rows of no sequence
+template <class T>
+__global__ __launch_bounds__(kBlock) void zero_rows_kernel(const int32_t *__restrict__ pos, int64_t rows, int32_t cols, T *p, T *q, T *r) {
+    const int lane = lane_id();
+    for (int64_t base = ((int64_t)blockIdx.x * kWavesPerBlock + wave_in_block()) * kWave; base < rows;
+         base += (int64_t)gridDim.x * kBlock) {
+        unsigned long long none = __ballot(base + lane < rows && pos[base + lane < rows ? base + lane : base] < 0);
+        while (none) {
+            const int64_t row = base + __ffsll((long long)none) - 1;
+            none &= none - 1;
+            for (int c = lane; c < cols; c += kWave) {
+                p[row * cols + c] = T(0.0f);
+                if (q) q[row * cols + c] = T(0.0f);
+                if (r) r[row * cols + c] = T(0.0f);
+            }
+        }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kBlock) void scan_step_kernel(ScanArgs a, const float *state, float *next) {
+    const int64_t n = a.n_rays * a.channels;
+    for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < n; e += (int64_t)gridDim.x * kBlock) {
+        const int64_t ray = e / a.channels, ch = e - ray * a.channels;
+        const float u = to_f(reinterpret_cast<const T *>(a.u)[ray * a.ld_u + ch]);
+        float step = to_f(reinterpret_cast<const T *>(a.dt)[ray * a.ld_dt + ch]) + (a.bias ? a.bias[ch] : 0.0f);
+        if (a.softplus) step = softplus_f(step);
+        const float in = step * u, d2 = step * kLog2e;
+        float y = 0.0f;
+        for (int s = 0; s < a.states; ++s) {
+            const float B = to_f(reinterpret_cast<const T *>(a.B)[ray * a.ld_B + s]), C = to_f(reinterpret_cast<const T *>(a.C)[ray * a.ld_C + s]);
+            const float h = fmaf(fast_exp2(d2 * a.A[ch * a.states + s]), state[e * a.states + s], in * B);
+            next[e * a.states + s] = h;
+            y = fmaf(C, h, y);
+        }
+        if (a.D) y = fmaf(a.D[ch], u, y);
+        if (a.z) {
+            const float z = to_f(reinterpret_cast<const T *>(a.z)[ray * a.ld_z + ch]);
+            y *= z * sigmoid_f(z);
+        }
+        reinterpret_cast<T *>(a.y)[e] = from_f<T>(y);
+    }
+}
+
+// lanes per channel and states per lane
+struct Shape { int ns, p; };
+Shape shape_of(int states, int most) {
+    Shape s{4, 1};
+    while (s.ns < most && s.ns < states) s.ns *= 2;
+    while (s.ns * s.p < states) s.p *= 2;
+    return s;
+}
+constexpr int kFwdStates = 16, kBwdStates = 8;
+
+// calls f(T{}, integral NS, integral P)
+template <int MOST, class F>
+void with_shape(int32_t dtype, Shape sh, F &&f) {
+    with_dtype(dtype, [&](auto t) {
+        if constexpr (MOST >= 16) {
+            if (sh.ns == 16) {
+                auto ns = std::integral_constant<int, 16>{};
+                if (sh.p == 1) f(t, ns, std::integral_constant<int, 1>{});
+                else if (sh.p == 2) f(t, ns, std::integral_constant<int, 2>{});
+                else if (sh.p == 4) f(t, ns, std::integral_constant<int, 4>{});
+                else if (sh.p == 8) f(t, ns, std::integral_constant<int, 8>{});
+                else f(t, ns, std::integral_constant<int, 16>{});
+                return;
+            }
+        }
+        if (sh.ns == 4) {
+            f(t, std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+            return;
+        }
+        auto ns = std::integral_constant<int, 8>{};
+        if constexpr (MOST >= 16) {
+            f(t, ns, std::integral_constant<int, 1>{});
+        } else {
+            if (sh.p == 1) f(t, ns, std::integral_constant<int, 1>{});
+            else if (sh.p == 2) f(t, ns, std::integral_constant<int, 2>{});
+            else if (sh.p == 4) f(t, ns, std::integral_constant<int, 4>{});
+            else if (sh.p == 8) f(t, ns, std::integral_constant<int, 8>{});
+            else if (sh.p == 16) f(t, ns, std::integral_constant<int, 16>{});
+            else f(t, ns, std::integral_constant<int, 32>{});
+        }
+    });
+}
+
+// How a call is cut: whole sequences where they give every SIMD a wave; otherwise chunks of at least 32 rows, enough for two waves per
+// SIMD.  (Cutting costs a second pass over the exponentials, so it has to more than double the waves.)
+struct ScanPlan { Shape sh; int blocks; int64_t chunk, chunks, slots, tasks, workers; };
+ScanPlan scan_plan(int64_t n_rays, int64_t rows, int channels, int states, bool packed, bool backward) {
+    ScanPlan p{};
+    p.sh = shape_of(states, backward ? kBwdStates : kFwdStates);
+    p.blocks = (int)ceil_div(channels, kWave / p.sh.p);
+    const int64_t waves = n_rays * p.blocks, want = (int64_t)kNumCU * 8;
+    p.tasks = n_rays;
+    if (n_rays > 0 && waves < kNumCU * 4 && rows / n_rays >= 64) {
+        int64_t chunk = ceil_div(ceil_div(rows * p.blocks, want), kTile) * kTile;
+        if (chunk < 32) chunk = 32;
+        if (chunk < rows / n_rays) {
+            p.chunk = chunk;
+            p.chunks = ceil_div(rows / n_rays, chunk);
+            p.slots = rows / chunk + 1 + n_rays;
+            p.tasks = packed ? n_rays + ceil_div(rows, chunk) : n_rays * p.chunks;
+        }
+    }
+    p.workers = p.tasks;
+    const int64_t most = ceil_div(4096, p.blocks);
+    if (backward && p.workers > most) p.workers = most;
+    return p;
+}
+int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
+struct ScanSpace { int64_t ends, sums, bc, w, total; };
+ScanSpace scan_space(const ScanPlan &p, int64_t rows, int channels, int states, bool backward) {
+    ScanSpace s{};
+    s.ends = align256(p.slots * states * channels * 4);
+    s.sums = align256(p.slots * channels * 4);
+    if (backward) {
+        s.bc = align256((int64_t)p.blocks * rows * 2 * p.sh.ns * p.sh.p * 4);
+        s.w = align256(p.workers * channels * (states + 2) * 4);
+    }
+    s.total = s.ends + s.sums + s.bc + s.w;
+    return s;
+}
+
+int check_scan(const nfa_selective_scan_args *a, const char *who, bool step) {
+    NFA_REQUIRE(a, "%s: NULL arguments", who);
+    NFA_REQUIRE(a->n_rays >= 0 && a->rows >= 0 && a->channels >= 1, "%s: bad size", who);
+    NFA_REQUIRE(a->states >= 1 && a->states <= NFA_SCAN_MAX_STATES, "%s: states must be 1 .. %d, got %d", who, NFA_SCAN_MAX_STATES, a->states);
+    NFA_REQUIRE(dtype_ok(a->dtype), "%s: bad dtype %d", who, a->dtype);
+    NFA_REQUIRE(a->rows < (1ll << 31) && a->n_rays < (1ll << 31) && a->channels <= (1 << 24), "%s: too many rows, rays or channels", who);
+    const int64_t rows = step ? a->n_rays : a->rows;
+    NFA_REQUIRE(a->A, "%s: NULL pointer", who);
+    NFA_REQUIRE(rows == 0 || (a->inputs && a->delta && a->B && a->C), "%s: NULL pointer", who);
+    NFA_REQUIRE(rows <= 1 || (a->inputs_stride >= a->channels && a->delta_stride >= a->channels && (!a->gate || a->gate_stride >= a->channels) &&
+                              a->B_stride >= a->states && a->C_stride >= a->states), "%s: a row stride is shorter than its row", who);
+    if (step) return NFA_OK;
+    NFA_REQUIRE(a->packed_info || a->n_rays == 0 || a->rows % a->n_rays == 0, "%s: rows do not divide into equal sequences", who);
+    NFA_REQUIRE(a->n_rays > 0 || a->packed_info || a->rows == 0, "%s: rows without sequences", who);
+    NFA_REQUIRE(!a->packed_info || a->rows == 0 || (a->row_ray && a->row_pos), "%s: packed sequences need their row map", who);
+    return NFA_OK;
+}
+
+ScanArgs scan_args(const nfa_selective_scan_args *a) {
+    ScanArgs d{};
+    d.u = a->inputs; d.ld_u = a->inputs_stride;
+    d.dt = a->delta; d.ld_dt = a->delta_stride;
+    d.z = a->gate; d.ld_z = a->gate_stride;
+    d.B = a->B; d.ld_B = a->B_stride;
+    d.C = a->C; d.ld_C = a->C_stride;
+    d.gy = a->grad_outputs; d.ld_gy = a->grad_outputs_stride;
+    d.A = a->A; d.D = a->D; d.bias = a->delta_bias; d.init = a->initial_state; d.gfinal = a->grad_final_state;
+    d.info = a->packed_info; d.ray = a->row_ray; d.pos = a->row_pos;
+    d.rows = a->rows; d.n_rays = a->n_rays;
+    d.length = a->n_rays > 0 ? a->rows / a->n_rays : 0;
+    d.channels = a->channels; d.states = a->states; d.softplus = a->delta_softplus != 0;
+    return d;
+}
+void use_plan(ScanArgs &d, const ScanPlan &p, const ScanSpace &sp, void *workspace) {
+    d.chunk = p.chunk; d.chunks = p.chunks; d.slots = p.slots; d.tasks = p.tasks; d.workers = p.workers; d.blocks = p.blocks;
+    char *w = (char *)workspace;
+    d.ends = (float *)w;
+    d.sums = (float *)(w + sp.ends);
+    d.part_bc = (float *)(w + sp.ends + sp.sums);
+    d.part_w = (float *)(w + sp.ends + sp.sums + sp.bc);
+}
+
+template <bool REV>
+void launch_chain(const ScanArgs &d, hipStream_t s) {
+    const dim3 grid((unsigned)ceil_div((int64_t)d.channels * d.states, kBlock), (unsigned)d.n_rays);
+    hipLaunchKernelGGL((scan_chain_kernel<REV>), grid, dim3(kBlock), 0, s, d);
+}
+void launch_zero_rows(const ScanArgs &d, int32_t dtype, void *p, void *q, void *r, hipStream_t s) {
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((zero_rows_kernel<T>), dim3(blocks_for(d.rows)), dim3(kBlock), 0, s, d.pos, d.rows, d.channels, (T *)p, (T *)q, (T *)r);
+    });
+}
+
+}  // namespace
+}  // namespace nfa
+
+using namespace nfa;
+
+NFA_EXPORT int64_t nfa_selective_scan_checkpoint_bytes(int64_t rows, int32_t channels, int32_t states) {
+    if (rows <= 0 || channels <= 0 || states <= 0) return 0;
+    return ceil_div(rows, kTile) * channels * states * 4;
+}
+
+NFA_EXPORT int64_t nfa_selective_scan_workspace_bytes(int64_t n_rays, int64_t rows, int32_t channels, int32_t states, int32_t backward) {
+    if (n_rays <= 0 || rows <= 0 || channels <= 0 || states <= 0 || states > NFA_SCAN_MAX_STATES) return 0;
+    const ScanPlan p = scan_plan(n_rays, rows, channels, states, true, backward != 0), q = scan_plan(n_rays, rows, channels, states, false, backward != 0);
+    const int64_t x = scan_space(p, rows, channels, states, backward != 0).total, y = scan_space(q, rows, channels, states, backward != 0).total;
+    return x > y ? x : y;
+}
+
+NFA_EXPORT int nfa_selective_scan_fwd(const nfa_selective_scan_args *a, void *outputs, float *final_state, float *checkpoints,
+                                      void *workspace, void *stream) {
+    if (int rc = check_scan(a, "selective_scan_fwd", false)) return rc;
+    NFA_REQUIRE(outputs || a->rows == 0, "selective_scan_fwd: NULL pointer");
+    hipStream_t s = (hipStream_t)stream;
+    ScanArgs d = scan_args(a);
+    const ScanPlan p = scan_plan(a->n_rays, a->rows, a->channels, a->states, a->packed_info != nullptr, false);
+    const ScanSpace sp = scan_space(p, a->rows, a->channels, a->states, false);
+    NFA_REQUIRE(workspace || sp.total == 0, "selective_scan_fwd: NULL workspace");
+    use_plan(d, p, sp, workspace);
+    d.y = outputs; d.final_state = final_state; d.kept = checkpoints;
+    if (a->packed_info && a->rows > 0) launch_zero_rows(d, a->dtype, outputs, nullptr, nullptr, s);
+    if (p.tasks > 0) {
+        const int64_t grid = ceil_div(p.tasks * p.blocks, kWavesPerBlock);
+        NFA_REQUIRE(grid < (1ll << 31) && a->n_rays * (int64_t)(p.chunk ? 1 : 0) < 65536, "selective_scan_fwd: too large for one launch");
+        with_shape<kFwdStates>(a->dtype, p.sh, [&](auto t, auto ns, auto pp) {
+            using T = decltype(t);
+            if (p.chunk) {
+                hipLaunchKernelGGL((scan_fwd_kernel<T, ns(), pp(), true>), dim3((unsigned)grid), dim3(kBlock), 0, s, d);
+                launch_chain<false>(d, s);
+            }
+            hipLaunchKernelGGL((scan_fwd_kernel<T, ns(), pp(), false>), dim3((unsigned)grid), dim3(kBlock), 0, s, d);
+        });
+    }
+    return check_launch("scan_fwd_kernel");
+}
+
+NFA_EXPORT int nfa_selective_scan_bwd(const nfa_selective_scan_args *a, const float *checkpoints, const nfa_selective_scan_grads *g,
+                                      void *workspace, void *stream) {
+    if (int rc = check_scan(a, "selective_scan_bwd", false)) return rc;
+    if (a->rows == 0 || a->n_rays == 0) return NFA_OK;
+    NFA_REQUIRE(g && g->inputs && g->delta && g->B && g->C && g->A && a->grad_outputs && checkpoints && workspace, "selective_scan_bwd: NULL pointer");
+    NFA_REQUIRE(!a->gate || g->gate, "selective_scan_bwd: NULL pointer");
+    NFA_REQUIRE(a->grad_outputs_stride >= a->channels || a->rows <= 1, "selective_scan_bwd: grad_outputs_stride < channels");
+    hipStream_t s = (hipStream_t)stream;
+    ScanArgs d = scan_args(a);
+    const ScanPlan p = scan_plan(a->n_rays, a->rows, a->channels, a->states, a->packed_info != nullptr, true);
+    const ScanSpace sp = scan_space(p, a->rows, a->channels, a->states, true);
+    use_plan(d, p, sp, workspace);
+    d.kept = (float *)checkpoints;
+    d.gu = g->inputs; d.gdt = g->delta; d.gz = a->gate ? g->gate : nullptr; d.ginit = g->initial_state;
+    const int64_t grid = ceil_div(p.tasks * p.blocks, kWavesPerBlock), main_grid = ceil_div(p.workers * p.blocks, kWavesPerBlock);
+    NFA_REQUIRE(grid < (1ll << 31) && a->n_rays * (int64_t)(p.chunk ? 1 : 0) < 65536, "selective_scan_bwd: too large for one launch");
+    if (a->packed_info) launch_zero_rows(d, a->dtype, d.gu, d.gdt, d.gz, s);
+    with_shape<kBwdStates>(a->dtype, p.sh, [&](auto t, auto ns, auto pp) {
+        using T = decltype(t);
+        if (p.chunk) {
+            hipLaunchKernelGGL((scan_bwd_local_kernel<T, ns(), pp()>), dim3((unsigned)grid), dim3(kBlock), 0, s, d);
+            launch_chain<true>(d, s);
+        }
+        hipLaunchKernelGGL((scan_bwd_kernel<T, ns(), pp()>), dim3((unsigned)main_grid), dim3(kBlock), 0, s, d);
+        hipLaunchKernelGGL((scan_join_bc_kernel<T>), dim3(blocks_for(a->rows * 2 * a->states)), dim3(kBlock), 0, s, d, (int)(ns() * pp()), (T *)g->B, (T *)g->C);
+    });
+    const int64_t per = (int64_t)a->channels * (a->states + 2), n = (int64_t)a->channels * a->states;
+    launch_reduce_rows(d.part_w, p.workers, n, per, g->A, NFA_DTYPE_F32, s);
+    if (g->D) launch_reduce_rows(d.part_w + n, p.workers, a->channels, per, g->D, NFA_DTYPE_F32, s);
+    if (g->delta_bias) launch_reduce_rows(d.part_w + n + a->channels, p.workers, a->channels, per, g->delta_bias, NFA_DTYPE_F32, s);
+    return check_launch("scan_bwd_kernel");
+}
+
+NFA_EXPORT int nfa_selective_scan_step(const nfa_selective_scan_args *a, const float *state, void *outputs, float *out_state, void *stream) {
+    if (int rc = check_scan(a, "selective_scan_step", true)) return rc;
+    if (a->n_rays == 0) return NFA_OK;
+    NFA_REQUIRE(state && outputs && out_state, "selective_scan_step: NULL pointer");
+    ScanArgs d = scan_args(a);
+    d.y = outputs;
+    with_dtype(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((scan_step_kernel<T>), dim3(blocks_for(a->n_rays * a->channels)), dim3(kBlock), 0, (hipStream_t)stream, d, state, out_state);
+    });
+    return check_launch("scan_step_kernel");
+}

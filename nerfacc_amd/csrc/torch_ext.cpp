@@ -1505,6 +1505,204 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_bwd(const Tensor &g_, const T
     return {some(gx), some(gw), some(gb)};
 }
 
+std::tuple<Tensor, Tensor> row_map(const Tensor &info, int64_t rows) {
+    check_input(info, "packed_info", at::kLong);
+    TORCH_CHECK(info.dim() == 2 && info.size(1) == 2 && rows >= 0, "packed_info must be [n_rays, 2]");
+    Guard g(device_of(info));
+    Tensor ray = at::empty({rows}, opts(info, at::kInt)), pos = at::empty({rows}, opts(info, at::kInt));
+    check_rc(nfa_row_map(ptr<int64_t>(info), info.size(0), rows, ptr<int32_t>(ray), ptr<int32_t>(pos), stream_of(info)));
+    return {ray, pos};
+}
+
+// the sequences of a call: packed (info and its row map) or equal ones
+struct Sequences {
+    OptTensor info, ray, pos;
+    int64_t n_rays;
+    Sequences(const OptTensor &info_, const OptTensor &ray_, const OptTensor &pos_, int64_t n, int64_t rows, const Tensor &like) : n_rays(n) {
+        info = dense_of(info_, "packed_info", at::kLong, 2 * n, like);
+        TORCH_CHECK(n >= 0 && (info || (n > 0 && rows % n == 0)), "nerfacc_amd: rows do not divide into equal sequences");
+        if (!info) return;
+        ray = dense_of(ray_, "row_ray", at::kInt, rows, like);
+        pos = dense_of(pos_, "row_pos", at::kInt, rows, like);
+        TORCH_CHECK(ray && pos, "nerfacc_amd: packed sequences need their row map");
+    }
+    template <class A> void into(A &a) const {
+        a.n_rays = n_rays;
+        a.packed_info = ptr<int64_t>(info);
+        a.row_ray = ptr<int32_t>(ray);
+        a.row_pos = ptr<int32_t>(pos);
+    }
+};
+
+std::tuple<Tensor, OptTensor> causal_conv_fwd(const Tensor &x_, const Tensor &w_, const OptTensor &b_, const OptTensor &init_, const OptTensor &info,
+                                              const OptTensor &ray, const OptTensor &pos, int64_t n_rays, int64_t act, bool want_final) {
+    TORCH_CHECK(x_.dim() == 2 && w_.dim() == 2, "causal_conv: 2-D inputs and weight expected");
+    const int64_t n = x_.size(0), d = x_.size(1), width = w_.size(1);
+    const auto dt = x_.scalar_type();
+    const Tensor x = as_rows(x_, "inputs", n, d, x_), w = dense_of(w_, "weight", dt, d * width, x_);
+    const OptTensor b = dense_of(b_, "bias", dt, d, x_), init = dense_of(init_, "initial_state", dt, n_rays * (width - 1) * d, x_);
+    const Sequences seq(info, ray, pos, n_rays, n, x_);
+    Guard g(device_of(x_));
+    Tensor out = at::empty({n, d}, x_.options()), last;
+    if (want_final) last = at::empty({n_rays, width - 1, d}, x_.options());
+    if (n_rays == 0) return {out.zero_(), some(last)};
+    nfa_causal_conv_args a{};
+    seq.into(a);
+    a.rows = n; a.channels = (int32_t)d; a.width = (int32_t)width; a.dtype = dtype_of(x); a.activation = (int32_t)act;
+    a.inputs = x.data_ptr(); a.inputs_stride = row_stride(x);
+    a.weight = w.data_ptr(); a.bias = ptr<void>(b); a.initial_state = ptr<void>(init);
+    check_rc(nfa_causal_conv_fwd(&a, out.data_ptr(), ptr<void>(last), stream_of(x)));
+    return {out, some(last)};
+}
+
+std::tuple<OptTensor, OptTensor, OptTensor, OptTensor> causal_conv_bwd(
+    const Tensor &g_, const OptTensor &gfinal_, const Tensor &x_, const Tensor &w_, const OptTensor &b_, const OptTensor &init_, const OptTensor &info,
+    const OptTensor &ray, const OptTensor &pos, int64_t n_rays, int64_t act, bool need_x, bool need_w, bool need_b, bool need_init) {
+    TORCH_CHECK(x_.dim() == 2 && w_.dim() == 2, "causal_conv: 2-D inputs and weight expected");
+    const int64_t n = x_.size(0), d = x_.size(1), width = w_.size(1), ns = n_rays * (width - 1) * d;
+    const auto dt = x_.scalar_type();
+    const Tensor x = as_rows(x_, "inputs", n, d, x_), w = dense_of(w_, "weight", dt, d * width, x_), gy = as_rows(g_, "grad_outputs", n, d, x_);
+    const OptTensor b = dense_of(b_, "bias", dt, d, x_), init = dense_of(init_, "initial_state", dt, ns, x_),
+                    gfinal = dense_of(gfinal_, "grad_final_state", dt, ns, x_);
+    const Sequences seq(info, ray, pos, n_rays, n, x_);
+    Guard g(device_of(x_));
+    Tensor gx, gw, gb, gi, ws;
+    const bool none = n == 0 || n_rays == 0;
+    auto make = [&](at::IntArrayRef shape) { return none ? at::zeros(shape, x_.options()) : at::empty(shape, x_.options()); };
+    if (need_x) gx = make({n, d});
+    if (need_w) gw = make({d, width});
+    if (need_b) gb = make({d});
+    if (need_init) gi = make({n_rays, width - 1, d});
+    if (n_rays == 0) return {some(gx), some(gw), some(gb), some(gi)};
+    nfa_causal_conv_args a{};
+    seq.into(a);
+    a.rows = n; a.channels = (int32_t)d; a.width = (int32_t)width; a.dtype = dtype_of(x); a.activation = (int32_t)act;
+    a.inputs = x.data_ptr(); a.inputs_stride = row_stride(x);
+    a.weight = w.data_ptr(); a.bias = ptr<void>(b); a.initial_state = ptr<void>(init);
+    a.grad_outputs = gy.data_ptr(); a.grad_outputs_stride = row_stride(gy); a.grad_final_state = ptr<void>(gfinal);
+    if (need_w || need_b) ws = at::empty({nfa_causal_conv_bwd_workspace_bytes(n, a.channels, a.width, a.dtype)}, opts(x, at::kByte));
+    check_rc(nfa_causal_conv_bwd(&a, ptr<void>(gx), ptr<void>(gw), ptr<void>(gb), ptr<void>(gi), ptr<void>(ws), stream_of(x)));
+    return {some(gx), some(gw), some(gb), some(gi)};
+}
+
+Tensor causal_conv_step(const Tensor &x_, const Tensor &state_, const Tensor &w_, const OptTensor &b_, int64_t act, const Tensor &to) {
+    TORCH_CHECK(x_.dim() == 2 && w_.dim() == 2, "causal_conv_step: 2-D inputs and weight expected");
+    const int64_t r = x_.size(0), d = x_.size(1), width = w_.size(1), ns = r * (width - 1) * d;
+    const auto dt = x_.scalar_type();
+    const Tensor x = as_rows(x_, "inputs", r, d, x_), w = dense_of(w_, "weight", dt, d * width, x_), state = dense_of(state_, "state", dt, ns, x_);
+    const OptTensor b = dense_of(b_, "bias", dt, d, x_);
+    check_len(to, "out_state", dt, ns, x_);
+    Guard g(device_of(x_));
+    Tensor out = at::empty({r, d}, x_.options());
+    nfa_causal_conv_args a{};
+    a.n_rays = r; a.rows = r; a.channels = (int32_t)d; a.width = (int32_t)width; a.dtype = dtype_of(x); a.activation = (int32_t)act;
+    a.inputs = x.data_ptr(); a.inputs_stride = row_stride(x);
+    a.weight = w.data_ptr(); a.bias = ptr<void>(b);
+    check_rc(nfa_causal_conv_step(&a, state.data_ptr(), out.data_ptr(), to.data_ptr(), stream_of(x)));
+    return out;
+}
+
+// the tensors of a scan, checked and with contiguous rows
+struct ScanInputs {
+    int64_t n, d, s;
+    Tensor u, dt, z, B, C, A;
+    OptTensor D, bias, init;
+    ScanInputs(const Tensor &u_, const Tensor &dt_, const OptTensor &z_, const Tensor &B_, const Tensor &C_, const Tensor &A_, const OptTensor &D_,
+               const OptTensor &bias_, const OptTensor &init_, int64_t n_rays) {
+        TORCH_CHECK(u_.dim() == 2 && A_.dim() == 2, "selective_scan: 2-D inputs and A expected");
+        n = u_.size(0); d = u_.size(1); s = A_.size(1);
+        u = as_rows(u_, "inputs", n, d, u_);
+        dt = as_rows(dt_, "delta", n, d, u_);
+        if (z_ && z_->defined()) z = as_rows(*z_, "gate", n, d, u_);
+        B = as_rows(B_, "B", n, s, u_);
+        C = as_rows(C_, "C", n, s, u_);
+        A = dense_of(A_, "A", at::kFloat, d * s, u_);
+        D = dense_of(D_, "D", at::kFloat, d, u_);
+        bias = dense_of(bias_, "delta_bias", at::kFloat, d, u_);
+        init = dense_of(init_, "initial_state", at::kFloat, n_rays * d * s, u_);
+    }
+    nfa_selective_scan_args args(bool softplus) const {
+        nfa_selective_scan_args a{};
+        a.rows = n; a.channels = (int32_t)d; a.states = (int32_t)s; a.dtype = dtype_of(u); a.delta_softplus = softplus;
+        a.inputs = u.data_ptr(); a.inputs_stride = row_stride(u);
+        a.delta = dt.data_ptr(); a.delta_stride = row_stride(dt);
+        if (z.defined()) { a.gate = z.data_ptr(); a.gate_stride = row_stride(z); }
+        a.B = B.data_ptr(); a.B_stride = row_stride(B);
+        a.C = C.data_ptr(); a.C_stride = row_stride(C);
+        a.A = ptr<float>(A); a.D = ptr<float>(D); a.delta_bias = ptr<float>(bias); a.initial_state = ptr<float>(init);
+        return a;
+    }
+};
+
+std::tuple<Tensor, OptTensor, OptTensor> selective_scan_fwd(
+    const Tensor &u, const Tensor &dt, const OptTensor &z, const Tensor &B, const Tensor &C, const Tensor &A, const OptTensor &D, const OptTensor &bias,
+    const OptTensor &init, const OptTensor &info, const OptTensor &ray, const OptTensor &pos, int64_t n_rays, bool softplus, bool want_final, bool keep) {
+    const ScanInputs in(u, dt, z, B, C, A, D, bias, init, n_rays);
+    const Sequences seq(info, ray, pos, n_rays, in.n, u);
+    Guard g(device_of(u));
+    Tensor out = at::empty({in.n, in.d}, u.options()), last, kept, ws;
+    if (want_final) last = at::empty({n_rays, in.d, in.s}, opts(u, at::kFloat));
+    if (n_rays == 0) out.zero_();
+    if (keep) kept = at::empty({nfa_selective_scan_checkpoint_bytes(in.n, (int32_t)in.d, (int32_t)in.s)}, opts(u, at::kByte));
+    const int64_t bytes = nfa_selective_scan_workspace_bytes(n_rays, in.n, (int32_t)in.d, (int32_t)in.s, 0);
+    if (bytes > 0) ws = at::empty({bytes}, opts(u, at::kByte));
+    if (n_rays == 0) return {out, some(last), some(kept)};
+    auto a = in.args(softplus);
+    seq.into(a);
+    check_rc(nfa_selective_scan_fwd(&a, out.data_ptr(), ptr<float>(last), ptr<float>(kept), ptr<void>(ws), stream_of(u)));
+    return {out, some(last), some(kept)};
+}
+
+// (inputs, delta, gate, B, C, A, D, delta_bias, initial_state)
+std::vector<OptTensor> selective_scan_bwd(
+    const Tensor &g_, const OptTensor &gfinal_, const Tensor &u, const Tensor &dt, const OptTensor &z, const Tensor &B, const Tensor &C, const Tensor &A,
+    const OptTensor &D, const OptTensor &bias, const OptTensor &init, const Tensor &kept, const OptTensor &info, const OptTensor &ray, const OptTensor &pos,
+    int64_t n_rays, bool softplus) {
+    const ScanInputs in(u, dt, z, B, C, A, D, bias, init, n_rays);
+    const Sequences seq(info, ray, pos, n_rays, in.n, u);
+    const Tensor gy = as_rows(g_, "grad_outputs", in.n, in.d, u);
+    const OptTensor gfinal = dense_of(gfinal_, "grad_final_state", at::kFloat, n_rays * in.d * in.s, u);
+    check_len(kept, "checkpoints", at::kByte, nfa_selective_scan_checkpoint_bytes(in.n, (int32_t)in.d, (int32_t)in.s), u);
+    Guard g(device_of(u));
+    const auto f32 = opts(u, at::kFloat);
+    const bool none = in.n == 0 || n_rays == 0;
+    auto make = [&](at::IntArrayRef shape, at::TensorOptions o) { return none ? at::zeros(shape, o) : at::empty(shape, o); };
+    Tensor gu = make({in.n, in.d}, u.options()), gdt = make({in.n, in.d}, u.options()), gz, gB = make({in.n, in.s}, u.options()),
+           gC = make({in.n, in.s}, u.options()), gA = make({in.d, in.s}, f32), gD, gbias, ginit;
+    if (in.z.defined()) gz = make({in.n, in.d}, u.options());
+    if (in.D) gD = make({in.d}, f32);
+    if (in.bias) gbias = make({in.d}, f32);
+    if (in.init) {
+        ginit = make({n_rays, in.d, in.s}, f32);
+        if (none && gfinal) ginit.copy_(gfinal->view({n_rays, in.d, in.s}));
+    }
+    if (!none) {
+        auto a = in.args(softplus);
+        seq.into(a);
+        a.grad_outputs = gy.data_ptr(); a.grad_outputs_stride = row_stride(gy); a.grad_final_state = ptr<float>(gfinal);
+        Tensor ws = at::empty({nfa_selective_scan_workspace_bytes(n_rays, in.n, a.channels, a.states, 1)}, opts(u, at::kByte));
+        nfa_selective_scan_grads gr{};
+        gr.inputs = gu.data_ptr(); gr.delta = gdt.data_ptr(); gr.gate = ptr<void>(gz); gr.B = gB.data_ptr(); gr.C = gC.data_ptr();
+        gr.A = ptr<float>(gA); gr.D = ptr<float>(gD); gr.delta_bias = ptr<float>(gbias); gr.initial_state = ptr<float>(ginit);
+        check_rc(nfa_selective_scan_bwd(&a, ptr<float>(kept), &gr, ws.data_ptr(), stream_of(u)));
+    }
+    return {gu, gdt, some(gz), gB, gC, gA, some(gD), some(gbias), some(ginit)};
+}
+
+Tensor selective_scan_step(const Tensor &u, const Tensor &dt, const OptTensor &z, const Tensor &B, const Tensor &C, const Tensor &A, const OptTensor &D,
+                           const OptTensor &bias, const Tensor &state_, bool softplus, const Tensor &to) {
+    const ScanInputs in(u, dt, z, B, C, A, D, bias, std::nullopt, u.dim() ? u.size(0) : 0);
+    const int64_t ns = in.n * in.d * in.s;
+    const Tensor state = dense_of(state_, "state", at::kFloat, ns, u);
+    check_len(to, "out_state", at::kFloat, ns, u);
+    Guard g(device_of(u));
+    Tensor out = at::empty({in.n, in.d}, u.options());
+    auto a = in.args(softplus);
+    a.n_rays = in.n;
+    check_rc(nfa_selective_scan_step(&a, ptr<float>(state), out.data_ptr(), ptr<float>(to), stream_of(u)));
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1595,4 +1793,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("foreign_nodes", &foreign_nodes);
     m.def("linear_fwd", &linear_fwd);
     m.def("linear_bwd", &linear_bwd);
+    m.def("row_map", &row_map);
+    m.def("causal_conv_fwd", &causal_conv_fwd);
+    m.def("causal_conv_bwd", &causal_conv_bwd);
+    m.def("causal_conv_step", &causal_conv_step);
+    m.def("selective_scan_fwd", &selective_scan_fwd);
+    m.def("selective_scan_bwd", &selective_scan_bwd);
+    m.def("selective_scan_step", &selective_scan_step);
 }

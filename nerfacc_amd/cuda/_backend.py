@@ -1158,6 +1158,131 @@ class _CtypesC:
                 _check(L.nfa_linear_bwd(ctypes.byref(a), _ptr(saved), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), _stream(x)))
         return gx, gw, gb
 
+    @staticmethod
+    def row_map(info, rows: int):
+        """(the ray of every row, its position there; -1: none): nfa_row_map"""
+        _check_input(info, "packed_info", torch.int64)
+        with _Guard(info):
+            ray, pos = (torch.empty(rows, dtype=torch.int32, device=info.device) for _ in range(2))
+            _check(load_library().nfa_row_map(_ptr(info), info.shape[0], rows, _ptr(ray), _ptr(pos), _stream(info)))
+        return ray, pos
+
+    @staticmethod
+    def _conv_args(x, w, b, init, info, ray, pos, n_rays, act, **more):
+        return _STRUCTS["nfa_causal_conv_args"](
+            n_rays=n_rays, rows=x.shape[0], channels=x.shape[1], width=w.shape[1], dtype=_dtype_id(x), activation=act, inputs=_ptr(x),
+            inputs_stride=_row_stride(x), weight=_ptr(w), bias=_ptr(b), initial_state=_ptr(init), packed_info=_ptr(info), row_ray=_ptr(ray),
+            row_pos=_ptr(pos), **more)
+
+    @staticmethod
+    def causal_conv_fwd(x, w, b, init, info, ray, pos, n_rays: int, act: int, want_final: bool):
+        """(outputs, final_state or None): nfa_causal_conv_fwd"""
+        x, w, b, init = _as_rows(x), _dense(w), _dense(b), _dense(init)
+        with _Guard(x):
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            last = torch.empty((n_rays, w.shape[1] - 1, x.shape[1]), dtype=x.dtype, device=x.device) if want_final else None
+            if n_rays == 0:
+                return out.zero_(), last
+            a = _CtypesC._conv_args(x, w, b, init, info, ray, pos, n_rays, act)
+            _check(load_library().nfa_causal_conv_fwd(ctypes.byref(a), _ptr(out), _ptr(last), _stream(x)))
+        return out, last
+
+    @staticmethod
+    def causal_conv_bwd(g, gfinal, x, w, b, init, info, ray, pos, n_rays: int, act: int, need_x: bool, need_w: bool, need_b: bool,
+                        need_init: bool):
+        """(grad_inputs, grad_weight, grad_bias, grad_initial_state), None where not asked for: nfa_causal_conv_bwd"""
+        g, gfinal, x, w, b, init = _as_rows(g), _dense(gfinal), _as_rows(x), _dense(w), _dense(b), _dense(init)
+        (n, d), width = x.shape, w.shape[1]
+        new = torch.empty if n and n_rays else torch.zeros
+        with _Guard(x):
+            kw = {"dtype": x.dtype, "device": x.device}
+            gx = new((n, d), **kw) if need_x else None
+            gw = new((d, width), **kw) if need_w else None
+            gb = new((d,), **kw) if need_b else None
+            gi = new((n_rays, width - 1, d), **kw) if need_init else None
+            if n_rays == 0:
+                return gx, gw, gb, gi
+            L = load_library()
+            ws = torch.empty(L.nfa_causal_conv_bwd_workspace_bytes(n, d, width, _dtype_id(x)), dtype=torch.uint8, device=x.device)
+            a = _CtypesC._conv_args(x, w, b, init, info, ray, pos, n_rays, act, grad_outputs=_ptr(g), grad_outputs_stride=_row_stride(g),
+                                    grad_final_state=_ptr(gfinal))
+            _check(L.nfa_causal_conv_bwd(ctypes.byref(a), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(gi), _ptr(ws), _stream(x)))
+        return gx, gw, gb, gi
+
+    @staticmethod
+    def causal_conv_step(x, state, w, b, act: int, to):
+        """outputs; the new state goes to `to`: nfa_causal_conv_step"""
+        x, state, w, b = _as_rows(x), _dense(state), _dense(w), _dense(b)
+        with _Guard(x):
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            a = _CtypesC._conv_args(x, w, b, None, None, None, None, x.shape[0], act)
+            _check(load_library().nfa_causal_conv_step(ctypes.byref(a), _ptr(state), _ptr(out), _ptr(to), _stream(x)))
+        return out
+
+    @staticmethod
+    def _scan_args(u, dt, z, B, C, A, D, bias, init, info, ray, pos, n_rays, softplus, **more):
+        return _STRUCTS["nfa_selective_scan_args"](
+            n_rays=n_rays, rows=u.shape[0], channels=u.shape[1], states=A.shape[1], dtype=_dtype_id(u), delta_softplus=int(softplus),
+            inputs=_ptr(u), inputs_stride=_row_stride(u), delta=_ptr(dt), delta_stride=_row_stride(dt), gate=_ptr(z),
+            gate_stride=0 if z is None else _row_stride(z), B=_ptr(B), B_stride=_row_stride(B), C=_ptr(C), C_stride=_row_stride(C), A=_ptr(A),
+            D=_ptr(D), delta_bias=_ptr(bias), initial_state=_ptr(init), packed_info=_ptr(info), row_ray=_ptr(ray), row_pos=_ptr(pos), **more)
+
+    @staticmethod
+    def selective_scan_fwd(u, dt, z, B, C, A, D, bias, init, info, ray, pos, n_rays: int, softplus: bool, want_final: bool, keep: bool):
+        """(outputs, final_state or None, checkpoints or None): nfa_selective_scan_fwd"""
+        u, dt, z, B, C = (_as_rows(t) for t in (u, dt, z, B, C))
+        A, D, bias, init = (_dense(t) for t in (A, D, bias, init))
+        (n, d), s = u.shape, A.shape[1]
+        L = load_library()
+        with _Guard(u):
+            kw = {"device": u.device}
+            out = torch.empty((n, d), dtype=u.dtype, **kw)
+            last = torch.empty((n_rays, d, s), dtype=torch.float32, **kw) if want_final else None
+            kept = torch.empty(L.nfa_selective_scan_checkpoint_bytes(n, d, s), dtype=torch.uint8, **kw) if keep else None
+            if n_rays == 0:
+                return out.zero_(), last, kept
+            bytes_ = L.nfa_selective_scan_workspace_bytes(n_rays, n, d, s, 0)
+            ws = torch.empty(bytes_, dtype=torch.uint8, **kw) if bytes_ else None
+            a = _CtypesC._scan_args(u, dt, z, B, C, A, D, bias, init, info, ray, pos, n_rays, softplus)
+            _check(L.nfa_selective_scan_fwd(ctypes.byref(a), _ptr(out), _ptr(last), _ptr(kept), _ptr(ws), _stream(u)))
+        return out, last, kept
+
+    @staticmethod
+    def selective_scan_bwd(g, gfinal, u, dt, z, B, C, A, D, bias, init, kept, info, ray, pos, n_rays: int, softplus: bool):
+        """gradients of (inputs, delta, gate, B, C, A, D, delta_bias, initial_state): nfa_selective_scan_bwd"""
+        g, u, dt, z, B, C = (_as_rows(t) for t in (g, u, dt, z, B, C))
+        gfinal, A, D, bias, init = (_dense(t) for t in (gfinal, A, D, bias, init))
+        (n, d), s, none = u.shape, A.shape[1], u.shape[0] == 0 or n_rays == 0
+        new = torch.zeros if none else torch.empty
+        L = load_library()
+        with _Guard(u):
+            kw, f32 = {"dtype": u.dtype, "device": u.device}, {"dtype": torch.float32, "device": u.device}
+            gu, gdt, gz = new((n, d), **kw), new((n, d), **kw), None if z is None else new((n, d), **kw)
+            gB, gC, gA = new((n, s), **kw), new((n, s), **kw), new((d, s), **f32)
+            gD, gbias = (None if t is None else new((d,), **f32) for t in (D, bias))
+            ginit = None if init is None else new((n_rays, d, s), **f32)
+            if none and ginit is not None and gfinal is not None:
+                ginit.copy_(gfinal)
+            if not none:
+                ws = torch.empty(L.nfa_selective_scan_workspace_bytes(n_rays, n, d, s, 1), dtype=torch.uint8, device=u.device)
+                a = _CtypesC._scan_args(u, dt, z, B, C, A, D, bias, init, info, ray, pos, n_rays, softplus, grad_outputs=_ptr(g),
+                                        grad_outputs_stride=_row_stride(g), grad_final_state=_ptr(gfinal))
+                gr = _STRUCTS["nfa_selective_scan_grads"](inputs=_ptr(gu), delta=_ptr(gdt), gate=_ptr(gz), B=_ptr(gB), C=_ptr(gC), A=_ptr(gA),
+                                                          D=_ptr(gD), delta_bias=_ptr(gbias), initial_state=_ptr(ginit))
+                _check(L.nfa_selective_scan_bwd(ctypes.byref(a), _ptr(kept), ctypes.byref(gr), _ptr(ws), _stream(u)))
+        return gu, gdt, gz, gB, gC, gA, gD, gbias, ginit
+
+    @staticmethod
+    def selective_scan_step(u, dt, z, B, C, A, D, bias, state, softplus: bool, to):
+        """outputs; the new state goes to `to`: nfa_selective_scan_step"""
+        u, dt, z, B, C = (_as_rows(t) for t in (u, dt, z, B, C))
+        A, D, bias, state = (_dense(t) for t in (A, D, bias, state))
+        with _Guard(u):
+            out = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+            a = _CtypesC._scan_args(u, dt, z, B, C, A, D, bias, None, None, None, None, u.shape[0], softplus)
+            _check(load_library().nfa_selective_scan_step(ctypes.byref(a), _ptr(state), _ptr(out), _ptr(to), _stream(u)))
+        return out
+
 
 def _select_backend():
     """The torch C++ extension (nerfacc_amd/_hip*.so, csrc/torch_ext.cpp) is THE boundary, as the reference's pybind
