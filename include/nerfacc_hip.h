@@ -467,7 +467,7 @@ int nfa_pdf_loss_bwd(const float *g_loss, const int32_t *ids_left, const int32_t
  * nfa_linear_fwd  inputs [rows, in_features], weight [out_features, in_features] and bias [out_features] (nullable), residual
  *                 [rows, out_features] (nullable) -> outputs [rows, out_features] contiguous.  saved (nullable unless a backward
  *                 pass follows): what nfa_linear_bwd differentiates the activation from, nfa_linear_saved_bytes(...) bytes; 0
- *                 bytes = it needs none, or (relu, exp, softplus without a residual) the outputs themselves.
+ *                 bytes = it needs none, or (exp, softplus and some sizes of relu, without a residual) the outputs themselves.
  * nfa_linear_bwd  grad_outputs [rows, out_features] -> grad_inputs [rows, in_features] contiguous, grad_weight, grad_bias (each
  *                 nullable); the residual's gradient is grad_outputs.  saved = the forward call's saved array, or its outputs where
  *                 nfa_linear_saved_bytes says 0 and the activation is not NONE.  workspace: nfa_linear_bwd_workspace_bytes(...). */
@@ -487,7 +487,7 @@ typedef struct nfa_linear_args {
 
 int64_t nfa_linear_saved_bytes(int64_t rows, int32_t out_features, int32_t dtype, int32_t activation, int32_t has_residual);
 int nfa_linear_fwd(const nfa_linear_args *args, void *outputs, void *saved, void *stream);
-int64_t nfa_linear_bwd_workspace_bytes(int64_t rows, int32_t in_features, int32_t out_features, int32_t dtype);
+int64_t nfa_linear_bwd_workspace_bytes(int64_t rows, int32_t in_features, int32_t out_features, int32_t dtype, int32_t activation);
 int nfa_linear_bwd(const nfa_linear_args *args, const void *saved, void *grad_inputs, void *grad_weight, void *grad_bias,
                    void *workspace, void *stream);
 

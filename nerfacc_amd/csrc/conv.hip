@@ -209,7 +209,7 @@ __global__ __launch_bounds__(kBlock) void conv_bwd_kernel(ConvArgs a) {
                         float z = b[i];
 #pragma unroll
                         for (int j = 0; j < W; ++j) z = fmaf(w[j][i], win[j][i], z);
-                        g *= act_slope(NFA_ACT_SILU, z);
+                        g *= act_slope<NFA_ACT_SILU>(z);
                     }
                     acc[0][i] = 0.0f;
                     if (in) {
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(kBlock) void conv_init_grad_kernel(ConvArgs a, T *g
             g[p] = 0.0f;
             if (p < count) {
                 g[p] = to_f(reinterpret_cast<const T *>(a.gy)[(start + p) * a.ld_gy + c]);
-                if (a.act == NFA_ACT_SILU) g[p] *= act_slope(NFA_ACT_SILU, z);
+                if (a.act == NFA_ACT_SILU) g[p] *= act_slope<NFA_ACT_SILU>(z);
             }
         }
 #pragma unroll

@@ -9,9 +9,10 @@
 //   wgrad     p = n, q = k, c = m    P = dz, Q = x        both transposed; c is split over workgroups, partial sums joined in order
 // dz is formed from dy and the saved number while a tile is staged: it never goes to memory.
 //
-// A field's layers are narrow (8 .. 256 features) and their batches long (2^18 samples): reading x and writing y bounds them, so a
-// workgroup takes 128 rows of samples and the whole width where it can, x goes through the chip once, and everything elementwise
-// rides on the tile in registers.
+// A field's layers are narrow (8 .. 256 features) and their batches long (2^18 samples): reading x and writing y bounds them.  For
+// a contraction of up to 256 the forward pass and dgrad keep the weight in LDS for the life of a workgroup and every wave takes rows
+// straight from memory into the registers that feed the matrix units: no barrier after the first, x read once, everything elementwise
+// in registers (resident_kernel).  Longer contractions and wgrad go tile by tile through LDS (tile_kernel).
 #include "feature.hpp"
 
 namespace nfa {
@@ -34,9 +35,9 @@ struct DenseArgs {
     float *partial;                             // wgrad: [splits][P * Q + P]
     int64_t n_p, n_c;                           // rows of the output; length of the contraction
     int32_t n_q;
-    int64_t ld_p, ld_q, ld_saved, ld_residual;  // in elements
+    int64_t ld_p, ld_q, ld_saved, ld_residual;  // in elements (ld_saved of bits: in bytes)
     int64_t split;                              // wgrad: contraction steps of one workgroup
-    int32_t act, vec_p, vec_q, vec_out, want_bias, tiles_q, tiles;
+    int32_t act, mask, vec_p, vec_q, vec_out, want_bias, tiles_q, tiles, block_q, splits;
 };
 
 enum { kForward, kDgrad, kWgrad };
@@ -55,7 +56,291 @@ __device__ __forceinline__ u32x4 load_chunk(const T *row, int64_t col, int64_t c
     }
     return v;
 }
+// what dz is formed from beside dy: a chunk of saved numbers, or a byte of relu's bits
+template <class T>
+__device__ __forceinline__ u32x4 load_saved(const DenseArgs &a, int64_t row, int64_t col, int64_t cols, bool inside) {
+    u32x4 v = {0, 0, 0, 0};
+    if (a.mask) {
+        if (inside && col < cols) v[0] = reinterpret_cast<const uint8_t *>(a.saved)[row * a.ld_saved + col / kChunk<T>];
+    } else if (a.act != NFA_ACT_NONE) {
+        v = load_chunk<T>(reinterpret_cast<const T *>(a.saved) + row * a.ld_saved, col, cols, inside, a.vec_p);
+    }
+    return v;
+}
 
+template <class T> struct Frag { T v[kChunk<T>]; };
+
+// dz = dy act'(.) of N chunks, rounded to T.  SPLIT (16-bit types, smooth activations): what the rounding lost goes into `rest`, and
+// the product is taken of both parts, so that a gradient carries the rounding of its own result and of the saved number only.  relu's
+// dz is dy or 0: nothing is lost there.  each(chunk, dz of one number in 32 bits, place in the chunk)
+template <class T, bool SPLIT, int N, class F>
+__device__ __forceinline__ void form_dz(const DenseArgs &a, u32x4 (&g)[N], const u32x4 (&s)[N], u32x4 (&rest)[SPLIT ? N : 1], F &&each) {
+    auto with = [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            Frag<T> v = __builtin_bit_cast(Frag<T>, g[k]), lo;
+            const Frag<T> w = __builtin_bit_cast(Frag<T>, s[k]);
+#pragma unroll
+            for (int i = 0; i < kChunk<T>; ++i) {
+                float dz = to_f(v.v[i]);
+                if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((s[k][0] >> i) & 1u) != 0 : to_f(w.v[i]) > 0.0f) ? dz : 0.0f;
+                else if constexpr (ACT != NFA_ACT_NONE) dz *= act_slope<ACT>(to_f(w.v[i]));
+                each(k, dz, i);
+                if constexpr (ACT != NFA_ACT_NONE) v.v[i] = from_f<T>(dz);
+                if constexpr (SPLIT) lo.v[i] = from_f<T>(dz - to_f(v.v[i]));
+            }
+            if constexpr (ACT != NFA_ACT_NONE) g[k] = __builtin_bit_cast(u32x4, v);
+            if constexpr (SPLIT) rest[k] = __builtin_bit_cast(u32x4, lo);
+        }
+    };
+    if constexpr (sizeof(T) == 4) {
+        with_act(a.act, with);
+    } else if constexpr (SPLIT) {
+        switch (a.act) {
+            case NFA_ACT_SIGMOID: with(std::integral_constant<int, NFA_ACT_SIGMOID>{}); break;
+            case NFA_ACT_SOFTPLUS: with(std::integral_constant<int, NFA_ACT_SOFTPLUS>{}); break;
+            case NFA_ACT_SILU: with(std::integral_constant<int, NFA_ACT_SILU>{}); break;
+            case NFA_ACT_GELU: with(std::integral_constant<int, NFA_ACT_GELU>{}); break;
+            default: with(std::integral_constant<int, NFA_ACT_EXP>{}); break;
+        }
+    } else {
+        if (a.act == NFA_ACT_RELU) with(std::integral_constant<int, NFA_ACT_RELU>{});
+        else with(std::integral_constant<int, NFA_ACT_NONE>{});
+    }
+}
+template <class T> bool splits(int32_t act) { return sizeof(T) == 2 && act != NFA_ACT_NONE && act != NFA_ACT_RELU; }
+
+// acc[q][p] += Q P over the lane's chunk.  32-bit numbers go in four steps: the contraction may run in any order as long as both
+// sides agree, so lane group g feeds chunk g and each step takes one number of it.
+template <class T>
+__device__ __forceinline__ f32x4 multiply(u32x4 q, u32x4 p, f32x4 acc) {
+    if constexpr (std::is_same_v<T, bf16>) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, q), __builtin_bit_cast(bf16x8, p), acc, 0, 0, 0);
+    } else if constexpr (std::is_same_v<T, f16>) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, q), __builtin_bit_cast(f16x8, p), acc, 0, 0, 0);
+    } else {
+        const f32x4 a = __builtin_bit_cast(f32x4, q), b = __builtin_bit_cast(f32x4, p);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], acc, 0, 0, 0);
+        return acc;
+    }
+}
+// ds_read_b64_tr_b16: sixteen lanes read four rows of four times four columns, lane i gets the i-th column of the four rows
+__device__ __forceinline__ s16x4 read_transposed(const char *at) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
+}
+
+// y = act(z) (+ residual) of N chunks in place; `kept`: what the backward pass wants of them (bits: in the first word of a chunk)
+template <class T, int N>
+__device__ __forceinline__ void finish_chunks(const DenseArgs &a, float (&z)[N][kChunk<T>], const u32x4 (&res)[N], u32x4 (&y)[N], u32x4 (&kept)[N]) {
+    with_act(a.act, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+        constexpr bool VALUE = ACT == NFA_ACT_RELU || ACT == NFA_ACT_EXP || ACT == NFA_ACT_SOFTPLUS;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            Frag<T> out, keep;
+            const Frag<T> add = __builtin_bit_cast(Frag<T>, res[k]);
+            uint32_t bits = 0;
+#pragma unroll
+            for (int i = 0; i < kChunk<T>; ++i) {
+                const float v = act_fwd<ACT>(z[k][i]);
+                if constexpr (ACT == NFA_ACT_RELU) bits |= (v > 0.0f ? 1u : 0u) << i;
+                keep.v[i] = from_f<T>(VALUE ? v : z[k][i]);
+                out.v[i] = from_f<T>(a.residual ? v + to_f(add.v[i]) : v);
+            }
+            y[k] = __builtin_bit_cast(u32x4, out);
+            kept[k] = __builtin_bit_cast(u32x4, keep);
+            if (a.mask) kept[k][0] = bits;
+        }
+    });
+}
+// a chunk of a contiguous output row, as far as it lies inside
+template <class T>
+__device__ __forceinline__ void store_chunk(T *row, int q, int n_q, bool vec, u32x4 v) {
+    if (vec) {
+        if (q < n_q) *reinterpret_cast<u32x4 *>(row + q) = v;
+    } else {
+        const Frag<T> f = __builtin_bit_cast(Frag<T>, v);
+#pragma unroll
+        for (int i = 0; i < kChunk<T>; ++i)
+            if (q + i < n_q) row[q + i] = f.v[i];
+    }
+}
+// the epilogue of N chunks of row p (columns q[k] ..): acc in, outputs and the saved numbers out
+template <class T, int MODE, int N>
+__device__ __forceinline__ void epilogue(const DenseArgs &a, int64_t p, const int (&q)[N], float (&z)[N][kChunk<T>], const u32x4 (&res)[N]) {
+    u32x4 y[N], kept[N];
+    T *out = reinterpret_cast<T *>(a.out) + p * a.n_q;
+    if constexpr (MODE == kForward) {
+        finish_chunks<T, N>(a, z, res, y, kept);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            store_chunk<T>(out, q[k], a.n_q, a.vec_out, y[k]);
+            if (!a.saved_out) continue;
+            if (a.mask) {
+                if (q[k] < a.n_q) reinterpret_cast<uint8_t *>(a.saved_out)[p * a.ld_saved + q[k] / kChunk<T>] = (uint8_t)kept[k][0];
+            } else {
+                store_chunk<T>(reinterpret_cast<T *>(a.saved_out) + p * a.n_q, q[k], a.n_q, a.vec_out, kept[k]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            Frag<T> o;
+#pragma unroll
+            for (int i = 0; i < kChunk<T>; ++i) o.v[i] = from_f<T>(z[k][i]);
+            store_chunk<T>(out, q[k], a.n_q, a.vec_out, __builtin_bit_cast(u32x4, o));
+        }
+    }
+}
+
+// Columns of a group of 32 and the two fragments that compute them.  A lane of a fragment's result holds four neighbouring of its
+// sixteen columns; 16-bit types exchange columns between the two fragments so that a lane's eight are neighbours (one 16-byte store).
+// column of number r of lane group g in fragment j
+template <class T> __device__ __forceinline__ int column_of(int j, int g, int r) { return sizeof(T) == 2 ? g * 8 + j * 4 + r : j * 16 + g * 4 + r; }
+// place (16 j + row of the fragment) of column c
+template <class T> __device__ __forceinline__ int place_of_column(int c) {
+    return sizeof(T) == 2 ? ((c >> 2) & 1) * 16 + (c >> 3) * 4 + (c & 3) : c;
+}
+
+// ---- the weight stays in LDS -------------------------------------------------------------------------------------------
+// LDS: forward, rows of the weight in the order of place_of_column, 16 KS-byte-chunked along c; dgrad, rows along c as they are, read
+// transposed.  Chunks are exchanged inside a row so that the lanes of one read lie in different banks.
+constexpr int kResidentBytes = 144 * 1024;
+template <class T, int KS>
+__device__ __forceinline__ int weight_offset(int row, int chunk) {                   // forward
+    constexpr int CH = KS * 4, L = CH >= 16 ? 4 : (CH == 8 ? 3 : 2);
+    return (row * CH + (chunk ^ ((row >> (4 - L)) & ((1 << L) - 1)))) * 16;
+}
+template <class T>
+__device__ __forceinline__ int weight_offset_t(int row, int chunk, int pitch) {      // dgrad; pitch: chunks in a row, 4, 8 or a multiple of 16
+    if (sizeof(T) == 2) return (row * pitch + (chunk ^ (pitch >= 16 ? (row & 3) << 2 : pitch == 8 ? ((row >> 1) & 1) << 2 : 0))) * 16;
+    return (row * pitch + (chunk ^ (pitch >= 16 ? ((row >> 2) & 3) << 2 : pitch == 8 ? ((row >> 2) & 1) << 2 : 0))) * 16;
+}
+
+// waves on a CU: sixteen while a wave's rows leave room in the registers, eight beyond (its loads in flight are twice as many then)
+constexpr int resident_threads(int ks) { return ks <= 2 ? 1024 : 512; }
+template <class T, int MODE, int KS, bool SPLIT>
+__global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArgs a) {
+    constexpr int CE = kChunk<T>, RT = SPLIT || KS == 16 ? 1 : 2;       // rows of a wave: RT fragments of sixteen
+    constexpr int NC = sizeof(T) == 2 ? 1 : 2;                          // chunks of a lane in a group of 32 columns
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = lane_id(), i = lane & 15, g = lane >> 4;
+    const int q0 = blockIdx.y * a.block_q, nq = a.n_q - q0 < a.block_q ? a.n_q - q0 : a.block_q;
+    const int q_rows = (nq + 31) & ~31, pitch = a.block_q / CE;         // (dgrad: block_q is 32, 64 or a multiple of 128)
+    const T *Q = reinterpret_cast<const T *>(a.q), *P = reinterpret_cast<const T *>(a.p);
+    if (MODE == kForward) {
+        for (int e = threadIdx.x; e < q_rows * KS * 4; e += blockDim.x) {
+            const int q = e / (KS * 4), chunk = e % (KS * 4);
+            const u32x4 v = load_chunk<T>(Q + (int64_t)(q0 + q) * a.ld_q, chunk * CE, a.n_c, q < nq, a.vec_q);
+            *reinterpret_cast<u32x4 *>(lds + weight_offset<T, KS>((q & ~31) + place_of_column<T>(q & 31), chunk)) = v;
+        }
+    } else {
+        for (int e = threadIdx.x; e < KS * 4 * CE * pitch; e += blockDim.x) {
+            const int n = e / pitch, chunk = e - n * pitch;
+            const u32x4 v = load_chunk<T>(Q + (int64_t)n * a.ld_q + q0, chunk * CE, nq, n < a.n_c, a.vec_q);
+            *reinterpret_cast<u32x4 *>(lds + weight_offset_t<T>(n, chunk, pitch)) = v;
+        }
+    }
+    __syncthreads();
+
+    const T *bias = reinterpret_cast<const T *>(a.bias);
+    const int64_t waves = (int64_t)gridDim.x * (blockDim.x >> 6);
+    for (int64_t tile = (int64_t)blockIdx.x * (blockDim.x >> 6) + wave_in_block(); tile < a.tiles; tile += waves) {
+        const int64_t p0 = tile * (16 * RT);
+        u32x4 x[RT * KS], lo[SPLIT ? RT * KS : 1];
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const int64_t p = p0 + r * 16 + i;
+                x[r * KS + k] = load_chunk<T>(P + p * a.ld_p, (k * 4 + g) * CE, a.n_c, p < a.n_p, a.vec_p);
+            }
+        if constexpr (MODE == kDgrad) {
+            if (a.act != NFA_ACT_NONE) {
+                u32x4 s[RT * KS];
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        const int64_t p = p0 + r * 16 + i;
+                        s[r * KS + k] = load_saved<T>(a, p, (k * 4 + g) * CE, a.n_c, p < a.n_p);
+                    }
+                form_dz<T, SPLIT, RT * KS>(a, x, s, lo, [](int, float, int) {});
+            }
+        }
+        for (int q = 0; q < nq; q += 32) {
+            f32x4 acc[RT][2];
+            u32x4 res[RT][NC];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                acc[r][0] = acc[r][1] = f32x4{0, 0, 0, 0};
+                const int64_t p = p0 + r * 16 + i;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    res[r][c] = u32x4{0, 0, 0, 0};
+                    if (MODE == kForward && a.residual)
+                        res[r][c] = load_chunk<T>(reinterpret_cast<const T *>(a.residual) + p * a.ld_residual, q0 + q + column_of<T>(c, g, 0), a.n_q,
+                                                  p < a.n_p, a.vec_out);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                if (k * 4 * CE >= a.n_c) continue;
+                u32x4 w[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if constexpr (MODE == kForward) {
+                        w[j] = *reinterpret_cast<const u32x4 *>(lds + weight_offset<T, KS>(q + j * 16 + i, k * 4 + g));
+                    } else if constexpr (sizeof(T) == 2) {
+                        s16x4 h[2];
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            const int n = k * 32 + g * 8 + s * 4 + (i >> 2), c = q + (i & 3) * 8 + j * 4;
+                            h[s] = read_transposed(lds + weight_offset_t<T>(n, c >> 3, pitch) + (c & 7) * 2);
+                        }
+                        w[j] = __builtin_bit_cast(u32x4, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    } else {
+                        f32x4 e;
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            const int n = k * 16 + g * 4 + s, c = q + j * 16 + i;
+                            e[s] = *reinterpret_cast<const float *>(lds + weight_offset_t<T>(n, c >> 2, pitch) + (c & 3) * 4);
+                        }
+                        w[j] = __builtin_bit_cast(u32x4, e);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        acc[r][j] = multiply<T>(w[j], x[r * KS + k], acc[r][j]);
+                        if constexpr (SPLIT) acc[r][j] = multiply<T>(w[j], lo[r * KS + k], acc[r][j]);
+                    }
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const int64_t p = p0 + r * 16 + i;
+                float z[NC][CE];
+                int col[NC];
+#pragma unroll
+                for (int c = 0; c < NC; ++c) col[c] = q0 + q + column_of<T>(c, g, 0);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int c = q0 + q + column_of<T>(j, g, e);
+                        const float b = MODE == kForward && bias && c < a.n_q ? to_f(bias[c]) : 0.0f;
+                        z[NC == 1 ? 0 : j][NC == 1 ? j * 4 + e : e] = acc[r][j][e] + b;
+                    }
+                if (p < a.n_p) epilogue<T, MODE, NC>(a, p, col, z, res[r]);
+            }
+        }
+    }
+}
+
+// ---- tile by tile ------------------------------------------------------------------------------------------------------
 // LDS layouts.  c-contiguous tiles: 128-byte rows, the 16-byte chunks of row r exchanged by r & 7.  Transposed tiles (rows along c,
 // 64 or 128 columns): the 32-byte (16-bit types) or 64-byte units of a row exchanged so that the rows that one instruction reads
 // lie in different banks.
@@ -71,8 +356,6 @@ __device__ __forceinline__ int stage_offset(int row, int chunk) {        // byte
     if (sizeof(T) == 4) return row * ROWS * 4 + (((chunk >> 2) ^ unit_swizzle<T, ROWS>(row)) << 6) + ((chunk & 3) << 4);
     return row * ROWS * 2 + (((chunk >> 1) ^ unit_swizzle<T, ROWS>(row)) << 5) + ((chunk & 1) << 4);
 }
-
-template <class T> struct Frag { T v[kChunk<T>]; };
 
 // the sixteen bytes that lane l feeds to the matrix units for rows (or columns) c0 .. c0 + 15 and half `ks` of the tile
 template <class T, bool TR, int ROWS>
@@ -90,66 +373,49 @@ __device__ __forceinline__ u32x4 read_frag(const char *tile, int c0, int ks, int
         }
         __builtin_memcpy(&v, e, 16);
     } else {
-        // ds_read_b64_tr_b16: sixteen lanes read four rows of sixteen columns, lane i gets column i of the four
         s16x4 h[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int row = ks * 32 + g * 8 + s * 4 + (i >> 2);
-            const char *at = tile + row * ROWS * 2 + (((c0 >> 4) ^ unit_swizzle<T, ROWS>(row)) << 5) + ((i & 3) << 3);
-            h[s] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
+            h[s] = read_transposed(tile + row * ROWS * 2 + (((c0 >> 4) ^ unit_swizzle<T, ROWS>(row)) << 5) + ((i & 3) << 3));
         }
-        s16x8 w = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
-        __builtin_memcpy(&v, &w, 16);
+        v = __builtin_bit_cast(u32x4, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
     }
     return v;
 }
 
-// acc[q][p] += Q P over the lane's chunk.  32-bit numbers go in four steps: the contraction may run in any order as long as both
-// sides agree, so lane group g feeds chunk g and each step takes one number of it.
-template <class T>
-__device__ __forceinline__ f32x4 multiply(u32x4 q, u32x4 p, f32x4 acc) {
-    if constexpr (std::is_same_v<T, bf16>) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, q), __builtin_bit_cast(bf16x8, p), acc, 0, 0, 0);
-    } else if constexpr (std::is_same_v<T, f16>) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, q), __builtin_bit_cast(f16x8, p), acc, 0, 0, 0);
-    } else {
-        const f32x4 a = __builtin_bit_cast(f32x4, q), b = __builtin_bit_cast(f32x4, p);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], acc, 0, 0, 0);
-        return acc;
-    }
-}
-
-template <class T, int MODE, int BP, int BQ>
-__global__ __launch_bounds__(kBlock) void dense_kernel(DenseArgs a) {
+template <class T, int MODE, int BP, int BQ, bool SPLIT>
+__global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
     constexpr bool PT = MODE == kWgrad, QT = MODE != kForward, FUSE = MODE != kForward;
     constexpr int CE = kChunk<T>, ST = kStage<T>;
     constexpr int NP = BP / 32, NQ = BQ / 32;               // chunks a thread stages per tile = 16-wide fragments per wave
+    constexpr int kP = BP * kRowBytes, kBuf = kP * (SPLIT ? 2 : 1) + BQ * kRowBytes;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
     const int wp = wave >> 1, wq = wave & 1;
 
-    // tile of this workgroup: eight runs of tiles, one per XCD (workgroups are dealt to them in turn), so that the column tiles of
-    // a row tile share an L2
-    int tile = blockIdx.x;
-    const int per = (a.tiles + kNumXCD - 1) / kNumXCD;
-    tile = (tile % kNumXCD) * per + tile / kNumXCD;
-    if (tile >= a.tiles) return;
+    // tile (and, for wgrad, stretch of rows) of this workgroup: eight runs of them, one per XCD (workgroups are dealt to the XCDs in
+    // turn), so that the tiles that read the same rows share an L2
+    const int per = (int)((gridDim.x + kNumXCD - 1) / kNumXCD);
+    const int64_t at = (int64_t)(blockIdx.x % kNumXCD) * per + blockIdx.x / kNumXCD;
+    if (at >= (int64_t)a.tiles * a.splits) return;
+    const int64_t stretch = at / a.tiles;
+    const int tile = (int)(at - stretch * a.tiles);
     const int64_t p0 = (int64_t)(tile / a.tiles_q) * BP;
     const int q0 = (tile % a.tiles_q) * BQ;
-    const int64_t c_begin = MODE == kWgrad ? (int64_t)blockIdx.y * a.split : 0;
+    const int64_t c_begin = MODE == kWgrad ? stretch * a.split : 0;
     const int64_t c_end = MODE == kWgrad ? (c_begin + a.split < a.n_c ? c_begin + a.split : a.n_c) : a.n_c;
 
-    const T *P = reinterpret_cast<const T *>(a.p), *Q = reinterpret_cast<const T *>(a.q), *S = reinterpret_cast<const T *>(a.saved);
+    const T *P = reinterpret_cast<const T *>(a.p), *Q = reinterpret_cast<const T *>(a.q);
     u32x4 rp[NP], rs[NP], rq[NQ];
     f32x4 acc[NP][NQ];
 #pragma unroll
     for (int i = 0; i < NP; ++i)
 #pragma unroll
         for (int j = 0; j < NQ; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    float db[FUSE ? CE : 1];
+    float db[MODE == kWgrad ? CE : 1];
 #pragma unroll
-    for (int i = 0; i < (FUSE ? CE : 1); ++i) db[i] = 0.0f;
+    for (int i = 0; i < (MODE == kWgrad ? CE : 1); ++i) db[i] = 0.0f;
 
     // which row and chunk of a tile this thread stages in its k-th turn
     auto place = [&](bool tr, int rows, int k, int &row, int &chunk) {
@@ -165,7 +431,7 @@ __global__ __launch_bounds__(kBlock) void dense_kernel(DenseArgs a) {
             const int64_t r = PT ? c + row : p0 + row, col = PT ? p0 + chunk * CE : c + chunk * CE;
             const int64_t rows = PT ? c_end : a.n_p, cols = PT ? a.n_p : a.n_c;
             rp[k] = load_chunk<T>(P + r * a.ld_p, col, cols, r < rows, a.vec_p);
-            if (FUSE && a.act != NFA_ACT_NONE) rs[k] = load_chunk<T>(S + r * a.ld_saved, col, cols, r < rows, a.vec_p);
+            if (FUSE) rs[k] = load_saved<T>(a, r, col, cols, r < rows);
         }
 #pragma unroll
         for (int k = 0; k < NQ; ++k) {
@@ -177,33 +443,23 @@ __global__ __launch_bounds__(kBlock) void dense_kernel(DenseArgs a) {
         }
     };
     auto store = [&](char *buf) {
+        u32x4 lo[SPLIT ? NP : 1];
+        if constexpr (FUSE)
+            form_dz<T, SPLIT, NP>(a, rp, rs, lo, [&](int, float dz, int e) {
+                if constexpr (MODE == kWgrad) db[e] += dz;
+            });
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
             int row, chunk;
             place(PT, BP, k, row, chunk);
-            if (FUSE) {
-                Frag<T> g = __builtin_bit_cast(Frag<T>, rp[k]);
-                if (a.act != NFA_ACT_NONE) {
-                    const Frag<T> s = __builtin_bit_cast(Frag<T>, rs[k]);
-#pragma unroll
-                    for (int i = 0; i < CE; ++i) {
-                        const float dz = to_f(g.v[i]) * act_slope(a.act, to_f(s.v[i]));
-                        if (MODE == kWgrad) db[i] += dz;
-                        g.v[i] = from_f<T>(dz);             // rounded: the matrix units take T
-                    }
-                    rp[k] = __builtin_bit_cast(u32x4, g);
-                } else if (MODE == kWgrad) {
-#pragma unroll
-                    for (int i = 0; i < CE; ++i) db[i] += to_f(g.v[i]);
-                }
-            }
             *reinterpret_cast<u32x4 *>(buf + stage_offset<T, PT, BP>(row, chunk)) = rp[k];
+            if constexpr (SPLIT) *reinterpret_cast<u32x4 *>(buf + kP + stage_offset<T, PT, BP>(row, chunk)) = lo[k];
         }
 #pragma unroll
         for (int k = 0; k < NQ; ++k) {
             int row, chunk;
             place(QT, BQ, k, row, chunk);
-            *reinterpret_cast<u32x4 *>(buf + BP * kRowBytes + stage_offset<T, QT, BQ>(row, chunk)) = rq[k];
+            *reinterpret_cast<u32x4 *>(buf + kBuf - BQ * kRowBytes + stage_offset<T, QT, BQ>(row, chunk)) = rq[k];
         }
     };
     auto compute = [&](const char *buf, int64_t c) {
@@ -212,17 +468,19 @@ __global__ __launch_bounds__(kBlock) void dense_kernel(DenseArgs a) {
             if (c + ks * (ST / 2) >= c_end) break;          // a half that holds only zeros
             u32x4 fp[NP], fq[NQ];
 #pragma unroll
-            for (int i = 0; i < NP; ++i) fp[i] = read_frag<T, PT, BP>(buf, wp * (BP / 2) + i * 16, ks, lane);
+            for (int j = 0; j < NQ; ++j) fq[j] = read_frag<T, QT, BQ>(buf + kBuf - BQ * kRowBytes, wq * (BQ / 2) + j * 16, ks, lane);
 #pragma unroll
-            for (int j = 0; j < NQ; ++j) fq[j] = read_frag<T, QT, BQ>(buf + BP * kRowBytes, wq * (BQ / 2) + j * 16, ks, lane);
+            for (int half = 0; half < (SPLIT ? 2 : 1); ++half) {
 #pragma unroll
-            for (int i = 0; i < NP; ++i)
+                for (int i = 0; i < NP; ++i) fp[i] = read_frag<T, PT, BP>(buf + half * kP, wp * (BP / 2) + i * 16, ks, lane);
 #pragma unroll
-                for (int j = 0; j < NQ; ++j) acc[i][j] = multiply<T>(fq[j], fp[i], acc[i][j]);
+                for (int i = 0; i < NP; ++i)
+#pragma unroll
+                    for (int j = 0; j < NQ; ++j) acc[i][j] = multiply<T>(fq[j], fp[i], acc[i][j]);
+            }
         }
     };
 
-    constexpr int kBuf = (BP + BQ) * kRowBytes;
     load(c_begin);
     store(lds);
     __syncthreads();
@@ -238,17 +496,22 @@ __global__ __launch_bounds__(kBlock) void dense_kernel(DenseArgs a) {
 
     // lane l holds row p = l % 16 of each fragment and four neighbouring columns q
     const int i = lane & 15, g = lane >> 4;
-    if (MODE == kWgrad) {
-        float *part = a.partial + (int64_t)blockIdx.y * (a.n_p * a.n_q + a.n_p);
+    if constexpr (MODE == kWgrad) {
+        float *part = a.partial + stretch * (a.n_p * a.n_q + a.n_p);
 #pragma unroll
         for (int pi = 0; pi < NP; ++pi)
 #pragma unroll
             for (int qi = 0; qi < NQ; ++qi) {
                 const int64_t p = p0 + wp * (BP / 2) + pi * 16 + i;
                 const int q = q0 + wq * (BQ / 2) + qi * 16 + g * 4;
+                if (p >= a.n_p) continue;
+                if (a.vec_out) {
+                    if (q < a.n_q) *reinterpret_cast<f32x4 *>(part + p * a.n_q + q) = acc[pi][qi];
+                } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (p < a.n_p && q + r < a.n_q) part[p * a.n_q + q + r] = acc[pi][qi][r];
+                    for (int r = 0; r < 4; ++r)
+                        if (q + r < a.n_q) part[p * a.n_q + q + r] = acc[pi][qi][r];
+                }
             }
         if (q0 == 0 && a.want_bias) {                       // db: the threads that staged the same columns, in order
             constexpr int per_row = BP / CE, n = kBlock / per_row;
@@ -262,51 +525,33 @@ __global__ __launch_bounds__(kBlock) void dense_kernel(DenseArgs a) {
                 part[a.n_p * a.n_q + p0 + tid] = v;
             }
         }
-        return;
-    }
-    T *out = reinterpret_cast<T *>(a.out), *kept = reinterpret_cast<T *>(a.saved_out);
-    const T *bias = reinterpret_cast<const T *>(a.bias), *res = reinterpret_cast<const T *>(a.residual);
-    struct alignas(4 * sizeof(T)) V4 { T v[4]; };
-#pragma unroll
-    for (int qi = 0; qi < NQ; ++qi) {
-        const int q = q0 + wq * (BQ / 2) + qi * 16 + g * 4;
-        float b[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) b[r] = (MODE == kForward && bias && q + r < a.n_q) ? to_f(bias[q + r]) : 0.0f;
+    } else {
+        // through LDS, so that a thread holds whole chunks of a row: 32 rows of each wave's half at a time
+        const T *bias = reinterpret_cast<const T *>(a.bias);
+        constexpr int W = BQ / 2 + 4;                       // floats in a row: the half's columns, shifted by a bank group per row
+        float *mine = reinterpret_cast<float *>(lds) + wave * 16 * W;
 #pragma unroll
         for (int pi = 0; pi < NP; ++pi) {
-            const int64_t p = p0 + wp * (BP / 2) + pi * 16 + i;
-            if (p >= a.n_p || q >= a.n_q) continue;
-            V4 y, k;
-            if (MODE == kForward) {
-                V4 add{};
-                if (res) {
-                    if (a.vec_out) add = *reinterpret_cast<const V4 *>(res + p * a.ld_residual + q);
-                    else
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) add.v[r] = q + r < a.n_q ? res[p * a.ld_residual + q + r] : T(0.0f);
-                }
+            for (int qi = 0; qi < NQ; ++qi) *reinterpret_cast<f32x4 *>(mine + i * W + qi * 16 + g * 4) = acc[pi][qi];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            constexpr int per_row = BQ / 2 / CE;            // chunks of a row in this half
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float z = acc[pi][qi][r] + b[r], v = act_fwd(a.act, z);
-                    k.v[r] = from_f<T>(a.want_bias ? v : z);        // (forward: want_bias = the saved number is act(z))
-                    y.v[r] = from_f<T>(res ? v + to_f(add.v[r]) : v);
-                }
-            } else {
+            for (int k = 0; k < 16 * per_row / kWave; ++k) {
+                const int e = k * kWave + lane, row = e / per_row, chunk = e % per_row;
+                const int64_t p = p0 + wp * (BP / 2) + pi * 16 + row;
+                const int col[1] = {q0 + wq * (BQ / 2) + chunk * CE};
+                float z[1][CE];
+                u32x4 res[1] = {{0, 0, 0, 0}};
+                if (MODE == kForward && a.residual)
+                    res[0] = load_chunk<T>(reinterpret_cast<const T *>(a.residual) + p * a.ld_residual, col[0], a.n_q, p < a.n_p, a.vec_out);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y.v[r] = from_f<T>(acc[pi][qi][r]);
+                for (int v = 0; v < CE; ++v)
+                    z[0][v] = mine[row * W + chunk * CE + v] + (MODE == kForward && bias && col[0] + v < a.n_q ? to_f(bias[col[0] + v]) : 0.0f);
+                if (p < a.n_p && col[0] < a.n_q) epilogue<T, MODE, 1>(a, p, col, z, res);
             }
-            if (a.vec_out) {
-                *reinterpret_cast<V4 *>(out + p * a.n_q + q) = y;
-                if (MODE == kForward && kept) *reinterpret_cast<V4 *>(kept + p * a.n_q + q) = k;
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (q + r < a.n_q) {
-                        out[p * a.n_q + q + r] = y.v[r];
-                        if (MODE == kForward && kept) kept[p * a.n_q + q + r] = k.v[r];
-                    }
-            }
+            __builtin_amdgcn_wave_barrier();
         }
     }
 }
@@ -337,26 +582,74 @@ bool aligned(const void *p, int64_t ld, int64_t cols, int64_t bytes, int64_t to)
     return (uintptr_t)p % to == 0 && ld * bytes % to == 0 && cols * bytes % to == 0;
 }
 
-template <class T, int MODE, int BP, int BQ>
+template <class K>
+int allow_lds(K kernel, size_t bytes) {
+    if (bytes <= 64 * 1024) return NFA_OK;
+    const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return e == hipSuccess ? NFA_OK : fail(NFA_ERR_LAUNCH, "linear: %zu bytes of LDS: %s", bytes, hipGetErrorString(e));
+}
+
+template <class T, int MODE, int BP, int BQ, bool SPLIT>
 int launch_tiles(DenseArgs a, int64_t splits, hipStream_t s) {
     const int64_t tiles_p = ceil_div(a.n_p, BP);
     a.tiles_q = (int32_t)ceil_div(a.n_q, BQ);
     NFA_REQUIRE(tiles_p * a.tiles_q < (1 << 30), "linear: too many rows for one launch");
     a.tiles = (int32_t)(tiles_p * a.tiles_q);
     const int64_t steps = MODE == kWgrad ? a.split : a.n_c;
-    const size_t bytes = (size_t)(BP + BQ) * kRowBytes * (steps > kStage<T> ? 2 : 1);
-    const dim3 grid((unsigned)(ceil_div(a.tiles, kNumXCD) * kNumXCD), (unsigned)splits);
-    hipLaunchKernelGGL((dense_kernel<T, MODE, BP, BQ>), grid, dim3(kBlock), bytes, s, a);
-    return check_launch("dense_kernel");
+    const size_t bytes = (size_t)(BP * (SPLIT ? 2 : 1) + BQ) * kRowBytes * (steps > kStage<T> ? 2 : 1);
+    if (int rc = allow_lds(tile_kernel<T, MODE, BP, BQ, SPLIT>, bytes)) return rc;
+    a.splits = (int32_t)splits;
+    const unsigned grid = (unsigned)(ceil_div(a.tiles * splits, kNumXCD) * kNumXCD);
+    hipLaunchKernelGGL((tile_kernel<T, MODE, BP, BQ, SPLIT>), dim3(grid), dim3(kBlock), bytes, s, a);
+    return check_launch("tile_kernel");
+}
+
+template <class T, int MODE, int KS, bool SPLIT>
+int launch_resident(DenseArgs a, hipStream_t s) {
+    constexpr int RT = SPLIT || KS == 16 ? 1 : 2, C = KS * 4 * kChunk<T>;
+    const int64_t tiles = ceil_div(a.n_p, 16 * RT);
+    NFA_REQUIRE(tiles < (1ll << 31), "linear: too many rows for one launch");
+    a.tiles = (int32_t)tiles;
+    // columns of a workgroup: all that fit, fewer where the rows alone do not give every SIMD a wave
+    auto round_q = [](int64_t q) { return q <= 32 ? 32 : q <= 64 ? 64 : ceil_div(q, 128) * 128; };
+    int64_t block = round_q(a.n_q), most = 32;
+    while (round_q(most + 32) * C * (int64_t)sizeof(T) <= kResidentBytes && most < block) most = round_q(most + 32);
+    if (block > most) block = most;
+    while (block > 32 && tiles * ceil_div(a.n_q, block) < kNumCU * 4) block = block > 128 ? round_q(block / 2) : block / 2;
+    a.block_q = (int32_t)block;
+    const int64_t blocks_q = ceil_div(a.n_q, block);
+    const size_t bytes = (size_t)(block * C * (int64_t)sizeof(T));
+    if (int rc = allow_lds(resident_kernel<T, MODE, KS, SPLIT>, bytes)) return rc;
+    const int per_cu = bytes <= 36 * 1024 ? 4 : bytes <= 72 * 1024 ? 2 : 1, threads = resident_threads(KS) / per_cu;   // as many workgroups as weights fit
+    int64_t grid = ceil_div((int64_t)kNumCU * per_cu, blocks_q);
+    const int64_t need = ceil_div(tiles, threads / kWave);
+    if (grid > need) grid = need;
+    NFA_REQUIRE(blocks_q < 65536, "linear: too many features for one launch");
+    hipLaunchKernelGGL((resident_kernel<T, MODE, KS, SPLIT>), dim3((unsigned)grid, (unsigned)blocks_q), dim3(threads), bytes, s, a);
+    return check_launch("resident_kernel");
+}
+
+// forward or dgrad: the weight in LDS for contractions of up to 256, tiles beyond
+template <class T, int MODE, bool SPLIT>
+int launch_rows(const DenseArgs &a, hipStream_t s) {
+    constexpr int step = 4 * kChunk<T>;
+    if (a.n_c <= step) return launch_resident<T, MODE, 1, SPLIT>(a, s);
+    if (a.n_c <= 2 * step) return launch_resident<T, MODE, 2, SPLIT>(a, s);
+    if (a.n_c <= 4 * step) return launch_resident<T, MODE, 4, SPLIT>(a, s);
+    if (a.n_c <= 8 * step) return launch_resident<T, MODE, 8, SPLIT>(a, s);
+    if constexpr (sizeof(T) == 4)
+        if (a.n_c <= 16 * step) return launch_resident<T, MODE, 16, SPLIT>(a, s);
+    constexpr int BP = SPLIT ? 64 : 128;
+    return a.n_q <= 64 ? launch_tiles<T, MODE, BP, 64, SPLIT>(a, 1, s) : launch_tiles<T, MODE, BP, 128, SPLIT>(a, 1, s);
 }
 
 // rows of the long axis that one workgroup of the weight gradient sums: enough workgroups for every CU twice, and not so many that
 // their partial sums (a whole weight each) outweigh the rows read
 struct WgradPlan { int64_t split, splits, bp, bq; };
-WgradPlan wgrad_plan(int64_t rows, int64_t n, int64_t k, int32_t dtype) {
+WgradPlan wgrad_plan(int64_t rows, int64_t n, int64_t k, int32_t dtype, bool two_parts) {
     const int64_t stage = dtype == NFA_DTYPE_F32 ? 32 : 64;
     WgradPlan w;
-    w.bp = n <= 64 ? 64 : 128;
+    w.bp = n <= 64 || two_parts ? 64 : 128;
     w.bq = k <= 64 ? 64 : 128;
     const int64_t tiles = ceil_div(n, w.bp) * ceil_div(k, w.bq);
     int64_t splits = ceil_div(2 * kNumCU, tiles);
@@ -367,6 +660,11 @@ WgradPlan wgrad_plan(int64_t rows, int64_t n, int64_t k, int32_t dtype) {
     w.splits = ceil_div(rows, w.split);
     return w;
 }
+
+bool keeps_bits(int64_t out_features, int32_t dtype, int32_t act) {
+    return act == NFA_ACT_RELU && out_features % (16 / dtype_bytes(dtype)) == 0;
+}
+bool two_parts(int32_t dtype, int32_t act) { return dtype != NFA_DTYPE_F32 && act != NFA_ACT_NONE && act != NFA_ACT_RELU; }
 
 }  // namespace
 
@@ -395,6 +693,7 @@ static int check_linear(const nfa_linear_args *a, const char *who) {
 }
 
 NFA_EXPORT int64_t nfa_linear_saved_bytes(int64_t rows, int32_t out_features, int32_t dtype, int32_t activation, int32_t has_residual) {
+    if (keeps_bits(out_features, dtype, activation)) return rows * (out_features / (16 / dtype_bytes(dtype)));
     if (activation == NFA_ACT_NONE || (act_from_value(activation) && !has_residual)) return 0;
     return rows * out_features * dtype_bytes(dtype);
 }
@@ -412,23 +711,20 @@ NFA_EXPORT int nfa_linear_fwd(const nfa_linear_args *a, void *outputs, void *sav
     d.out = outputs; d.saved_out = saved;
     d.n_p = a->rows; d.n_q = a->out_features; d.n_c = a->in_features;
     d.act = a->activation;
-    d.want_bias = act_from_value(a->activation);
+    d.mask = keeps_bits(a->out_features, a->dtype, a->activation);
+    d.ld_saved = d.mask ? a->out_features / (16 / bytes) : a->out_features;
     d.vec_p = aligned(d.p, d.ld_p, a->in_features, bytes, 16);
     d.vec_q = aligned(d.q, d.ld_q, a->in_features, bytes, 16);
-    d.vec_out = aligned(outputs, d.n_q, d.n_q, bytes, 4 * bytes) && (!saved || aligned(saved, d.n_q, d.n_q, bytes, 4 * bytes)) &&
-                (!a->residual || aligned(a->residual, a->residual_stride, d.n_q, bytes, 4 * bytes));
+    d.vec_out = aligned(outputs, d.n_q, d.n_q, bytes, 16) && (!saved || d.mask || aligned(saved, d.n_q, d.n_q, bytes, 16)) &&
+                (!a->residual || aligned(a->residual, a->residual_stride, d.n_q, bytes, 16));
     int rc = NFA_OK;
-    with_dtype(a->dtype, [&](auto t) {
-        using T = decltype(t);
-        rc = d.n_q <= 64 ? launch_tiles<T, kForward, 128, 64>(d, 1, (hipStream_t)stream)
-                         : launch_tiles<T, kForward, 128, 128>(d, 1, (hipStream_t)stream);
-    });
+    with_dtype(a->dtype, [&](auto t) { rc = launch_rows<decltype(t), kForward, false>(d, (hipStream_t)stream); });
     return rc;
 }
 
-NFA_EXPORT int64_t nfa_linear_bwd_workspace_bytes(int64_t rows, int32_t in_features, int32_t out_features, int32_t dtype) {
+NFA_EXPORT int64_t nfa_linear_bwd_workspace_bytes(int64_t rows, int32_t in_features, int32_t out_features, int32_t dtype, int32_t activation) {
     if (rows <= 0 || in_features <= 0 || out_features <= 0) return 0;
-    const WgradPlan w = wgrad_plan(rows, out_features, in_features, dtype);
+    const WgradPlan w = wgrad_plan(rows, out_features, in_features, dtype, two_parts(dtype, activation));
     return w.splits * ((int64_t)out_features * in_features + out_features) * 4;
 }
 
@@ -442,39 +738,50 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
     NFA_REQUIRE(saved || a->activation == NFA_ACT_NONE, "linear_bwd: the activation needs what the forward call saved");
     NFA_REQUIRE(workspace || !(grad_weight || grad_bias), "linear_bwd: NULL workspace");
     const int64_t bytes = dtype_bytes(a->dtype), n = a->out_features, k = a->in_features;
-    const bool vec_g = aligned(a->grad_outputs, a->grad_outputs_stride, n, bytes, 16) && (!saved || aligned(saved, n, n, bytes, 16));
+    const bool split = two_parts(a->dtype, a->activation);
     DenseArgs d{};
     d.p = a->grad_outputs; d.ld_p = a->grad_outputs_stride;
-    d.saved = saved; d.ld_saved = n;
+    d.saved = saved;
     d.act = a->activation;
-    d.vec_p = vec_g;
+    d.mask = keeps_bits(n, a->dtype, a->activation);
+    d.ld_saved = d.mask ? n / (16 / bytes) : n;
+    d.vec_p = aligned(a->grad_outputs, a->grad_outputs_stride, n, bytes, 16) &&
+              (!saved || a->activation == NFA_ACT_NONE || d.mask || aligned(saved, n, n, bytes, 16));
     int rc = NFA_OK;
     if (grad_inputs) {
         DenseArgs e = d;
         e.q = a->weight; e.ld_q = k;
         e.vec_q = aligned(a->weight, k, k, bytes, 16);
         e.out = grad_inputs;
-        e.vec_out = aligned(grad_inputs, k, k, bytes, 4 * bytes);
+        e.vec_out = aligned(grad_inputs, k, k, bytes, 16);
         e.n_p = a->rows; e.n_q = (int32_t)k; e.n_c = n;
         with_dtype(a->dtype, [&](auto t) {
             using T = decltype(t);
-            rc = k <= 64 ? launch_tiles<T, kDgrad, 128, 64>(e, 1, s) : launch_tiles<T, kDgrad, 128, 128>(e, 1, s);
+            if constexpr (sizeof(T) == 2)
+                if (split) { rc = launch_rows<T, kDgrad, true>(e, s); return; }
+            rc = launch_rows<T, kDgrad, false>(e, s);
         });
         if (rc) return rc;
     }
     if (grad_weight || grad_bias) {
-        const WgradPlan w = wgrad_plan(a->rows, n, k, a->dtype);
+        const WgradPlan w = wgrad_plan(a->rows, n, k, a->dtype, split);
         DenseArgs e = d;
         e.q = a->inputs; e.ld_q = a->inputs_stride;
         e.vec_q = aligned(a->inputs, a->inputs_stride, k, bytes, 16);
         e.partial = (float *)workspace;
+        e.vec_out = k % 4 == 0 && n % 4 == 0;
         e.n_p = n; e.n_q = (int32_t)k; e.n_c = a->rows;
         e.split = w.split;
         e.want_bias = grad_bias != nullptr;
         with_dtype(a->dtype, [&](auto t) {
             using T = decltype(t);
-            if (w.bp == 64) rc = w.bq == 64 ? launch_tiles<T, kWgrad, 64, 64>(e, w.splits, s) : launch_tiles<T, kWgrad, 64, 128>(e, w.splits, s);
-            else rc = w.bq == 64 ? launch_tiles<T, kWgrad, 128, 64>(e, w.splits, s) : launch_tiles<T, kWgrad, 128, 128>(e, w.splits, s);
+            if constexpr (sizeof(T) == 2)
+                if (split) {
+                    rc = w.bq == 64 ? launch_tiles<T, kWgrad, 64, 64, true>(e, w.splits, s) : launch_tiles<T, kWgrad, 64, 128, true>(e, w.splits, s);
+                    return;
+                }
+            if (w.bp == 64) rc = w.bq == 64 ? launch_tiles<T, kWgrad, 64, 64, false>(e, w.splits, s) : launch_tiles<T, kWgrad, 64, 128, false>(e, w.splits, s);
+            else rc = w.bq == 64 ? launch_tiles<T, kWgrad, 128, 64, false>(e, w.splits, s) : launch_tiles<T, kWgrad, 128, 128, false>(e, w.splits, s);
         });
         if (rc) return rc;
         const int64_t ld = n * k + n;

@@ -56,32 +56,44 @@ __device__ __forceinline__ float softplus_f(float x) {
 
 constexpr float kInvSqrt2 = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f;
 
-// What a layer keeps for its backward pass (include/nerfacc_hip.h: nfa_linear_saved): relu, exp and softplus are differentiated from
-// their own value a = act(z), which loses nothing by its rounding (the sign; e^z itself; 1 - e^-a with the relative error of a); the
-// others from z, whose relative rounding error is the derivative's.
+// What a layer keeps for its backward pass (include/nerfacc_hip.h: nfa_linear_saved_bytes): of relu one bit; exp and softplus are
+// differentiated from their own value a = act(z), which loses little by its rounding (e^z itself; 1 - e^-a with the relative error of
+// a); the others from z, whose relative rounding error is the derivative's.
 inline bool act_from_value(int32_t act) { return act == NFA_ACT_RELU || act == NFA_ACT_EXP || act == NFA_ACT_SOFTPLUS; }
 
-__device__ __forceinline__ float act_fwd(int act, float z) {
-    switch (act) {
-        case NFA_ACT_RELU: return z < 0.0f ? 0.0f : z;      // (NaN stays NaN)
-        case NFA_ACT_SIGMOID: return sigmoid_f(z);
-        case NFA_ACT_SOFTPLUS: return softplus_f(z);
-        case NFA_ACT_SILU: return z * sigmoid_f(z);
-        case NFA_ACT_GELU: return 0.5f * z * erfcf(-z * kInvSqrt2);
-        case NFA_ACT_EXP: return expf(z);
-        default: return z;
-    }
+template <int ACT>
+__device__ __forceinline__ float act_fwd(float z) {
+    if constexpr (ACT == NFA_ACT_RELU) return z < 0.0f ? 0.0f : z;      // (NaN stays NaN)
+    else if constexpr (ACT == NFA_ACT_SIGMOID) return sigmoid_f(z);
+    else if constexpr (ACT == NFA_ACT_SOFTPLUS) return softplus_f(z);
+    else if constexpr (ACT == NFA_ACT_SILU) return z * sigmoid_f(z);
+    else if constexpr (ACT == NFA_ACT_GELU) return 0.5f * z * erfcf(-z * kInvSqrt2);
+    else if constexpr (ACT == NFA_ACT_EXP) return expf(z);
+    else return z;
 }
 // the derivative, from the saved number (act_from_value)
-__device__ __forceinline__ float act_slope(int act, float s) {
+template <int ACT>
+__device__ __forceinline__ float act_slope(float s) {
+    if constexpr (ACT == NFA_ACT_RELU) return s > 0.0f ? 1.0f : (s != s ? s : 0.0f);
+    else if constexpr (ACT == NFA_ACT_SIGMOID) return sigmoid_f(s) * sigmoid_f(-s);
+    else if constexpr (ACT == NFA_ACT_SOFTPLUS) return -expm1f(-s);
+    else if constexpr (ACT == NFA_ACT_SILU) return sigmoid_f(s) * fmaf(s, sigmoid_f(-s), 1.0f);
+    else if constexpr (ACT == NFA_ACT_GELU) return fmaf(s * kInvSqrt2Pi, expf(-0.5f * s * s), 0.5f * erfcf(-s * kInvSqrt2));
+    else if constexpr (ACT == NFA_ACT_EXP) return s;
+    else return 1.0f;
+}
+// calls f(integral ACT): the choice is made once around a loop, not once per number (a switch inside an unrolled loop is many times
+// the instruction cache)
+template <class F>
+__device__ __forceinline__ void with_act(int act, F &&f) {
     switch (act) {
-        case NFA_ACT_RELU: return s > 0.0f ? 1.0f : (s != s ? s : 0.0f);
-        case NFA_ACT_SIGMOID: { const float r = sigmoid_f(s); return r * sigmoid_f(-s); }
-        case NFA_ACT_SOFTPLUS: return -expm1f(-s);
-        case NFA_ACT_SILU: { const float r = sigmoid_f(s); return r * fmaf(s, sigmoid_f(-s), 1.0f); }
-        case NFA_ACT_GELU: return fmaf(s * kInvSqrt2Pi, expf(-0.5f * s * s), 0.5f * erfcf(-s * kInvSqrt2));
-        case NFA_ACT_EXP: return s;
-        default: return 1.0f;
+        case NFA_ACT_RELU: f(std::integral_constant<int, NFA_ACT_RELU>{}); break;
+        case NFA_ACT_SIGMOID: f(std::integral_constant<int, NFA_ACT_SIGMOID>{}); break;
+        case NFA_ACT_SOFTPLUS: f(std::integral_constant<int, NFA_ACT_SOFTPLUS>{}); break;
+        case NFA_ACT_SILU: f(std::integral_constant<int, NFA_ACT_SILU>{}); break;
+        case NFA_ACT_GELU: f(std::integral_constant<int, NFA_ACT_GELU>{}); break;
+        case NFA_ACT_EXP: f(std::integral_constant<int, NFA_ACT_EXP>{}); break;
+        default: f(std::integral_constant<int, NFA_ACT_NONE>{}); break;
     }
 }
 

@@ -1465,7 +1465,8 @@ std::tuple<Tensor, OptTensor> linear_fwd(const Tensor &x_, const Tensor &w_, con
     if (r_ && r_->defined()) r = as_rows(*r_, "residual", m, n, x_);
     Guard g(device_of(x_));
     Tensor out = at::empty({m, n}, x_.options()), saved;
-    if (save && nfa_linear_saved_bytes(m, (int32_t)n, dtype_of(x), (int32_t)act, r.defined()) > 0) saved = at::empty({m, n}, x_.options());
+    if (const int64_t bytes = save ? nfa_linear_saved_bytes(m, (int32_t)n, dtype_of(x), (int32_t)act, r.defined()) : 0; bytes > 0)
+        saved = at::empty({bytes}, opts(x, at::kByte));
     nfa_linear_args a{};
     a.rows = m; a.in_features = (int32_t)k; a.out_features = (int32_t)n;
     a.dtype = dtype_of(x); a.activation = (int32_t)act;
@@ -1482,7 +1483,13 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_bwd(const Tensor &g_, const T
     const int64_t m = x_.size(0), k = w_.size(1), n = w_.size(0);
     const Tensor x = as_rows(x_, "inputs", m, k, x_), w = dense_of(w_, "weight", x_.scalar_type(), n * k, x_);
     const Tensor gy = as_rows(g_, "grad_outputs", m, n, x_);
-    const OptTensor saved = dense_of(saved_, "saved", x_.scalar_type(), m * n, x_);
+    OptTensor saved;                            // what linear_fwd kept, or its outputs
+    if (act != NFA_ACT_NONE && m > 0) {
+        TORCH_CHECK(saved_ && saved_->defined() && saved_->is_cuda() && saved_->device() == x.device() && saved_->is_contiguous(), "linear: saved is missing");
+        const int64_t kept = nfa_linear_saved_bytes(m, (int32_t)n, dtype_of(x), (int32_t)act, 0);
+        TORCH_CHECK((int64_t)saved_->nbytes() == (kept ? kept : m * n * (int64_t)x.element_size()), "linear: saved differs in size");
+        saved = saved_;
+    }
     Guard g(device_of(x_));
     Tensor gx, gw, gb;
     if (need_x) gx = at::empty({m, k}, x_.options());
@@ -1500,7 +1507,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_bwd(const Tensor &g_, const T
     a.weight = w.data_ptr();
     a.grad_outputs = gy.data_ptr(); a.grad_outputs_stride = row_stride(gy);
     Tensor ws;
-    if (need_w || need_b) ws = at::empty({nfa_linear_bwd_workspace_bytes(m, (int32_t)k, (int32_t)n, a.dtype)}, opts(x, at::kByte));
+    if (need_w || need_b) ws = at::empty({nfa_linear_bwd_workspace_bytes(m, (int32_t)k, (int32_t)n, a.dtype, a.activation)}, opts(x, at::kByte));
     check_rc(nfa_linear_bwd(&a, ptr<void>(saved), ptr<void>(gx), ptr<void>(gw), ptr<void>(gb), ptr<void>(ws), stream_of(x)));
     return {some(gx), some(gw), some(gb)};
 }

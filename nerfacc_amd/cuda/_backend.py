@@ -1131,8 +1131,8 @@ class _CtypesC:
         with _Guard(x):
             out = torch.empty((m, n), dtype=x.dtype, device=x.device)
             L = load_library()
-            kept = save and L.nfa_linear_saved_bytes(m, n, _dtype_id(x), act, int(r is not None)) > 0
-            saved = torch.empty_like(out) if kept else None
+            kept = L.nfa_linear_saved_bytes(m, n, _dtype_id(x), act, int(r is not None)) if save else 0
+            saved = torch.empty(kept, dtype=torch.uint8, device=x.device) if kept else None
             a = _STRUCTS["nfa_linear_args"](rows=m, in_features=k, out_features=n, dtype=_dtype_id(x), activation=act, inputs=_ptr(x),
                                             inputs_stride=_row_stride(x), weight=_ptr(w), bias=_ptr(b), residual=_ptr(r),
                                             residual_stride=0 if r is None else _row_stride(r))
@@ -1151,7 +1151,7 @@ class _CtypesC:
             gb = new((n,), dtype=x.dtype, device=x.device) if need_b else None
             if m:
                 L = load_library()
-                ws = torch.empty(L.nfa_linear_bwd_workspace_bytes(m, k, n, _dtype_id(x)), dtype=torch.uint8, device=x.device)
+                ws = torch.empty(L.nfa_linear_bwd_workspace_bytes(m, k, n, _dtype_id(x), act), dtype=torch.uint8, device=x.device)
                 a = _STRUCTS["nfa_linear_args"](rows=m, in_features=k, out_features=n, dtype=_dtype_id(x), activation=act, inputs=_ptr(x),
                                                 inputs_stride=_row_stride(x), weight=_ptr(w), grad_outputs=_ptr(g),
                                                 grad_outputs_stride=_row_stride(g))

@@ -65,7 +65,8 @@ def test_the_c_abi_checks_before_it_launches():
     assert "NULL" in _error(L.nfa_linear_fwd(None, p, None, None)) and "NULL" in _error(L.nfa_linear_fwd(ctypes.byref(a), None, None, None))
     assert "saved" in _error(L.nfa_linear_bwd(ctypes.byref(a), None, p, p, p, p, None))
     assert "workspace" in _error(L.nfa_linear_bwd(ctypes.byref(a), p, p, p, p, None, None))
-    assert L.nfa_linear_saved_bytes(10, 8, 1, 0, 1) == 0 and L.nfa_linear_saved_bytes(10, 8, 1, 1, 0) == 0 and L.nfa_linear_saved_bytes(10, 8, 1, 4, 0) == 160
+    assert L.nfa_linear_saved_bytes(10, 8, 1, 0, 1) == 0 and L.nfa_linear_saved_bytes(10, 8, 1, 6, 0) == 0 and L.nfa_linear_saved_bytes(10, 8, 1, 4, 0) == 160
+    assert [L.nfa_linear_saved_bytes(10, n, t, 1, r) for n, t, r in ((16, 1, 1), (16, 0, 0), (9, 1, 0), (9, 1, 1))] == [20, 40, 0, 180]     # relu: bits
     good = dict(n_rays=2, rows=4, channels=8, width=4, dtype=0, activation=4, inputs=p, inputs_stride=8, weight=p, grad_outputs=p, grad_outputs_stride=8)
     for bad, text in ((dict(width=5), "width"), (dict(width=1), "width"), (dict(rows=5), "equal sequences"), (dict(packed_info=p), "row map"),
                       (dict(activation=1), "activation"), (dict(inputs_stride=2), "inputs_stride"), (dict(weight=None), "NULL"),
@@ -91,4 +92,4 @@ def test_workspaces_cover_both_layouts():
     assert L.nfa_selective_scan_workspace_bytes(4096, 1 << 18, 64, 16, 0) == 0                      # whole rays: nothing to chain
     assert L.nfa_selective_scan_workspace_bytes(1, 1 << 15, 1024, 16, 0) >= 2 * 1024 * 17 * 4
     assert L.nfa_selective_scan_checkpoint_bytes(17, 3, 5) == 3 * 3 * 5 * 4
-    assert L.nfa_causal_conv_bwd_workspace_bytes(0, 8, 4, 1) == 0 and L.nfa_linear_bwd_workspace_bytes(0, 8, 8, 1) == 0
+    assert L.nfa_causal_conv_bwd_workspace_bytes(0, 8, 4, 1) == 0 and L.nfa_linear_bwd_workspace_bytes(0, 8, 8, 1, 0) == 0
