@@ -37,33 +37,39 @@ struct DenseArgs {
     int32_t n_q;
     int64_t ld_p, ld_q, ld_saved, ld_residual;  // in elements (ld_saved of bits: in bytes)
     int64_t split;                              // wgrad: contraction steps of one workgroup
-    int32_t act, mask, vec_p, vec_q, vec_out, want_bias, tiles_q, tiles, block_q, splits;
+    int32_t act, mask, vec, want_bias, tiles_q, tiles, block_q, splits;
 };
 
 enum { kForward, kDgrad, kWgrad };
 
-// sixteen bytes of a row, zero outside it; `vec`: every row starts on 16 bytes and holds whole chunks
-template <class T>
-__device__ __forceinline__ u32x4 load_chunk(const T *row, int64_t col, int64_t cols, bool inside, bool vec) {
+// sixteen bytes of row `row`, zeros outside the array.  VEC: every row starts on 16 bytes and holds whole chunks; the load is then
+// made in any case, from a place that exists, so that a tile's loads are one block without branches
+template <class T, bool VEC>
+__device__ __forceinline__ u32x4 load_chunk(const T *base, int64_t row, int64_t rows, int64_t ld, int64_t col, int64_t cols) {
     u32x4 v = {0, 0, 0, 0};
-    if (vec) {
-        if (inside && col < cols) v = *reinterpret_cast<const u32x4 *>(row + col);
+    const bool inside = row < rows && col < cols;
+    if constexpr (VEC) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(base + (row < rows ? row : rows - 1) * ld + (col < cols ? col : 0));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = inside ? w[i] : 0;
     } else if (inside) {
         T e[kChunk<T>];
+        base += row * ld + col;
 #pragma unroll
-        for (int i = 0; i < kChunk<T>; ++i) e[i] = col + i < cols ? row[col + i] : T(0.0f);
+        for (int i = 0; i < kChunk<T>; ++i) e[i] = col + i < cols ? base[i] : T(0.0f);
         __builtin_memcpy(&v, e, 16);
     }
     return v;
 }
 // what dz is formed from beside dy: a chunk of saved numbers, or a byte of relu's bits
-template <class T>
-__device__ __forceinline__ u32x4 load_saved(const DenseArgs &a, int64_t row, int64_t col, int64_t cols, bool inside) {
+template <class T, bool VEC>
+__device__ __forceinline__ u32x4 load_saved(const DenseArgs &a, int64_t row, int64_t rows, int64_t col, int64_t cols) {
     u32x4 v = {0, 0, 0, 0};
     if (a.mask) {
-        if (inside && col < cols) v[0] = reinterpret_cast<const uint8_t *>(a.saved)[row * a.ld_saved + col / kChunk<T>];
+        const bool inside = row < rows && col < cols;
+        v[0] = reinterpret_cast<const uint8_t *>(a.saved)[inside ? row * a.ld_saved + col / kChunk<T> : 0];
     } else if (a.act != NFA_ACT_NONE) {
-        v = load_chunk<T>(reinterpret_cast<const T *>(a.saved) + row * a.ld_saved, col, cols, inside, a.vec_p);
+        v = load_chunk<T, VEC>(reinterpret_cast<const T *>(a.saved), row, rows, a.ld_saved, col, cols);
     }
     return v;
 }
@@ -156,9 +162,9 @@ __device__ __forceinline__ void finish_chunks(const DenseArgs &a, float (&z)[N][
     });
 }
 // a chunk of a contiguous output row, as far as it lies inside
-template <class T>
-__device__ __forceinline__ void store_chunk(T *row, int q, int n_q, bool vec, u32x4 v) {
-    if (vec) {
+template <class T, bool VEC>
+__device__ __forceinline__ void store_chunk(T *row, int q, int n_q, u32x4 v) {
+    if constexpr (VEC) {
         if (q < n_q) *reinterpret_cast<u32x4 *>(row + q) = v;
     } else {
         const Frag<T> f = __builtin_bit_cast(Frag<T>, v);
@@ -168,7 +174,7 @@ __device__ __forceinline__ void store_chunk(T *row, int q, int n_q, bool vec, u3
     }
 }
 // the epilogue of N chunks of row p (columns q[k] ..): acc in, outputs and the saved numbers out
-template <class T, int MODE, int N>
+template <class T, int MODE, bool VEC, int N>
 __device__ __forceinline__ void epilogue(const DenseArgs &a, int64_t p, const int (&q)[N], float (&z)[N][kChunk<T>], const u32x4 (&res)[N]) {
     u32x4 y[N], kept[N];
     T *out = reinterpret_cast<T *>(a.out) + p * a.n_q;
@@ -176,12 +182,12 @@ __device__ __forceinline__ void epilogue(const DenseArgs &a, int64_t p, const in
         finish_chunks<T, N>(a, z, res, y, kept);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            store_chunk<T>(out, q[k], a.n_q, a.vec_out, y[k]);
+            store_chunk<T, VEC>(out, q[k], a.n_q, y[k]);
             if (!a.saved_out) continue;
             if (a.mask) {
                 if (q[k] < a.n_q) reinterpret_cast<uint8_t *>(a.saved_out)[p * a.ld_saved + q[k] / kChunk<T>] = (uint8_t)kept[k][0];
             } else {
-                store_chunk<T>(reinterpret_cast<T *>(a.saved_out) + p * a.n_q, q[k], a.n_q, a.vec_out, kept[k]);
+                store_chunk<T, VEC>(reinterpret_cast<T *>(a.saved_out) + p * a.n_q, q[k], a.n_q, kept[k]);
             }
         }
     } else {
@@ -190,7 +196,7 @@ __device__ __forceinline__ void epilogue(const DenseArgs &a, int64_t p, const in
             Frag<T> o;
 #pragma unroll
             for (int i = 0; i < kChunk<T>; ++i) o.v[i] = from_f<T>(z[k][i]);
-            store_chunk<T>(out, q[k], a.n_q, a.vec_out, __builtin_bit_cast(u32x4, o));
+            store_chunk<T, VEC>(out, q[k], a.n_q, __builtin_bit_cast(u32x4, o));
         }
     }
 }
@@ -221,7 +227,7 @@ __device__ __forceinline__ int weight_offset_t(int row, int chunk, int pitch) { 
 
 // waves on a CU: sixteen while a wave's rows leave room in the registers, eight beyond (its loads in flight are twice as many then)
 constexpr int resident_threads(int ks) { return ks <= 2 ? 1024 : 512; }
-template <class T, int MODE, int KS, bool SPLIT>
+template <class T, int MODE, int KS, bool SPLIT, bool VEC>
 __global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArgs a) {
     constexpr int CE = kChunk<T>, RT = SPLIT || KS == 16 ? 1 : 2;       // rows of a wave: RT fragments of sixteen
     constexpr int NC = sizeof(T) == 2 ? 1 : 2;                          // chunks of a lane in a group of 32 columns
@@ -233,40 +239,47 @@ __global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArg
     if (MODE == kForward) {
         for (int e = threadIdx.x; e < q_rows * KS * 4; e += blockDim.x) {
             const int q = e / (KS * 4), chunk = e % (KS * 4);
-            const u32x4 v = load_chunk<T>(Q + (int64_t)(q0 + q) * a.ld_q, chunk * CE, a.n_c, q < nq, a.vec_q);
+            const u32x4 v = load_chunk<T, VEC>(Q, q0 + q, q0 + nq, a.ld_q, chunk * CE, a.n_c);
             *reinterpret_cast<u32x4 *>(lds + weight_offset<T, KS>((q & ~31) + place_of_column<T>(q & 31), chunk)) = v;
         }
     } else {
         for (int e = threadIdx.x; e < KS * 4 * CE * pitch; e += blockDim.x) {
             const int n = e / pitch, chunk = e - n * pitch;
-            const u32x4 v = load_chunk<T>(Q + (int64_t)n * a.ld_q + q0, chunk * CE, nq, n < a.n_c, a.vec_q);
+            const u32x4 v = load_chunk<T, VEC>(Q + q0, n, a.n_c, a.ld_q, chunk * CE, nq);
             *reinterpret_cast<u32x4 *>(lds + weight_offset_t<T>(n, chunk, pitch)) = v;
         }
     }
+    float *bias = reinterpret_cast<float *>(lds + a.block_q * (KS * 4 * CE * (int)sizeof(T)));
+    if (MODE == kForward)
+        for (int c = threadIdx.x; c < a.block_q; c += blockDim.x) bias[c] = a.bias && c < nq ? to_f(reinterpret_cast<const T *>(a.bias)[q0 + c]) : 0.0f;
     __syncthreads();
 
-    const T *bias = reinterpret_cast<const T *>(a.bias);
+    const bool whole = a.n_c == KS * 4 * CE;
     const int64_t waves = (int64_t)gridDim.x * (blockDim.x >> 6);
     for (int64_t tile = (int64_t)blockIdx.x * (blockDim.x >> 6) + wave_in_block(); tile < a.tiles; tile += waves) {
         const int64_t p0 = tile * (16 * RT);
         u32x4 x[RT * KS], lo[SPLIT ? RT * KS : 1];
+        if (VEC && whole) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
+            for (int r = 0; r < RT; ++r) {
                 const int64_t p = p0 + r * 16 + i;
-                x[r * KS + k] = load_chunk<T>(P + p * a.ld_p, (k * 4 + g) * CE, a.n_c, p < a.n_p, a.vec_p);
+                const T *row = P + (p < a.n_p ? p : a.n_p - 1) * a.ld_p + g * CE;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) x[r * KS + k] = *reinterpret_cast<const u32x4 *>(row + k * 4 * CE);
             }
+        } else {
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int k = 0; k < KS; ++k) x[r * KS + k] = load_chunk<T, VEC>(P, p0 + r * 16 + i, a.n_p, a.ld_p, (k * 4 + g) * CE, a.n_c);
+        }
         if constexpr (MODE == kDgrad) {
             if (a.act != NFA_ACT_NONE) {
                 u32x4 s[RT * KS];
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) {
-                        const int64_t p = p0 + r * 16 + i;
-                        s[r * KS + k] = load_saved<T>(a, p, (k * 4 + g) * CE, a.n_c, p < a.n_p);
-                    }
+                    for (int k = 0; k < KS; ++k) s[r * KS + k] = load_saved<T, VEC>(a, p0 + r * 16 + i, a.n_p, (k * 4 + g) * CE, a.n_c);
                 form_dz<T, SPLIT, RT * KS>(a, x, s, lo, [](int, float, int) {});
             }
         }
@@ -276,13 +289,12 @@ __global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArg
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 acc[r][0] = acc[r][1] = f32x4{0, 0, 0, 0};
-                const int64_t p = p0 + r * 16 + i;
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     res[r][c] = u32x4{0, 0, 0, 0};
                     if (MODE == kForward && a.residual)
-                        res[r][c] = load_chunk<T>(reinterpret_cast<const T *>(a.residual) + p * a.ld_residual, q0 + q + column_of<T>(c, g, 0), a.n_q,
-                                                  p < a.n_p, a.vec_out);
+                        res[r][c] = load_chunk<T, VEC>(reinterpret_cast<const T *>(a.residual), p0 + r * 16 + i, a.n_p, a.ld_residual,
+                                                       q0 + q + column_of<T>(c, g, 0), a.n_q);
                 }
             }
 #pragma unroll
@@ -328,13 +340,13 @@ __global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArg
                 for (int c = 0; c < NC; ++c) col[c] = q0 + q + column_of<T>(c, g, 0);
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
+                {
+                    f32x4 b = {0, 0, 0, 0};
+                    if (MODE == kForward) b = *reinterpret_cast<const f32x4 *>(bias + q + column_of<T>(j, g, 0));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int c = q0 + q + column_of<T>(j, g, e);
-                        const float b = MODE == kForward && bias && c < a.n_q ? to_f(bias[c]) : 0.0f;
-                        z[NC == 1 ? 0 : j][NC == 1 ? j * 4 + e : e] = acc[r][j][e] + b;
-                    }
-                if (p < a.n_p) epilogue<T, MODE, NC>(a, p, col, z, res[r]);
+                    for (int e = 0; e < 4; ++e) z[NC == 1 ? 0 : j][NC == 1 ? j * 4 + e : e] = acc[r][j][e] + b[e];
+                }
+                if (p < a.n_p) epilogue<T, MODE, VEC, NC>(a, p, col, z, res[r]);
             }
         }
     }
@@ -384,7 +396,7 @@ __device__ __forceinline__ u32x4 read_frag(const char *tile, int c0, int ks, int
     return v;
 }
 
-template <class T, int MODE, int BP, int BQ, bool SPLIT>
+template <class T, int MODE, int BP, int BQ, bool SPLIT, bool VEC>
 __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
     constexpr bool PT = MODE == kWgrad, QT = MODE != kForward, FUSE = MODE != kForward;
     constexpr int CE = kChunk<T>, ST = kStage<T>;
@@ -430,8 +442,8 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
             place(PT, BP, k, row, chunk);
             const int64_t r = PT ? c + row : p0 + row, col = PT ? p0 + chunk * CE : c + chunk * CE;
             const int64_t rows = PT ? c_end : a.n_p, cols = PT ? a.n_p : a.n_c;
-            rp[k] = load_chunk<T>(P + r * a.ld_p, col, cols, r < rows, a.vec_p);
-            if (FUSE) rs[k] = load_saved<T>(a, r, col, cols, r < rows);
+            rp[k] = load_chunk<T, VEC>(P, r, rows, a.ld_p, col, cols);
+            if (FUSE) rs[k] = load_saved<T, VEC>(a, r, rows, col, cols);
         }
 #pragma unroll
         for (int k = 0; k < NQ; ++k) {
@@ -439,7 +451,7 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
             place(QT, BQ, k, row, chunk);
             const int64_t r = QT ? c + row : q0 + row, col = QT ? q0 + chunk * CE : c + chunk * CE;
             const int64_t rows = QT ? c_end : a.n_q, cols = QT ? a.n_q : a.n_c;
-            rq[k] = load_chunk<T>(Q + r * a.ld_q, col, cols, r < rows, a.vec_q);
+            rq[k] = load_chunk<T, VEC>(Q, r, rows, a.ld_q, col, cols);
         }
     };
     auto store = [&](char *buf) {
@@ -505,7 +517,7 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
                 const int64_t p = p0 + wp * (BP / 2) + pi * 16 + i;
                 const int q = q0 + wq * (BQ / 2) + qi * 16 + g * 4;
                 if (p >= a.n_p) continue;
-                if (a.vec_out) {
+                if (VEC) {                                  // (whole chunks of 16 bytes: n_p and n_q divide by 4)
                     if (q < a.n_q) *reinterpret_cast<f32x4 *>(part + p * a.n_q + q) = acc[pi][qi];
                 } else {
 #pragma unroll
@@ -545,11 +557,11 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
                 float z[1][CE];
                 u32x4 res[1] = {{0, 0, 0, 0}};
                 if (MODE == kForward && a.residual)
-                    res[0] = load_chunk<T>(reinterpret_cast<const T *>(a.residual) + p * a.ld_residual, col[0], a.n_q, p < a.n_p, a.vec_out);
+                    res[0] = load_chunk<T, VEC>(reinterpret_cast<const T *>(a.residual), p, a.n_p, a.ld_residual, col[0], a.n_q);
 #pragma unroll
                 for (int v = 0; v < CE; ++v)
                     z[0][v] = mine[row * W + chunk * CE + v] + (MODE == kForward && bias && col[0] + v < a.n_q ? to_f(bias[col[0] + v]) : 0.0f);
-                if (p < a.n_p && col[0] < a.n_q) epilogue<T, MODE, 1>(a, p, col, z, res);
+                if (p < a.n_p && col[0] < a.n_q) epilogue<T, MODE, VEC, 1>(a, p, col, z, res);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -597,10 +609,11 @@ int launch_tiles(DenseArgs a, int64_t splits, hipStream_t s) {
     a.tiles = (int32_t)(tiles_p * a.tiles_q);
     const int64_t steps = MODE == kWgrad ? a.split : a.n_c;
     const size_t bytes = (size_t)(BP * (SPLIT ? 2 : 1) + BQ) * kRowBytes * (steps > kStage<T> ? 2 : 1);
-    if (int rc = allow_lds(tile_kernel<T, MODE, BP, BQ, SPLIT>, bytes)) return rc;
+    const auto kernel = a.vec ? tile_kernel<T, MODE, BP, BQ, SPLIT, true> : tile_kernel<T, MODE, BP, BQ, SPLIT, false>;
+    if (int rc = allow_lds(kernel, bytes)) return rc;
     a.splits = (int32_t)splits;
     const unsigned grid = (unsigned)(ceil_div(a.tiles * splits, kNumXCD) * kNumXCD);
-    hipLaunchKernelGGL((tile_kernel<T, MODE, BP, BQ, SPLIT>), dim3(grid), dim3(kBlock), bytes, s, a);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kBlock), bytes, s, a);
     return check_launch("tile_kernel");
 }
 
@@ -618,14 +631,15 @@ int launch_resident(DenseArgs a, hipStream_t s) {
     while (block > 32 && tiles * ceil_div(a.n_q, block) < kNumCU * 4) block = block > 128 ? round_q(block / 2) : block / 2;
     a.block_q = (int32_t)block;
     const int64_t blocks_q = ceil_div(a.n_q, block);
-    const size_t bytes = (size_t)(block * C * (int64_t)sizeof(T));
-    if (int rc = allow_lds(resident_kernel<T, MODE, KS, SPLIT>, bytes)) return rc;
+    const size_t bytes = (size_t)(block * (C * (int64_t)sizeof(T) + 4));       // and the bias in 32 bits
+    const auto kernel = a.vec ? resident_kernel<T, MODE, KS, SPLIT, true> : resident_kernel<T, MODE, KS, SPLIT, false>;
+    if (int rc = allow_lds(kernel, bytes)) return rc;
     const int per_cu = bytes <= 36 * 1024 ? 4 : bytes <= 72 * 1024 ? 2 : 1, threads = resident_threads(KS) / per_cu;   // as many workgroups as weights fit
     int64_t grid = ceil_div((int64_t)kNumCU * per_cu, blocks_q);
     const int64_t need = ceil_div(tiles, threads / kWave);
     if (grid > need) grid = need;
     NFA_REQUIRE(blocks_q < 65536, "linear: too many features for one launch");
-    hipLaunchKernelGGL((resident_kernel<T, MODE, KS, SPLIT>), dim3((unsigned)grid, (unsigned)blocks_q), dim3(threads), bytes, s, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid, (unsigned)blocks_q), dim3(threads), bytes, s, a);
     return check_launch("resident_kernel");
 }
 
@@ -713,9 +727,8 @@ NFA_EXPORT int nfa_linear_fwd(const nfa_linear_args *a, void *outputs, void *sav
     d.act = a->activation;
     d.mask = keeps_bits(a->out_features, a->dtype, a->activation);
     d.ld_saved = d.mask ? a->out_features / (16 / bytes) : a->out_features;
-    d.vec_p = aligned(d.p, d.ld_p, a->in_features, bytes, 16);
-    d.vec_q = aligned(d.q, d.ld_q, a->in_features, bytes, 16);
-    d.vec_out = aligned(outputs, d.n_q, d.n_q, bytes, 16) && (!saved || d.mask || aligned(saved, d.n_q, d.n_q, bytes, 16)) &&
+    d.vec = aligned(d.p, d.ld_p, a->in_features, bytes, 16) && aligned(d.q, d.ld_q, a->in_features, bytes, 16) &&
+            aligned(outputs, d.n_q, d.n_q, bytes, 16) && (!saved || d.mask || aligned(saved, d.n_q, d.n_q, bytes, 16)) &&
                 (!a->residual || aligned(a->residual, a->residual_stride, d.n_q, bytes, 16));
     int rc = NFA_OK;
     with_dtype(a->dtype, [&](auto t) { rc = launch_rows<decltype(t), kForward, false>(d, (hipStream_t)stream); });
@@ -745,15 +758,14 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
     d.act = a->activation;
     d.mask = keeps_bits(n, a->dtype, a->activation);
     d.ld_saved = d.mask ? n / (16 / bytes) : n;
-    d.vec_p = aligned(a->grad_outputs, a->grad_outputs_stride, n, bytes, 16) &&
+    const bool vec = aligned(a->grad_outputs, a->grad_outputs_stride, n, bytes, 16) &&
               (!saved || a->activation == NFA_ACT_NONE || d.mask || aligned(saved, n, n, bytes, 16));
     int rc = NFA_OK;
     if (grad_inputs) {
         DenseArgs e = d;
         e.q = a->weight; e.ld_q = k;
-        e.vec_q = aligned(a->weight, k, k, bytes, 16);
         e.out = grad_inputs;
-        e.vec_out = aligned(grad_inputs, k, k, bytes, 16);
+        e.vec = vec && aligned(a->weight, k, k, bytes, 16) && aligned(grad_inputs, k, k, bytes, 16);
         e.n_p = a->rows; e.n_q = (int32_t)k; e.n_c = n;
         with_dtype(a->dtype, [&](auto t) {
             using T = decltype(t);
@@ -767,9 +779,8 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
         const WgradPlan w = wgrad_plan(a->rows, n, k, a->dtype, split);
         DenseArgs e = d;
         e.q = a->inputs; e.ld_q = a->inputs_stride;
-        e.vec_q = aligned(a->inputs, a->inputs_stride, k, bytes, 16);
+        e.vec = vec && aligned(a->inputs, a->inputs_stride, k, bytes, 16);
         e.partial = (float *)workspace;
-        e.vec_out = k % 4 == 0 && n % 4 == 0;
         e.n_p = n; e.n_q = (int32_t)k; e.n_c = a->rows;
         e.split = w.split;
         e.want_bias = grad_bias != nullptr;
