@@ -359,7 +359,7 @@ __global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArg
 template <class T, int COLS>
 __device__ __forceinline__ int unit_swizzle(int row) {
     if (sizeof(T) == 4) return (row >> 2) & 3;
-    if (COLS == 128) return (row & 3) | (((row >> 3) & 1) << 2);
+    if (COLS >= 128) return (row & 3) | (((row >> 3) & 1) << 2);
     return ((row >> 1) & 1) | (((row >> 3) & 1) << 1);
 }
 template <class T, bool TR, int ROWS>
@@ -396,15 +396,18 @@ __device__ __forceinline__ u32x4 read_frag(const char *tile, int c0, int ks, int
     return v;
 }
 
-template <class T, int MODE, int BP, int BQ, bool SPLIT, bool VEC>
-__global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
+// WP x WQ waves, each with BP / WP x BQ / WQ of the tile
+template <class T, int MODE, int BP, int BQ, int WP, int WQ, bool SPLIT, bool VEC>
+__global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
+    constexpr int TH = WP * WQ * kWave;
     constexpr bool PT = MODE == kWgrad, QT = MODE != kForward, FUSE = MODE != kForward;
     constexpr int CE = kChunk<T>, ST = kStage<T>;
-    constexpr int NP = BP / 32, NQ = BQ / 32;               // chunks a thread stages per tile = 16-wide fragments per wave
+    constexpr int CP = BP * 8 / TH, CQ = BQ * 8 / TH;       // chunks a thread stages per tile
+    constexpr int NP = BP / WP / 16, NQ = BQ / WQ / 16;     // sixteen-wide fragments of a wave
     constexpr int kP = BP * kRowBytes, kBuf = kP * (SPLIT ? 2 : 1) + BQ * kRowBytes;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
-    const int wp = wave >> 1, wq = wave & 1;
+    const int wp = wave / WQ, wq = wave % WQ;
 
     // tile (and, for wgrad, stretch of rows) of this workgroup: eight runs of them, one per XCD (workgroups are dealt to the XCDs in
     // turn), so that the tiles that read the same rows share an L2
@@ -419,7 +422,7 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
     const int64_t c_end = MODE == kWgrad ? (c_begin + a.split < a.n_c ? c_begin + a.split : a.n_c) : a.n_c;
 
     const T *P = reinterpret_cast<const T *>(a.p), *Q = reinterpret_cast<const T *>(a.q);
-    u32x4 rp[NP], rs[NP], rq[NQ];
+    u32x4 rp[CP], rs[CP], rq[CQ];
     f32x4 acc[NP][NQ];
 #pragma unroll
     for (int i = 0; i < NP; ++i)
@@ -433,11 +436,11 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
     auto place = [&](bool tr, int rows, int k, int &row, int &chunk) {
         const int per_row = tr ? rows / CE : 8;
         chunk = tid % per_row;
-        row = tid / per_row + k * (kBlock / per_row);
+        row = tid / per_row + k * (TH / per_row);
     };
     auto load = [&](int64_t c) {
 #pragma unroll
-        for (int k = 0; k < NP; ++k) {
+        for (int k = 0; k < CP; ++k) {
             int row, chunk;
             place(PT, BP, k, row, chunk);
             const int64_t r = PT ? c + row : p0 + row, col = PT ? p0 + chunk * CE : c + chunk * CE;
@@ -446,7 +449,7 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
             if (FUSE) rs[k] = load_saved<T, VEC>(a, r, rows, col, cols);
         }
 #pragma unroll
-        for (int k = 0; k < NQ; ++k) {
+        for (int k = 0; k < CQ; ++k) {
             int row, chunk;
             place(QT, BQ, k, row, chunk);
             const int64_t r = QT ? c + row : q0 + row, col = QT ? q0 + chunk * CE : c + chunk * CE;
@@ -455,20 +458,20 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
         }
     };
     auto store = [&](char *buf) {
-        u32x4 lo[SPLIT ? NP : 1];
+        u32x4 lo[SPLIT ? CP : 1];
         if constexpr (FUSE)
-            form_dz<T, SPLIT, NP>(a, rp, rs, lo, [&](int, float dz, int e) {
+            form_dz<T, SPLIT, CP>(a, rp, rs, lo, [&](int, float dz, int e) {
                 if constexpr (MODE == kWgrad) db[e] += dz;
             });
 #pragma unroll
-        for (int k = 0; k < NP; ++k) {
+        for (int k = 0; k < CP; ++k) {
             int row, chunk;
             place(PT, BP, k, row, chunk);
             *reinterpret_cast<u32x4 *>(buf + stage_offset<T, PT, BP>(row, chunk)) = rp[k];
             if constexpr (SPLIT) *reinterpret_cast<u32x4 *>(buf + kP + stage_offset<T, PT, BP>(row, chunk)) = lo[k];
         }
 #pragma unroll
-        for (int k = 0; k < NQ; ++k) {
+        for (int k = 0; k < CQ; ++k) {
             int row, chunk;
             place(QT, BQ, k, row, chunk);
             *reinterpret_cast<u32x4 *>(buf + kBuf - BQ * kRowBytes + stage_offset<T, QT, BQ>(row, chunk)) = rq[k];
@@ -480,11 +483,11 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
             if (c + ks * (ST / 2) >= c_end) break;          // a half that holds only zeros
             u32x4 fp[NP], fq[NQ];
 #pragma unroll
-            for (int j = 0; j < NQ; ++j) fq[j] = read_frag<T, QT, BQ>(buf + kBuf - BQ * kRowBytes, wq * (BQ / 2) + j * 16, ks, lane);
+            for (int j = 0; j < NQ; ++j) fq[j] = read_frag<T, QT, BQ>(buf + kBuf - BQ * kRowBytes, wq * (BQ / WQ) + j * 16, ks, lane);
 #pragma unroll
             for (int half = 0; half < (SPLIT ? 2 : 1); ++half) {
 #pragma unroll
-                for (int i = 0; i < NP; ++i) fp[i] = read_frag<T, PT, BP>(buf + half * kP, wp * (BP / 2) + i * 16, ks, lane);
+                for (int i = 0; i < NP; ++i) fp[i] = read_frag<T, PT, BP>(buf + half * kP, wp * (BP / WP) + i * 16, ks, lane);
 #pragma unroll
                 for (int i = 0; i < NP; ++i)
 #pragma unroll
@@ -514,8 +517,8 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
         for (int pi = 0; pi < NP; ++pi)
 #pragma unroll
             for (int qi = 0; qi < NQ; ++qi) {
-                const int64_t p = p0 + wp * (BP / 2) + pi * 16 + i;
-                const int q = q0 + wq * (BQ / 2) + qi * 16 + g * 4;
+                const int64_t p = p0 + wp * (BP / WP) + pi * 16 + i;
+                const int q = q0 + wq * (BQ / WQ) + qi * 16 + g * 4;
                 if (p >= a.n_p) continue;
                 if (VEC) {                                  // (whole chunks of 16 bytes: n_p and n_q divide by 4)
                     if (q < a.n_q) *reinterpret_cast<f32x4 *>(part + p * a.n_q + q) = acc[pi][qi];
@@ -526,7 +529,7 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
                 }
             }
         if (q0 == 0 && a.want_bias) {                       // db: the threads that staged the same columns, in order
-            constexpr int per_row = BP / CE, n = kBlock / per_row;
+            constexpr int per_row = BP / CE, n = TH / per_row;
             float *sum = reinterpret_cast<float *>(lds);
 #pragma unroll
             for (int e = 0; e < CE; ++e) sum[(tid / per_row) * BP + (tid % per_row) * CE + e] = db[e];
@@ -538,9 +541,9 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
             }
         }
     } else {
-        // through LDS, so that a thread holds whole chunks of a row: 32 rows of each wave's half at a time
+        // through LDS, so that a thread holds whole chunks of a row: sixteen rows of each wave at a time
         const T *bias = reinterpret_cast<const T *>(a.bias);
-        constexpr int W = BQ / 2 + 4;                       // floats in a row: the half's columns, shifted by a bank group per row
+        constexpr int W = BQ / WQ + 4;                      // floats in a row: the wave's columns, shifted by a bank group per row
         float *mine = reinterpret_cast<float *>(lds) + wave * 16 * W;
 #pragma unroll
         for (int pi = 0; pi < NP; ++pi) {
@@ -548,12 +551,12 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(DenseArgs a) {
             for (int qi = 0; qi < NQ; ++qi) *reinterpret_cast<f32x4 *>(mine + i * W + qi * 16 + g * 4) = acc[pi][qi];
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            constexpr int per_row = BQ / 2 / CE;            // chunks of a row in this half
+            constexpr int per_row = BQ / WQ / CE;           // chunks of a row
 #pragma unroll
             for (int k = 0; k < 16 * per_row / kWave; ++k) {
                 const int e = k * kWave + lane, row = e / per_row, chunk = e % per_row;
-                const int64_t p = p0 + wp * (BP / 2) + pi * 16 + row;
-                const int col[1] = {q0 + wq * (BQ / 2) + chunk * CE};
+                const int64_t p = p0 + wp * (BP / WP) + pi * 16 + row;
+                const int col[1] = {q0 + wq * (BQ / WQ) + chunk * CE};
                 float z[1][CE];
                 u32x4 res[1] = {{0, 0, 0, 0}};
                 if (MODE == kForward && a.residual)
@@ -601,7 +604,7 @@ int allow_lds(K kernel, size_t bytes) {
     return e == hipSuccess ? NFA_OK : fail(NFA_ERR_LAUNCH, "linear: %zu bytes of LDS: %s", bytes, hipGetErrorString(e));
 }
 
-template <class T, int MODE, int BP, int BQ, bool SPLIT>
+template <class T, int MODE, int BP, int BQ, int WP, int WQ, bool SPLIT>
 int launch_tiles(DenseArgs a, int64_t splits, hipStream_t s) {
     const int64_t tiles_p = ceil_div(a.n_p, BP);
     a.tiles_q = (int32_t)ceil_div(a.n_q, BQ);
@@ -609,11 +612,11 @@ int launch_tiles(DenseArgs a, int64_t splits, hipStream_t s) {
     a.tiles = (int32_t)(tiles_p * a.tiles_q);
     const int64_t steps = MODE == kWgrad ? a.split : a.n_c;
     const size_t bytes = (size_t)(BP * (SPLIT ? 2 : 1) + BQ) * kRowBytes * (steps > kStage<T> ? 2 : 1);
-    const auto kernel = a.vec ? tile_kernel<T, MODE, BP, BQ, SPLIT, true> : tile_kernel<T, MODE, BP, BQ, SPLIT, false>;
+    const auto kernel = a.vec ? tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, true> : tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, false>;
     if (int rc = allow_lds(kernel, bytes)) return rc;
     a.splits = (int32_t)splits;
     const unsigned grid = (unsigned)(ceil_div(a.tiles * splits, kNumXCD) * kNumXCD);
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kBlock), bytes, s, a);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(WP * WQ * kWave), bytes, s, a);
     return check_launch("tile_kernel");
 }
 
@@ -653,8 +656,12 @@ int launch_rows(const DenseArgs &a, hipStream_t s) {
     if (a.n_c <= 8 * step) return launch_resident<T, MODE, 8, SPLIT>(a, s);
     if constexpr (sizeof(T) == 4)
         if (a.n_c <= 16 * step) return launch_resident<T, MODE, 16, SPLIT>(a, s);
+    // 16-bit types, aligned and large enough for every CU: 256 x 256 by eight waves, whose fragments are used often enough that the matrix
+    // units and not LDS set the pace
     constexpr int BP = SPLIT ? 64 : 128;
-    return a.n_q <= 64 ? launch_tiles<T, MODE, BP, 64, SPLIT>(a, 1, s) : launch_tiles<T, MODE, BP, 128, SPLIT>(a, 1, s);
+    if constexpr (sizeof(T) == 2 && !SPLIT)
+        if (a.vec && a.n_q > 128 && ceil_div(a.n_p, 256) * ceil_div(a.n_q, 256) >= kNumCU) return launch_tiles<T, MODE, 256, 256, 2, 4, SPLIT>(a, 1, s);
+    return a.n_q <= 64 ? launch_tiles<T, MODE, BP, 64, 2, 2, SPLIT>(a, 1, s) : launch_tiles<T, MODE, BP, 128, 2, 2, SPLIT>(a, 1, s);
 }
 
 // rows of the long axis that one workgroup of the weight gradient sums: enough workgroups for every CU twice, and not so many that
@@ -788,11 +795,11 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
             using T = decltype(t);
             if constexpr (sizeof(T) == 2)
                 if (split) {
-                    rc = w.bq == 64 ? launch_tiles<T, kWgrad, 64, 64, true>(e, w.splits, s) : launch_tiles<T, kWgrad, 64, 128, true>(e, w.splits, s);
+                    rc = w.bq == 64 ? launch_tiles<T, kWgrad, 64, 64, 2, 2, true>(e, w.splits, s) : launch_tiles<T, kWgrad, 64, 128, 2, 2, true>(e, w.splits, s);
                     return;
                 }
-            if (w.bp == 64) rc = w.bq == 64 ? launch_tiles<T, kWgrad, 64, 64, false>(e, w.splits, s) : launch_tiles<T, kWgrad, 64, 128, false>(e, w.splits, s);
-            else rc = w.bq == 64 ? launch_tiles<T, kWgrad, 128, 64, false>(e, w.splits, s) : launch_tiles<T, kWgrad, 128, 128, false>(e, w.splits, s);
+            if (w.bp == 64) rc = w.bq == 64 ? launch_tiles<T, kWgrad, 64, 64, 2, 2, false>(e, w.splits, s) : launch_tiles<T, kWgrad, 64, 128, 2, 2, false>(e, w.splits, s);
+            else rc = w.bq == 64 ? launch_tiles<T, kWgrad, 128, 64, 2, 2, false>(e, w.splits, s) : launch_tiles<T, kWgrad, 128, 128, 2, 2, false>(e, w.splits, s);
         });
         if (rc) return rc;
         const int64_t ld = n * k + n;
