@@ -15,6 +15,8 @@
 // in registers (resident_kernel).  Longer contractions and wgrad go tile by tile through LDS (tile_kernel).
 #include "feature.hpp"
 
+#include <algorithm>
+
 namespace nfa {
 namespace {
 
@@ -175,19 +177,19 @@ __device__ __forceinline__ void store_chunk(T *row, int q, int n_q, u32x4 v) {
 }
 // the epilogue of N chunks of row p (columns q[k] ..): acc in, outputs and the saved numbers out
 template <class T, int MODE, bool VEC, int N>
-__device__ __forceinline__ void epilogue(const DenseArgs &a, int64_t p, const int (&q)[N], float (&z)[N][kChunk<T>], const u32x4 (&res)[N]) {
+__device__ __forceinline__ void epilogue(const DenseArgs &a, int64_t p, const int (&q)[N], int n_q, float (&z)[N][kChunk<T>], const u32x4 (&res)[N]) {
     u32x4 y[N], kept[N];
     T *out = reinterpret_cast<T *>(a.out) + p * a.n_q;
     if constexpr (MODE == kForward) {
         finish_chunks<T, N>(a, z, res, y, kept);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            store_chunk<T, VEC>(out, q[k], a.n_q, y[k]);
+            store_chunk<T, VEC>(out, q[k], n_q, y[k]);
             if (!a.saved_out) continue;
             if (a.mask) {
-                if (q[k] < a.n_q) reinterpret_cast<uint8_t *>(a.saved_out)[p * a.ld_saved + q[k] / kChunk<T>] = (uint8_t)kept[k][0];
+                if (q[k] < n_q) reinterpret_cast<uint8_t *>(a.saved_out)[p * a.ld_saved + q[k] / kChunk<T>] = (uint8_t)kept[k][0];
             } else {
-                store_chunk<T, VEC>(reinterpret_cast<T *>(a.saved_out) + p * a.n_q, q[k], a.n_q, kept[k]);
+                store_chunk<T, VEC>(reinterpret_cast<T *>(a.saved_out) + p * a.n_q, q[k], n_q, kept[k]);
             }
         }
     } else {
@@ -196,7 +198,7 @@ __device__ __forceinline__ void epilogue(const DenseArgs &a, int64_t p, const in
             Frag<T> o;
 #pragma unroll
             for (int i = 0; i < kChunk<T>; ++i) o.v[i] = from_f<T>(z[k][i]);
-            store_chunk<T, VEC>(out, q[k], a.n_q, __builtin_bit_cast(u32x4, o));
+            store_chunk<T, VEC>(out, q[k], n_q, __builtin_bit_cast(u32x4, o));
         }
     }
 }
@@ -225,12 +227,15 @@ __device__ __forceinline__ int weight_offset_t(int row, int chunk, int pitch) { 
     return (row * pitch + (chunk ^ (pitch >= 16 ? ((row >> 2) & 3) << 2 : pitch == 8 ? ((row >> 2) & 1) << 2 : 0))) * 16;
 }
 
-// waves on a CU: sixteen while a wave's rows leave room in the registers, eight beyond (its loads in flight are twice as many then)
-constexpr int resident_threads(int ks) { return ks <= 2 ? 1024 : 512; }
+// waves of a CU: sixteen for short rows, eight for long ones (each with twice the loads in flight)
+constexpr int resident_waves(int ks) { return ks <= 2 ? 16 : 8; }
 template <class T, int MODE, int KS, bool SPLIT, bool VEC>
-__global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArgs a) {
+__global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
     constexpr int CE = kChunk<T>, RT = SPLIT || KS == 16 ? 1 : 2;       // rows of a wave: RT fragments of sixteen
     constexpr int NC = sizeof(T) == 2 ? 1 : 2;                          // chunks of a lane in a group of 32 columns
+    // groups of 32 columns at a time: two for long rows (whole 128-byte lines in a store, twice the independent products: 130 -> 106 us at
+    // 2^18 x 256 x 256 bf16), one for short ones (31 against 41 us at 100003 x 63 x 65 fp16, where the second is mostly empty)
+    constexpr int NG = KS >= 4 ? 2 : 1;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = lane_id(), i = lane & 15, g = lane >> 4;
     const int q0 = blockIdx.y * a.block_q, nq = a.n_q - q0 < a.block_q ? a.n_q - q0 : a.block_q;
@@ -276,6 +281,21 @@ __global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArg
         if constexpr (MODE == kDgrad) {
             if (a.act != NFA_ACT_NONE) {
                 u32x4 s[RT * KS];
+                if (KS >= 4 && a.mask && whole && a.ld_saved % 16 == 0 && (uintptr_t)a.saved % 16 == 0) {
+                    // relu's bits, four steps of the contraction in one access: word k of a row, byte g
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        const int64_t p = p0 + r * 16 + i;
+                        const u32x4 *row = reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint8_t *>(a.saved) + (p < a.n_p ? p : a.n_p - 1) * a.ld_saved);
+#pragma unroll
+                        for (int k = 0; k < KS; k += 4) {
+                            const u32x4 b = row[k / 4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (k + e < KS) s[r * KS + k + e] = u32x4{b[e] >> (8 * g), 0, 0, 0};
+                        }
+                    }
+                } else
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -283,33 +303,45 @@ __global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArg
                 form_dz<T, SPLIT, RT * KS>(a, x, s, lo, [](int, float, int) {});
             }
         }
-        for (int q = 0; q < nq; q += 32) {
-            f32x4 acc[RT][2];
-            u32x4 res[RT][NC];
+        u32x4 ahead[MODE == kForward ? RT * NC * NG : 1];
+        auto load_residual = [&](int q) {                   // of the columns q .. q + 32 NG - 1
+            if constexpr (MODE == kForward) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int c = 0; c < NC * NG; ++c)
+                        ahead[r * NC * NG + c] = load_chunk<T, VEC>(reinterpret_cast<const T *>(a.residual), p0 + r * 16 + i, a.n_p, a.ld_residual,
+                                                                   q0 + q + (c / NC) * 32 + column_of<T>(c % NC, g, 0), a.n_q);
+            }
+        };
+        if (MODE == kForward && a.residual) load_residual(0);
+        for (int q = 0; q < nq; q += 32 * NG) {
+            f32x4 acc[RT][2 * NG];
+            u32x4 res[RT * NC * NG];
+            const bool both = q + 32 < nq;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                acc[r][0] = acc[r][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    res[r][c] = u32x4{0, 0, 0, 0};
-                    if (MODE == kForward && a.residual)
-                        res[r][c] = load_chunk<T, VEC>(reinterpret_cast<const T *>(a.residual), p0 + r * 16 + i, a.n_p, a.ld_residual,
-                                                       q0 + q + column_of<T>(c, g, 0), a.n_q);
-                }
+                for (int j = 0; j < 2 * NG; ++j) acc[r][j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < NC * NG; ++c) res[r * NC * NG + c] = MODE == kForward && a.residual ? ahead[r * NC * NG + c] : u32x4{0, 0, 0, 0};
             }
+            if (MODE == kForward && a.residual && q + 32 * NG < nq) load_residual(q + 32 * NG);
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 if (k * 4 * CE >= a.n_c) continue;
-                u32x4 w[2];
+                u32x4 w[2 * NG];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < 2 * NG; ++j) {
+                    if (j >= 2 && !both) continue;
+                    const int qj = q + (j >> 1) * 32;
                     if constexpr (MODE == kForward) {
-                        w[j] = *reinterpret_cast<const u32x4 *>(lds + weight_offset<T, KS>(q + j * 16 + i, k * 4 + g));
+                        w[j] = *reinterpret_cast<const u32x4 *>(lds + weight_offset<T, KS>(qj + (j & 1) * 16 + i, k * 4 + g));
                     } else if constexpr (sizeof(T) == 2) {
                         s16x4 h[2];
 #pragma unroll
                         for (int s = 0; s < 2; ++s) {
-                            const int n = k * 32 + g * 8 + s * 4 + (i >> 2), c = q + (i & 3) * 8 + j * 4;
+                            const int n = k * 32 + g * 8 + s * 4 + (i >> 2), c = qj + (i & 3) * 8 + (j & 1) * 4;
                             h[s] = read_transposed(lds + weight_offset_t<T>(n, c >> 3, pitch) + (c & 7) * 2);
                         }
                         w[j] = __builtin_bit_cast(u32x4, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -317,7 +349,7 @@ __global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArg
                         f32x4 e;
 #pragma unroll
                         for (int s = 0; s < 4; ++s) {
-                            const int n = k * 16 + g * 4 + s, c = q + j * 16 + i;
+                            const int n = k * 16 + g * 4 + s, c = qj + (j & 1) * 16 + i;
                             e[s] = *reinterpret_cast<const float *>(lds + weight_offset_t<T>(n, c >> 2, pitch) + (c & 3) * 4);
                         }
                         w[j] = __builtin_bit_cast(u32x4, e);
@@ -326,7 +358,8 @@ __global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArg
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
+                    for (int j = 0; j < 2 * NG; ++j) {
+                        if (j >= 2 && !both) continue;
                         acc[r][j] = multiply<T>(w[j], x[r * KS + k], acc[r][j]);
                         if constexpr (SPLIT) acc[r][j] = multiply<T>(w[j], lo[r * KS + k], acc[r][j]);
                     }
@@ -334,19 +367,22 @@ __global__ __launch_bounds__(resident_threads(KS)) void resident_kernel(DenseArg
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 const int64_t p = p0 + r * 16 + i;
-                float z[NC][CE];
-                int col[NC];
+                float z[NC * NG][CE];
+                int col[NC * NG];
+                u32x4 add[NC * NG];
 #pragma unroll
-                for (int c = 0; c < NC; ++c) col[c] = q0 + q + column_of<T>(c, g, 0);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                {
-                    f32x4 b = {0, 0, 0, 0};
-                    if (MODE == kForward) b = *reinterpret_cast<const f32x4 *>(bias + q + column_of<T>(j, g, 0));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) z[NC == 1 ? 0 : j][NC == 1 ? j * 4 + e : e] = acc[r][j][e] + b[e];
+                for (int c = 0; c < NC * NG; ++c) {
+                    col[c] = q0 + q + (c / NC) * 32 + column_of<T>(c % NC, g, 0);
+                    add[c] = res[r * NC * NG + c];
                 }
-                if (p < a.n_p) epilogue<T, MODE, VEC, NC>(a, p, col, z, res[r]);
+#pragma unroll
+                for (int j = 0; j < 2 * NG; ++j) {
+                    f32x4 b = {0, 0, 0, 0};
+                    if (MODE == kForward && (j < 2 || both)) b = *reinterpret_cast<const f32x4 *>(bias + q + (j >> 1) * 32 + column_of<T>(j & 1, g, 0));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[NC == 1 ? j >> 1 : j][NC == 1 ? (j & 1) * 4 + e : e] = acc[r][j][e] + b[e];
+                }
+                if (p < a.n_p) epilogue<T, MODE, VEC, NC * NG>(a, p, col, q0 + nq, z, add);
             }
         }
     }
@@ -545,10 +581,14 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
         const T *bias = reinterpret_cast<const T *>(a.bias);
         constexpr int W = BQ / WQ + 4;                      // floats in a row: the wave's columns, shifted by a bank group per row
         float *mine = reinterpret_cast<float *>(lds) + wave * 16 * W;
+#pragma unroll 1
+        for (int pi = 0; pi < NP; ++pi) {                   // (one body for all fragments: unrolled it would not fit the instruction cache)
 #pragma unroll
-        for (int pi = 0; pi < NP; ++pi) {
+            for (int t = 0; t < NP; ++t) {
+                if (t != pi) continue;
 #pragma unroll
-            for (int qi = 0; qi < NQ; ++qi) *reinterpret_cast<f32x4 *>(mine + i * W + qi * 16 + g * 4) = acc[pi][qi];
+                for (int qi = 0; qi < NQ; ++qi) *reinterpret_cast<f32x4 *>(mine + i * W + qi * 16 + g * 4) = acc[t][qi];
+            }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             constexpr int per_row = BQ / WQ / CE;           // chunks of a row
@@ -564,7 +604,7 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
 #pragma unroll
                 for (int v = 0; v < CE; ++v)
                     z[0][v] = mine[row * W + chunk * CE + v] + (MODE == kForward && bias && col[0] + v < a.n_q ? to_f(bias[col[0] + v]) : 0.0f);
-                if (p < a.n_p && col[0] < a.n_q) epilogue<T, MODE, VEC, 1>(a, p, col, z, res);
+                if (p < a.n_p && col[0] < a.n_q) epilogue<T, MODE, VEC, 1>(a, p, col, a.n_q, z, res);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -637,7 +677,7 @@ int launch_resident(DenseArgs a, hipStream_t s) {
     const size_t bytes = (size_t)(block * (C * (int64_t)sizeof(T) + 4));       // and the bias in 32 bits
     const auto kernel = a.vec ? resident_kernel<T, MODE, KS, SPLIT, true> : resident_kernel<T, MODE, KS, SPLIT, false>;
     if (int rc = allow_lds(kernel, bytes)) return rc;
-    const int per_cu = bytes <= 36 * 1024 ? 4 : bytes <= 72 * 1024 ? 2 : 1, threads = resident_threads(KS) / per_cu;   // as many workgroups as weights fit
+    const int per_cu = bytes <= 36 * 1024 ? 4 : bytes <= 72 * 1024 ? 2 : 1, threads = std::min(512, resident_waves(KS) * kWave / per_cu);
     int64_t grid = ceil_div((int64_t)kNumCU * per_cu, blocks_q);
     const int64_t need = ceil_div(tiles, threads / kWave);
     if (grid > need) grid = need;
@@ -671,9 +711,9 @@ WgradPlan wgrad_plan(int64_t rows, int64_t n, int64_t k, int32_t dtype, bool two
     const int64_t stage = dtype == NFA_DTYPE_F32 ? 32 : 64;
     WgradPlan w;
     w.bp = n <= 64 || two_parts ? 64 : 128;
-    w.bq = k <= 64 ? 64 : 128;
+    w.bq = k <= 64 ? 64 : k <= 128 || two_parts || w.bp == 64 ? 128 : 256;
     const int64_t tiles = ceil_div(n, w.bp) * ceil_div(k, w.bq);
-    int64_t splits = ceil_div(2 * kNumCU, tiles);
+    int64_t splits = ceil_div((w.bq == 256 ? 1 : 2) * kNumCU, tiles);
     const int64_t most = ceil_div(rows, 4 * stage);
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
@@ -799,7 +839,8 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
                     return;
                 }
             if (w.bp == 64) rc = w.bq == 64 ? launch_tiles<T, kWgrad, 64, 64, 2, 2, false>(e, w.splits, s) : launch_tiles<T, kWgrad, 64, 128, 2, 2, false>(e, w.splits, s);
-            else rc = w.bq == 64 ? launch_tiles<T, kWgrad, 128, 64, 2, 2, false>(e, w.splits, s) : launch_tiles<T, kWgrad, 128, 128, 2, 2, false>(e, w.splits, s);
+            else if (w.bq == 64) rc = launch_tiles<T, kWgrad, 128, 64, 2, 2, false>(e, w.splits, s);
+            else rc = w.bq == 128 ? launch_tiles<T, kWgrad, 128, 128, 2, 2, false>(e, w.splits, s) : launch_tiles<T, kWgrad, 128, 256, 2, 4, false>(e, w.splits, s);
         });
         if (rc) return rc;
         const int64_t ld = n * k + n;
