@@ -505,9 +505,8 @@ NFA_EXPORT int nfa_causal_conv_bwd(const nfa_causal_conv_args *a, void *grad_inp
             hipLaunchKernelGGL((conv_bwd_kernel<T, w(), vc()>), dim3((unsigned)p.blocks_x, (unsigned)p.blocks_y), dim3(kBlock), lds, s, d);
         });
         if (int rc = check_launch("conv_bwd_kernel")) return rc;
-        const int64_t ld = (int64_t)a->channels * (a->width + 1);
-        if (grad_weight) launch_reduce_rows(d.partial, p.blocks_x, (int64_t)a->channels * a->width, ld, grad_weight, a->dtype, s);
-        if (grad_bias) launch_reduce_rows(d.partial + (int64_t)a->channels * a->width, p.blocks_x, a->channels, ld, grad_bias, a->dtype, s);
+        if (grad_weight || grad_bias)
+            launch_reduce_rows(d.partial, p.blocks_x, {{grad_weight, (int64_t)a->channels * a->width}, {grad_bias, a->channels}}, a->dtype, s);
         if (int rc = check_launch("reduce_rows_kernel")) return rc;
     }
     if (grad_initial_state && a->n_rays > 0) {

@@ -611,25 +611,31 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
     }
 }
 
-// columns by lane, sixteen rows side by side; a column's sum is formed in the same order every time
+// columns by lane, sixteen rows side by side; a column's sum is formed in the same order every time.  The columns go to up to three
+// outputs, one behind the other (nullptr: not wanted)
+struct Outputs { void *to[3]; int64_t cols[3]; };
 template <class T>
-__global__ __launch_bounds__(1024) void reduce_rows_kernel(const float *__restrict__ part, int64_t rows, int64_t cols, int64_t ld,
-                                                           T *__restrict__ out) {
+__global__ __launch_bounds__(1024) void reduce_rows_kernel(const float *__restrict__ part, int64_t rows, int64_t ld, Outputs o) {
     __shared__ float sum[16][64];
     const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
     const int64_t c = (int64_t)blockIdx.x * 64 + lane;
     float v = 0.0f;
-    if (c < cols) {
+    if (c < ld) {
 #pragma unroll 8
         for (int64_t r = grp; r < rows; r += 16) v += part[r * ld + c];
     }
     sum[grp][lane] = v;
     __syncthreads();
-    if (grp == 0 && c < cols) {
+    if (grp == 0 && c < ld) {
         float t = 0.0f;
 #pragma unroll
         for (int k = 0; k < 16; ++k) t += sum[k][lane];
-        out[c] = from_f<T>(t);
+        int64_t at = c;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            if (at >= 0 && at < o.cols[k] && o.to[k]) reinterpret_cast<T *>(o.to[k])[at] = from_f<T>(t);
+            at -= o.cols[k];
+        }
     }
 }
 
@@ -713,7 +719,8 @@ WgradPlan wgrad_plan(int64_t rows, int64_t n, int64_t k, int32_t dtype, bool two
     w.bp = n <= 64 || two_parts ? 64 : 128;
     w.bq = k <= 64 ? 64 : k <= 128 || two_parts || w.bp == 64 ? 128 : 256;
     const int64_t tiles = ceil_div(n, w.bp) * ceil_div(k, w.bq);
-    int64_t splits = ceil_div((w.bq == 256 ? 1 : 2) * kNumCU, tiles);
+    const int64_t per_cu = w.bq == 256 ? 1 : std::max<int64_t>(2, 256 / w.bp + 256 / w.bq - 4);      // 4 of 64 x 64, 2 of 128 x 128
+    int64_t splits = ceil_div(per_cu * kNumCU, tiles);
     const int64_t most = ceil_div(rows, 4 * stage);
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
@@ -729,10 +736,16 @@ bool two_parts(int32_t dtype, int32_t act) { return dtype != NFA_DTYPE_F32 && ac
 
 }  // namespace
 
-void launch_reduce_rows(const float *part, int64_t rows, int64_t cols, int64_t ld, void *out, int32_t dtype, hipStream_t s) {
+void launch_reduce_rows(const float *part, int64_t rows, std::initializer_list<std::pair<void *, int64_t>> outputs, int32_t dtype, hipStream_t s) {
+    Outputs o{};
+    int64_t cols = 0, k = 0;
+    for (auto &p : outputs) {
+        o.to[k] = p.first;
+        o.cols[k++] = p.second;
+        cols += p.second;
+    }
     with_dtype(dtype, [&](auto t) {
-        using T = decltype(t);
-        hipLaunchKernelGGL((reduce_rows_kernel<T>), dim3((unsigned)ceil_div(cols, 64)), dim3(1024), 0, s, part, rows, cols, ld, (T *)out);
+        hipLaunchKernelGGL((reduce_rows_kernel<decltype(t)>), dim3((unsigned)ceil_div(cols, 64)), dim3(1024), 0, s, part, rows, cols, o);
     });
 }
 
@@ -843,9 +856,7 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
             else rc = w.bq == 128 ? launch_tiles<T, kWgrad, 128, 128, 2, 2, false>(e, w.splits, s) : launch_tiles<T, kWgrad, 128, 256, 2, 4, false>(e, w.splits, s);
         });
         if (rc) return rc;
-        const int64_t ld = n * k + n;
-        if (grad_weight) launch_reduce_rows(e.partial, w.splits, n * k, ld, grad_weight, a->dtype, s);
-        if (grad_bias) launch_reduce_rows(e.partial + n * k, w.splits, n, ld, grad_bias, a->dtype, s);
+        launch_reduce_rows(e.partial, w.splits, {{grad_weight, n * k}, {grad_bias, n}}, a->dtype, s);
         return check_launch("reduce_rows_kernel");
     }
     return NFA_OK;

@@ -790,10 +790,7 @@ NFA_EXPORT int nfa_selective_scan_bwd(const nfa_selective_scan_args *a, const fl
         hipLaunchKernelGGL((scan_bwd_kernel<T, ns(), pp()>), dim3((unsigned)main_grid), dim3(kBlock), 0, s, d);
         hipLaunchKernelGGL((scan_join_bc_kernel<T>), dim3(blocks_for(a->rows * 2 * a->states)), dim3(kBlock), 0, s, d, (int)(ns() * pp()), (T *)g->B, (T *)g->C);
     });
-    const int64_t per = (int64_t)a->channels * (a->states + 2), n = (int64_t)a->channels * a->states;
-    launch_reduce_rows(d.part_w, p.workers, n, per, g->A, NFA_DTYPE_F32, s);
-    if (g->D) launch_reduce_rows(d.part_w + n, p.workers, a->channels, per, g->D, NFA_DTYPE_F32, s);
-    if (g->delta_bias) launch_reduce_rows(d.part_w + n + a->channels, p.workers, a->channels, per, g->delta_bias, NFA_DTYPE_F32, s);
+    launch_reduce_rows(d.part_w, p.workers, {{g->A, (int64_t)a->channels * a->states}, {g->D, a->channels}, {g->delta_bias, a->channels}}, NFA_DTYPE_F32, s);
     return check_launch("scan_bwd_kernel");
 }
 
