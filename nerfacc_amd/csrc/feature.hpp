@@ -42,8 +42,7 @@ __device__ __forceinline__ float sigmoid_f(float x) {
 // log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1], with log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, as its odd
 // series: every term is positive, so small steps (x around -7 in a scan) keep their relative accuracy, which log(1 + e) would not.
 // The series is cut after s^15 / 15: the rest is below 3^-16 / 17 = 1.4e-9 of the first term.
-__device__ __forceinline__ float softplus_f(float x) {
-    const float e = fast_exp2(-fabsf(x) * kLog2e);
+__device__ __forceinline__ float softplus_from(float x, float e) {         // e = exp(-|x|)
     const float s = e * fast_rcp(2.0f + e), q = s * s;
     float p = 1.0f / 15.0f;
     p = fmaf(p, q, 1.0f / 13.0f);
@@ -55,6 +54,7 @@ __device__ __forceinline__ float softplus_f(float x) {
     p = fmaf(p, q, 1.0f);
     return x != x ? x : fmaxf(x, 0.0f) + 2.0f * s * p;
 }
+__device__ __forceinline__ float softplus_f(float x) { return softplus_from(x, fast_exp2(-fabsf(x) * kLog2e)); }
 
 constexpr float kInvSqrt2 = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f;
 

@@ -52,8 +52,8 @@ __device__ __forceinline__ void sequence_rows(const ScanArgs &a, int64_t ray, in
     if (count > a.rows - start) count = a.rows - start;
 }
 // chunk k >= 1 of a sequence begins `chunk` rows behind the one before it, so no two of them begin in the same block of `chunk` rows
-__device__ __forceinline__ int64_t chunk_slot(const ScanArgs &a, int64_t ray, int64_t start, int64_t k) {
-    return k == 0 ? a.slots - a.n_rays + ray : (start + k * a.chunk) / a.chunk;
+__device__ __forceinline__ int64_t chunk_slot(const ScanArgs &a, int64_t ray, int64_t first, int64_t k) {       // first: start / chunk
+    return k == 0 ? a.slots - a.n_rays + ray : first + k;
 }
 
 __device__ __forceinline__ Task find_task(const ScanArgs &a, int64_t id, int lane) {
@@ -87,7 +87,7 @@ __device__ __forceinline__ Task find_task(const ScanArgs &a, int64_t id, int lan
     t.n = t.count - t.first;
     if (a.chunk && t.n > a.chunk) t.n = a.chunk;
     if (t.n < 0) t.n = 0;
-    t.slot = a.chunk ? chunk_slot(a, t.ray, t.start, k) : 0;
+    t.slot = a.chunk ? chunk_slot(a, t.ray, t.start / a.chunk, k) : 0;
     if (k > 0 && t.n == 0) t.live = false;
     return t;
 }
@@ -158,34 +158,33 @@ __device__ __forceinline__ float sum_parts(float v) {
     return v;
 }
 
-// what a wave has in hand of the next eight rows
-template <class T, int NS, int P, bool HAS_C, bool HAS_Z, bool HAS_G>
+// What a wave has in hand of the next eight rows.  Rows and bases are the same in all lanes (scalar registers); lanes without a channel
+// read the last one's, rows behind the end the last row's, so that all loads are one block without branches.
+template <class T, int NS, int P, bool HAS_U, bool HAS_C, bool HAS_Z, bool HAS_G>
 struct Rows {
-    static constexpr int SP = NS * P, kStates = kTile * SP / kWave > 0 ? (kTile * SP + kWave - 1) / kWave : 1;
-    T u[kTile], dt[kTile], z[HAS_Z ? kTile : 1], g[HAS_G ? kTile : 1];
+    static constexpr int SP = NS * P, kStates = (kTile * SP + kWave - 1) / kWave;
+    T u[HAS_U ? kTile : 1], dt[kTile], z[HAS_Z ? kTile : 1], g[HAS_G ? kTile : 1];
     T b[kStates], c[HAS_C ? kStates : 1];
 
-    __device__ __forceinline__ void load(const ScanArgs &a, int64_t row, int n, int64_t ch, bool on, int lane) {
+    __device__ __forceinline__ void load(const ScanArgs &a, int64_t row, int n, uint32_t ch, int lane) {
 #pragma unroll
         for (int t = 0; t < kTile; ++t) {
-            u[t] = dt[t] = T(0.0f);
-            if (HAS_Z) z[t] = T(0.0f);
-            if (HAS_G) g[t] = T(0.0f);
-            if (t < n && on) {
-                if (!HAS_G || a.u) u[t] = reinterpret_cast<const T *>(a.u)[(row + t) * a.ld_u + ch];
-                dt[t] = reinterpret_cast<const T *>(a.dt)[(row + t) * a.ld_dt + ch];
-                if (HAS_Z && a.z) z[t] = reinterpret_cast<const T *>(a.z)[(row + t) * a.ld_z + ch];
-                if (HAS_G) g[t] = reinterpret_cast<const T *>(a.gy)[(row + t) * a.ld_gy + ch];
-            }
+            const int64_t r = row + (t < n ? t : n - 1);
+            if (HAS_U) u[t] = (reinterpret_cast<const T *>(a.u) + r * a.ld_u)[ch];
+            dt[t] = (reinterpret_cast<const T *>(a.dt) + r * a.ld_dt)[ch];
+            if (HAS_G) g[t] = (reinterpret_cast<const T *>(a.gy) + r * a.ld_gy)[ch];
         }
+        if (HAS_Z && a.z)
+#pragma unroll
+            for (int t = 0; t < kTile; ++t) z[t] = (reinterpret_cast<const T *>(a.z) + (row + (t < n ? t : n - 1)) * a.ld_z)[ch];
 #pragma unroll
         for (int k = 0; k < kStates; ++k) {
-            const int e = k * kWave + lane, t = e / SP, s = e % SP;
-            b[k] = T(0.0f);
-            if (HAS_C) c[k] = T(0.0f);
-            if (t < n && s < a.states) {
-                b[k] = reinterpret_cast<const T *>(a.B)[(row + t) * a.ld_B + s];
-                if (HAS_C) c[k] = reinterpret_cast<const T *>(a.C)[(row + t) * a.ld_C + s];
+            const int e = k * kWave + lane, t = e / SP < n ? e / SP : n - 1, s = e % SP, sc = s < a.states ? s : 0;
+            b[k] = (reinterpret_cast<const T *>(a.B) + row * a.ld_B)[(int64_t)t * a.ld_B + sc];
+            if (HAS_C) c[k] = (reinterpret_cast<const T *>(a.C) + row * a.ld_C)[(int64_t)t * a.ld_C + sc];
+            if (s >= a.states) {
+                b[k] = T(0.0f);
+                if (HAS_C) c[k] = T(0.0f);
             }
         }
     }
@@ -205,6 +204,13 @@ struct Rows {
     }
 };
 
+// softplus and its derivative from one exponential
+struct Step { float step, slope; };
+__device__ __forceinline__ Step softplus_step(float raw) {
+    const float e = fast_exp2(-fabsf(raw) * kLog2e), r = fast_rcp(1.0f + e);
+    return {softplus_from(raw, e), raw != raw ? raw : (raw >= 0.0f ? r : e * r)};
+}
+
 template <int NS> __device__ __forceinline__ void read_states(const float *at, float (&v)[NS]) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) v[i] = at[i];
@@ -212,18 +218,17 @@ template <int NS> __device__ __forceinline__ void read_states(const float *at, f
 
 // main pass (LOCAL = false): outputs, kept states, final state; first pass over chunks (LOCAL): what a chunk adds, and its steps' sum
 template <class T, int NS, int P, bool LOCAL>
-__global__ __launch_bounds__(kBlock) void scan_fwd_kernel(ScanArgs a) {
+__global__ __launch_bounds__(kWave) void scan_fwd_kernel(ScanArgs a) {
     constexpr int SP = NS * P, CH = kWave / P;
-    __shared__ __attribute__((aligned(16))) float shared[kWavesPerBlock][2 * kTile * SP];
-    const int lane = lane_id(), wave = wave_in_block(), part = lane / CH;
-    const int64_t id = (int64_t)blockIdx.x * kWavesPerBlock + wave;
+    __shared__ __attribute__((aligned(16))) float lds[2 * kTile * SP];
+    const int lane = lane_id(), part = lane / CH;
+    const int64_t id = blockIdx.x;
     const int64_t task = id / a.blocks;
     if (task >= a.tasks) return;
-    const int64_t ch = (id - task * a.blocks) * CH + lane % CH;
-    const bool on = ch < a.channels;
+    const uint32_t ch = (uint32_t)(id - task * a.blocks) * CH + lane % CH, last = a.channels - 1, chc = ch < last ? ch : last;
+    const bool on = ch <= last;
     const Task t = find_task(a, task, lane);
     if (!t.live) return;
-    float *lds = shared[wave];
     float A2[NS], h[NS];
     const float D = on && a.D ? a.D[ch] : 0.0f, bias = on && a.bias ? a.bias[ch] : 0.0f;
     float sum = 0.0f;
@@ -238,17 +243,17 @@ __global__ __launch_bounds__(kBlock) void scan_fwd_kernel(ScanArgs a) {
             else if (a.init) h[i] = a.init[(t.ray * a.channels + ch) * a.states + s];
         }
     }
-    Rows<T, NS, P, !LOCAL, !LOCAL, false> next;
+    Rows<T, NS, P, true, !LOCAL, !LOCAL, false> next;
     const int64_t row0 = t.start + t.first;
     int left = (int)(t.n < kTile ? t.n : kTile);
-    next.load(a, row0, left, ch, on, lane);
+    if (left > 0) next.load(a, row0, left, chc, lane);
     for (int64_t k = 0; k < t.n; k += kTile) {
         const auto rows = next;
         const int n = left;
         rows.stage(lds, lane);
         const int64_t rest = t.n - k - kTile;
         left = (int)(rest < kTile ? (rest > 0 ? rest : 0) : kTile);
-        if (left > 0) next.load(a, row0 + k + kTile, left, ch, on, lane);
+        if (left > 0) next.load(a, row0 + k + kTile, left, chc, lane);
         if (!LOCAL && a.kept && t.first + k > 0) {
             float *to = a.kept + ((row0 + k) / kTile) * a.states * a.channels;
 #pragma unroll
@@ -279,7 +284,7 @@ __global__ __launch_bounds__(kBlock) void scan_fwd_kernel(ScanArgs a) {
                     const float z = to_f(rows.z[j]);
                     y *= z * sigmoid_f(z);
                 }
-                if (on && part == 0) reinterpret_cast<T *>(a.y)[(row0 + k + j) * a.channels + ch] = from_f<T>(y);
+                if (on && part == 0) (reinterpret_cast<T *>(a.y) + (row0 + k + j) * a.channels)[ch] = from_f<T>(y);
             }
         }
     }
@@ -312,20 +317,20 @@ __global__ __launch_bounds__(kBlock) void scan_chain_kernel(ScanArgs a) {
     const float A2 = a.A[ch * a.states + s] * kLog2e;
     const float *from = REV ? a.gfinal : a.init;
     float h = from ? from[(ray * a.channels + ch) * a.states + s] : 0.0f;
-    const int64_t chunks = count > 0 ? (count + a.chunk - 1) / a.chunk : 1;
-    constexpr int kAhead = 8;
+    const int64_t chunks = count > 0 ? (count + a.chunk - 1) / a.chunk : 1, first = start / a.chunk;
+    constexpr int kAhead = 32;                              // chunks in flight: the chain itself is one fma each
     for (int64_t k0 = 0; k0 < chunks; k0 += kAhead) {
         float add[kAhead], decay[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int64_t k = k0 + i < chunks ? k0 + i : chunks - 1, slot = chunk_slot(a, ray, start, REV ? chunks - 1 - k : k);
+            const int64_t k = k0 + i < chunks ? k0 + i : chunks - 1, slot = chunk_slot(a, ray, first, REV ? chunks - 1 - k : k);
             add[i] = a.ends[(slot * a.states + s) * a.channels + ch];
             decay[i] = fast_exp2(a.sums[slot * a.channels + ch] * A2);
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             if (k0 + i >= chunks) break;
-            const int64_t k = k0 + i, slot = chunk_slot(a, ray, start, REV ? chunks - 1 - k : k);
+            const int64_t k = k0 + i, slot = chunk_slot(a, ray, first, REV ? chunks - 1 - k : k);
             a.ends[(slot * a.states + s) * a.channels + ch] = h;
             h = fmaf(decay[i], h, add[i]);
         }
@@ -334,18 +339,17 @@ __global__ __launch_bounds__(kBlock) void scan_chain_kernel(ScanArgs a) {
 
 // the gradient that a chunk adds at its first row, and its steps' sum
 template <class T, int NS, int P>
-__global__ __launch_bounds__(kBlock) void scan_bwd_local_kernel(ScanArgs a) {
+__global__ __launch_bounds__(kWave) void scan_bwd_local_kernel(ScanArgs a) {
     constexpr int SP = NS * P, CH = kWave / P;
-    __shared__ __attribute__((aligned(16))) float shared[kWavesPerBlock][2 * kTile * SP];
-    const int lane = lane_id(), wave = wave_in_block(), part = lane / CH;
-    const int64_t id = (int64_t)blockIdx.x * kWavesPerBlock + wave;
+    __shared__ __attribute__((aligned(16))) float lds[2 * kTile * SP];
+    const int lane = lane_id(), part = lane / CH;
+    const int64_t id = blockIdx.x;
     const int64_t task = id / a.blocks;
     if (task >= a.tasks) return;
-    const int64_t ch = (id - task * a.blocks) * CH + lane % CH;
-    const bool on = ch < a.channels;
+    const uint32_t ch = (uint32_t)(id - task * a.blocks) * CH + lane % CH, last = a.channels - 1, chc = ch < last ? ch : last;
+    const bool on = ch <= last;
     const Task t = find_task(a, task, lane);
     if (!t.live) return;
-    float *lds = shared[wave];
     float A2[NS], G[NS], sum = 0.0f;
     const float bias = on && a.bias ? a.bias[ch] : 0.0f;
 #pragma unroll
@@ -355,16 +359,14 @@ __global__ __launch_bounds__(kBlock) void scan_bwd_local_kernel(ScanArgs a) {
         G[i] = 0.0f;
     }
     const int64_t row0 = t.start + t.first, tiles = (t.n + kTile - 1) / kTile;
-    Rows<T, NS, P, true, true, true> next;
+    Rows<T, NS, P, false, true, true, true> next;
     auto rows_in = [&](int64_t k) { const int64_t r = t.n - k * kTile; return (int)(r < kTile ? r : kTile); };
-    ScanArgs b = a;
-    b.u = nullptr;                                          // not needed here
-    if (tiles > 0) next.load(b, row0 + (tiles - 1) * kTile, rows_in(tiles - 1), ch, on, lane);
+    if (tiles > 0) next.load(a, row0 + (tiles - 1) * kTile, rows_in(tiles - 1), chc, lane);
     for (int64_t k = tiles - 1; k >= 0; --k) {
         const auto rows = next;
         const int n = rows_in(k);
         rows.stage(lds, lane);
-        if (k > 0) next.load(b, row0 + (k - 1) * kTile, kTile, ch, on, lane);
+        if (k > 0) next.load(a, row0 + (k - 1) * kTile, kTile, chc, lane);
 #pragma unroll
         for (int j = kTile - 1; j >= 0; --j) {
             if (j >= n) continue;
@@ -391,17 +393,16 @@ __global__ __launch_bounds__(kBlock) void scan_bwd_local_kernel(ScanArgs a) {
 }
 
 template <class T, int NS, int P>
-__global__ __launch_bounds__(kBlock) void scan_bwd_kernel(ScanArgs a) {
+__global__ __launch_bounds__(kWave, 2) void scan_bwd_kernel(ScanArgs a) {
     constexpr int SP = NS * P, CH = kWave / P;
-    __shared__ __attribute__((aligned(16))) float shared[kWavesPerBlock][2 * kTile * SP];
-    const int lane = lane_id(), wave = wave_in_block(), part = lane / CH;
-    const int64_t id = (int64_t)blockIdx.x * kWavesPerBlock + wave;
+    __shared__ __attribute__((aligned(16))) float lds[2 * kTile * SP];
+    const int lane = lane_id(), part = lane / CH;
+    const int64_t id = blockIdx.x;
     const int64_t worker = id / a.blocks;
     if (worker >= a.workers) return;
     const int block = (int)(id - worker * a.blocks);
-    const int64_t ch = (int64_t)block * CH + lane % CH;
-    const bool on = ch < a.channels;
-    float *lds = shared[wave];
+    const uint32_t ch = (uint32_t)block * CH + lane % CH, last = a.channels - 1, chc = ch < last ? ch : last;
+    const bool on = ch <= last;
     float A[NS], A2[NS], dA[NS], dD = 0.0f, dbias = 0.0f;
     const float D = on && a.D ? a.D[ch] : 0.0f, bias = on && a.bias ? a.bias[ch] : 0.0f;
 #pragma unroll
@@ -431,41 +432,47 @@ __global__ __launch_bounds__(kBlock) void scan_bwd_kernel(ScanArgs a) {
             else if (here && a.gfinal) G[i] = a.gfinal[(t.ray * a.channels + ch) * a.states + s];
         }
         const int64_t row0 = t.start + t.first, tiles = (t.n + kTile - 1) / kTile;
-        Rows<T, NS, P, true, true, true> rows;
+        Rows<T, NS, P, true, true, true, true> rows;
         for (int64_t k = tiles - 1; k >= 0; --k) {
             const int64_t row = row0 + k * kTile;
             const int n = (int)(t.n - k * kTile < kTile ? t.n - k * kTile : kTile);
-            rows.load(a, row, n, ch, on, lane);
+            rows.load(a, row, n, chc, lane);
             float h0[NS], h[kTile][NS], e[kTile][NS];
+            Step st[kTile];
+            const bool inside = t.first + k > 0;
+            const float *from = inside ? a.kept + (row / kTile) * a.states * a.channels : a.init;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 const int s = part * NS + i;
                 h0[i] = 0.0f;
-                if (on && s < a.states) {
-                    if (t.first + k > 0) h0[i] = a.kept[((row / kTile) * a.states + s) * a.channels + ch];
-                    else if (a.init) h0[i] = a.init[(t.ray * a.channels + ch) * a.states + s];
-                }
+                if (from && on && s < a.states) h0[i] = from[inside ? (uint32_t)s * a.channels + ch : (t.ray * a.channels + ch) * a.states + s];
             }
             rows.stage(lds, lane);
 #pragma unroll
             for (int j = 0; j < kTile; ++j) {
-                float step = to_f(rows.dt[j]) + bias;
-                if (a.softplus) step = softplus_f(step);
-                const float in = step * to_f(rows.u[j]);
+                const float raw = to_f(rows.dt[j]) + bias;
+                st[j] = {raw, 1.0f};
+                if (a.softplus) st[j] = softplus_step(raw);
+                const float in = st[j].step * to_f(rows.u[j]);
                 float B[NS];
                 read_states<NS>(lds + j * SP + part * NS, B);
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
-                    e[j][i] = fast_exp2(step * A2[i]);
+                    e[j][i] = fast_exp2(st[j].step * A2[i]);
                     h[j][i] = fmaf(e[j][i], j ? h[j - 1][i] : h0[i], in * B[i]);
                 }
             }
 #pragma unroll
             for (int j = kTile - 1; j >= 0; --j) {
                 if (j >= n) continue;
-                const float u = to_f(rows.u[j]), raw = to_f(rows.dt[j]) + bias, step = a.softplus ? softplus_f(raw) : raw;
-                const float gy = to_f(rows.g[j]), z = to_f(rows.z[j]), sig = sigmoid_f(z);
-                const float dy = a.z ? gy * z * sig : gy, in = step * u;
+                // (lanes without a channel: no input and no gradient, so that they add nothing to dB and dC)
+                const float u = on ? to_f(rows.u[j]) : 0.0f, gy = on ? to_f(rows.g[j]) : 0.0f, step = st[j].step, in = step * u;
+                float z = 0.0f, sig = 0.0f, dy = gy;
+                if (a.z) {
+                    z = to_f(rows.z[j]);
+                    sig = sigmoid_f(z);
+                    dy = on ? gy * (z * sig) : 0.0f;
+                }
                 float B[NS], C[NS], v[2 * NS], y = 0.0f, sB = 0.0f, sA = 0.0f;
                 read_states<NS>(lds + j * SP + part * NS, B);
                 read_states<NS>(lds + (kTile + j) * SP + part * NS, C);
@@ -473,33 +480,32 @@ __global__ __launch_bounds__(kBlock) void scan_bwd_kernel(ScanArgs a) {
                 for (int i = 0; i < NS; ++i) {
                     const float g = fmaf(C[i], dy, G[i]);
                     y = fmaf(C[i], h[j][i], y);
-                    v[i] = g * in;
-                    v[NS + i] = dy * h[j][i];
+                    v[i] = on ? g * in : 0.0f;
+                    v[NS + i] = on ? dy * h[j][i] : 0.0f;
                     sB = fmaf(g, B[i], sB);
-                    const float w = g * (e[j][i] * (j ? h[j - 1][i] : h0[i]));
+                    G[i] = g * e[j][i];
+                    const float w = G[i] * (j ? h[j - 1][i] : h0[i]);
                     sA = fmaf(w, A[i], sA);
                     dA[i] = fmaf(w, step, dA[i]);
-                    G[i] = g * e[j][i];
                 }
                 sB = sum_parts<P>(sB);
                 sA = sum_parts<P>(sA);
-                float dstep = fmaf(u, sB, sA);
-                if (a.softplus) dstep *= sigmoid_f(raw);
+                const float dstep = fmaf(u, sB, sA) * st[j].slope;
                 if (a.z) y = fmaf(D, u, sum_parts<P>(y));
                 if (on && part == 0) {
-                    const int64_t at = (row + j) * a.channels + ch;
-                    reinterpret_cast<T *>(a.gu)[at] = from_f<T>(fmaf(step, sB, D * dy));
-                    reinterpret_cast<T *>(a.gdt)[at] = from_f<T>(dstep);
-                    if (a.z) reinterpret_cast<T *>(a.gz)[at] = from_f<T>(gy * y * (sig * fmaf(z, 1.0f - sig, 1.0f)));
+                    const int64_t at = (row + j) * a.channels;
+                    (reinterpret_cast<T *>(a.gu) + at)[ch] = from_f<T>(fmaf(step, sB, D * dy));
+                    (reinterpret_cast<T *>(a.gdt) + at)[ch] = from_f<T>(dstep);
+                    if (a.z) (reinterpret_cast<T *>(a.gz) + at)[ch] = from_f<T>(gy * y * (sig * fmaf(z, 1.0f - sig, 1.0f)));
                     dD = fmaf(dy, u, dD);
                     dbias += dstep;
                 }
                 sum_over_lanes<2 * NS, CH / 2>(v, lane);
-                float *to = a.part_bc + ((int64_t)block * a.rows + row + j) * (2 * SP);
                 if (stores) {
+                    float *to = a.part_bc + ((int64_t)block * a.rows + row + j) * (2 * SP);
 #pragma unroll
                     for (int i = 0; i < kLeft; ++i) {
-                        const int q = i * (1 << kHalvings) + number;
+                        const uint32_t q = i * (1 << kHalvings) + number;
                         to[(q / NS) * SP + part * NS + q % NS] = v[i];
                     }
                 }
@@ -750,15 +756,15 @@ NFA_EXPORT int nfa_selective_scan_fwd(const nfa_selective_scan_args *a, void *ou
     d.y = outputs; d.final_state = final_state; d.kept = checkpoints;
     if (a->packed_info && a->rows > 0) launch_zero_rows(d, a->dtype, outputs, nullptr, nullptr, s);
     if (p.tasks > 0) {
-        const int64_t grid = ceil_div(p.tasks * p.blocks, kWavesPerBlock);
+        const int64_t grid = p.tasks * p.blocks;
         NFA_REQUIRE(grid < (1ll << 31) && a->n_rays * (int64_t)(p.chunk ? 1 : 0) < 65536, "selective_scan_fwd: too large for one launch");
         with_shape<kFwdStates>(a->dtype, p.sh, [&](auto t, auto ns, auto pp) {
             using T = decltype(t);
             if (p.chunk) {
-                hipLaunchKernelGGL((scan_fwd_kernel<T, ns(), pp(), true>), dim3((unsigned)grid), dim3(kBlock), 0, s, d);
+                hipLaunchKernelGGL((scan_fwd_kernel<T, ns(), pp(), true>), dim3((unsigned)grid), dim3(kWave), 0, s, d);
                 launch_chain<false>(d, s);
             }
-            hipLaunchKernelGGL((scan_fwd_kernel<T, ns(), pp(), false>), dim3((unsigned)grid), dim3(kBlock), 0, s, d);
+            hipLaunchKernelGGL((scan_fwd_kernel<T, ns(), pp(), false>), dim3((unsigned)grid), dim3(kWave), 0, s, d);
         });
     }
     return check_launch("scan_fwd_kernel");
@@ -778,16 +784,16 @@ NFA_EXPORT int nfa_selective_scan_bwd(const nfa_selective_scan_args *a, const fl
     use_plan(d, p, sp, workspace);
     d.kept = (float *)checkpoints;
     d.gu = g->inputs; d.gdt = g->delta; d.gz = a->gate ? g->gate : nullptr; d.ginit = g->initial_state;
-    const int64_t grid = ceil_div(p.tasks * p.blocks, kWavesPerBlock), main_grid = ceil_div(p.workers * p.blocks, kWavesPerBlock);
+    const int64_t grid = p.tasks * p.blocks, main_grid = p.workers * p.blocks;
     NFA_REQUIRE(grid < (1ll << 31) && a->n_rays * (int64_t)(p.chunk ? 1 : 0) < 65536, "selective_scan_bwd: too large for one launch");
     if (a->packed_info) launch_zero_rows(d, a->dtype, d.gu, d.gdt, d.gz, s);
     with_shape<kBwdStates>(a->dtype, p.sh, [&](auto t, auto ns, auto pp) {
         using T = decltype(t);
         if (p.chunk) {
-            hipLaunchKernelGGL((scan_bwd_local_kernel<T, ns(), pp()>), dim3((unsigned)grid), dim3(kBlock), 0, s, d);
+            hipLaunchKernelGGL((scan_bwd_local_kernel<T, ns(), pp()>), dim3((unsigned)grid), dim3(kWave), 0, s, d);
             launch_chain<true>(d, s);
         }
-        hipLaunchKernelGGL((scan_bwd_kernel<T, ns(), pp()>), dim3((unsigned)main_grid), dim3(kBlock), 0, s, d);
+        hipLaunchKernelGGL((scan_bwd_kernel<T, ns(), pp()>), dim3((unsigned)main_grid), dim3(kWave), 0, s, d);
         hipLaunchKernelGGL((scan_join_bc_kernel<T>), dim3(blocks_for(a->rows * 2 * a->states)), dim3(kBlock), 0, s, d, (int)(ns() * pp()), (T *)g->B, (T *)g->C);
     });
     launch_reduce_rows(d.part_w, p.workers, {{g->A, (int64_t)a->channels * a->states}, {g->D, a->channels}, {g->delta_bias, a->channels}}, NFA_DTYPE_F32, s);
