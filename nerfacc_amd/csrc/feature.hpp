@@ -26,7 +26,7 @@ inline void with_dtype(int32_t dtype, F &&f) {
     else f(f16{});
 }
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 // 2^x in one v_exp_f32: 1 ulp, results below 2^-126 become 0
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }

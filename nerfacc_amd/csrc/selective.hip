@@ -403,13 +403,12 @@ __global__ __launch_bounds__(kWave, 2) void scan_bwd_kernel(ScanArgs a) {
     const int block = (int)(id - worker * a.blocks);
     const uint32_t ch = (uint32_t)block * CH + lane % CH, last = a.channels - 1, chc = ch < last ? ch : last;
     const bool on = ch <= last;
-    float A[NS], A2[NS], dA[NS], dD = 0.0f, dbias = 0.0f;
+    float A2[NS], dA[NS], dD = 0.0f, dbias = 0.0f;          // A2 = A log2(e): dstep is summed with it and scaled once
     const float D = on && a.D ? a.D[ch] : 0.0f, bias = on && a.bias ? a.bias[ch] : 0.0f;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
         const int s = part * NS + i;
-        A[i] = on && s < a.states ? a.A[ch * a.states + s] : 0.0f;
-        A2[i] = A[i] * kLog2e;
+        A2[i] = on && s < a.states ? a.A[ch * a.states + s] * kLog2e : 0.0f;
         dA[i] = 0.0f;
     }
     // after the exchange over channels: this lane's values, their places, and whether it is the one that stores them
@@ -437,7 +436,7 @@ __global__ __launch_bounds__(kWave, 2) void scan_bwd_kernel(ScanArgs a) {
             const int64_t row = row0 + k * kTile;
             const int n = (int)(t.n - k * kTile < kTile ? t.n - k * kTile : kTile);
             rows.load(a, row, n, chc, lane);
-            float h0[NS], h[kTile][NS], e[kTile][NS];
+            float h0[NS], h[kTile][NS];
             Step st[kTile];
             const bool inside = t.first + k > 0;
             const float *from = inside ? a.kept + (row / kTile) * a.states * a.channels : a.init;
@@ -458,15 +457,16 @@ __global__ __launch_bounds__(kWave, 2) void scan_bwd_kernel(ScanArgs a) {
                 read_states<NS>(lds + j * SP + part * NS, B);
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
-                    e[j][i] = fast_exp2(st[j].step * A2[i]);
-                    h[j][i] = fmaf(e[j][i], j ? h[j - 1][i] : h0[i], in * B[i]);
+                    h[j][i] = fmaf(fast_exp2(st[j].step * A2[i]), j ? h[j - 1][i] : h0[i], in * B[i]);
                 }
             }
 #pragma unroll
             for (int j = kTile - 1; j >= 0; --j) {
                 if (j >= n) continue;
                 // (lanes without a channel: no input and no gradient, so that they add nothing to dB and dC)
-                const float u = on ? to_f(rows.u[j]) : 0.0f, gy = on ? to_f(rows.g[j]) : 0.0f, step = st[j].step, in = step * u;
+                const float u = on ? to_f(rows.u[j]) : 0.0f, gy = on ? to_f(rows.g[j]) : 0.0f, in = st[j].step * u;
+                float step = st[j].step;
+                asm volatile("" : "+v"(step));              // (or the compiler keeps the exponentials of the first loop after all)
                 float z = 0.0f, sig = 0.0f, dy = gy;
                 if (a.z) {
                     z = to_f(rows.z[j]);
@@ -483,14 +483,14 @@ __global__ __launch_bounds__(kWave, 2) void scan_bwd_kernel(ScanArgs a) {
                     v[i] = on ? g * in : 0.0f;
                     v[NS + i] = on ? dy * h[j][i] : 0.0f;
                     sB = fmaf(g, B[i], sB);
-                    G[i] = g * e[j][i];
+                    G[i] = g * fast_exp2(step * A2[i]);     // (formed again: kept, it would take 64 registers and a wave per SIMD)
                     const float w = G[i] * (j ? h[j - 1][i] : h0[i]);
-                    sA = fmaf(w, A[i], sA);
+                    sA = fmaf(w, A2[i], sA);
                     dA[i] = fmaf(w, step, dA[i]);
                 }
                 sB = sum_parts<P>(sB);
                 sA = sum_parts<P>(sA);
-                const float dstep = fmaf(u, sB, sA) * st[j].slope;
+                const float dstep = fmaf(u, sB, sA * kLn2) * st[j].slope;
                 if (a.z) y = fmaf(D, u, sum_parts<P>(y));
                 if (on && part == 0) {
                     const int64_t at = (row + j) * a.channels;
@@ -509,6 +509,7 @@ __global__ __launch_bounds__(kWave, 2) void scan_bwd_kernel(ScanArgs a) {
                         to[(q / NS) * SP + part * NS + q % NS] = v[i];
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);          // one row at a time: rows in parallel would need twice the registers
             }
         }
         if (a.ginit && t.first == 0) {
