@@ -10,6 +10,8 @@
 // and then in order over the workgroups: no atomics.
 #include "feature.hpp"
 
+#include <algorithm>
+
 namespace nfa {
 namespace {
 
@@ -84,15 +86,27 @@ __global__ __launch_bounds__(kBlock) void conv_fwd_kernel(ConvArgs a) {
     Place p = place_of(a, begin);
 #pragma unroll
     for (int j = 1; j < W; ++j) load_before<T, W, VC>(a, begin, p, W - j, c, win[j]);
+    // the next rows' loads are in flight while these are computed; rows behind the piece read its last row again
+    Vec<T, VC> next[kAhead];
+    Place after[kAhead];
+    auto load = [&](int64_t row, Place before) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int64_t r = row + k < end ? row + k : end - 1;
+            after[k] = r == begin ? p : place_after(a, k ? after[k - 1] : before, r);
+            next[k] = *reinterpret_cast<const Vec<T, VC> *>(reinterpret_cast<const T *>(a.x) + r * a.ld_x + c);
+        }
+    };
+    load(begin, p);
     for (int64_t row = begin; row < end; row += kAhead) {
-        Vec<T, VC> next[kAhead];
+        Vec<T, VC> now[kAhead];
         Place at[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-            if (row + k >= end) continue;
-            at[k] = row + k == begin ? p : place_after(a, k ? at[k - 1] : p, row + k);
-            next[k] = *reinterpret_cast<const Vec<T, VC> *>(reinterpret_cast<const T *>(a.x) + (row + k) * a.ld_x + c);
+            now[k] = next[k];
+            at[k] = after[k];
         }
+        if (row + kAhead < end) load(row + kAhead, at[kAhead - 1]);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
             if (row + k >= end) continue;
@@ -107,19 +121,20 @@ __global__ __launch_bounds__(kBlock) void conv_fwd_kernel(ConvArgs a) {
             float y[VC];
 #pragma unroll
             for (int i = 0; i < VC; ++i) {
-                win[W - 1][i] = to_f(next[k].v[i]);
+                win[W - 1][i] = to_f(now[k].v[i]);
                 float z = b[i];
 #pragma unroll
                 for (int j = 0; j < W; ++j) z = fmaf(w[j][i], win[j][i], z);
-                if (a.act == NFA_ACT_SILU) z = z * sigmoid_f(z);
-                y[i] = at[k].pos < 0 ? 0.0f : z;
+                y[i] = z;
             }
+            if (a.act == NFA_ACT_SILU)
+#pragma unroll
+                for (int i = 0; i < VC; ++i) y[i] *= sigmoid_f(y[i]);
+            if (at[k].pos < 0)
+#pragma unroll
+                for (int i = 0; i < VC; ++i) y[i] = 0.0f;
             store_row<T, VC>(a.y, (row + k) * a.channels + c, y);
         }
-        const int last = end - row < kAhead ? (int)(end - row) - 1 : kAhead - 1;
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-            if (k == last) p = at[k];
     }
 }
 
@@ -319,22 +334,34 @@ __global__ __launch_bounds__(kBlock) void conv_init_grad_kernel(ConvArgs a, T *g
     }
 }
 
-template <class T, int W>
+template <class T, int W, int VC>
 __global__ __launch_bounds__(kBlock) void conv_step_kernel(ConvArgs a, const T *state, T *y, T *next) {
-    const int64_t n = a.n_rays * a.channels;
-    for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < n; e += (int64_t)gridDim.x * kBlock) {
-        const int64_t c = e % a.channels, ray = e / a.channels;
-        T line[W];
+    const int64_t c = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * VC;
+    if (c >= a.channels) return;
+    float w[W][VC], b[VC];
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) line[j] = state[(ray * (W - 1) + j) * a.channels + c];
-        line[W - 1] = reinterpret_cast<const T *>(a.x)[ray * a.ld_x + c];
-        float z = a.bias ? to_f(reinterpret_cast<const T *>(a.bias)[c]) : 0.0f;
+    for (int i = 0; i < VC; ++i) {
+        b[i] = a.bias ? to_f(reinterpret_cast<const T *>(a.bias)[c + i]) : 0.0f;
 #pragma unroll
-        for (int j = 0; j < W; ++j) z = fmaf(to_f(reinterpret_cast<const T *>(a.w)[c * W + j]), to_f(line[j]), z);
-        if (a.act == NFA_ACT_SILU) z = z * sigmoid_f(z);
-        y[e] = from_f<T>(z);
+        for (int j = 0; j < W; ++j) w[j][i] = to_f(reinterpret_cast<const T *>(a.w)[(c + i) * W + j]);
+    }
+    for (int64_t ray = blockIdx.y; ray < a.n_rays; ray += gridDim.y) {
+        using V = Vec<T, VC>;
+        V line[W], out;
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) next[(ray * (W - 1) + j) * a.channels + c] = line[j + 1];
+        for (int j = 0; j < W - 1; ++j) line[j] = *reinterpret_cast<const V *>(state + (ray * (W - 1) + j) * a.channels + c);
+        line[W - 1] = *reinterpret_cast<const V *>(reinterpret_cast<const T *>(a.x) + ray * a.ld_x + c);
+#pragma unroll
+        for (int i = 0; i < VC; ++i) {
+            float z = b[i];
+#pragma unroll
+            for (int j = 0; j < W; ++j) z = fmaf(w[j][i], to_f(line[j].v[i]), z);
+            if (a.act == NFA_ACT_SILU) z = z * sigmoid_f(z);
+            out.v[i] = from_f<T>(z);
+        }
+        *reinterpret_cast<V *>(y + ray * a.channels + c) = out;
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) *reinterpret_cast<V *>(next + (ray * (W - 1) + j) * a.channels + c) = line[j + 1];
     }
 }
 
@@ -525,10 +552,13 @@ NFA_EXPORT int nfa_causal_conv_step(const nfa_causal_conv_args *a, const void *s
     NFA_REQUIRE(a->inputs && a->weight && state && outputs && out_state, "causal_conv_step: NULL pointer");
     NFA_REQUIRE(a->inputs_stride >= a->channels || a->n_rays <= 1, "causal_conv_step: inputs_stride < channels");
     ConvArgs d = conv_args(a);
-    with_conv(a->dtype, a->width, 1, [&](auto t, auto w, auto) {
+    const int64_t bytes = dtype_bytes(a->dtype);
+    int vec = (int)(16 / bytes);
+    if (a->channels % vec || !fits(d.x, d.ld_x, bytes, vec) || !fits(state, 0, bytes, vec) || !fits(outputs, 0, bytes, vec) || !fits(out_state, 0, bytes, vec)) vec = 1;
+    const dim3 grid((unsigned)ceil_div(ceil_div(a->channels, vec), kBlock), (unsigned)std::min<int64_t>(a->n_rays, 32768));
+    with_conv(a->dtype, a->width, vec, [&](auto t, auto w, auto vc) {
         using T = decltype(t);
-        hipLaunchKernelGGL((conv_step_kernel<T, w()>), dim3(blocks_for(a->n_rays * a->channels)), dim3(kBlock), 0, (hipStream_t)stream, d,
-                           (const T *)state, (T *)outputs, (T *)out_state);
+        hipLaunchKernelGGL((conv_step_kernel<T, w(), vc()>), grid, dim3(kBlock), 0, (hipStream_t)stream, d, (const T *)state, (T *)outputs, (T *)out_state);
     });
     return check_launch("conv_step_kernel");
 }

@@ -19,10 +19,15 @@
 // the sums over rows stay in registers over all rows of a wave; both are joined in a fixed order.
 #include "feature.hpp"
 
+#include <algorithm>
+
 namespace nfa {
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kTile = 8;                // rows between kept states, and rows whose loads are in flight together
+constexpr int64_t kMaxStride = 1 << 26; // elements: eight rows of four bytes are 2^31 bytes apart at most
 
 struct ScanArgs {
     const void *u, *dt, *z, *B, *C, *gy;
@@ -166,22 +171,29 @@ struct Rows {
     T u[HAS_U ? kTile : 1], dt[kTile], z[HAS_Z ? kTile : 1], g[HAS_G ? kTile : 1];
     T b[kStates], c[HAS_C ? kStates : 1];
 
+    // one scalar base per tensor, 32-bit offsets from it (row strides are at most kMaxStride)
+    static __device__ __forceinline__ T at(const void *base, int64_t row, int64_t ld, uint32_t offset) {
+        return *reinterpret_cast<const T *>(reinterpret_cast<const char *>(base) + row * ld * (int64_t)sizeof(T) + offset);
+    }
     __device__ __forceinline__ void load(const ScanArgs &a, int64_t row, int n, uint32_t ch, int lane) {
+        const uint32_t z0 = sizeof(T), lu = (uint32_t)a.ld_u * z0, ld = (uint32_t)a.ld_dt * z0, lg = (uint32_t)a.ld_gy * z0, lz = (uint32_t)a.ld_z * z0,
+                       c0 = ch * z0;
 #pragma unroll
         for (int t = 0; t < kTile; ++t) {
-            const int64_t r = row + (t < n ? t : n - 1);
-            if (HAS_U) u[t] = (reinterpret_cast<const T *>(a.u) + r * a.ld_u)[ch];
-            dt[t] = (reinterpret_cast<const T *>(a.dt) + r * a.ld_dt)[ch];
-            if (HAS_G) g[t] = (reinterpret_cast<const T *>(a.gy) + r * a.ld_gy)[ch];
+            const uint32_t r = t < n ? t : n - 1;
+            if (HAS_U) u[t] = at(a.u, row, a.ld_u, r * lu + c0);
+            dt[t] = at(a.dt, row, a.ld_dt, r * ld + c0);
+            if (HAS_G) g[t] = at(a.gy, row, a.ld_gy, r * lg + c0);
         }
         if (HAS_Z && a.z)
 #pragma unroll
-            for (int t = 0; t < kTile; ++t) z[t] = (reinterpret_cast<const T *>(a.z) + (row + (t < n ? t : n - 1)) * a.ld_z)[ch];
+            for (int t = 0; t < kTile; ++t) z[t] = at(a.z, row, a.ld_z, (uint32_t)(t < n ? t : n - 1) * lz + c0);
 #pragma unroll
         for (int k = 0; k < kStates; ++k) {
-            const int e = k * kWave + lane, t = e / SP < n ? e / SP : n - 1, s = e % SP, sc = s < a.states ? s : 0;
-            b[k] = (reinterpret_cast<const T *>(a.B) + row * a.ld_B)[(int64_t)t * a.ld_B + sc];
-            if (HAS_C) c[k] = (reinterpret_cast<const T *>(a.C) + row * a.ld_C)[(int64_t)t * a.ld_C + sc];
+            const int e = k * kWave + lane, s = e % SP;
+            const uint32_t t = e / SP < n ? e / SP : n - 1, sc = s < a.states ? s : 0;
+            b[k] = at(a.B, row, a.ld_B, (t * (uint32_t)a.ld_B + sc) * z0);
+            if (HAS_C) c[k] = at(a.C, row, a.ld_C, (t * (uint32_t)a.ld_C + sc) * z0);
             if (s >= a.states) {
                 b[k] = T(0.0f);
                 if (HAS_C) c[k] = T(0.0f);
@@ -456,9 +468,8 @@ __global__ __launch_bounds__(kWave, 2) void scan_bwd_kernel(ScanArgs a) {
                 float B[NS];
                 read_states<NS>(lds + j * SP + part * NS, B);
 #pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    h[j][i] = fmaf(fast_exp2(st[j].step * A2[i]), j ? h[j - 1][i] : h0[i], in * B[i]);
-                }
+                for (int i = 0; i < NS; ++i) h[j][i] = fmaf(fast_exp2(st[j].step * A2[i]), j ? h[j - 1][i] : h0[i], in * B[i]);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int j = kTile - 1; j >= 0; --j) {
@@ -493,10 +504,11 @@ __global__ __launch_bounds__(kWave, 2) void scan_bwd_kernel(ScanArgs a) {
                 const float dstep = fmaf(u, sB, sA * kLn2) * st[j].slope;
                 if (a.z) y = fmaf(D, u, sum_parts<P>(y));
                 if (on && part == 0) {
-                    const int64_t at = (row + j) * a.channels;
-                    (reinterpret_cast<T *>(a.gu) + at)[ch] = from_f<T>(fmaf(step, sB, D * dy));
-                    (reinterpret_cast<T *>(a.gdt) + at)[ch] = from_f<T>(dstep);
-                    if (a.z) (reinterpret_cast<T *>(a.gz) + at)[ch] = from_f<T>(gy * y * (sig * fmaf(z, 1.0f - sig, 1.0f)));
+                    const int64_t at = row * a.channels;
+                    const uint32_t to = (uint32_t)j * a.channels + ch;
+                    (reinterpret_cast<T *>(a.gu) + at)[to] = from_f<T>(fmaf(step, sB, D * dy));
+                    (reinterpret_cast<T *>(a.gdt) + at)[to] = from_f<T>(dstep);
+                    if (a.z) (reinterpret_cast<T *>(a.gz) + at)[to] = from_f<T>(gy * y * (sig * fmaf(z, 1.0f - sig, 1.0f)));
                     dD = fmaf(dy, u, dD);
                     dbias += dstep;
                 }
@@ -567,28 +579,48 @@ __global__ __launch_bounds__(kBlock) void zero_rows_kernel(const int32_t *__rest
     }
 }
 
-template <class T>
+// One row per sequence: reading and writing the state bounds it (8 bytes per state).  L lanes share a channel, each with four
+// neighbouring states (one 16-byte access); L = 0: a lane per channel and states one by one, for numbers of states that do not divide.
+template <class T, int L>
 __global__ __launch_bounds__(kBlock) void scan_step_kernel(ScanArgs a, const float *state, float *next) {
-    const int64_t n = a.n_rays * a.channels;
-    for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < n; e += (int64_t)gridDim.x * kBlock) {
-        const int64_t ray = e / a.channels, ch = e - ray * a.channels;
-        const float u = to_f(reinterpret_cast<const T *>(a.u)[ray * a.ld_u + ch]);
-        float step = to_f(reinterpret_cast<const T *>(a.dt)[ray * a.ld_dt + ch]) + (a.bias ? a.bias[ch] : 0.0f);
+    constexpr int LL = L ? L : 1;
+    const uint32_t e = blockIdx.x * kBlock + threadIdx.x, ch = e / LL, s0 = e % LL * 4;
+    if (ch >= (uint32_t)a.channels) return;                 // (whole groups of lanes: LL divides the wave)
+    const float bias = a.bias ? a.bias[ch] : 0.0f, D = a.D ? a.D[ch] : 0.0f;
+    f32x4 A = {0, 0, 0, 0};
+    if (L) A = *reinterpret_cast<const f32x4 *>(a.A + ch * a.states + s0);
+    for (int64_t ray = blockIdx.y; ray < a.n_rays; ray += gridDim.y) {
+        const int64_t at = (ray * a.channels + ch) * a.states + s0;
+        const float u = to_f((reinterpret_cast<const T *>(a.u) + ray * a.ld_u)[ch]);
+        float step = to_f((reinterpret_cast<const T *>(a.dt) + ray * a.ld_dt)[ch]) + bias, y = 0.0f;
+        const T *B = reinterpret_cast<const T *>(a.B) + ray * a.ld_B, *C = reinterpret_cast<const T *>(a.C) + ray * a.ld_C;
+        f32x4 h = {0, 0, 0, 0};
+        if (L) h = *reinterpret_cast<const f32x4 *>(state + at);
+        float z = 0.0f;
+        if (a.z) z = to_f((reinterpret_cast<const T *>(a.z) + ray * a.ld_z)[ch]);
         if (a.softplus) step = softplus_f(step);
         const float in = step * u, d2 = step * kLog2e;
-        float y = 0.0f;
-        for (int s = 0; s < a.states; ++s) {
-            const float B = to_f(reinterpret_cast<const T *>(a.B)[ray * a.ld_B + s]), C = to_f(reinterpret_cast<const T *>(a.C)[ray * a.ld_C + s]);
-            const float h = fmaf(fast_exp2(d2 * a.A[ch * a.states + s]), state[e * a.states + s], in * B);
-            next[e * a.states + s] = h;
-            y = fmaf(C, h, y);
+        if (L) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h[i] = fmaf(fast_exp2(d2 * A[i]), h[i], in * to_f(B[s0 + i]));
+                y = fmaf(to_f(C[s0 + i]), h[i], y);
+            }
+            *reinterpret_cast<f32x4 *>(next + at) = h;
+            if constexpr (L >= 2) y = add_other<1>(y);
+            if constexpr (L >= 4) y = add_other<2>(y);
+            if constexpr (L >= 8) y = add_other<4>(y);
+            if constexpr (L >= 16) y = add_other<8>(y);
+        } else {
+            for (int s = 0; s < a.states; ++s) {
+                const float v = fmaf(fast_exp2(d2 * a.A[ch * a.states + s]), state[at + s], in * to_f(B[s]));
+                next[at + s] = v;
+                y = fmaf(to_f(C[s]), v, y);
+            }
         }
-        if (a.D) y = fmaf(a.D[ch], u, y);
-        if (a.z) {
-            const float z = to_f(reinterpret_cast<const T *>(a.z)[ray * a.ld_z + ch]);
-            y *= z * sigmoid_f(z);
-        }
-        reinterpret_cast<T *>(a.y)[e] = from_f<T>(y);
+        y = fmaf(D, u, y);
+        if (a.z) y *= z * sigmoid_f(z);
+        if (s0 == 0) (reinterpret_cast<T *>(a.y) + ray * a.channels)[ch] = from_f<T>(y);
     }
 }
 
@@ -685,6 +717,8 @@ int check_scan(const nfa_selective_scan_args *a, const char *who, bool step) {
     NFA_REQUIRE(rows <= 1 || (a->inputs_stride >= a->channels && a->delta_stride >= a->channels && (!a->gate || a->gate_stride >= a->channels) &&
                               a->B_stride >= a->states && a->C_stride >= a->states), "%s: a row stride is shorter than its row", who);
     if (step) return NFA_OK;
+    for (int64_t ld : {a->inputs_stride, a->delta_stride, a->gate_stride, a->B_stride, a->C_stride, a->grad_outputs_stride})
+        NFA_REQUIRE(ld <= kMaxStride, "%s: a row stride is over 2^26", who);
     NFA_REQUIRE(a->packed_info || a->n_rays == 0 || a->rows % a->n_rays == 0, "%s: rows do not divide into equal sequences", who);
     NFA_REQUIRE(a->n_rays > 0 || a->packed_info || a->rows == 0, "%s: rows without sequences", who);
     NFA_REQUIRE(!a->packed_info || a->rows == 0 || (a->row_ray && a->row_pos), "%s: packed sequences need their row map", who);
@@ -807,9 +841,17 @@ NFA_EXPORT int nfa_selective_scan_step(const nfa_selective_scan_args *a, const f
     NFA_REQUIRE(state && outputs && out_state, "selective_scan_step: NULL pointer");
     ScanArgs d = scan_args(a);
     d.y = outputs;
+    const bool whole = ((uintptr_t)state | (uintptr_t)out_state | (uintptr_t)a->A) % 16 == 0;
+    int lanes = 0;
+    for (int l : {1, 2, 4, 8, 16})
+        if (whole && a->states == 4 * l) lanes = l;
+    const int64_t per = (int64_t)a->channels * (lanes ? lanes : 1);
+    const dim3 grid((unsigned)ceil_div(per, kBlock), (unsigned)std::min<int64_t>(a->n_rays, 32768));
     with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL((scan_step_kernel<T>), dim3(blocks_for(a->n_rays * a->channels)), dim3(kBlock), 0, (hipStream_t)stream, d, state, out_state);
+        const auto kernel = lanes == 1 ? scan_step_kernel<T, 1> : lanes == 2 ? scan_step_kernel<T, 2> : lanes == 4 ? scan_step_kernel<T, 4>
+                          : lanes == 8 ? scan_step_kernel<T, 8> : lanes == 16 ? scan_step_kernel<T, 16> : scan_step_kernel<T, 0>;
+        hipLaunchKernelGGL(kernel, grid, dim3(kBlock), 0, (hipStream_t)stream, d, state, out_state);
     });
     return check_launch("scan_step_kernel");
 }
