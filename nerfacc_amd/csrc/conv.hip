@@ -70,7 +70,7 @@ __device__ __forceinline__ void load_before(const ConvArgs &a, int64_t row, Plac
 constexpr int kAhead = 4;               // rows whose loads are in flight together
 
 template <class T, int W, int VC>
-__global__ __launch_bounds__(kBlock) void conv_fwd_kernel(ConvArgs a) {
+__global__ __launch_bounds__(kBlock, 3) void conv_fwd_kernel(ConvArgs a) {
     const int lane = threadIdx.x % a.lanes;
     const int64_t c = ((int64_t)blockIdx.y * a.lanes + lane) * VC;
     const int64_t piece = (int64_t)blockIdx.x * (kBlock / a.lanes) + threadIdx.x / a.lanes;
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(kBlock) void conv_fwd_kernel(ConvArgs a) {
 }
 
 template <class T, int W, int VC>
-__global__ __launch_bounds__(kBlock) void conv_bwd_kernel(ConvArgs a) {
+__global__ __launch_bounds__(kBlock, 3) void conv_bwd_kernel(ConvArgs a) {
     extern __shared__ float joined[];
     const int lane = threadIdx.x % a.lanes, group = threadIdx.x / a.lanes, groups = kBlock / a.lanes;
     const int64_t c = ((int64_t)blockIdx.y * a.lanes + lane) * VC;
@@ -195,10 +195,10 @@ __global__ __launch_bounds__(kBlock) void conv_bwd_kernel(ConvArgs a) {
             Place at[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                if (row + k >= stop) continue;
-                at[k] = row + k == begin ? p : place_after(a, k ? at[k - 1] : p, row + k);
-                nx[k] = *reinterpret_cast<const Vec<T, VC> *>(reinterpret_cast<const T *>(a.x) + (row + k) * a.ld_x + c);
-                ng[k] = *reinterpret_cast<const Vec<T, VC> *>(reinterpret_cast<const T *>(a.gy) + (row + k) * a.ld_gy + c);
+                const int64_t r = row + k < stop ? row + k : stop - 1;
+                at[k] = r == begin ? p : place_after(a, k ? at[k - 1] : p, r);
+                nx[k] = *reinterpret_cast<const Vec<T, VC> *>(reinterpret_cast<const T *>(a.x) + r * a.ld_x + c);
+                ng[k] = *reinterpret_cast<const Vec<T, VC> *>(reinterpret_cast<const T *>(a.gy) + r * a.ld_gy + c);
             }
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
@@ -401,7 +401,7 @@ void with_conv(int32_t dtype, int width, int vec, F &&f) {
     });
 }
 
-constexpr int64_t kBwdGroups = 1024;            // workgroups (and partial sums) of a backward pass, at most
+constexpr int64_t kBwdGroups = 3 * kNumCU;      // workgroups (and partial sums) of a backward pass, at most: all resident
 
 struct ConvPlan { int vec, lanes, piece; int64_t pieces, blocks_x, blocks_y; };
 ConvPlan conv_plan(int64_t rows, int64_t channels, int vec, bool backward) {
@@ -411,9 +411,11 @@ ConvPlan conv_plan(int64_t rows, int64_t channels, int vec, bool backward) {
     p.lanes = 1;
     while (p.lanes < vecs && p.lanes < 64) p.lanes *= 2;
     p.blocks_y = ceil_div(vecs, p.lanes);
-    // long pieces read their halo rows rarely; short ones fill the chip
-    p.piece = 32;
-    while (p.piece > 4 && ceil_div(rows, p.piece) * vecs < (int64_t)kNumCU * 1024) p.piece /= 2;
+    // as many rows per wave as fill the chip's 3 x 1024 wave places once, at most 64 (then twice, ...): long pieces read their halo rows
+    // rarely, and a launch of one and a third rounds takes two (43 rows against 32 at 32768 x 2048: 64 against 75 us)
+    const int64_t each = ceil_div(ceil_div(rows * p.lanes * p.blocks_y, kWave), 3 * 4 * kNumCU);
+    p.piece = (int)ceil_div(each, ceil_div(each, 64));
+    if (p.piece < 4) p.piece = 4;
     p.pieces = ceil_div(rows, p.piece);
     p.blocks_x = ceil_div(p.pieces, kBlock / p.lanes);
     if (backward && p.blocks_x > ceil_div(kBwdGroups, p.blocks_y)) p.blocks_x = ceil_div(kBwdGroups, p.blocks_y);
