@@ -163,6 +163,12 @@ __device__ __forceinline__ float sum_parts(float v) {
     return v;
 }
 
+// column c of row `row` + r: one scalar base per tensor, a 32-bit offset from it (row strides are at most kMaxStride)
+template <class T>
+__device__ __forceinline__ T row_at(const void *base, int64_t row, int64_t ld, uint32_t r, uint32_t c) {
+    return *reinterpret_cast<const T *>(reinterpret_cast<const char *>(base) + row * ld * (int64_t)sizeof(T) + (r * (uint32_t)ld + c) * (uint32_t)sizeof(T));
+}
+
 // What a wave has in hand of the next eight rows.  Rows and bases are the same in all lanes (scalar registers); lanes without a channel
 // read the last one's, rows behind the end the last row's, so that all loads are one block without branches.
 template <class T, int NS, int P, bool HAS_U, bool HAS_C, bool HAS_Z, bool HAS_G>
@@ -171,29 +177,23 @@ struct Rows {
     T u[HAS_U ? kTile : 1], dt[kTile], z[HAS_Z ? kTile : 1], g[HAS_G ? kTile : 1];
     T b[kStates], c[HAS_C ? kStates : 1];
 
-    // one scalar base per tensor, 32-bit offsets from it (row strides are at most kMaxStride)
-    static __device__ __forceinline__ T at(const void *base, int64_t row, int64_t ld, uint32_t offset) {
-        return *reinterpret_cast<const T *>(reinterpret_cast<const char *>(base) + row * ld * (int64_t)sizeof(T) + offset);
-    }
     __device__ __forceinline__ void load(const ScanArgs &a, int64_t row, int n, uint32_t ch, int lane) {
-        const uint32_t z0 = sizeof(T), lu = (uint32_t)a.ld_u * z0, ld = (uint32_t)a.ld_dt * z0, lg = (uint32_t)a.ld_gy * z0, lz = (uint32_t)a.ld_z * z0,
-                       c0 = ch * z0;
 #pragma unroll
         for (int t = 0; t < kTile; ++t) {
             const uint32_t r = t < n ? t : n - 1;
-            if (HAS_U) u[t] = at(a.u, row, a.ld_u, r * lu + c0);
-            dt[t] = at(a.dt, row, a.ld_dt, r * ld + c0);
-            if (HAS_G) g[t] = at(a.gy, row, a.ld_gy, r * lg + c0);
+            if (HAS_U) u[t] = row_at<T>(a.u, row, a.ld_u, r, ch);
+            dt[t] = row_at<T>(a.dt, row, a.ld_dt, r, ch);
+            if (HAS_G) g[t] = row_at<T>(a.gy, row, a.ld_gy, r, ch);
         }
         if (HAS_Z && a.z)
 #pragma unroll
-            for (int t = 0; t < kTile; ++t) z[t] = at(a.z, row, a.ld_z, (uint32_t)(t < n ? t : n - 1) * lz + c0);
+            for (int t = 0; t < kTile; ++t) z[t] = row_at<T>(a.z, row, a.ld_z, t < n ? t : n - 1, ch);
 #pragma unroll
         for (int k = 0; k < kStates; ++k) {
             const int e = k * kWave + lane, s = e % SP;
             const uint32_t t = e / SP < n ? e / SP : n - 1, sc = s < a.states ? s : 0;
-            b[k] = at(a.B, row, a.ld_B, (t * (uint32_t)a.ld_B + sc) * z0);
-            if (HAS_C) c[k] = at(a.C, row, a.ld_C, (t * (uint32_t)a.ld_C + sc) * z0);
+            b[k] = row_at<T>(a.B, row, a.ld_B, t, sc);
+            if (HAS_C) c[k] = row_at<T>(a.C, row, a.ld_C, t, sc);
             if (s >= a.states) {
                 b[k] = T(0.0f);
                 if (HAS_C) c[k] = T(0.0f);
@@ -404,16 +404,23 @@ __global__ __launch_bounds__(kWave) void scan_bwd_local_kernel(ScanArgs a) {
     if (on && part == 0) a.sums[t.slot * a.channels + ch] = sum;
 }
 
+// The backward main pass.  A tile of eight rows at a time, from the last to the first: the lanes of a channel share the rows' own
+// numbers (step and its slope, dy, ...: each lane forms them for 8 / P rows) through LDS, which also keeps h before each row; so a lane's
+// registers hold one row, the loops stay loops (the body is several hundred instructions), and LDS alone (22 KiB a wave with sixteen
+// states) sets how many waves a CU holds.
 template <class T, int NS, int P>
-__global__ __launch_bounds__(kWave, 2) void scan_bwd_kernel(ScanArgs a) {
-    constexpr int SP = NS * P, CH = kWave / P;
-    __shared__ __attribute__((aligned(16))) float lds[2 * kTile * SP];
-    const int lane = lane_id(), part = lane / CH;
+__global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
+    constexpr int SP = NS * P, CH = kWave / P, PR = P < kTile ? kTile / P : 1, kStates = (kTile * SP + kWave - 1) / kWave;
+    __shared__ f32x4 hist[kTile][NS / 4][kWave];            // h before row j
+    __shared__ __attribute__((aligned(16))) float bc[2][kTile * SP];
+    __shared__ float own_rows[5][kTile][CH];                // step, u, slope, dy, dL/dy of the gate; later du, dstep, dgate
+    enum { kStep, kU, kSlope, kDy, kGate };
+    const int lane = lane_id(), part = lane / CH, col = lane % CH;
     const int64_t id = blockIdx.x;
     const int64_t worker = id / a.blocks;
     if (worker >= a.workers) return;
     const int block = (int)(id - worker * a.blocks);
-    const uint32_t ch = (uint32_t)block * CH + lane % CH, last = a.channels - 1, chc = ch < last ? ch : last;
+    const uint32_t ch = (uint32_t)block * CH + col, last = a.channels - 1, chc = ch < last ? ch : last;
     const bool on = ch <= last;
     float A2[NS], dA[NS], dD = 0.0f, dbias = 0.0f;          // A2 = A log2(e): dstep is summed with it and scaled once
     const float D = on && a.D ? a.D[ch] : 0.0f, bias = on && a.bias ? a.bias[ch] : 0.0f;
@@ -443,75 +450,130 @@ __global__ __launch_bounds__(kWave, 2) void scan_bwd_kernel(ScanArgs a) {
             else if (here && a.gfinal) G[i] = a.gfinal[(t.ray * a.channels + ch) * a.states + s];
         }
         const int64_t row0 = t.start + t.first, tiles = (t.n + kTile - 1) / kTile;
-        Rows<T, NS, P, true, true, true, true> rows;
-        for (int64_t k = tiles - 1; k >= 0; --k) {
+        auto rows_in = [&](int64_t k) { const int64_t r = t.n - k * kTile; return (int)(r < kTile ? r : kTile); };
+
+        // what the next tile needs from memory
+        T nu[PR], ndt[PR], nz[PR], ng[PR], nb[kStates], nc[kStates];
+        float nh[NS];
+        auto load = [&](int64_t k) {
             const int64_t row = row0 + k * kTile;
-            const int n = (int)(t.n - k * kTile < kTile ? t.n - k * kTile : kTile);
-            rows.load(a, row, n, chc, lane);
-            float h0[NS], h[kTile][NS];
-            Step st[kTile];
+            const int n = rows_in(k);
+#pragma unroll
+            for (int r = 0; r < PR; ++r) {
+                const int j = part * PR + r;
+                const uint32_t at = j < n ? j : n - 1;
+                nu[r] = row_at<T>(a.u, row, a.ld_u, at, chc);
+                ndt[r] = row_at<T>(a.dt, row, a.ld_dt, at, chc);
+                ng[r] = row_at<T>(a.gy, row, a.ld_gy, at, chc);
+                nz[r] = a.z ? row_at<T>(a.z, row, a.ld_z, at, chc) : T(0.0f);
+            }
+#pragma unroll
+            for (int q = 0; q < kStates; ++q) {
+                const int e = q * kWave + lane, s = e % SP;
+                const uint32_t at = e / SP < n ? e / SP : n - 1, sc = s < a.states ? s : 0;
+                nb[q] = row_at<T>(a.B, row, a.ld_B, at, sc);
+                nc[q] = row_at<T>(a.C, row, a.ld_C, at, sc);
+                if (s >= a.states) nb[q] = nc[q] = T(0.0f);
+            }
             const bool inside = t.first + k > 0;
             const float *from = inside ? a.kept + (row / kTile) * a.states * a.channels : a.init;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 const int s = part * NS + i;
-                h0[i] = 0.0f;
-                if (from && on && s < a.states) h0[i] = from[inside ? (uint32_t)s * a.channels + ch : (t.ray * a.channels + ch) * a.states + s];
+                nh[i] = 0.0f;
+                if (from && on && s < a.states) nh[i] = from[inside ? (uint32_t)s * a.channels + ch : (t.ray * a.channels + ch) * a.states + s];
             }
-            rows.stage(lds, lane);
+        };
+        if (tiles > 0) load(tiles - 1);
+        for (int64_t k = tiles - 1; k >= 0; --k) {
+            const int64_t row = row0 + k * kTile;
+            const int n = rows_in(k);
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int j = 0; j < kTile; ++j) {
-                const float raw = to_f(rows.dt[j]) + bias;
-                st[j] = {raw, 1.0f};
-                if (a.softplus) st[j] = softplus_step(raw);
-                const float in = st[j].step * to_f(rows.u[j]);
-                float B[NS];
-                read_states<NS>(lds + j * SP + part * NS, B);
-#pragma unroll
-                for (int i = 0; i < NS; ++i) h[j][i] = fmaf(fast_exp2(st[j].step * A2[i]), j ? h[j - 1][i] : h0[i], in * B[i]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int j = kTile - 1; j >= 0; --j) {
-                if (j >= n) continue;
-                // (lanes without a channel: no input and no gradient, so that they add nothing to dB and dC)
-                const float u = on ? to_f(rows.u[j]) : 0.0f, gy = on ? to_f(rows.g[j]) : 0.0f, in = st[j].step * u;
-                float step = st[j].step;
-                asm volatile("" : "+v"(step));              // (or the compiler keeps the exponentials of the first loop after all)
-                float z = 0.0f, sig = 0.0f, dy = gy;
+            for (int r = 0; r < PR; ++r) {
+                const int j = part * PR + r;
+                // lanes without a channel: no input and no gradient, so that they add nothing to dB and dC
+                const float raw = to_f(ndt[r]) + bias, u = on ? to_f(nu[r]) : 0.0f, gy = on ? to_f(ng[r]) : 0.0f;
+                Step st = {raw, 1.0f};
+                if (a.softplus) st = softplus_step(raw);
+                float dy = gy, gate = 0.0f;
                 if (a.z) {
-                    z = to_f(rows.z[j]);
-                    sig = sigmoid_f(z);
-                    dy = on ? gy * (z * sig) : 0.0f;
+                    const float z = on ? to_f(nz[r]) : 0.0f, sig = sigmoid_f(z);
+                    dy = gy * (z * sig);
+                    gate = gy * (sig * fmaf(z, 1.0f - sig, 1.0f));
                 }
-                float B[NS], C[NS], v[2 * NS], y = 0.0f, sB = 0.0f, sA = 0.0f;
-                read_states<NS>(lds + j * SP + part * NS, B);
-                read_states<NS>(lds + (kTile + j) * SP + part * NS, C);
+                if (P <= kTile || j < kTile) {
+                    own_rows[kStep][j][col] = on ? st.step : 0.0f;
+                    own_rows[kU][j][col] = u;
+                    own_rows[kSlope][j][col] = st.slope;
+                    own_rows[kDy][j][col] = dy;
+                    own_rows[kGate][j][col] = gate;
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < kStates; ++q) {
+                const int e = q * kWave + lane;
+                if (e < kTile * SP) {
+                    bc[0][e] = to_f(nb[q]);
+                    bc[1][e] = to_f(nc[q]);
+                }
+            }
+            float h[NS];
+#pragma unroll
+            for (int i = 0; i < NS; ++i) h[i] = nh[i];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (k > 0) load(k - 1);
+
+            auto states_at = [&](int which, int j, float (&v)[NS]) { read_states<NS>(&bc[which][j * SP + part * NS], v); };
+#pragma unroll 2
+            for (int j = 0; j < n; ++j) {
+                const float step = own_rows[kStep][j][col], in = step * own_rows[kU][j][col];
+                float B[NS];
+                states_at(0, j, B);
+#pragma unroll
+                for (int i = 0; i < NS; i += 4) hist[j][i / 4][lane] = f32x4{h[i], h[i + 1], h[i + 2], h[i + 3]};
+#pragma unroll
+                for (int i = 0; i < NS; ++i) h[i] = fmaf(fast_exp2(step * A2[i]), h[i], in * B[i]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 2
+            for (int j = n - 1; j >= 0; --j) {
+                const float step = own_rows[kStep][j][col], u = own_rows[kU][j][col], slope = own_rows[kSlope][j][col], dy = own_rows[kDy][j][col],
+                            gate = own_rows[kGate][j][col], in = step * u;
+                float B[NS], C[NS], before[NS], v[2 * NS], y = 0.0f, sB = 0.0f, sA = 0.0f;
+                states_at(0, j, B);
+                states_at(1, j, C);
+#pragma unroll
+                for (int i = 0; i < NS; i += 4) {
+                    const f32x4 q = hist[j][i / 4][lane];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) before[i + r] = q[r];
+                }
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
                     const float g = fmaf(C[i], dy, G[i]);
-                    y = fmaf(C[i], h[j][i], y);
-                    v[i] = on ? g * in : 0.0f;
-                    v[NS + i] = on ? dy * h[j][i] : 0.0f;
+                    y = fmaf(C[i], h[i], y);
+                    v[i] = g * in;
+                    v[NS + i] = dy * h[i];
                     sB = fmaf(g, B[i], sB);
-                    G[i] = g * fast_exp2(step * A2[i]);     // (formed again: kept, it would take 64 registers and a wave per SIMD)
-                    const float w = G[i] * (j ? h[j - 1][i] : h0[i]);
+                    G[i] = g * fast_exp2(step * A2[i]);
+                    const float w = G[i] * before[i];
                     sA = fmaf(w, A2[i], sA);
                     dA[i] = fmaf(w, step, dA[i]);
+                    h[i] = before[i];
                 }
                 sB = sum_parts<P>(sB);
                 sA = sum_parts<P>(sA);
-                const float dstep = fmaf(u, sB, sA * kLn2) * st[j].slope;
+                const float dstep = fmaf(u, sB, sA * kLn2) * slope;
                 if (a.z) y = fmaf(D, u, sum_parts<P>(y));
-                if (on && part == 0) {
-                    const int64_t at = row * a.channels;
-                    const uint32_t to = (uint32_t)j * a.channels + ch;
-                    (reinterpret_cast<T *>(a.gu) + at)[to] = from_f<T>(fmaf(step, sB, D * dy));
-                    (reinterpret_cast<T *>(a.gdt) + at)[to] = from_f<T>(dstep);
-                    if (a.z) (reinterpret_cast<T *>(a.gz) + at)[to] = from_f<T>(gy * y * (sig * fmaf(z, 1.0f - sig, 1.0f)));
-                    dD = fmaf(dy, u, dD);
-                    dbias += dstep;
+                if (part == 0) {
+                    own_rows[kU][j][col] = fmaf(step, sB, D * dy);
+                    own_rows[kSlope][j][col] = dstep;
+                    own_rows[kGate][j][col] = gate * y;
                 }
+                dD = fmaf(dy, u, dD);
+                dbias += dstep;
                 sum_over_lanes<2 * NS, CH / 2>(v, lane);
                 if (stores) {
                     float *to = a.part_bc + ((int64_t)block * a.rows + row + j) * (2 * SP);
@@ -521,7 +583,18 @@ __global__ __launch_bounds__(kWave, 2) void scan_bwd_kernel(ScanArgs a) {
                         to[(q / NS) * SP + part * NS + q % NS] = v[i];
                     }
                 }
-                __builtin_amdgcn_sched_barrier(0);          // one row at a time: rows in parallel would need twice the registers
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int r = 0; r < PR; ++r) {
+                const int j = part * PR + r;
+                if (!on || j >= n) continue;
+                const int64_t at = row * a.channels;
+                const uint32_t to = (uint32_t)j * a.channels + ch;
+                (reinterpret_cast<T *>(a.gu) + at)[to] = from_f<T>(own_rows[kU][j][col]);
+                (reinterpret_cast<T *>(a.gdt) + at)[to] = from_f<T>(own_rows[kSlope][j][col]);
+                if (a.z) (reinterpret_cast<T *>(a.gz) + at)[to] = from_f<T>(own_rows[kGate][j][col]);
             }
         }
         if (a.ginit && t.first == 0) {
@@ -687,7 +760,7 @@ ScanPlan scan_plan(int64_t n_rays, int64_t rows, int channels, int states, bool 
         }
     }
     p.workers = p.tasks;
-    const int64_t most = ceil_div(4096, p.blocks);
+    const int64_t most = ceil_div(16384, p.blocks);
     if (backward && p.workers > most) p.workers = most;
     return p;
 }
