@@ -406,12 +406,12 @@ __global__ __launch_bounds__(kWave) void scan_bwd_local_kernel(ScanArgs a) {
 
 // The backward main pass.  A tile of eight rows at a time, from the last to the first: the lanes of a channel share the rows' own
 // numbers (step and its slope, dy, ...: each lane forms them for 8 / P rows) through LDS, which also keeps h before each row; so a lane's
-// registers hold one row, the loops stay loops (the body is several hundred instructions), and LDS alone (22 KiB a wave with sixteen
-// states) sets how many waves a CU holds.
+// registers hold one row, the loops stay loops (the body is several hundred instructions), and LDS (20 KiB a wave with sixteen states:
+// eight waves on a CU) sets how many waves a CU holds.
 template <class T, int NS, int P>
 __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
     constexpr int SP = NS * P, CH = kWave / P, PR = P < kTile ? kTile / P : 1, kStates = (kTile * SP + kWave - 1) / kWave;
-    __shared__ f32x4 hist[kTile][NS / 4][kWave];            // h before row j
+    __shared__ f32x4 hist[kTile - 1][NS / 4][kWave];        // h after row j; before row 0 it stays in registers
     __shared__ __attribute__((aligned(16))) float bc[2][kTile * SP];
     __shared__ float own_rows[5][kTile][CH];                // step, u, slope, dy, dL/dy of the gate; later du, dstep, dgate
     enum { kStep, kU, kSlope, kDy, kGate };
@@ -518,9 +518,9 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
                     bc[1][e] = to_f(nc[q]);
                 }
             }
-            float h[NS];
+            float h[NS], h0[NS];
 #pragma unroll
-            for (int i = 0; i < NS; ++i) h[i] = nh[i];
+            for (int i = 0; i < NS; ++i) h[i] = h0[i] = nh[i];
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             if (k > 0) load(k - 1);
@@ -532,12 +532,12 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
                 float B[NS];
                 states_at(0, j, B);
 #pragma unroll
-                for (int i = 0; i < NS; i += 4) hist[j][i / 4][lane] = f32x4{h[i], h[i + 1], h[i + 2], h[i + 3]};
-#pragma unroll
                 for (int i = 0; i < NS; ++i) h[i] = fmaf(fast_exp2(step * A2[i]), h[i], in * B[i]);
+                if (j + 1 < n)
+#pragma unroll
+                    for (int i = 0; i < NS; i += 4) hist[j][i / 4][lane] = f32x4{h[i], h[i + 1], h[i + 2], h[i + 3]};
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 2
             for (int j = n - 1; j >= 0; --j) {
                 const float step = own_rows[kStep][j][col], u = own_rows[kU][j][col], slope = own_rows[kSlope][j][col], dy = own_rows[kDy][j][col],
                             gate = own_rows[kGate][j][col], in = step * u;
@@ -546,7 +546,8 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
                 states_at(1, j, C);
 #pragma unroll
                 for (int i = 0; i < NS; i += 4) {
-                    const f32x4 q = hist[j][i / 4][lane];
+                    f32x4 q = {h0[i], h0[i + 1], h0[i + 2], h0[i + 3]};
+                    if (j > 0) q = hist[j - 1][i / 4][lane];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) before[i + r] = q[r];
                 }
