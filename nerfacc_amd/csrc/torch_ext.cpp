@@ -8,6 +8,7 @@
 // argument checks (CHECK_INPUT, utils_cuda.cuh:12-17), allocation, the readback of the few integers that size
 // an output, the cache of the bit-packed occupancy grid.  No CPU path: a host tensor is an error.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -1710,6 +1711,311 @@ Tensor selective_scan_step(const Tensor &u, const Tensor &dt, const OptTensor &z
     return out;
 }
 
+// ---------------------------------------------------------------------------------------------------
+// the feature operators as a whole: refusals, autograd and the calls above in one go (the Python layer above this only names the
+// activation; nerfacc_amd/dense.py and selective.py hold the same steps for the ctypes face)
+// ---------------------------------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+inline Tensor get(const OptTensor &t) { return t && t->defined() ? *t : Tensor(); }
+
+void check_native(const char *op, const Tensor &x) {
+    TORCH_CHECK(x.is_cuda(), op, ": inputs must be a CUDA/HIP tensor (nerfacc_amd has no CPU kernels)");
+    const auto t = x.scalar_type();
+    TORCH_CHECK_TYPE(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, op, ": inputs must be float32, bfloat16 or float16, got ", t);
+}
+void check_like(const char *op, const char *what, const Tensor &t, const Tensor &x, at::IntArrayRef shape, at::ScalarType dtype) {
+    if (!t.defined()) return;
+    TORCH_CHECK(t.device() == x.device(), op, ": ", what, " is on ", t.device(), ", inputs on ", x.device());
+    TORCH_CHECK_TYPE(t.scalar_type() == dtype, op, ": ", what, " must have dtype ", dtype, ", got ", t.scalar_type());
+    TORCH_CHECK_VALUE(t.sizes() == shape, op, ": ", what, " must have shape ", shape, ", got ", t.sizes());
+}
+// whether autograd records the call; refuses one whose captured backward pass would end the process
+bool records_grad(const char *op, const Tensor &x, std::initializer_list<OptTensor> tensors) {
+    if (!at::GradMode::is_enabled()) return false;
+    bool any = false;
+    for (auto &t : tensors) any |= t && t->defined() && t->requires_grad();
+    if (!any) return false;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream_of(x), &status) != hipSuccess) (void)hipGetLastError();
+    TORCH_CHECK(status == hipStreamCaptureStatusNone || foreign_nodes(std::vector<OptTensor>(tensors)) == 0, op,
+                ": captured into a graph while an eager autograd graph of the same tensors lives (its backward pass could not be captured): drop the "
+                "eager outputs first, or call under torch.no_grad()");
+    return true;
+}
+// the results of a backward pass that differentiates once: using them in another one is an error, as torch's once_differentiable does it
+variable_list once(variable_list grads, const variable_list &outer) {
+    bool any = false;
+    for (auto &g : outer) any |= g.defined() && g.requires_grad();
+    if (!at::GradMode::is_enabled() || !any) return grads;
+    for (auto &g : grads)
+        if (g.defined()) g = g.detach().requires_grad_(true);
+    const size_t n = grads.size();
+    auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", n);
+    return (*error)(std::move(grads));
+}
+
+struct LinearFn : torch::autograd::Function<LinearFn> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &b, const OptTensor &r, int64_t act, bool learns) {
+        auto res = linear_fwd(x, w, b, r, act, learns);
+        const Tensor out = std::get<0>(res), kept = get(std::get<1>(res));
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["bias"] = b && b->defined();
+        ctx->saved_data["residual"] = r && r->defined();
+        if (learns) ctx->save_for_backward({x, w, !kept.defined() && act != NFA_ACT_NONE ? out : kept});
+        return out;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        variable_list out(6);
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+        const bool has_bias = ctx->saved_data["bias"].toBool(), need_b = has_bias && ctx->needs_input_grad(2);
+        if (need_x || need_w || need_b) {
+            const auto saved = ctx->get_saved_variables();
+            auto g = linear_bwd(grads[0], saved[0], saved[1], some(saved[2]), ctx->saved_data["act"].toInt(), need_x, need_w, need_b);
+            out[0] = get(std::get<0>(g));
+            out[1] = get(std::get<1>(g));
+            out[2] = get(std::get<2>(g));
+        }
+        if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(has_bias ? 3 : 2)) out[3] = grads[0];     // (counts the given tensors)
+        return once(out, grads);
+    }
+};
+
+Tensor linear(const Tensor &x, const Tensor &w, const OptTensor &b, const OptTensor &r, int64_t act) {
+    TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1), "linear: inputs (..., in) and weight (out, in) expected, got ", x.sizes(),
+                      " and ", w.sizes());
+    const int64_t n = w.size(0), k = w.size(1);
+    TORCH_CHECK_VALUE(n > 0 && k > 0, "linear: in_features and out_features must be at least 1");
+    check_native("linear", x);
+    at::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = n;
+    const auto dt = x.scalar_type();
+    check_like("linear", "weight", w, x, {n, k}, dt);
+    check_like("linear", "bias", get(b), x, {n}, dt);
+    check_like("linear", "residual", get(r), x, shape, dt);
+    const bool flat = x.dim() == 2;
+    const Tensor x2 = flat ? x : x.reshape({-1, k});
+    OptTensor r2 = some(get(r));
+    if (r2 && !flat) r2 = r2->reshape({-1, n});
+    const OptTensor b2 = some(get(b));
+    Tensor out;
+    if (records_grad("linear", x, {x, w, b, r})) {
+        const bool learns = x.requires_grad() || w.requires_grad() || (b2 && b2->requires_grad());
+        out = LinearFn::apply(x2, w, b2, r2, act, learns);
+    } else {
+        out = std::get<0>(linear_fwd(x2, w, b2, r2, act, false));
+    }
+    return flat ? out : out.view(shape);
+}
+
+// number of sequences of a batched or packed tensor
+int64_t sequences_of(const char *op, const Tensor &x, const OptTensor &info) {
+    int64_t n = 0;
+    if (!info || !info->defined()) {
+        TORCH_CHECK_VALUE(x.dim() == 3, op, ": inputs must be (n_rays, n, channels), or (n_samples, channels) with packed_info; got ", x.sizes());
+        n = x.size(0);
+    } else {
+        TORCH_CHECK_VALUE(x.dim() == 2, op, ": with packed_info inputs must be (n_samples, channels), got ", x.sizes());
+        TORCH_CHECK_VALUE(info->dim() == 2 && info->size(1) == 2, op, ": packed_info must be 2-D with shape (n_rays, 2), got ", info->sizes());
+        n = info->size(0);
+    }
+    TORCH_CHECK_VALUE(x.size(-1) > 0, op, ": at least one channel expected");
+    TORCH_CHECK_VALUE(n < (1ll << 31) && x.numel() / x.size(-1) < (1ll << 31), op, ": more than 2^31 - 1 rays or samples");
+    return n;
+}
+struct RowMap {
+    OptTensor info, ray, pos;
+    RowMap(const OptTensor &info_, const Tensor &x, int64_t n_rays) {
+        if (info_ && info_->defined()) info = info_->contiguous();
+        else if (n_rays == 0) info = at::empty({0, 2}, opts(x, at::kLong));
+        if (info) std::tie(ray, pos) = row_map(*info, x.size(0));
+    }
+};
+inline Tensor flat_rows(const Tensor &t) { return !t.defined() || t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
+
+struct CausalConvFn : torch::autograd::Function<CausalConvFn> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &b, const OptTensor &init, const OptTensor &info,
+                                 const OptTensor &ray, const OptTensor &pos, int64_t n_rays, int64_t act, bool want_final) {
+        ctx->set_materialize_grads(false);
+        auto res = causal_conv_fwd(x, w, b, init, info, ray, pos, n_rays, act, want_final);
+        ctx->save_for_backward({x, w, get(b), get(init), get(info), get(ray), get(pos)});
+        ctx->saved_data["n_rays"] = n_rays;
+        ctx->saved_data["act"] = act;
+        if (!want_final) return {std::get<0>(res)};
+        return {std::get<0>(res), *std::get<1>(res)};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const auto s = ctx->get_saved_variables();
+        const bool has_b = s[2].defined(), has_init = s[3].defined();
+        const Tensor gy = grads[0].defined() ? grads[0] : at::zeros_like(s[0]);
+        auto g = causal_conv_bwd(gy, grads.size() > 1 ? some(grads[1]) : std::nullopt, s[0], s[1], some(s[2]), some(s[3]), some(s[4]), some(s[5]), some(s[6]),
+                                 ctx->saved_data["n_rays"].toInt(), ctx->saved_data["act"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                 has_b && ctx->needs_input_grad(2), has_init && ctx->needs_input_grad(has_b ? 3 : 2));
+        variable_list out(10);
+        out[0] = get(std::get<0>(g)); out[1] = get(std::get<1>(g)); out[2] = get(std::get<2>(g)); out[3] = get(std::get<3>(g));
+        return once(out, grads);
+    }
+};
+
+int64_t check_width(const char *op, const Tensor &w, int64_t channels) {
+    TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) == channels && w.size(1) >= 2 && w.size(1) <= 4, op, ": weight must be (channels, width) with ", channels,
+                      " channels and width 2, 3 or 4, got ", w.sizes());
+    return w.size(1);
+}
+
+std::tuple<Tensor, OptTensor> causal_conv(const Tensor &x_, const Tensor &w, const OptTensor &b, const OptTensor &info, const OptTensor &init, int64_t act,
+                                          bool want_final) {
+    const int64_t n_rays = sequences_of("causal_conv", x_, info), d = x_.size(-1), width = check_width("causal_conv", w, d);
+    check_native("causal_conv", x_);
+    const auto dt = x_.scalar_type();
+    check_like("causal_conv", "weight", w, x_, {d, width}, dt);
+    check_like("causal_conv", "bias", get(b), x_, {d}, dt);
+    check_like("causal_conv", "packed_info", get(info), x_, {n_rays, 2}, at::kLong);
+    check_like("causal_conv", "initial_state", get(init), x_, {n_rays, width - 1, d}, dt);
+    const Tensor x = flat_rows(x_);
+    Guard g(device_of(x));
+    const RowMap m(info, x, n_rays);
+    const OptTensor b2 = some(get(b)), init2 = some(get(init));
+    Tensor out;
+    OptTensor last;
+    if (records_grad("causal_conv", x, {x_, w, b, init})) {
+        auto res = CausalConvFn::apply(x, w, b2, init2, m.info, m.ray, m.pos, n_rays, act, want_final);
+        out = res[0];
+        if (want_final) last = res[1];
+    } else {
+        std::tie(out, last) = causal_conv_fwd(x, w, b2, init2, m.info, m.ray, m.pos, n_rays, act, want_final);
+    }
+    return {x_.dim() == 2 ? out : out.view(x_.sizes()), last};
+}
+
+// where a step leaves its new state: `state` itself, or a buffer that shares no memory with it
+Tensor state_buffer(const char *op, const Tensor &state, const OptTensor &to_) {
+    const Tensor to = get(to_);
+    if (!to.defined()) return at::empty(state.sizes(), state.options());
+    TORCH_CHECK_VALUE(to.is_contiguous(), op, ": out_state must be contiguous");
+    if (state.numel() > 0 && !(to.data_ptr() == state.data_ptr() && state.is_contiguous())) {
+        int64_t reach = 1;
+        for (int64_t i = 0; i < state.dim(); ++i) reach += (state.size(i) - 1) * state.stride(i);
+        const char *a = (const char *)state.data_ptr(), *b = a + reach * state.element_size(), *c = (const char *)to.data_ptr(), *d = c + to.nbytes();
+        TORCH_CHECK_VALUE(!(a < d && c < b), op, ": out_state overlaps state; pass state itself to update it in place");
+    }
+    return to;
+}
+void refuse_grad(const char *op, const char *other, std::initializer_list<OptTensor> tensors) {
+    if (!at::GradMode::is_enabled()) return;
+    for (auto &t : tensors)
+        TORCH_CHECK(!(t && t->defined() && t->requires_grad()), op, " is not differentiable: call it under torch.no_grad(), or use ", other,
+                    " with initial_state");
+}
+void written(const OptTensor &to) {
+    if (to && to->defined() && !to->is_inference()) to->unsafeGetTensorImpl()->bump_version();
+}
+
+std::tuple<Tensor, Tensor> causal_conv_one(const Tensor &x, const Tensor &state, const Tensor &w, const OptTensor &b, int64_t act, const OptTensor &to_) {
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) > 0, "causal_conv_step: inputs must be (n_rays, channels)");
+    const int64_t r = x.size(0), d = x.size(1), width = check_width("causal_conv_step", w, d);
+    check_native("causal_conv_step", x);
+    const auto dt = x.scalar_type();
+    check_like("causal_conv_step", "state", state, x, {r, width - 1, d}, dt);
+    check_like("causal_conv_step", "weight", w, x, {d, width}, dt);
+    check_like("causal_conv_step", "bias", get(b), x, {d}, dt);
+    check_like("causal_conv_step", "out_state", get(to_), x, {r, width - 1, d}, dt);
+    refuse_grad("causal_conv_step", "causal_conv", {x, state, w, b, to_});
+    const Tensor to = state_buffer("causal_conv_step", state, to_);
+    const Tensor out = causal_conv_step(x, state, w, some(get(b)), act, to);
+    written(to_);
+    return {out, to};
+}
+
+struct SelectiveScanFn : torch::autograd::Function<SelectiveScanFn> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &u, const Tensor &dt, const Tensor &B, const Tensor &C, const Tensor &A, const OptTensor &z,
+                                 const OptTensor &D, const OptTensor &bias, const OptTensor &init, const OptTensor &info, const OptTensor &ray,
+                                 const OptTensor &pos, int64_t n_rays, bool softplus, bool want_final) {
+        ctx->set_materialize_grads(false);
+        auto res = selective_scan_fwd(u, dt, z, B, C, A, D, bias, init, info, ray, pos, n_rays, softplus, want_final, true);
+        ctx->save_for_backward({u, dt, B, C, A, get(z), get(D), get(bias), get(init), get(info), get(ray), get(pos), get(std::get<2>(res))});
+        ctx->saved_data["n_rays"] = n_rays;
+        ctx->saved_data["softplus"] = softplus;
+        if (!want_final) return {std::get<0>(res)};
+        return {std::get<0>(res), *std::get<1>(res)};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const auto s = ctx->get_saved_variables();
+        const Tensor gy = grads[0].defined() ? grads[0] : at::zeros_like(s[0]);
+        const auto g = selective_scan_bwd(gy, grads.size() > 1 ? some(grads[1]) : std::nullopt, s[0], s[1], some(s[5]), s[2], s[3], s[4], some(s[6]), some(s[7]),
+                                          some(s[8]), s[12], some(s[9]), some(s[10]), some(s[11]), ctx->saved_data["n_rays"].toInt(),
+                                          ctx->saved_data["softplus"].toBool());
+        // forward's order: u, dt, B, C, A, z, D, bias, init; needs_input_grad counts the tensors that were given
+        static constexpr int from[9] = {0, 1, 3, 4, 5, 2, 6, 7, 8};
+        variable_list out(15);
+        int given = 0;
+        for (int i = 0; i < 9; ++i) {
+            if (!s[i].defined()) continue;
+            if (ctx->needs_input_grad(given++)) out[i] = get(g[from[i]]);
+        }
+        return once(out, grads);
+    }
+};
+
+void check_scan(const char *op, const Tensor &x, at::IntArrayRef rows, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const OptTensor &D,
+                const OptTensor &z, const OptTensor &bias) {
+    TORCH_CHECK_VALUE(A.dim() == 2 && A.size(1) >= 1 && A.size(1) <= NFA_SCAN_MAX_STATES, op, ": A must be (channels, states) with 1 to ", NFA_SCAN_MAX_STATES,
+                      " states, got ", A.sizes());
+    check_native(op, x);
+    const int64_t d = x.size(-1), s = A.size(1);
+    at::DimVector wide(rows.begin(), rows.end()), narrow(wide);
+    wide.push_back(d);
+    narrow.push_back(s);
+    const auto t = x.scalar_type();
+    check_like(op, "delta", dt, x, wide, t);
+    check_like(op, "A", A, x, {d, s}, at::kFloat);
+    check_like(op, "B", B, x, narrow, t);
+    check_like(op, "C", C, x, narrow, t);
+    check_like(op, "D", get(D), x, {d}, at::kFloat);
+    check_like(op, "gate", get(z), x, wide, t);
+    check_like(op, "delta_bias", get(bias), x, {d}, at::kFloat);
+}
+
+std::tuple<Tensor, OptTensor> selective_scan(const Tensor &x_, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const OptTensor &D,
+                                             const OptTensor &z, const OptTensor &bias, bool softplus, const OptTensor &info, const OptTensor &init,
+                                             bool want_final) {
+    const int64_t n_rays = sequences_of("selective_scan", x_, info);
+    check_scan("selective_scan", x_, x_.sizes().slice(0, x_.dim() - 1), dt, A, B, C, D, z, bias);
+    check_like("selective_scan", "packed_info", get(info), x_, {n_rays, 2}, at::kLong);
+    check_like("selective_scan", "initial_state", get(init), x_, {n_rays, x_.size(-1), A.size(1)}, at::kFloat);
+    Guard g(device_of(x_));
+    const Tensor x = flat_rows(x_);
+    const RowMap m(info, x, n_rays);
+    const OptTensor z2 = some(flat_rows(get(z))), D2 = some(get(D)), bias2 = some(get(bias)), init2 = some(get(init));
+    Tensor out;
+    OptTensor last;
+    if (records_grad("selective_scan", x, {x_, dt, A, B, C, D, z, bias, init})) {
+        auto res = SelectiveScanFn::apply(x, flat_rows(dt), flat_rows(B), flat_rows(C), A, z2, D2, bias2, init2, m.info, m.ray, m.pos, n_rays, softplus, want_final);
+        out = res[0];
+        if (want_final) last = res[1];
+    } else {
+        OptTensor kept;
+        std::tie(out, last, kept) = selective_scan_fwd(x, flat_rows(dt), z2, flat_rows(B), flat_rows(C), A, D2, bias2, init2, m.info, m.ray, m.pos, n_rays, softplus,
+                                                       want_final, false);
+    }
+    return {x_.dim() == 2 ? out : out.view(x_.sizes()), last};
+}
+
+std::tuple<Tensor, Tensor> selective_scan_one(const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Tensor &state,
+                                              const OptTensor &D, const OptTensor &z, const OptTensor &bias, bool softplus, const OptTensor &to_) {
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) > 0, "selective_scan_step: inputs must be (n_rays, channels)");
+    check_scan("selective_scan_step", x, x.sizes().slice(0, 1), dt, A, B, C, D, z, bias);
+    const int64_t r = x.size(0), d = x.size(1), s = A.size(1);
+    check_like("selective_scan_step", "state", state, x, {r, d, s}, at::kFloat);
+    check_like("selective_scan_step", "out_state", get(to_), x, {r, d, s}, at::kFloat);
+    refuse_grad("selective_scan_step", "selective_scan", {x, dt, A, B, C, D, z, bias, state, to_});
+    const Tensor to = state_buffer("selective_scan_step", state, to_);
+    const Tensor out = selective_scan_step(x, dt, some(get(z)), B, C, A, some(get(D)), some(get(bias)), state, softplus, to);
+    written(to_);
+    return {out, to};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1797,6 +2103,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("grid_occupied_cells", &grid_occupied_cells);
     m.def("set_timing", &set_timing, "names"_a = py::none());
     m.def("timing_summary", &timing_summary);
+    m.def("linear", &linear);
+    m.def("causal_conv", &causal_conv);
+    m.def("causal_conv_one", &causal_conv_one);
+    m.def("selective_scan", &selective_scan);
+    m.def("selective_scan_one", &selective_scan_one);
     m.def("foreign_nodes", &foreign_nodes);
     m.def("linear_fwd", &linear_fwd);
     m.def("linear_bwd", &linear_bwd);

@@ -14,6 +14,20 @@ _ACTIVATIONS = {None: 0, "relu": 1, "sigmoid": 2, "softplus": 3, "silu": 4, "gel
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
+_EXT = None                   # the torch extension, False on the ctypes face, None before the first call
+
+
+def _ext():
+    """the torch extension, which holds each operator as one call (refusals, autograd and launch); False on the ctypes face, where the
+    same steps are Python"""
+    global _EXT
+    if _EXT is None:
+        from .cuda import _backend
+
+        _EXT = _backend._C if _backend.BACKEND == "ext" else False
+    return _EXT
+
+
 def _check_native(name: str, ref: Tensor, others) -> None:
     """the refusals that every feature operator shares; `others`: (name, tensor or None, shape, dtype)"""
     if not ref.is_cuda:
@@ -68,6 +82,9 @@ def linear(inputs: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activa
         tensor([[3., 0.]], device='cuda:0')
     """
     act = _activation_id("linear", activation)
+    ext = _EXT or _ext()
+    if ext:
+        return ext.linear(inputs, weight, bias, residual, act)
     if not isinstance(inputs, Tensor) or not isinstance(weight, Tensor):
         raise TypeError("linear: inputs and weight must be torch.Tensors")
     if inputs.dim() < 1 or weight.dim() != 2 or inputs.shape[-1] != weight.shape[1]:

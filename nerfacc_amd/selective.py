@@ -12,7 +12,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import cuda as _C
-from .dense import _activation_id, _check_native, _records_grad
+from .dense import _activation_id, _check_native, _ext, _records_grad
 
 _MAX_STATES = 256
 
@@ -92,6 +92,10 @@ def causal_conv(inputs: Tensor, weight: Tensor, bias: Optional[Tensor] = None, a
         tensor([[10.], [21.], [30.]], device='cuda:0')
     """
     act = _activation_id("causal_conv", activation, (None, "silu"))
+    ext = _ext()
+    if ext:
+        out = ext.causal_conv(inputs, weight, bias, packed_info, initial_state, act, return_final_state)
+        return out if return_final_state else out[0]
     n_rays = _sequences("causal_conv", inputs, packed_info)
     channels, dt = inputs.shape[-1], inputs.dtype
     width = _width("causal_conv", weight, channels)
@@ -144,6 +148,9 @@ def causal_conv_step(inputs: Tensor, state: Tensor, weight: Tensor, bias: Option
         (tensor([[32.]], device='cuda:0'), tensor([[[3.]]], device='cuda:0'))
     """
     act = _activation_id("causal_conv_step", activation, (None, "silu"))
+    ext = _ext()
+    if ext:
+        return ext.causal_conv_one(inputs, state, weight, bias, act, out_state)
     if not isinstance(inputs, Tensor) or inputs.dim() != 2 or inputs.shape[1] == 0:
         raise ValueError("causal_conv_step: inputs must be (n_rays, channels)")
     n_rays, channels = inputs.shape
@@ -191,6 +198,10 @@ def selective_scan(inputs: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tenso
         >>> selective_scan(one, one, torch.zeros(1, 1, device="cuda"), one, one, packed_info=torch.tensor([[0, 2], [2, 1]], device="cuda"))
         tensor([[1.], [2.], [1.]], device='cuda:0')
     """
+    ext = _ext()
+    if ext:
+        out = ext.selective_scan(inputs, delta, A, B, C, D, gate, delta_bias, bool(delta_softplus), packed_info, initial_state, return_final_state)
+        return out if return_final_state else out[0]
     n_rays = _sequences("selective_scan", inputs, packed_info)
     rows, channels = inputs.shape[:-1], inputs.shape[-1]
     _check_scan("selective_scan", inputs, rows, channels, n_rays, delta, A, B, C, D, gate, delta_bias,
@@ -244,6 +255,9 @@ def selective_scan_step(inputs: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: 
     """One more sample of every ray: inputs, delta, gate (n_rays, channels), B, C (n_rays, states) and the rays' state (n_rays, channels,
     states) float32 -> (outputs, new state), as `selective_scan` of one row each.  The new state goes to `out_state` if given
     (`out_state=state` updates it in place).  Not differentiable."""
+    ext = _ext()
+    if ext:
+        return ext.selective_scan_one(inputs, delta, A, B, C, state, D, gate, delta_bias, bool(delta_softplus), out_state)
     if not isinstance(inputs, Tensor) or inputs.dim() != 2 or inputs.shape[1] == 0:
         raise ValueError("selective_scan_step: inputs must be (n_rays, channels)")
     if not isinstance(state, Tensor):

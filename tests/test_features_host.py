@@ -9,7 +9,18 @@ import nerfacc_amd as nerfacc
 from nerfacc_amd.cuda import _backend
 
 
-def test_arguments_are_refused_before_the_device_is_asked_for():
+@pytest.fixture(params=["extension", "python"])
+def face(request, monkeypatch):
+    """the operators as one call of the extension, and as the Python steps of the ctypes face"""
+    from nerfacc_amd import dense
+
+    if request.param == "python":
+        monkeypatch.setattr(dense, "_EXT", False)
+    elif _backend.BACKEND != "ext":
+        pytest.skip("torch extension not the active backend")
+
+
+def test_arguments_are_refused_before_the_device_is_asked_for(face):
     x, w = torch.rand(4, 8), torch.rand(8, 4)
     info = torch.tensor([[0, 4]])
     with pytest.raises(ValueError):
@@ -38,7 +49,7 @@ def test_arguments_are_refused_before_the_device_is_asked_for():
         nerfacc.causal_conv_step(x, None, w)
 
 
-def test_host_tensors_are_refused():
+def test_host_tensors_are_refused(face):
     x, w, info = torch.rand(4, 8), torch.rand(8, 4), torch.tensor([[0, 4]])
     A, bc = torch.rand(8, 3), torch.rand(4, 3)
     for call in (lambda: nerfacc.linear(x, torch.rand(3, 8)), lambda: nerfacc.causal_conv(x, w, packed_info=info),

@@ -470,3 +470,75 @@ def test_both_host_faces_agree():
     same(*(f.selective_scan_bwd(c["gy"], c["gf"], *flat, c["init"], kept, info, *maps, 9, True) for f, kept in ((ext, a[2]), (ct, b[2]))))
     first = [t[:9] if t.shape[0] == 85 else t for t in flat]
     same(*((f.selective_scan_step(*first, c["init"], True, to), to) for f, to in ((ext, c["init"].clone()), (ct, c["init"].clone()))))
+
+
+def test_python_and_extension_steps_agree(monkeypatch):
+    """the operators as one call of the extension and as the Python steps of the ctypes face: the same bits, gradients included"""
+    import nerfacc_amd as nerfacc
+    from nerfacc_amd import dense
+
+    c, info = layer_inputs(80, torch.bfloat16, seed=3), packed(LENS)
+    gy = torch.randn(80, 24, generator=generator(7), device=DEV).bfloat16()
+    s = scan_inputs(80, 9, 24, 16, torch.float32, seed=2)
+    k = conv_inputs(80, 9, 24, 4, torch.float32, seed=2, state=True)
+
+    def everything():
+        own = {n: v.detach().requires_grad_(True) for n, v in c.items()}
+        out = layer(own, info)
+        res = [out.detach(), *torch.autograd.grad(out, list(own.values()), gy)]
+        own = {n: s[n].detach().requires_grad_(True) for n in NAMES}
+        for outs in (call_scan(s, own, info), call_scan(s, own, info)[:1], call_scan(s, own, info)[1:]):      # both results used, or one
+            gs = [s["gy"] if o.dim() == 2 else s["gf"] for o in outs]
+            res += [g for g in torch.autograd.grad(outs, list(own.values()), gs, allow_unused=True) if g is not None]
+        x, w, init = (k[n].detach().requires_grad_(True) for n in ("x", "w", "init"))
+        for w_, b_ in ((w, k["b"]), (k["w"], None)):
+            outs = nerfacc.causal_conv(x, w_, b_, packed_info=info, initial_state=init, return_final_state=True)
+            res += torch.autograd.grad(outs, [t for t in (x, w_, init) if t.requires_grad], [k["gy"], k["gf"]])
+        with torch.no_grad():
+            res += [*nerfacc.causal_conv_step(k["x"][:9], k["init"], k["w"], k["b"]),
+                    *nerfacc.selective_scan_step(s["u"][:9], s["delta"][:9], s["A"], s["B"][:9], s["C"][:9], s["init"], D=s["D"], delta_bias=s["bias"],
+                                                 delta_softplus=True)]
+        return res
+
+    a = everything()
+    monkeypatch.setattr(dense, "_EXT", False)
+    b = everything()
+    assert len(a) == len(b) and all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_steps_refuse_gradients_and_overlapping_states(monkeypatch):
+    import nerfacc_amd as nerfacc
+    from nerfacc_amd import dense
+
+    for ext in (None, False):
+        monkeypatch.setattr(dense, "_EXT", ext)
+        w, A = torch.rand(8, 4, device=DEV), torch.rand(8, 4, device=DEV)
+        x, bc = torch.rand(2, 8, device=DEV), torch.rand(2, 4, device=DEV)
+        pool, wide = torch.rand(3, 3, 8, device=DEV), torch.rand(3, 8, 4, device=DEV)
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            nerfacc.causal_conv_step(x, pool[:2], w.clone().requires_grad_(True))
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            nerfacc.selective_scan_step(x, x, A, bc, bc, wide[:2].clone().requires_grad_(True))
+        with pytest.raises(ValueError, match="overlaps"):
+            nerfacc.causal_conv_step(x, pool[:2], w, out_state=pool[1:])
+        with pytest.raises(ValueError, match="overlaps"):
+            nerfacc.selective_scan_step(x, x, A, bc, bc, wide[:2], out_state=wide[1:])
+        with pytest.raises(ValueError, match="contiguous"):
+            nerfacc.causal_conv_step(x, pool[:2], w, out_state=torch.rand(2, 8, 3, device=DEV).transpose(1, 2))
+        before = pool._version
+        nerfacc.causal_conv_step(x, pool[:2], w, out_state=pool[:2])
+        assert pool._version > before                                 # autograd and views see the write
+
+
+def test_differentiating_twice_is_refused(monkeypatch):
+    import nerfacc_amd as nerfacc
+    from nerfacc_amd import dense
+
+    for ext in (None, False):
+        monkeypatch.setattr(dense, "_EXT", ext)
+        x = torch.rand(4, 8, device=DEV, requires_grad=True)
+        w = torch.rand(8, 8, device=DEV)
+        gy = torch.rand(4, 8, device=DEV, requires_grad=True)
+        gx = torch.autograd.grad(nerfacc.linear(x, w, activation="silu"), x, gy, create_graph=True)[0]
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            gx.sum().backward()
