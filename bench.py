@@ -304,9 +304,10 @@ def parse_args():
     ap.add_argument("--exchange-mode", choices=("allreduce", "rs_ag"), default="allreduce",
                     help="gradient exchange of ExchangeAdam (N > 1): chunked all-reduce + Adam on every rank, or reduce-scatter -> Adam on the "
                          "local 1/N -> all-gather of the parameters; the OTHER mode is timed for a few steps as aux.exchange_modes")
-    ap.add_argument("--field", choices=("grid", "grid+mlp"), default="grid",
+    ap.add_argument("--field", choices=("grid", "grid+mlp", "grid+mlp-fused"), default="grid",
                     help="grid = the headline's dense-grid field (one parameter tensor); grid+mlp = feature grid + two-layer MLP (seven "
-                         "tensors: exercises the gradient hooks and the chunk order of the exchange on a multi-tensor graph; dry runs)")
+                         "tensors: exercises the gradient hooks and the chunk order of the exchange on a multi-tensor graph; dry runs); "
+                         "grid+mlp-fused = the same field, its layers through nerfacc.linear")
     ap.add_argument("--dist-backend", default="nccl", help="torch.distributed backend for N > 1 (nccl = RCCL; gloo for dry runs)")
     ap.add_argument("--all-ranks-on-device0", action="store_true",
                     help="dry run of the N > 1 code path on a single GPU (with --dist-backend gloo): every rank uses cuda:0")
@@ -368,8 +369,8 @@ def run(args):
 
     torch.manual_seed(42)
     teacher = DenseGridField(AABB, GRID_RES).to(device).eval()          # the analytic scene sampled on a grid
-    if args.field == "grid+mlp":
-        field = GridMlpField(AABB).to(device)
+    if args.field != "grid":
+        field = GridMlpField(AABB, fused=args.field == "grid+mlp-fused").to(device)
     else:
         field = DenseGridField(AABB, GRID_RES).to(device)
         with torch.no_grad():                                           # the student starts from fog and grey

@@ -74,8 +74,9 @@ class GridMlpField(torch.nn.Module):
     parameter tensors from 4 floats to 8 x res^3, reached by autograd in reverse order.  Not the headline field: it exists so that
     the multi-GPU path (ExchangeAdam's hooks, chunk order, both exchange modes) is exercised on a multi-tensor graph."""
 
-    def __init__(self, aabb, res=64, feat=8, hidden=32):
+    def __init__(self, aabb, res=64, feat=8, hidden=32, fused=False):
         super().__init__()
+        self.fused = fused                          # the decoder's layers through nerfacc.linear (`--field grid+mlp-fused`)
         self.register_buffer("aabb", torch.tensor(aabb, dtype=torch.float32))
         lo, hi = self.aabb[:3], self.aabb[3:]
         gen = torch.Generator().manual_seed(7)
@@ -90,6 +91,10 @@ class GridMlpField(torch.nn.Module):
     def _decode(self, x):
         u = torch.addcmul(self.u_shift, x, self.u_scale).view(1, 1, 1, -1, 3)
         f = F.grid_sample(self.grid, u, mode="bilinear", padding_mode="border", align_corners=False).view(self.grid.shape[1], -1).t()
+        if self.fused:
+            f = nerfacc.linear(f, self.l1.weight, self.l1.bias, activation="relu")
+            f = nerfacc.linear(f, self.l2.weight, self.l2.bias, activation="relu")
+            return nerfacc.linear(f, self.l3.weight, self.l3.bias)
         return self.l3(torch.relu(self.l2(torch.relu(self.l1(f)))))
 
     def query_density(self, x):

@@ -389,7 +389,8 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
 }
 
 // ---- tile by tile ------------------------------------------------------------------------------------------------------
-// LDS layouts.  c-contiguous tiles: 128-byte rows, the 16-byte chunks of row r exchanged by r & 7.  Transposed tiles (rows along c,
+// LDS layouts.  c-contiguous tiles: 128-byte rows, the 16-byte chunks of row r exchanged by r / 2 & 7: sixteen rows of one chunk lie
+// in all banks.  Transposed tiles (rows along c,
 // 64 or 128 columns): the 32-byte (16-bit types) or 64-byte units of a row exchanged so that the rows that one instruction reads
 // lie in different banks.
 template <class T, int COLS>
@@ -400,7 +401,7 @@ __device__ __forceinline__ int unit_swizzle(int row) {
 }
 template <class T, bool TR, int ROWS>
 __device__ __forceinline__ int stage_offset(int row, int chunk) {        // byte offset of a chunk in its tile
-    if (!TR) return row * kRowBytes + ((chunk ^ (row & 7)) << 4);
+    if (!TR) return row * kRowBytes + ((chunk ^ ((row >> 1) & 7)) << 4);
     if (sizeof(T) == 4) return row * ROWS * 4 + (((chunk >> 2) ^ unit_swizzle<T, ROWS>(row)) << 6) + ((chunk & 3) << 4);
     return row * ROWS * 2 + (((chunk >> 1) ^ unit_swizzle<T, ROWS>(row)) << 5) + ((chunk & 1) << 4);
 }

@@ -237,3 +237,26 @@ def test_refusals():
     gx = torch.autograd.grad(nerfacc.linear(xl, w).sum(), xl, create_graph=True)[0]
     with pytest.raises(RuntimeError):
         gx.sum().backward()
+
+
+def test_the_grid_and_mlp_field_through_it():
+    """a training step of the bench's grid + MLP field (sampling, field, rendering, gradients) with its decoder's layers fused"""
+    import nerfacc_amd as nerfacc
+    from benchlib.scene import AABB, GridMlpField, make_ray_pool, render_rays
+
+    torch.manual_seed(0)
+    plain, fused = GridMlpField(AABB, res=32).to(DEV), GridMlpField(AABB, res=32, fused=True).to(DEV)
+    fused.load_state_dict(plain.state_dict())
+    est = nerfacc.OccGridEstimator(roi_aabb=AABB, resolution=32, levels=1).to(DEV).eval()
+    est.binaries.fill_(True)
+    o, d = make_ray_pool(512, seed=3, device=DEV)
+    x = torch.rand(1000, 3, device=DEV) * 3 - 1.5
+    for a, b in zip(plain(x), fused(x)):                    # three layers of at most 32 terms: some hundred last places of 32 bits
+        assert torch.allclose(a, b, rtol=2e-5, atol=2e-6)
+    grads = []
+    for field in (plain, fused):
+        rgb, acc, depth, n = render_rays(field, est, o, d, torch.ones(3, device=DEV), False)
+        assert n > 1000
+        grads.append([rgb.detach(), *torch.autograd.grad((rgb - 0.3).square().sum(), list(field.parameters()))])
+    for a, b in zip(*grads):                                # atomic sums in torch's scatter and products: relative to the tensor's own size
+        assert (a - b).abs().max() <= 1e-4 * a.abs().max() + 1e-7
