@@ -44,22 +44,30 @@ struct DenseArgs {
 
 enum { kForward, kDgrad, kWgrad };
 
-// sixteen bytes of row `row`, zeros outside the array.  VEC: every row starts on 16 bytes and holds whole chunks; the load is then
-// made in any case, from a place that exists, so that a tile's loads are one block without branches
+// Sixteen bytes of row `row`.  VEC: every row starts on 16 bytes and holds whole chunks; the load is then made in any case, from a place
+// that exists, so that a tile's loads are one block without branches, and only_inside() clears what lies outside the array where the
+// value is used: a select right behind the load would wait for it.  Otherwise number by number, zeros outside.
 template <class T, bool VEC>
 __device__ __forceinline__ u32x4 load_chunk(const T *base, int64_t row, int64_t rows, int64_t ld, int64_t col, int64_t cols) {
-    u32x4 v = {0, 0, 0, 0};
-    const bool inside = row < rows && col < cols;
     if constexpr (VEC) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(base + (row < rows ? row : rows - 1) * ld + (col < cols ? col : 0));
+        return *reinterpret_cast<const u32x4 *>(base + (row < rows ? row : rows - 1) * ld + (col < cols ? col : 0));
+    } else {
+        u32x4 v = {0, 0, 0, 0};
+        if (row < rows && col < cols) {
+            T e[kChunk<T>];
+            base += row * ld + col;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = inside ? w[i] : 0;
-    } else if (inside) {
-        T e[kChunk<T>];
-        base += row * ld + col;
+            for (int i = 0; i < kChunk<T>; ++i) e[i] = col + i < cols ? base[i] : T(0.0f);
+            __builtin_memcpy(&v, e, 16);
+        }
+        return v;
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ u32x4 only_inside(u32x4 v, bool inside) {
+    if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < kChunk<T>; ++i) e[i] = col + i < cols ? base[i] : T(0.0f);
-        __builtin_memcpy(&v, e, 16);
+        for (int i = 0; i < 4; ++i) v[i] = inside ? v[i] : 0;
     }
     return v;
 }
@@ -244,13 +252,13 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
     if (MODE == kForward) {
         for (int e = threadIdx.x; e < q_rows * KS * 4; e += blockDim.x) {
             const int q = e / (KS * 4), chunk = e % (KS * 4);
-            const u32x4 v = load_chunk<T, VEC>(Q, q0 + q, q0 + nq, a.ld_q, chunk * CE, a.n_c);
+            const u32x4 v = only_inside<VEC>(load_chunk<T, VEC>(Q, q0 + q, q0 + nq, a.ld_q, chunk * CE, a.n_c), q < nq && chunk * CE < a.n_c);
             *reinterpret_cast<u32x4 *>(lds + weight_offset<T, KS>((q & ~31) + place_of_column<T>(q & 31), chunk)) = v;
         }
     } else {
         for (int e = threadIdx.x; e < KS * 4 * CE * pitch; e += blockDim.x) {
             const int n = e / pitch, chunk = e - n * pitch;
-            const u32x4 v = load_chunk<T, VEC>(Q + q0, n, a.n_c, a.ld_q, chunk * CE, nq);
+            const u32x4 v = only_inside<VEC>(load_chunk<T, VEC>(Q + q0, n, a.n_c, a.ld_q, chunk * CE, nq), n < a.n_c && chunk * CE < nq);
             *reinterpret_cast<u32x4 *>(lds + weight_offset_t<T>(n, chunk, pitch)) = v;
         }
     }
@@ -276,7 +284,8 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
 #pragma unroll
             for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int k = 0; k < KS; ++k) x[r * KS + k] = load_chunk<T, VEC>(P, p0 + r * 16 + i, a.n_p, a.ld_p, (k * 4 + g) * CE, a.n_c);
+                for (int k = 0; k < KS; ++k)
+                    x[r * KS + k] = only_inside<VEC>(load_chunk<T, VEC>(P, p0 + r * 16 + i, a.n_p, a.ld_p, (k * 4 + g) * CE, a.n_c), (k * 4 + g) * CE < a.n_c);
         }
         if constexpr (MODE == kDgrad) {
             if (a.act != NFA_ACT_NONE) {
@@ -299,7 +308,8 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) s[r * KS + k] = load_saved<T, VEC>(a, p0 + r * 16 + i, a.n_p, (k * 4 + g) * CE, a.n_c);
+                    for (int k = 0; k < KS; ++k)
+                        s[r * KS + k] = only_inside<VEC>(load_saved<T, VEC>(a, p0 + r * 16 + i, a.n_p, (k * 4 + g) * CE, a.n_c), (k * 4 + g) * CE < a.n_c);
                 form_dz<T, SPLIT, RT * KS>(a, x, s, lo, [](int, float, int) {});
             }
         }
@@ -494,8 +504,16 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
             rq[k] = load_chunk<T, VEC>(Q, r, rows, a.ld_q, col, cols);
         }
     };
-    auto store = [&](char *buf) {
+    auto store = [&](char *buf, int64_t c) {
         u32x4 lo[SPLIT ? CP : 1];
+#pragma unroll
+        for (int k = 0; k < CP; ++k) {
+            int row, chunk;
+            place(PT, BP, k, row, chunk);
+            const bool inside = PT ? c + row < c_end && p0 + chunk * CE < a.n_p : p0 + row < a.n_p && c + chunk * CE < a.n_c;
+            rp[k] = only_inside<VEC>(rp[k], inside);
+            if (FUSE) rs[k] = only_inside<VEC>(rs[k], inside);
+        }
         if constexpr (FUSE)
             form_dz<T, SPLIT, CP>(a, rp, rs, lo, [&](int, float dz, int e) {
                 if constexpr (MODE == kWgrad) db[e] += dz;
@@ -511,7 +529,8 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
         for (int k = 0; k < CQ; ++k) {
             int row, chunk;
             place(QT, BQ, k, row, chunk);
-            *reinterpret_cast<u32x4 *>(buf + kBuf - BQ * kRowBytes + stage_offset<T, QT, BQ>(row, chunk)) = rq[k];
+            const bool inside = QT ? c + row < c_end && q0 + chunk * CE < a.n_q : q0 + row < a.n_q && c + chunk * CE < a.n_c;
+            *reinterpret_cast<u32x4 *>(buf + kBuf - BQ * kRowBytes + stage_offset<T, QT, BQ>(row, chunk)) = only_inside<VEC>(rq[k], inside);
         }
     };
     auto compute = [&](const char *buf, int64_t c) {
@@ -534,14 +553,14 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
     };
 
     load(c_begin);
-    store(lds);
+    store(lds, c_begin);
     __syncthreads();
     int cur = 0;
     for (int64_t c = c_begin; c < c_end; c += ST) {
         const bool more = c + ST < c_end;
         if (more) load(c + ST);
         compute(lds + cur * kBuf, c);
-        if (more) store(lds + (cur ^ 1) * kBuf);
+        if (more) store(lds + (cur ^ 1) * kBuf, c + ST);
         __syncthreads();
         cur ^= 1;
     }
