@@ -36,7 +36,7 @@ __device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcp
 // sigmoid with the exponential taken of -|x|: no overflow at either end, and a relative error of a few ulp at both
 __device__ __forceinline__ float sigmoid_f(float x) {
     const float e = fast_exp2(-fabsf(x) * kLog2e), r = fast_rcp(1.0f + e);
-    return x != x ? x : (x >= 0.0f ? r : e * r);
+    return x >= 0.0f ? r : e * r;                            // (NaN: e and r are)
 }
 
 // log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1], with log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, as its odd
@@ -52,7 +52,7 @@ __device__ __forceinline__ float softplus_from(float x, float e) {         // e 
     p = fmaf(p, q, 1.0f / 5.0f);
     p = fmaf(p, q, 1.0f / 3.0f);
     p = fmaf(p, q, 1.0f);
-    return x != x ? x : fmaxf(x, 0.0f) + 2.0f * s * p;
+    return fmaf(s + s, p, fmaxf(x, 0.0f));                   // (NaN: s is)
 }
 __device__ __forceinline__ float softplus_f(float x) { return softplus_from(x, fast_exp2(-fabsf(x) * kLog2e)); }
 

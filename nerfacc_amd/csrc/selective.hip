@@ -169,46 +169,41 @@ __device__ __forceinline__ T row_at(const void *base, int64_t row, int64_t ld, u
     return *reinterpret_cast<const T *>(reinterpret_cast<const char *>(base) + row * ld * (int64_t)sizeof(T) + (r * (uint32_t)ld + c) * (uint32_t)sizeof(T));
 }
 
-// What a wave has in hand of the next eight rows.  Rows and bases are the same in all lanes (scalar registers); lanes without a channel
-// read the last one's, rows behind the end the last row's, so that all loads are one block without branches.
+// What a wave has in hand: eight rows' numbers, each replaced by those of the row eight further on as soon as it is used, so that one set
+// of registers keeps eight rows of loads in flight.  Rows and bases are the same in all lanes (scalar registers); lanes without a channel
+// read the last one's, rows beyond the end the end's, so that no load has a branch.
 template <class T, int NS, int P, bool HAS_U, bool HAS_C, bool HAS_Z, bool HAS_G>
 struct Rows {
     static constexpr int SP = NS * P, kStates = (kTile * SP + kWave - 1) / kWave;
     T u[HAS_U ? kTile : 1], dt[kTile], z[HAS_Z ? kTile : 1], g[HAS_G ? kTile : 1];
     T b[kStates], c[HAS_C ? kStates : 1];
 
-    __device__ __forceinline__ void load(const ScanArgs &a, int64_t row, int n, uint32_t ch, int lane) {
-#pragma unroll
-        for (int t = 0; t < kTile; ++t) {
-            const uint32_t r = t < n ? t : n - 1;
-            if (HAS_U) u[t] = row_at<T>(a.u, row, a.ld_u, r, ch);
-            dt[t] = row_at<T>(a.dt, row, a.ld_dt, r, ch);
-            if (HAS_G) g[t] = row_at<T>(a.gy, row, a.ld_gy, r, ch);
-        }
-        if (HAS_Z && a.z)
-#pragma unroll
-            for (int t = 0; t < kTile; ++t) z[t] = row_at<T>(a.z, row, a.ld_z, t < n ? t : n - 1, ch);
+    // row base + r into place j
+    __device__ __forceinline__ void load_row(const ScanArgs &a, int j, int64_t base, uint32_t r, uint32_t ch) {
+        if (HAS_U) u[j] = row_at<T>(a.u, base, a.ld_u, r, ch);
+        dt[j] = row_at<T>(a.dt, base, a.ld_dt, r, ch);
+        if (HAS_G) g[j] = row_at<T>(a.gy, base, a.ld_gy, r, ch);
+        if (HAS_Z && a.z) z[j] = row_at<T>(a.z, base, a.ld_z, r, ch);
+    }
+    // the n rows from `row` on: B and C
+    __device__ __forceinline__ void load_states(const ScanArgs &a, int64_t row, int n, int lane) {
 #pragma unroll
         for (int k = 0; k < kStates; ++k) {
             const int e = k * kWave + lane, s = e % SP;
             const uint32_t t = e / SP < n ? e / SP : n - 1, sc = s < a.states ? s : 0;
             b[k] = row_at<T>(a.B, row, a.ld_B, t, sc);
             if (HAS_C) c[k] = row_at<T>(a.C, row, a.ld_C, t, sc);
-            if (s >= a.states) {
-                b[k] = T(0.0f);
-                if (HAS_C) c[k] = T(0.0f);
-            }
         }
     }
     // B and C into this wave's LDS: [2][kTile][SP]
-    __device__ __forceinline__ void stage(float *lds, int lane) const {
+    __device__ __forceinline__ void stage(const ScanArgs &a, float *lds, int lane) const {
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int k = 0; k < kStates; ++k) {
             const int e = k * kWave + lane;
             if (e < kTile * SP) {
-                lds[e] = to_f(b[k]);
-                if (HAS_C) lds[kTile * SP + e] = to_f(c[k]);
+                lds[e] = e % SP < a.states ? to_f(b[k]) : 0.0f;
+                if (HAS_C) lds[kTile * SP + e] = e % SP < a.states ? to_f(c[k]) : 0.0f;
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -220,7 +215,7 @@ struct Rows {
 struct Step { float step, slope; };
 __device__ __forceinline__ Step softplus_step(float raw) {
     const float e = fast_exp2(-fabsf(raw) * kLog2e), r = fast_rcp(1.0f + e);
-    return {softplus_from(raw, e), raw != raw ? raw : (raw >= 0.0f ? r : e * r)};
+    return {softplus_from(raw, e), raw >= 0.0f ? r : e * r};
 }
 
 template <int NS> __device__ __forceinline__ void read_states(const float *at, float (&v)[NS]) {
@@ -255,17 +250,18 @@ __global__ __launch_bounds__(kWave) void scan_fwd_kernel(ScanArgs a) {
             else if (a.init) h[i] = a.init[(t.ray * a.channels + ch) * a.states + s];
         }
     }
-    Rows<T, NS, P, true, !LOCAL, !LOCAL, false> next;
+    Rows<T, NS, P, true, !LOCAL, !LOCAL, false> rows;
     const int64_t row0 = t.start + t.first;
-    int left = (int)(t.n < kTile ? t.n : kTile);
-    if (left > 0) next.load(a, row0, left, chc, lane);
-    for (int64_t k = 0; k < t.n; k += kTile) {
-        const auto rows = next;
-        const int n = left;
-        rows.stage(lds, lane);
-        const int64_t rest = t.n - k - kTile;
-        left = (int)(rest < kTile ? (rest > 0 ? rest : 0) : kTile);
-        if (left > 0) next.load(a, row0 + k + kTile, left, chc, lane);
+    const int total = (int)t.n;
+    if (total > 0) {
+#pragma unroll
+        for (int j = 0; j < kTile; ++j) rows.load_row(a, j, row0, j < total ? j : total - 1, chc);
+        rows.load_states(a, row0, total < kTile ? total : kTile, lane);
+    }
+    for (int k = 0; k < total; k += kTile) {
+        rows.stage(a, lds, lane);
+        const int n = total - k < kTile ? total - k : kTile, more = total - k - kTile;
+        if (more > 0) rows.load_states(a, row0 + k + kTile, more < kTile ? more : kTile, lane);
         if (!LOCAL && a.kept && t.first + k > 0) {
             float *to = a.kept + ((row0 + k) / kTile) * a.states * a.channels;
 #pragma unroll
@@ -298,6 +294,7 @@ __global__ __launch_bounds__(kWave) void scan_fwd_kernel(ScanArgs a) {
                 }
                 if (on && part == 0) (reinterpret_cast<T *>(a.y) + (row0 + k + j) * a.channels)[ch] = from_f<T>(y);
             }
+            if (more > 0) rows.load_row(a, j, row0 + k, kTile + (j < more ? j : more - 1), chc);
         }
     }
     if (LOCAL) {
@@ -371,24 +368,28 @@ __global__ __launch_bounds__(kWave) void scan_bwd_local_kernel(ScanArgs a) {
         G[i] = 0.0f;
     }
     const int64_t row0 = t.start + t.first, tiles = (t.n + kTile - 1) / kTile;
-    Rows<T, NS, P, false, true, true, true> next;
+    Rows<T, NS, P, false, true, true, true> rows;
     auto rows_in = [&](int64_t k) { const int64_t r = t.n - k * kTile; return (int)(r < kTile ? r : kTile); };
-    if (tiles > 0) next.load(a, row0 + (tiles - 1) * kTile, rows_in(tiles - 1), chc, lane);
+    if (tiles > 0) {
+        const int64_t row = row0 + (tiles - 1) * kTile;
+        const int n = rows_in(tiles - 1);
+#pragma unroll
+        for (int j = 0; j < kTile; ++j) rows.load_row(a, j, row, j < n ? j : n - 1, chc);
+        rows.load_states(a, row, n, lane);
+    }
     for (int64_t k = tiles - 1; k >= 0; --k) {
-        const auto rows = next;
         const int n = rows_in(k);
-        rows.stage(lds, lane);
-        if (k > 0) next.load(a, row0 + (k - 1) * kTile, kTile, chc, lane);
+        const int64_t before = row0 + (k - 1) * kTile;
+        rows.stage(a, lds, lane);
+        if (k > 0) rows.load_states(a, before, kTile, lane);
 #pragma unroll
         for (int j = kTile - 1; j >= 0; --j) {
+            float step = to_f(rows.dt[j]) + bias, dy = to_f(rows.g[j]), z = 0.0f;
+            if (a.z) z = to_f(rows.z[j]);
+            if (k > 0) rows.load_row(a, j, before, j, chc);
             if (j >= n) continue;
-            float step = to_f(rows.dt[j]) + bias;
             if (a.softplus) step = softplus_f(step);
-            float dy = to_f(rows.g[j]);
-            if (a.z) {
-                const float z = to_f(rows.z[j]);
-                dy *= z * sigmoid_f(z);
-            }
+            if (a.z) dy *= z * sigmoid_f(z);
             float C[NS];
             read_states<NS>(lds + (kTile + j) * SP + part * NS, C);
             sum += step;
