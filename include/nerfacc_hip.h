@@ -497,6 +497,9 @@ int nfa_linear_bwd(const nfa_linear_args *args, const void *saved, void *grad_in
  * nfa_row_map  row_ray / row_pos [rows] int32: the sequence of each row and its position there (-1: none), what the calls below take
  *              for packed sequences (NULL for equal ones). */
 int nfa_row_map(const int64_t *packed_info, int64_t n_rays, int64_t rows, int32_t *row_ray, int32_t *row_pos, void *stream);
+/* nfa_ray_order  order [n_rays] int32: the sequences from long to short (by 32 classes of length, in index order within one): dealt
+ *                out in this order, ragged sequences fill the chip evenly.  Results do not depend on it. */
+int nfa_ray_order(const int64_t *packed_info, int64_t n_rays, int64_t rows, int32_t *order, void *stream);
 
 /* Short causal convolution along each sequence, channel by channel:
  *   z[t] = bias + sum_j weight[:, j] x[t - width + 1 + j],  outputs = act(z);  rows before the first come from initial_state (zeros
@@ -553,6 +556,7 @@ typedef struct nfa_selective_scan_args {
     const float *initial_state;                     /* [n_rays, channels, states] nullable */
     const int64_t *packed_info;                     /* nullable */
     const int32_t *row_ray, *row_pos;               /* with packed_info */
+    const int32_t *ray_order;                       /* nullable */
     const void *grad_outputs;                       /* backward only */
     int64_t grad_outputs_stride;
     const float *grad_final_state;                  /* backward only, nullable */

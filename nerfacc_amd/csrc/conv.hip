@@ -382,6 +382,61 @@ __global__ __launch_bounds__(kBlock) void row_map_kernel(const int64_t *__restri
     }
 }
 
+// one workgroup: the longest length, the sequences in each of 32 classes of length, and every sequence's place behind the longer classes
+// and the earlier sequences of its own, by ballots (the same order every time)
+constexpr int kClasses = 32;
+__global__ __launch_bounds__(1024) void ray_order_kernel(const int64_t *__restrict__ info, int64_t n_rays, int64_t rows, int32_t *__restrict__ order) {
+    __shared__ int longest, place[kClasses], in_wave[16][kClasses];
+    const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6;
+    auto length = [&](int64_t r) {
+        int64_t start, count;
+        rows_of(info, r, rows, 0, start, count);
+        return (int)count;
+    };
+    if (tid == 0) longest = 0;
+    if (tid < kClasses) place[tid] = 0;
+    __syncthreads();
+    int most = 0;
+    for (int64_t r = tid; r < n_rays; r += 1024) {
+        const int n = length(r);
+        most = n > most ? n : most;
+    }
+    atomicMax(&longest, most);
+    __syncthreads();
+    const int64_t top = (int64_t)longest + 1;
+    auto class_of = [&](int64_t r) { return kClasses - 1 - (int)((int64_t)length(r) * kClasses / top); };
+    for (int64_t r = tid; r < n_rays; r += 1024) atomicAdd(&place[class_of(r)], 1);
+    __syncthreads();
+    if (tid == 0) {
+        int sum = 0;
+        for (int c = 0; c < kClasses; ++c) {
+            const int n = place[c];
+            place[c] = sum;
+            sum += n;
+        }
+    }
+    for (int64_t base = 0; base < n_rays; base += 1024) {
+        const int64_t r = base + tid;
+        const int mine = r < n_rays ? class_of(r) : -1;
+        int rank = 0;
+        for (int c = 0; c < kClasses; ++c) {
+            const unsigned long long same = __ballot(mine == c);
+            if (mine == c) rank = __popcll(same & lanes_lt(lane));
+            if (lane == 0) in_wave[wave][c] = __popcll(same);
+        }
+        __syncthreads();
+        if (mine >= 0) {
+            int at = place[mine] + rank;
+            for (int w = 0; w < wave; ++w) at += in_wave[w][mine];
+            order[at] = (int32_t)r;
+        }
+        __syncthreads();
+        if (tid < kClasses)
+            for (int w = 0; w < 16; ++w) place[tid] += in_wave[w][tid];
+        __syncthreads();
+    }
+}
+
 bool fits(const void *p, int64_t ld, int64_t bytes, int64_t vec) { return !p || ((uintptr_t)p % (vec * bytes) == 0 && ld % vec == 0); }
 
 // calls f(T{}, integral W, integral VC)
@@ -436,6 +491,15 @@ NFA_EXPORT int nfa_row_map(const int64_t *packed_info, int64_t n_rays, int64_t r
     hipLaunchKernelGGL(fill_map_kernel, dim3(blocks_for(rows)), dim3(kBlock), 0, s, row_ray, row_pos, rows);
     if (n_rays > 0) hipLaunchKernelGGL(row_map_kernel, dim3(blocks_for(n_rays * 16)), dim3(kBlock), 0, s, packed_info, n_rays, rows, row_ray, row_pos);
     return check_launch("row_map_kernel");
+}
+
+NFA_EXPORT int nfa_ray_order(const int64_t *packed_info, int64_t n_rays, int64_t rows, int32_t *order, void *stream) {
+    NFA_REQUIRE(n_rays >= 0 && rows >= 0, "ray_order: negative size");
+    NFA_REQUIRE(n_rays < (1ll << 31) && rows < (1ll << 31), "ray_order: more than 2^31 - 1 rays or rows");
+    if (n_rays == 0) return NFA_OK;
+    NFA_REQUIRE(packed_info && order, "ray_order: NULL pointer");
+    hipLaunchKernelGGL(ray_order_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, packed_info, n_rays, rows, order);
+    return check_launch("ray_order_kernel");
 }
 
 static int check_conv(const nfa_causal_conv_args *a, const char *who, bool step) {

@@ -34,7 +34,7 @@ struct ScanArgs {
     int64_t ld_u, ld_dt, ld_z, ld_B, ld_C, ld_gy;
     const float *A, *D, *bias, *init, *gfinal;
     const int64_t *info;
-    const int32_t *ray, *pos;
+    const int32_t *ray, *pos, *order;
     void *y, *gu, *gdt, *gz;
     float *final_state, *kept, *ginit;
     float *ends, *sums;                 // chunks: [slots][states][channels], [slots][channels]
@@ -65,7 +65,7 @@ __device__ __forceinline__ Task find_task(const ScanArgs &a, int64_t id, int lan
     Task t;
     int64_t k = 0;
     t.live = true;
-    if (a.chunk == 0) t.ray = id;
+    if (a.chunk == 0) t.ray = a.order ? __builtin_amdgcn_readfirstlane(a.order[id]) : id;
     else if (!a.info) { t.ray = id / a.chunks; k = id - t.ray * a.chunks; }
     else if (id < a.n_rays) t.ray = id;
     else {                              // the chunk that begins inside block id - n_rays, if one does
@@ -438,9 +438,11 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
     for (int i = 0; i < kHalvings; ++i) number |= ((lane >> (kBits - 1 - i)) & 1) << i;
     const bool stores = (lane & ((1 << (kBits - kHalvings)) - 1)) == 0;
 
+    int64_t place = worker;                                 // of this worker's sums; its ray's where it has one ray: the dealing order leaves no trace
     for (int64_t task = worker; task < a.tasks; task += a.workers) {
         const Task t = find_task(a, task, lane);
         if (!t.live) continue;
+        if (a.order) place = t.ray;
         float G[NS];                                        // dL/dh of the row behind, times its decay
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
@@ -608,7 +610,7 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
         }
     }
     const int64_t per = (int64_t)a.channels * (a.states + 2);
-    float *to = a.part_w + worker * per;
+    float *to = a.part_w + place * per;
     if (!on) return;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
@@ -810,6 +812,7 @@ ScanArgs scan_args(const nfa_selective_scan_args *a) {
     d.gy = a->grad_outputs; d.ld_gy = a->grad_outputs_stride;
     d.A = a->A; d.D = a->D; d.bias = a->delta_bias; d.init = a->initial_state; d.gfinal = a->grad_final_state;
     d.info = a->packed_info; d.ray = a->row_ray; d.pos = a->row_pos;
+    d.order = a->packed_info ? a->ray_order : nullptr;
     d.rows = a->rows; d.n_rays = a->n_rays;
     d.length = a->n_rays > 0 ? a->rows / a->n_rays : 0;
     d.channels = a->channels; d.states = a->states; d.softplus = a->delta_softplus != 0;
@@ -892,6 +895,7 @@ NFA_EXPORT int nfa_selective_scan_bwd(const nfa_selective_scan_args *a, const fl
     const ScanPlan p = scan_plan(a->n_rays, a->rows, a->channels, a->states, a->packed_info != nullptr, true);
     const ScanSpace sp = scan_space(p, a->rows, a->channels, a->states, true);
     use_plan(d, p, sp, workspace);
+    if (p.workers != a->n_rays || p.chunk) d.order = nullptr;
     d.kept = (float *)checkpoints;
     d.gu = g->inputs; d.gdt = g->delta; d.gz = a->gate ? g->gate : nullptr; d.ginit = g->initial_state;
     const int64_t grid = p.tasks * p.blocks, main_grid = p.workers * p.blocks;

@@ -1522,6 +1522,15 @@ std::tuple<Tensor, Tensor> row_map(const Tensor &info, int64_t rows) {
     return {ray, pos};
 }
 
+Tensor ray_order(const Tensor &info, int64_t rows) {
+    check_input(info, "packed_info", at::kLong);
+    TORCH_CHECK(info.dim() == 2 && info.size(1) == 2 && rows >= 0, "packed_info must be [n_rays, 2]");
+    Guard g(device_of(info));
+    Tensor order = at::empty({info.size(0)}, opts(info, at::kInt));
+    check_rc(nfa_ray_order(ptr<int64_t>(info), info.size(0), rows, ptr<int32_t>(order), stream_of(info)));
+    return order;
+}
+
 // the sequences of a call: packed (info and its row map) or equal ones
 struct Sequences {
     OptTensor info, ray, pos;
@@ -1644,9 +1653,11 @@ struct ScanInputs {
 
 std::tuple<Tensor, OptTensor, OptTensor> selective_scan_fwd(
     const Tensor &u, const Tensor &dt, const OptTensor &z, const Tensor &B, const Tensor &C, const Tensor &A, const OptTensor &D, const OptTensor &bias,
-    const OptTensor &init, const OptTensor &info, const OptTensor &ray, const OptTensor &pos, int64_t n_rays, bool softplus, bool want_final, bool keep) {
+    const OptTensor &init, const OptTensor &info, const OptTensor &ray, const OptTensor &pos, const OptTensor &order_, int64_t n_rays, bool softplus,
+    bool want_final, bool keep) {
     const ScanInputs in(u, dt, z, B, C, A, D, bias, init, n_rays);
     const Sequences seq(info, ray, pos, n_rays, in.n, u);
+    const OptTensor order = dense_of(order_, "ray_order", at::kInt, n_rays, u);
     Guard g(device_of(u));
     Tensor out = at::empty({in.n, in.d}, u.options()), last, kept, ws;
     if (want_final) last = at::empty({n_rays, in.d, in.s}, opts(u, at::kFloat));
@@ -1657,6 +1668,7 @@ std::tuple<Tensor, OptTensor, OptTensor> selective_scan_fwd(
     if (n_rays == 0) return {out, some(last), some(kept)};
     auto a = in.args(softplus);
     seq.into(a);
+    a.ray_order = ptr<int32_t>(order);
     check_rc(nfa_selective_scan_fwd(&a, out.data_ptr(), ptr<float>(last), ptr<float>(kept), ptr<void>(ws), stream_of(u)));
     return {out, some(last), some(kept)};
 }
@@ -1665,9 +1677,10 @@ std::tuple<Tensor, OptTensor, OptTensor> selective_scan_fwd(
 std::vector<OptTensor> selective_scan_bwd(
     const Tensor &g_, const OptTensor &gfinal_, const Tensor &u, const Tensor &dt, const OptTensor &z, const Tensor &B, const Tensor &C, const Tensor &A,
     const OptTensor &D, const OptTensor &bias, const OptTensor &init, const Tensor &kept, const OptTensor &info, const OptTensor &ray, const OptTensor &pos,
-    int64_t n_rays, bool softplus) {
+    const OptTensor &order_, int64_t n_rays, bool softplus) {
     const ScanInputs in(u, dt, z, B, C, A, D, bias, init, n_rays);
     const Sequences seq(info, ray, pos, n_rays, in.n, u);
+    const OptTensor order = dense_of(order_, "ray_order", at::kInt, n_rays, u);
     const Tensor gy = as_rows(g_, "grad_outputs", in.n, in.d, u);
     const OptTensor gfinal = dense_of(gfinal_, "grad_final_state", at::kFloat, n_rays * in.d * in.s, u);
     check_len(kept, "checkpoints", at::kByte, nfa_selective_scan_checkpoint_bytes(in.n, (int32_t)in.d, (int32_t)in.s), u);
@@ -1687,6 +1700,7 @@ std::vector<OptTensor> selective_scan_bwd(
     if (!none) {
         auto a = in.args(softplus);
         seq.into(a);
+    a.ray_order = ptr<int32_t>(order);
         a.grad_outputs = gy.data_ptr(); a.grad_outputs_stride = row_stride(gy); a.grad_final_state = ptr<float>(gfinal);
         Tensor ws = at::empty({nfa_selective_scan_workspace_bytes(n_rays, in.n, a.channels, a.states, 1)}, opts(u, at::kByte));
         nfa_selective_scan_grads gr{};
@@ -1831,6 +1845,11 @@ struct RowMap {
         else if (n_rays == 0) info = at::empty({0, 2}, opts(x, at::kLong));
         if (info) std::tie(ray, pos) = row_map(*info, x.size(0));
     }
+    // the dealing order of a scan: where whole rays are a few for each wave place of the chip, their lengths decide when the last one ends
+    OptTensor order(int64_t n_rays, int64_t rows) const {
+        if (!info || n_rays < 1024 || n_rays > 65536) return std::nullopt;
+        return ray_order(*info, rows);
+    }
 };
 inline Tensor flat_rows(const Tensor &t) { return !t.defined() || t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
 
@@ -1931,10 +1950,10 @@ std::tuple<Tensor, Tensor> causal_conv_one(const Tensor &x, const Tensor &state,
 struct SelectiveScanFn : torch::autograd::Function<SelectiveScanFn> {
     static variable_list forward(AutogradContext *ctx, const Tensor &u, const Tensor &dt, const Tensor &B, const Tensor &C, const Tensor &A, const OptTensor &z,
                                  const OptTensor &D, const OptTensor &bias, const OptTensor &init, const OptTensor &info, const OptTensor &ray,
-                                 const OptTensor &pos, int64_t n_rays, bool softplus, bool want_final) {
+                                 const OptTensor &pos, const OptTensor &order, int64_t n_rays, bool softplus, bool want_final) {
         ctx->set_materialize_grads(false);
-        auto res = selective_scan_fwd(u, dt, z, B, C, A, D, bias, init, info, ray, pos, n_rays, softplus, want_final, true);
-        ctx->save_for_backward({u, dt, B, C, A, get(z), get(D), get(bias), get(init), get(info), get(ray), get(pos), get(std::get<2>(res))});
+        auto res = selective_scan_fwd(u, dt, z, B, C, A, D, bias, init, info, ray, pos, order, n_rays, softplus, want_final, true);
+        ctx->save_for_backward({u, dt, B, C, A, get(z), get(D), get(bias), get(init), get(info), get(ray), get(pos), get(std::get<2>(res)), get(order)});
         ctx->saved_data["n_rays"] = n_rays;
         ctx->saved_data["softplus"] = softplus;
         if (!want_final) return {std::get<0>(res)};
@@ -1944,11 +1963,11 @@ struct SelectiveScanFn : torch::autograd::Function<SelectiveScanFn> {
         const auto s = ctx->get_saved_variables();
         const Tensor gy = grads[0].defined() ? grads[0] : at::zeros_like(s[0]);
         const auto g = selective_scan_bwd(gy, grads.size() > 1 ? some(grads[1]) : std::nullopt, s[0], s[1], some(s[5]), s[2], s[3], s[4], some(s[6]), some(s[7]),
-                                          some(s[8]), s[12], some(s[9]), some(s[10]), some(s[11]), ctx->saved_data["n_rays"].toInt(),
+                                          some(s[8]), s[12], some(s[9]), some(s[10]), some(s[11]), some(s[13]), ctx->saved_data["n_rays"].toInt(),
                                           ctx->saved_data["softplus"].toBool());
         // forward's order: u, dt, B, C, A, z, D, bias, init; needs_input_grad counts the tensors that were given
         static constexpr int from[9] = {0, 1, 3, 4, 5, 2, 6, 7, 8};
-        variable_list out(15);
+        variable_list out(16);
         int given = 0;
         for (int i = 0; i < 9; ++i) {
             if (!s[i].defined()) continue;
@@ -1987,16 +2006,17 @@ std::tuple<Tensor, OptTensor> selective_scan(const Tensor &x_, const Tensor &dt,
     Guard g(device_of(x_));
     const Tensor x = flat_rows(x_);
     const RowMap m(info, x, n_rays);
+    const OptTensor order = m.order(n_rays, x.size(0));
     const OptTensor z2 = some(flat_rows(get(z))), D2 = some(get(D)), bias2 = some(get(bias)), init2 = some(get(init));
     Tensor out;
     OptTensor last;
     if (records_grad("selective_scan", x, {x_, dt, A, B, C, D, z, bias, init})) {
-        auto res = SelectiveScanFn::apply(x, flat_rows(dt), flat_rows(B), flat_rows(C), A, z2, D2, bias2, init2, m.info, m.ray, m.pos, n_rays, softplus, want_final);
+        auto res = SelectiveScanFn::apply(x, flat_rows(dt), flat_rows(B), flat_rows(C), A, z2, D2, bias2, init2, m.info, m.ray, m.pos, order, n_rays, softplus, want_final);
         out = res[0];
         if (want_final) last = res[1];
     } else {
         OptTensor kept;
-        std::tie(out, last, kept) = selective_scan_fwd(x, flat_rows(dt), z2, flat_rows(B), flat_rows(C), A, D2, bias2, init2, m.info, m.ray, m.pos, n_rays, softplus,
+        std::tie(out, last, kept) = selective_scan_fwd(x, flat_rows(dt), z2, flat_rows(B), flat_rows(C), A, D2, bias2, init2, m.info, m.ray, m.pos, order, n_rays, softplus,
                                                        want_final, false);
     }
     return {x_.dim() == 2 ? out : out.view(x_.sizes()), last};
@@ -2112,6 +2132,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear_fwd", &linear_fwd);
     m.def("linear_bwd", &linear_bwd);
     m.def("row_map", &row_map);
+    m.def("ray_order", &ray_order);
     m.def("causal_conv_fwd", &causal_conv_fwd);
     m.def("causal_conv_bwd", &causal_conv_bwd);
     m.def("causal_conv_step", &causal_conv_step);

@@ -41,7 +41,7 @@ _FUSED_NAMES = (
     "rendering_fwd", "rendering_bwd",
     "grid_cell_points", "grid_ema_update", "grid_threshold", "grid_mark_invisible", "grid_occupied_counts", "grid_occupied_cells", "sample_positions",
     "transform_stot", "edge_cdfs_fwd", "edge_cdfs_bwd", "pdf_loss_fwd", "pdf_loss_bwd",
-    "foreign_nodes", "linear_fwd", "linear_bwd", "row_map", "causal_conv_fwd", "causal_conv_bwd", "causal_conv_step",
+    "foreign_nodes", "linear_fwd", "linear_bwd", "row_map", "ray_order", "causal_conv_fwd", "causal_conv_bwd", "causal_conv_step",
     "selective_scan_fwd", "selective_scan_bwd", "selective_scan_step",
 )
 

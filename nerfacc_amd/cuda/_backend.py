@@ -1168,6 +1168,15 @@ class _CtypesC:
         return ray, pos
 
     @staticmethod
+    def ray_order(info, rows: int):
+        """the rays from long to short: nfa_ray_order"""
+        _check_input(info, "packed_info", torch.int64)
+        with _Guard(info):
+            order = torch.empty(info.shape[0], dtype=torch.int32, device=info.device)
+            _check(load_library().nfa_ray_order(_ptr(info), info.shape[0], rows, _ptr(order), _stream(info)))
+        return order
+
+    @staticmethod
     def _conv_args(x, w, b, init, info, ray, pos, n_rays, act, **more):
         return _STRUCTS["nfa_causal_conv_args"](
             n_rays=n_rays, rows=x.shape[0], channels=x.shape[1], width=w.shape[1], dtype=_dtype_id(x), activation=act, inputs=_ptr(x),
@@ -1228,7 +1237,7 @@ class _CtypesC:
             D=_ptr(D), delta_bias=_ptr(bias), initial_state=_ptr(init), packed_info=_ptr(info), row_ray=_ptr(ray), row_pos=_ptr(pos), **more)
 
     @staticmethod
-    def selective_scan_fwd(u, dt, z, B, C, A, D, bias, init, info, ray, pos, n_rays: int, softplus: bool, want_final: bool, keep: bool):
+    def selective_scan_fwd(u, dt, z, B, C, A, D, bias, init, info, ray, pos, order, n_rays: int, softplus: bool, want_final: bool, keep: bool):
         """(outputs, final_state or None, checkpoints or None): nfa_selective_scan_fwd"""
         u, dt, z, B, C = (_as_rows(t) for t in (u, dt, z, B, C))
         A, D, bias, init = (_dense(t) for t in (A, D, bias, init))
@@ -1243,12 +1252,12 @@ class _CtypesC:
                 return out.zero_(), last, kept
             bytes_ = L.nfa_selective_scan_workspace_bytes(n_rays, n, d, s, 0)
             ws = torch.empty(bytes_, dtype=torch.uint8, **kw) if bytes_ else None
-            a = _CtypesC._scan_args(u, dt, z, B, C, A, D, bias, init, info, ray, pos, n_rays, softplus)
+            a = _CtypesC._scan_args(u, dt, z, B, C, A, D, bias, init, info, ray, pos, n_rays, softplus, ray_order=_ptr(order))
             _check(L.nfa_selective_scan_fwd(ctypes.byref(a), _ptr(out), _ptr(last), _ptr(kept), _ptr(ws), _stream(u)))
         return out, last, kept
 
     @staticmethod
-    def selective_scan_bwd(g, gfinal, u, dt, z, B, C, A, D, bias, init, kept, info, ray, pos, n_rays: int, softplus: bool):
+    def selective_scan_bwd(g, gfinal, u, dt, z, B, C, A, D, bias, init, kept, info, ray, pos, order, n_rays: int, softplus: bool):
         """gradients of (inputs, delta, gate, B, C, A, D, delta_bias, initial_state): nfa_selective_scan_bwd"""
         g, u, dt, z, B, C = (_as_rows(t) for t in (g, u, dt, z, B, C))
         gfinal, A, D, bias, init = (_dense(t) for t in (gfinal, A, D, bias, init))
@@ -1265,7 +1274,7 @@ class _CtypesC:
                 ginit.copy_(gfinal)
             if not none:
                 ws = torch.empty(L.nfa_selective_scan_workspace_bytes(n_rays, n, d, s, 1), dtype=torch.uint8, device=u.device)
-                a = _CtypesC._scan_args(u, dt, z, B, C, A, D, bias, init, info, ray, pos, n_rays, softplus, grad_outputs=_ptr(g),
+                a = _CtypesC._scan_args(u, dt, z, B, C, A, D, bias, init, info, ray, pos, n_rays, softplus, ray_order=_ptr(order), grad_outputs=_ptr(g),
                                         grad_outputs_stride=_row_stride(g), grad_final_state=_ptr(gfinal))
                 gr = _STRUCTS["nfa_selective_scan_grads"](inputs=_ptr(gu), delta=_ptr(gdt), gate=_ptr(gz), B=_ptr(gB), C=_ptr(gC), A=_ptr(gA),
                                                           D=_ptr(gD), delta_bias=_ptr(gbias), initial_state=_ptr(ginit))

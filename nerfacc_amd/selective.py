@@ -49,6 +49,13 @@ def _map_of(packed_info: Optional[Tensor], x: Tensor, n_rays: int):
     return (info, *_C.row_map(info, rows))
 
 
+def _scan_map_of(packed_info: Optional[Tensor], x: Tensor, n_rays: int):
+    """_map_of and the dealing order of a scan: where whole rays are a few for each wave place of the chip, their lengths decide when the
+    last one ends"""
+    rows = _map_of(packed_info, x, n_rays)
+    return (*rows, _C.ray_order(rows[0], x.shape[0]) if packed_info is not None and 1024 <= n_rays <= 65536 else None)
+
+
 def _flat(t: Optional[Tensor]) -> Optional[Tensor]:
     return t if t is None or t.dim() == 2 else t.reshape(-1, t.shape[-1])
 
@@ -209,10 +216,10 @@ def selective_scan(inputs: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tenso
                  ("initial_state", initial_state, (n_rays, channels, A.shape[-1] if isinstance(A, Tensor) and A.dim() else 0), torch.float32)))
     flat = [_flat(t) for t in (inputs, delta, gate, B, C)]
     if _records_grad("selective_scan", inputs, delta, A, B, C, D, gate, delta_bias, initial_state):
-        out, final = _SelectiveScan.apply(*flat, A, D, delta_bias, initial_state, _map_of(packed_info, flat[0], n_rays), n_rays,
+        out, final = _SelectiveScan.apply(*flat, A, D, delta_bias, initial_state, _scan_map_of(packed_info, flat[0], n_rays), n_rays,
                                           bool(delta_softplus), return_final_state)
     else:
-        out, final, _ = _C.selective_scan_fwd(*flat, A, D, delta_bias, initial_state, *_map_of(packed_info, flat[0], n_rays), n_rays,
+        out, final, _ = _C.selective_scan_fwd(*flat, A, D, delta_bias, initial_state, *_scan_map_of(packed_info, flat[0], n_rays), n_rays,
                                               bool(delta_softplus), return_final_state, False)
     out = out.view(inputs.shape)
     return (out, final) if return_final_state else out
