@@ -497,8 +497,8 @@ int nfa_linear_bwd(const nfa_linear_args *args, const void *saved, void *grad_in
  * nfa_row_map  row_ray / row_pos [rows] int32: the sequence of each row and its position there (-1: none), what the calls below take
  *              for packed sequences (NULL for equal ones). */
 int nfa_row_map(const int64_t *packed_info, int64_t n_rays, int64_t rows, int32_t *row_ray, int32_t *row_pos, void *stream);
-/* nfa_ray_order  order [n_rays] int32: the sequences from long to short (by 32 classes of length, in index order within one): dealt
- *                out in this order, ragged sequences fill the chip evenly.  Results do not depend on it. */
+/* nfa_ray_order  order [n_rays] int32: the sequences from long to short (by 32 classes of length, in no order within one): dealt out
+ *                in this order, ragged sequences fill the chip evenly.  Results do not depend on it. */
 int nfa_ray_order(const int64_t *packed_info, int64_t n_rays, int64_t rows, int32_t *order, void *stream);
 
 /* Short causal convolution along each sequence, channel by channel:

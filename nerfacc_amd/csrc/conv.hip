@@ -382,12 +382,12 @@ __global__ __launch_bounds__(kBlock) void row_map_kernel(const int64_t *__restri
     }
 }
 
-// one workgroup: the longest length, the sequences in each of 32 classes of length, and every sequence's place behind the longer classes
-// and the earlier sequences of its own, by ballots (the same order every time)
+// One workgroup: the longest length, the sequences in each of 32 classes of length, and a place for every sequence behind the longer
+// classes.  (Within a class the order is the LDS atomics'; nothing depends on it.)
 constexpr int kClasses = 32;
 __global__ __launch_bounds__(1024) void ray_order_kernel(const int64_t *__restrict__ info, int64_t n_rays, int64_t rows, int32_t *__restrict__ order) {
-    __shared__ int longest, place[kClasses], in_wave[16][kClasses];
-    const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6;
+    __shared__ int longest, place[kClasses];
+    const int tid = threadIdx.x;
     auto length = [&](int64_t r) {
         int64_t start, count;
         rows_of(info, r, rows, 0, start, count);
@@ -397,14 +397,19 @@ __global__ __launch_bounds__(1024) void ray_order_kernel(const int64_t *__restri
     if (tid < kClasses) place[tid] = 0;
     __syncthreads();
     int most = 0;
+#pragma unroll 4
     for (int64_t r = tid; r < n_rays; r += 1024) {
         const int n = length(r);
         most = n > most ? n : most;
     }
     atomicMax(&longest, most);
     __syncthreads();
-    const int64_t top = (int64_t)longest + 1;
-    auto class_of = [&](int64_t r) { return kClasses - 1 - (int)((int64_t)length(r) * kClasses / top); };
+    const float scale = (float)kClasses / (float)(longest + 1.0f);
+    auto class_of = [&](int64_t r) {
+        const int c = (int)((float)length(r) * scale);
+        return c < kClasses ? kClasses - 1 - c : 0;
+    };
+#pragma unroll 4
     for (int64_t r = tid; r < n_rays; r += 1024) atomicAdd(&place[class_of(r)], 1);
     __syncthreads();
     if (tid == 0) {
@@ -415,26 +420,9 @@ __global__ __launch_bounds__(1024) void ray_order_kernel(const int64_t *__restri
             sum += n;
         }
     }
-    for (int64_t base = 0; base < n_rays; base += 1024) {
-        const int64_t r = base + tid;
-        const int mine = r < n_rays ? class_of(r) : -1;
-        int rank = 0;
-        for (int c = 0; c < kClasses; ++c) {
-            const unsigned long long same = __ballot(mine == c);
-            if (mine == c) rank = __popcll(same & lanes_lt(lane));
-            if (lane == 0) in_wave[wave][c] = __popcll(same);
-        }
-        __syncthreads();
-        if (mine >= 0) {
-            int at = place[mine] + rank;
-            for (int w = 0; w < wave; ++w) at += in_wave[w][mine];
-            order[at] = (int32_t)r;
-        }
-        __syncthreads();
-        if (tid < kClasses)
-            for (int w = 0; w < 16; ++w) place[tid] += in_wave[w][tid];
-        __syncthreads();
-    }
+    __syncthreads();
+#pragma unroll 4
+    for (int64_t r = tid; r < n_rays; r += 1024) order[atomicAdd(&place[class_of(r)], 1)] = (int32_t)r;
 }
 
 bool fits(const void *p, int64_t ld, int64_t bytes, int64_t vec) { return !p || ((uintptr_t)p % (vec * bytes) == 0 && ld % vec == 0); }

@@ -46,7 +46,8 @@ enum { kForward, kDgrad, kWgrad };
 
 // Sixteen bytes of row `row`.  VEC: every row starts on 16 bytes and holds whole chunks; the load is then made in any case, from a place
 // that exists, so that a tile's loads are one block without branches, and only_inside() clears what lies outside the array where the
-// value is used: a select right behind the load would wait for it.  Otherwise number by number, zeros outside.
+// value is used: a select right behind the load would wait for it.  Otherwise sixteen bytes at the alignment of a number (global memory
+// takes that), with zeros behind the row's end; number by number only at the end of the array.
 template <class T, bool VEC>
 __device__ __forceinline__ u32x4 load_chunk(const T *base, int64_t row, int64_t rows, int64_t ld, int64_t col, int64_t cols) {
     if constexpr (VEC) {
@@ -56,9 +57,19 @@ __device__ __forceinline__ u32x4 load_chunk(const T *base, int64_t row, int64_t 
         if (row < rows && col < cols) {
             T e[kChunk<T>];
             base += row * ld + col;
+            if ((row - rows + 1) * ld + col + kChunk<T> <= cols) {          // the array holds sixteen bytes from here on
+                __builtin_memcpy(&v, base, 16);
+                if (col + kChunk<T> > cols) {
+                    __builtin_memcpy(e, &v, 16);
 #pragma unroll
-            for (int i = 0; i < kChunk<T>; ++i) e[i] = col + i < cols ? base[i] : T(0.0f);
-            __builtin_memcpy(&v, e, 16);
+                    for (int i = 0; i < kChunk<T>; ++i) e[i] = col + i < cols ? e[i] : T(0.0f);
+                    __builtin_memcpy(&v, e, 16);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kChunk<T>; ++i) e[i] = col + i < cols ? base[i] : T(0.0f);
+                __builtin_memcpy(&v, e, 16);
+            }
         }
         return v;
     }
@@ -176,6 +187,8 @@ template <class T, bool VEC>
 __device__ __forceinline__ void store_chunk(T *row, int q, int n_q, u32x4 v) {
     if constexpr (VEC) {
         if (q < n_q) *reinterpret_cast<u32x4 *>(row + q) = v;
+    } else if (q + kChunk<T> <= n_q) {
+        __builtin_memcpy(row + q, &v, 16);
     } else {
         const Frag<T> f = __builtin_bit_cast(Frag<T>, v);
 #pragma unroll
@@ -631,18 +644,20 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
     }
 }
 
-// columns by lane, sixteen rows side by side; a column's sum is formed in the same order every time.  The columns go to up to three
-// outputs, one behind the other (nullptr: not wanted)
+// Columns by lane, sixteen rows side by side; a column's sum is formed in the same order every time.  A workgroup sums the rows
+// [first, first + each) of its 64 columns, first = blockIdx.y * each; of many rows a first launch leaves each stretch's sum in the
+// stretch's own first row (nobody else reads it), a second one sums those.  The columns go to up to three outputs, one behind the other
+// (nullptr: not wanted).
 struct Outputs { void *to[3]; int64_t cols[3]; };
-template <class T>
-__global__ __launch_bounds__(1024) void reduce_rows_kernel(const float *__restrict__ part, int64_t rows, int64_t ld, Outputs o) {
+template <class T, bool LAST>
+__global__ __launch_bounds__(1024) void reduce_rows_kernel(float *part, int64_t rows, int64_t each, int64_t step, int64_t ld, Outputs o) {
     __shared__ float sum[16][64];
     const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane, first = blockIdx.y * each, end = first + each < rows ? first + each : rows;
     float v = 0.0f;
     if (c < ld) {
 #pragma unroll 8
-        for (int64_t r = grp; r < rows; r += 16) v += part[r * ld + c];
+        for (int64_t r = first + grp * step; r < end; r += 16 * step) v += part[r * ld + c];
     }
     sum[grp][lane] = v;
     __syncthreads();
@@ -650,6 +665,10 @@ __global__ __launch_bounds__(1024) void reduce_rows_kernel(const float *__restri
         float t = 0.0f;
 #pragma unroll
         for (int k = 0; k < 16; ++k) t += sum[k][lane];
+        if (!LAST) {
+            part[first * ld + c] = t;
+            return;
+        }
         int64_t at = c;
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
@@ -678,7 +697,9 @@ int launch_tiles(DenseArgs a, int64_t splits, hipStream_t s) {
     a.tiles = (int32_t)(tiles_p * a.tiles_q);
     const int64_t steps = MODE == kWgrad ? a.split : a.n_c;
     const size_t bytes = (size_t)(BP * (SPLIT ? 2 : 1) + BQ) * kRowBytes * (steps > kStage<T> ? 2 : 1);
-    const auto kernel = a.vec ? tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, true> : tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, false>;
+    auto kernel = tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, true>;
+    if constexpr (BP < 256)                                 // (the largest tiles are for aligned rows)
+        if (!a.vec) kernel = tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, false>;
     if (int rc = allow_lds(kernel, bytes)) return rc;
     a.splits = (int32_t)splits;
     const unsigned grid = (unsigned)(ceil_div(a.tiles * splits, kNumXCD) * kNumXCD);
@@ -756,7 +777,7 @@ bool two_parts(int32_t dtype, int32_t act) { return dtype != NFA_DTYPE_F32 && ac
 
 }  // namespace
 
-void launch_reduce_rows(const float *part, int64_t rows, std::initializer_list<std::pair<void *, int64_t>> outputs, int32_t dtype, hipStream_t s) {
+void launch_reduce_rows(float *part, int64_t rows, std::initializer_list<std::pair<void *, int64_t>> outputs, int32_t dtype, hipStream_t s) {
     Outputs o{};
     int64_t cols = 0, k = 0;
     for (auto &p : outputs) {
@@ -764,8 +785,15 @@ void launch_reduce_rows(const float *part, int64_t rows, std::initializer_list<s
         o.cols[k++] = p.second;
         cols += p.second;
     }
+    const unsigned blocks = (unsigned)ceil_div(cols, 64);
+    // one launch while it fills the chip or its rows are few: 4096 rows of 1152 columns take 19 us in one, 10 in two
+    int64_t step = 1;
+    if (rows >= 1024 && blocks < 2 * kNumCU) {
+        step = 128;
+        hipLaunchKernelGGL((reduce_rows_kernel<float, false>), dim3(blocks, (unsigned)ceil_div(rows, step)), dim3(1024), 0, s, part, rows, step, (int64_t)1, cols, o);
+    }
     with_dtype(dtype, [&](auto t) {
-        hipLaunchKernelGGL((reduce_rows_kernel<decltype(t)>), dim3((unsigned)ceil_div(cols, 64)), dim3(1024), 0, s, part, rows, cols, o);
+        hipLaunchKernelGGL((reduce_rows_kernel<decltype(t), true>), dim3(blocks), dim3(1024), 0, s, part, rows, rows, step, cols, o);
     });
 }
 

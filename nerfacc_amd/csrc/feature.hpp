@@ -102,7 +102,7 @@ __device__ __forceinline__ void with_act(int act, F &&f) {
 inline bool act_ok(int32_t act) { return act >= NFA_ACT_NONE && act <= NFA_ACT_EXP; }
 
 // the sum over the rows of part [rows][all columns] in a fixed order (no atomics: the same bits every time), rounded once; the columns
-// go to up to three outputs (pointer or nullptr, columns), one behind the other
-void launch_reduce_rows(const float *part, int64_t rows, std::initializer_list<std::pair<void *, int64_t>> outputs, int32_t dtype, hipStream_t s);
+// go to up to three outputs (pointer or nullptr, columns), one behind the other.  part is written to.
+void launch_reduce_rows(float *part, int64_t rows, std::initializer_list<std::pair<void *, int64_t>> outputs, int32_t dtype, hipStream_t s);
 
 }  // namespace nfa

@@ -623,17 +623,25 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
     }
 }
 
-// dB and dC of a row: the channel blocks' sums in order; zeros for rows of no sequence
+// dB and dC of a row: the channel blocks' sums in order; zeros for rows of no sequence.  A thread: four neighbouring states.
 template <class T>
-__global__ __launch_bounds__(kBlock) void scan_join_bc_kernel(ScanArgs a, int sp, T *gB, T *gC) {
-    const int64_t n = a.rows * 2 * a.states;
+__global__ __launch_bounds__(kBlock) void scan_join_bc_kernel(ScanArgs a, int log_sp, T *gB, T *gC) {
+    const int64_t n = a.rows << (log_sp - 1);               // 2 sp / 4 groups in a row
     for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < n; e += (int64_t)gridDim.x * kBlock) {
-        const int64_t row = e / (2 * a.states);
-        const int q = (int)(e - row * 2 * a.states), which = q / a.states, s = q - which * a.states;
-        float v = 0.0f;
+        const int64_t row = e >> (log_sp - 1);
+        const int q = (int)(e & ((1 << (log_sp - 1)) - 1)) * 4, which = q >> log_sp, s = q & ((1 << log_sp) - 1);
+        if (s >= a.states) continue;
+        f32x4 v = {0, 0, 0, 0};
         if (!a.info || a.pos[row] >= 0)
-            for (int b = 0; b < a.blocks; ++b) v += a.part_bc[((int64_t)b * a.rows + row) * (2 * sp) + which * sp + s];
-        (which ? gC : gB)[row * a.states + s] = from_f<T>(v);
+            for (int b = 0; b < a.blocks; ++b) {
+                const f32x4 w = *reinterpret_cast<const f32x4 *>(a.part_bc + (((int64_t)b * a.rows + row) << (log_sp + 1)) + q);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += w[i];
+            }
+        T *to = (which ? gC : gB) + row * a.states + s;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s + i < a.states) to[i] = from_f<T>(v[i]);
     }
 }
 
@@ -908,7 +916,8 @@ NFA_EXPORT int nfa_selective_scan_bwd(const nfa_selective_scan_args *a, const fl
             launch_chain<true>(d, s);
         }
         hipLaunchKernelGGL((scan_bwd_kernel<T, ns(), pp()>), dim3((unsigned)main_grid), dim3(kWave), 0, s, d);
-        hipLaunchKernelGGL((scan_join_bc_kernel<T>), dim3(blocks_for(a->rows * 2 * a->states)), dim3(kBlock), 0, s, d, (int)(ns() * pp()), (T *)g->B, (T *)g->C);
+        hipLaunchKernelGGL((scan_join_bc_kernel<T>), dim3(blocks_for(a->rows * ns() * pp() / 2)), dim3(kBlock), 0, s, d, log2_of(ns() * pp()), (T *)g->B,
+                           (T *)g->C);
     });
     launch_reduce_rows(d.part_w, p.workers, {{g->A, (int64_t)a->channels * a->states}, {g->D, a->channels}, {g->delta_bias, a->channels}}, NFA_DTYPE_F32, s);
     return check_launch("scan_bwd_kernel");
