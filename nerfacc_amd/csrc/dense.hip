@@ -644,6 +644,62 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
     }
 }
 
+// ---- few rows, a long contraction ----------------------------------------------------------------------------------------
+// A tile of a long contraction is one step after the other, and few tiles leave the chip empty meanwhile: here sixteen rows and 32
+// columns are a workgroup, whose four waves take every fourth step each, straight from memory, and join their sums in LDS in order.
+template <class T, bool VEC>
+__global__ __launch_bounds__(kBlock) void stream_kernel(DenseArgs a) {
+    constexpr int CE = kChunk<T>, NC = sizeof(T) == 2 ? 1 : 2, kDeep = 4;      // kDeep: a wave's steps in flight
+    __shared__ f32x4 sums[kWavesPerBlock][2][kWave];
+    const int lane = lane_id(), i = lane & 15, g = lane >> 4, wave = wave_in_block();
+    const int64_t p0 = (int64_t)(blockIdx.x / a.tiles_q) * 16;
+    const int q0 = (int)(blockIdx.x % a.tiles_q) * 32;
+    const T *P = reinterpret_cast<const T *>(a.p), *Q = reinterpret_cast<const T *>(a.q);
+    f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    const int64_t steps = (a.n_c + 4 * CE - 1) / (4 * CE);
+    for (int64_t k0 = wave; k0 < steps; k0 += kWavesPerBlock * kDeep) {
+        u32x4 x[kDeep], w[kDeep][2];
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            const int64_t c = ((k0 + d * kWavesPerBlock) * 4 + g) * CE;
+            x[d] = load_chunk<T, VEC>(P, p0 + i, a.n_p, a.ld_p, c, a.n_c);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) w[d][j] = load_chunk<T, VEC>(Q, q0 + column_of<T>(j, i >> 2, i & 3), a.n_q, a.ld_q, c, a.n_c);
+        }
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            const bool inside = ((k0 + d * kWavesPerBlock) * 4 + g) * CE < a.n_c;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[j] = multiply<T>(only_inside<VEC>(w[d][j], inside), only_inside<VEC>(x[d], inside), acc[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) sums[wave][j][lane] = acc[j];
+    __syncthreads();
+    const int64_t p = p0 + i;
+    if (wave != 0 || p >= a.n_p) return;
+    float z[NC][CE];
+    int col[NC];
+    u32x4 res[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        col[c] = q0 + column_of<T>(c, g, 0);
+        res[c] = u32x4{0, 0, 0, 0};
+        if (a.residual) res[c] = load_chunk<T, VEC>(reinterpret_cast<const T *>(a.residual), p, a.n_p, a.ld_residual, col[c], a.n_q);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = q0 + column_of<T>(j, g, e);
+            float v = a.bias && c < a.n_q ? to_f(reinterpret_cast<const T *>(a.bias)[c]) : 0.0f, sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kWavesPerBlock; ++k) sum += sums[k][j][lane][e];
+            z[NC == 1 ? 0 : j][NC == 1 ? j * 4 + e : e] = sum + v;
+        }
+    epilogue<T, kForward, VEC, NC>(a, p, col, a.n_q, z, res);
+}
+
 // Columns by lane, sixteen rows side by side; a column's sum is formed in the same order every time.  A workgroup sums the rows
 // [first, first + each) of its 64 columns, first = blockIdx.y * each; of many rows a first launch leaves each stretch's sum in the
 // stretch's own first row (nobody else reads it), a second one sums those.  The columns go to up to three outputs, one behind the other
@@ -743,6 +799,14 @@ int launch_rows(const DenseArgs &a, hipStream_t s) {
     if (a.n_c <= 8 * step) return launch_resident<T, MODE, 8, SPLIT>(a, s);
     if constexpr (sizeof(T) == 4)
         if (a.n_c <= 16 * step) return launch_resident<T, MODE, 16, SPLIT>(a, s);
+    // few tiles: rows, and the contraction, over more workgroups (1781 x 826 x 2 fp32: 9 against 37 us; from 64 tiles on the tiles win)
+    if (MODE == kForward && ceil_div(a.n_p, 128) * ceil_div(a.n_q, 128) < (sizeof(T) == 4 ? kNumCU : kNumCU / 4)) {
+        DenseArgs b = a;
+        b.tiles_q = (int32_t)ceil_div(a.n_q, 32);
+        const auto kernel = a.vec ? stream_kernel<T, true> : stream_kernel<T, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(ceil_div(a.n_p, 16) * b.tiles_q)), dim3(kBlock), 0, s, b);
+        return check_launch("stream_kernel");
+    }
     // 16-bit types, aligned and large enough for every CU: 256 x 256 by eight waves, whose fragments are used often enough that the matrix
     // units and not LDS set the pace
     constexpr int BP = SPLIT ? 64 : 128;

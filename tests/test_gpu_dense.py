@@ -76,6 +76,20 @@ def test_sizes(dtype, m, k, n):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(1, 300, 3), (17, 1000, 33), (40, 257, 300), (300, 512, 64), (9000, 272, 130), (5, 64, 700)])
+def test_long_contractions_and_wide_outputs(dtype, m, k, n):
+    """contractions beyond what stays in LDS: few rows, tiles; and a weight in several blocks of columns"""
+    check(*make(m, k, n, dtype, seed=9, residual=True), "relu")
+    check(*make(m, k, n, dtype, seed=10), "silu")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_tiles(dtype):
+    """enough rows and columns for the largest tiles, with rows and columns that end inside them"""
+    check(*make(16500, 520, 1000, dtype, seed=11), "relu")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("residual", [False, True])
 def test_activations(dtype, act, residual):
