@@ -114,7 +114,9 @@ __device__ __forceinline__ void form_dz(const DenseArgs &a, u32x4 (&g)[N], const
                 if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((s[k][0] >> i) & 1u) != 0 : to_f(w.v[i]) > 0.0f) ? dz : 0.0f;
                 else if constexpr (ACT != NFA_ACT_NONE) dz *= act_slope<ACT>(to_f(w.v[i]));
                 each(k, dz, i);
-                if constexpr (ACT != NFA_ACT_NONE) v.v[i] = from_f<T>(dz);
+                float near = dz;                            // (fp16: the largest number in place of an overflow, the rest in the second part)
+                if constexpr (SPLIT && std::is_same_v<T, f16>) near = fabsf(dz) > 65504.0f ? copysignf(65504.0f, dz) : dz;
+                if constexpr (ACT != NFA_ACT_NONE) v.v[i] = from_f<T>(near);
                 if constexpr (SPLIT) lo.v[i] = from_f<T>(dz - to_f(v.v[i]));
             }
             if constexpr (ACT != NFA_ACT_NONE) g[k] = __builtin_bit_cast(u32x4, v);
@@ -799,7 +801,8 @@ int launch_rows(const DenseArgs &a, hipStream_t s) {
     if (a.n_c <= 8 * step) return launch_resident<T, MODE, 8, SPLIT>(a, s);
     if constexpr (sizeof(T) == 4)
         if (a.n_c <= 16 * step) return launch_resident<T, MODE, 16, SPLIT>(a, s);
-    // few tiles: rows, and the contraction, over more workgroups (1781 x 826 x 2 fp32: 9 against 37 us; from 64 tiles on the tiles win)
+    // few tiles: rows, and the contraction, over more workgroups.  4096 x 1024 x 256, 64 tiles: fp32 49 us against 84 by tiles (whose steps
+    // are four times as long as those of 16-bit types), bf16 25 against 20
     if (MODE == kForward && ceil_div(a.n_p, 128) * ceil_div(a.n_q, 128) < (sizeof(T) == 4 ? kNumCU : kNumCU / 4)) {
         DenseArgs b = a;
         b.tiles_q = (int32_t)ceil_div(a.n_q, 32);

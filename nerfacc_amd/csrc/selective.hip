@@ -27,7 +27,7 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 8;                // rows between kept states, and rows whose loads are in flight together
-constexpr int64_t kMaxStride = 1 << 26; // elements: eight rows of four bytes are 2^31 bytes apart at most
+constexpr int64_t kMaxStride = 1 << 25; // elements: sixteen rows of four bytes are 2^31 bytes apart at most
 
 struct ScanArgs {
     const void *u, *dt, *z, *B, *C, *gy;
@@ -795,7 +795,7 @@ int check_scan(const nfa_selective_scan_args *a, const char *who, bool step) {
     NFA_REQUIRE(a->n_rays >= 0 && a->rows >= 0 && a->channels >= 1, "%s: bad size", who);
     NFA_REQUIRE(a->states >= 1 && a->states <= NFA_SCAN_MAX_STATES, "%s: states must be 1 .. %d, got %d", who, NFA_SCAN_MAX_STATES, a->states);
     NFA_REQUIRE(dtype_ok(a->dtype), "%s: bad dtype %d", who, a->dtype);
-    NFA_REQUIRE(a->rows < (1ll << 31) && a->n_rays < (1ll << 31) && a->channels <= (1 << 24), "%s: too many rows, rays or channels", who);
+    NFA_REQUIRE(a->rows < (1ll << 31) && a->n_rays < (1ll << 31) && a->channels <= (1 << 23), "%s: too many rows, rays or channels", who);
     const int64_t rows = step ? a->n_rays : a->rows;
     NFA_REQUIRE(a->A, "%s: NULL pointer", who);
     NFA_REQUIRE(rows == 0 || (a->inputs && a->delta && a->B && a->C), "%s: NULL pointer", who);
@@ -803,7 +803,7 @@ int check_scan(const nfa_selective_scan_args *a, const char *who, bool step) {
                               a->B_stride >= a->states && a->C_stride >= a->states), "%s: a row stride is shorter than its row", who);
     if (step) return NFA_OK;
     for (int64_t ld : {a->inputs_stride, a->delta_stride, a->gate_stride, a->B_stride, a->C_stride, a->grad_outputs_stride})
-        NFA_REQUIRE(ld <= kMaxStride, "%s: a row stride is over 2^26", who);
+        NFA_REQUIRE(ld <= kMaxStride, "%s: a row stride is over 2^25", who);
     NFA_REQUIRE(a->packed_info || a->n_rays == 0 || a->rows % a->n_rays == 0, "%s: rows do not divide into equal sequences", who);
     NFA_REQUIRE(a->n_rays > 0 || a->packed_info || a->rows == 0, "%s: rows without sequences", who);
     NFA_REQUIRE(!a->packed_info || a->rows == 0 || (a->row_ray && a->row_pos), "%s: packed sequences need their row map", who);

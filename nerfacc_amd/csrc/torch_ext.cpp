@@ -1412,12 +1412,12 @@ inline int32_t dtype_of(const Tensor &t) {
     return NFA_DTYPE_F16;
 }
 
-// a [rows, cols] tensor whose rows are contiguous and do not overlap, at any row stride up to 2^26; copied if it is not one
+// a [rows, cols] tensor whose rows are contiguous and do not overlap, at any row stride up to 2^25; copied if it is not one
 inline Tensor as_rows(const Tensor &t, const char *name, int64_t rows, int64_t cols, const Tensor &like) {
     TORCH_CHECK(t.defined() && t.is_cuda(), name, " must be a CUDA/HIP tensor (nerfacc_amd has no CPU kernels)");
     TORCH_CHECK(t.device() == like.device() && t.scalar_type() == like.scalar_type(), name, " differs in device or dtype");
     TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, name, " must have shape [", rows, ", ", cols, "]");
-    if ((t.stride(1) == 1 || cols == 1) && ((t.stride(0) >= cols && t.stride(0) <= (1 << 26)) || rows <= 1)) return t;
+    if ((t.stride(1) == 1 || cols == 1) && ((t.stride(0) >= cols && t.stride(0) <= (1 << 25)) || rows <= 1)) return t;
     return t.contiguous();
 }
 inline int64_t row_stride(const Tensor &t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }

@@ -191,8 +191,8 @@ def _dtype_id(t: torch.Tensor) -> int:
 
 
 def _as_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """a 2-D tensor whose rows are contiguous and do not overlap, at any row stride up to 2^26; copied if it is not one"""
-    if t is None or ((t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[1] <= t.stride(0) <= 1 << 26 or t.shape[0] <= 1)):
+    """a 2-D tensor whose rows are contiguous and do not overlap, at any row stride up to 2^25; copied if it is not one"""
+    if t is None or ((t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[1] <= t.stride(0) <= 1 << 25 or t.shape[0] <= 1)):
         return t
     return t.contiguous()
 

@@ -274,3 +274,82 @@ def test_the_grid_and_mlp_field_through_it():
         grads.append([rgb.detach(), *torch.autograd.grad((rgb - 0.3).square().sum(), list(field.parameters()))])
     for a, b in zip(*grads):                                # atomic sums in torch's scatter and products: relative to the tensor's own size
         assert (a - b).abs().max() <= 1e-4 * a.abs().max() + 1e-7
+
+
+def test_fp16_dz_beyond_its_range():
+    """dz = dy act'(z) over 65504 with gradients that fit: the two parts of dz hold it, and an infinite gradient stays infinite"""
+    import nerfacc_amd as nerfacc
+
+    x = torch.full((3, 8), 1.0, device=DEV, dtype=torch.float16, requires_grad=True)
+    w = torch.full((16, 8), 0.5, device=DEV, dtype=torch.float16)
+    gy = torch.full((3, 16), 2000.0, device=DEV, dtype=torch.float16)                # e^4 = 54.6: dz = 109200
+    gy[2] = float("inf")
+    out = nerfacc.linear(x, w, activation="exp")
+    gx = torch.autograd.grad(out, x, gy)[0]
+    assert gx[2].isposinf().all() and gx[:2].isposinf().all()                        # 16 x 54600 does not fit fp16: inf, not NaN
+    gx = torch.autograd.grad(nerfacc.linear(x, w * torch.tensor([[1.0]] + [[0.0]] * 15, device=DEV).half(), activation="exp"), x, gy[:1].expand(3, 16))[0]
+    assert (gx.float() - 54.598 * 2000 * 0.5).abs().max() <= 2.0**-10 * 54600
+
+
+def test_offsets_beyond_32_bits():
+    """outputs of more than 2^31 numbers: their end is what the last rows give alone"""
+    import nerfacc_amd as nerfacc
+
+    x = torch.randn((1 << 23) + 77, 8, generator=torch.Generator(device=DEV).manual_seed(0), device=DEV).bfloat16()
+    w = torch.randn(264, 8, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).bfloat16()
+    out = nerfacc.linear(x, w, activation="relu")
+    assert out.numel() > 1 << 31 and torch.equal(out[-3000:], nerfacc.linear(x[-3000:], w, activation="relu"))
+    assert torch.equal(out[:500], nerfacc.linear(x[:500], w, activation="relu"))
+
+
+def test_a_large_weight_in_a_captured_step():
+    """the form whose workgroups take more than 64 KiB of LDS, captured and replayed"""
+    import nerfacc_amd as nerfacc
+
+    x, w, b, r, g = make(900, 256, 256, torch.bfloat16, seed=12, residual=True)
+    own = [t.detach().requires_grad_(True) for t in (x, w, b, r)]
+
+    def step():
+        out = nerfacc.linear(own[0], own[1], own[2], activation="relu", residual=own[3])
+        return [out.detach(), *torch.autograd.grad(out, own, g)]
+
+    step()
+    gc.collect()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, generator=torch.Generator(device=DEV).manual_seed(k), device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(held, step())), k
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    """a backward pass that could not be captured: the forward call says so instead"""
+    import nerfacc_amd as nerfacc
+    from nerfacc_amd.cuda import _backend
+
+    if _backend.BACKEND != "ext":
+        pytest.skip("torch extension not the active backend")
+    x, w, b, r, g = make(64, 32, 32, torch.float32, seed=13)
+    own = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    alive = nerfacc.linear(*own)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        with torch.cuda.graph(graph):
+            nerfacc.linear(*own)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()), torch.no_grad():
+        nerfacc.linear(*own)                                                         # without gradients there is nothing to capture
+    assert alive.shape == (64, 32)
+    torch.cuda.synchronize()
+
+
+def test_docstring_example():
+    import nerfacc_amd as nerfacc
+
+    x = torch.tensor([[1., 2.]], device=DEV)
+    assert nerfacc.linear(x, torch.tensor([[1., 1.], [1., -1.]], device=DEV), activation="relu").tolist() == [[3.0, 0.0]]

@@ -567,3 +567,30 @@ def test_differentiating_twice_is_refused(monkeypatch):
         gx = torch.autograd.grad(nerfacc.linear(x, w, activation="silu"), x, gy, create_graph=True)[0]
         with pytest.raises(RuntimeError, match="once_differentiable"):
             gx.sum().backward()
+
+
+def test_offsets_beyond_32_bits():
+    """tensors of more than 2^31 numbers: the last rays are what they give alone"""
+    import nerfacc_amd as nerfacc
+
+    rays, n, d = 2100, 1000, 1040
+    x = torch.randn(64, n, d, generator=generator(0), device=DEV).bfloat16().repeat(33, 1, 1)[:rays]
+    assert x.numel() > 1 << 31
+    w = torch.randn(d, 4, generator=generator(1), device=DEV).bfloat16()
+    assert torch.equal(nerfacc.causal_conv(x, w, activation="silu")[-2:], nerfacc.causal_conv(x[-2:], w, activation="silu"))
+    A, bc = -torch.rand(d, 1, generator=generator(2), device=DEV), torch.randn(rays, n, 1, generator=generator(3), device=DEV).bfloat16()
+    out = nerfacc.selective_scan(x, x, A, bc, bc, delta_softplus=True)
+    tail = nerfacc.selective_scan(x[-70:], x[-70:], A, bc[-70:], bc[-70:], delta_softplus=True)
+    assert torch.equal(out[-70:], tail)                               # (70 rays: whole ones there too)
+
+
+def test_docstring_examples():
+    import nerfacc_amd as nerfacc
+
+    info = torch.tensor([[0, 2], [2, 1]], device=DEV)
+    x = torch.tensor([[1.], [2.], [3.]], device=DEV)
+    assert nerfacc.causal_conv(x, torch.tensor([[1., 10.]], device=DEV), packed_info=info).flatten().tolist() == [10.0, 21.0, 30.0]
+    y, state = nerfacc.causal_conv_step(torch.tensor([[3.]], device=DEV), torch.tensor([[[2.]]], device=DEV), torch.tensor([[1., 10.]], device=DEV))
+    assert y.tolist() == [[32.0]] and state.tolist() == [[[3.0]]]
+    one = torch.ones(3, 1, device=DEV)
+    assert nerfacc.selective_scan(one, one, torch.zeros(1, 1, device=DEV), one, one, packed_info=info).flatten().tolist() == [1.0, 2.0, 1.0]
