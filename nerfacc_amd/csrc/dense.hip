@@ -459,7 +459,7 @@ __device__ __forceinline__ u32x4 read_frag(const char *tile, int c0, int ks, int
 }
 
 // WP x WQ waves, each with BP / WP x BQ / WQ of the tile
-template <class T, int MODE, int BP, int BQ, int WP, int WQ, bool SPLIT, bool VEC>
+template <class T, int MODE, int BP, int BQ, int WP, int WQ, bool SPLIT, bool VEC, bool DEEP>
 __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
     constexpr int TH = WP * WQ * kWave;
     constexpr bool PT = MODE == kWgrad, QT = MODE != kForward, FUSE = MODE != kForward;
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
     const int64_t c_end = MODE == kWgrad ? (c_begin + a.split < a.n_c ? c_begin + a.split : a.n_c) : a.n_c;
 
     const T *P = reinterpret_cast<const T *>(a.p), *Q = reinterpret_cast<const T *>(a.q);
-    u32x4 rp[CP], rs[CP], rq[CQ];
+    struct Staged { u32x4 p[CP], s[FUSE ? CP : 1], q[CQ]; };
     f32x4 acc[NP][NQ];
 #pragma unroll
     for (int i = 0; i < NP; ++i)
@@ -500,15 +500,15 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
         chunk = tid % per_row;
         row = tid / per_row + k * (TH / per_row);
     };
-    auto load = [&](int64_t c) {
+    auto load = [&](Staged &t, int64_t c) {
 #pragma unroll
         for (int k = 0; k < CP; ++k) {
             int row, chunk;
             place(PT, BP, k, row, chunk);
             const int64_t r = PT ? c + row : p0 + row, col = PT ? p0 + chunk * CE : c + chunk * CE;
             const int64_t rows = PT ? c_end : a.n_p, cols = PT ? a.n_p : a.n_c;
-            rp[k] = load_chunk<T, VEC>(P, r, rows, a.ld_p, col, cols);
-            if (FUSE) rs[k] = load_saved<T, VEC>(a, r, rows, col, cols);
+            t.p[k] = load_chunk<T, VEC>(P, r, rows, a.ld_p, col, cols);
+            if constexpr (FUSE) t.s[k] = load_saved<T, VEC>(a, r, rows, col, cols);
         }
 #pragma unroll
         for (int k = 0; k < CQ; ++k) {
@@ -516,28 +516,28 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
             place(QT, BQ, k, row, chunk);
             const int64_t r = QT ? c + row : q0 + row, col = QT ? q0 + chunk * CE : c + chunk * CE;
             const int64_t rows = QT ? c_end : a.n_q, cols = QT ? a.n_q : a.n_c;
-            rq[k] = load_chunk<T, VEC>(Q, r, rows, a.ld_q, col, cols);
+            t.q[k] = load_chunk<T, VEC>(Q, r, rows, a.ld_q, col, cols);
         }
     };
-    auto store = [&](char *buf, int64_t c) {
+    auto store = [&](Staged &t, char *buf, int64_t c) {
         u32x4 lo[SPLIT ? CP : 1];
 #pragma unroll
         for (int k = 0; k < CP; ++k) {
             int row, chunk;
             place(PT, BP, k, row, chunk);
             const bool inside = PT ? c + row < c_end && p0 + chunk * CE < a.n_p : p0 + row < a.n_p && c + chunk * CE < a.n_c;
-            rp[k] = only_inside<VEC>(rp[k], inside);
-            if (FUSE) rs[k] = only_inside<VEC>(rs[k], inside);
+            t.p[k] = only_inside<VEC>(t.p[k], inside);
+            if constexpr (FUSE) t.s[k] = only_inside<VEC>(t.s[k], inside);
         }
         if constexpr (FUSE)
-            form_dz<T, SPLIT, CP>(a, rp, rs, lo, [&](int, float dz, int e) {
+            form_dz<T, SPLIT, CP>(a, t.p, t.s, lo, [&](int, float dz, int e) {
                 if constexpr (MODE == kWgrad) db[e] += dz;
             });
 #pragma unroll
         for (int k = 0; k < CP; ++k) {
             int row, chunk;
             place(PT, BP, k, row, chunk);
-            *reinterpret_cast<u32x4 *>(buf + stage_offset<T, PT, BP>(row, chunk)) = rp[k];
+            *reinterpret_cast<u32x4 *>(buf + stage_offset<T, PT, BP>(row, chunk)) = t.p[k];
             if constexpr (SPLIT) *reinterpret_cast<u32x4 *>(buf + kP + stage_offset<T, PT, BP>(row, chunk)) = lo[k];
         }
 #pragma unroll
@@ -545,7 +545,7 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
             int row, chunk;
             place(QT, BQ, k, row, chunk);
             const bool inside = QT ? c + row < c_end && q0 + chunk * CE < a.n_q : q0 + row < a.n_q && c + chunk * CE < a.n_c;
-            *reinterpret_cast<u32x4 *>(buf + kBuf - BQ * kRowBytes + stage_offset<T, QT, BQ>(row, chunk)) = only_inside<VEC>(rq[k], inside);
+            *reinterpret_cast<u32x4 *>(buf + kBuf - BQ * kRowBytes + stage_offset<T, QT, BQ>(row, chunk)) = only_inside<VEC>(t.q[k], inside);
         }
     };
     auto compute = [&](const char *buf, int64_t c) {
@@ -567,17 +567,39 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
         }
     };
 
-    load(c_begin);
-    store(lds, c_begin);
-    __syncthreads();
-    int cur = 0;
-    for (int64_t c = c_begin; c < c_end; c += ST) {
-        const bool more = c + ST < c_end;
-        if (more) load(c + ST);
-        compute(lds + cur * kBuf, c);
-        if (more) store(lds + (cur ^ 1) * kBuf, c + ST);
+    if constexpr (DEEP) {
+        // Two tiles in flight behind the one that is multiplied.  Every load is made, also behind the end (from a place that exists; what
+        // lies outside is stored as zeros): with a branch around it the wait for one tile would be a wait for both.
+        static_assert(VEC, "loads behind the end need places that exist");
+        Staged even, odd;
+        load(even, c_begin);
+        load(odd, c_begin + ST);
+        store(even, lds, c_begin);
         __syncthreads();
-        cur ^= 1;
+        auto step = [&](Staged &next, Staged &after, int64_t c, int cur) {       // tile c is in buffer `cur`, tile c + ST in `next`
+            load(after, c + 2 * ST);
+            compute(lds + cur * kBuf, c);
+            store(next, lds + (cur ^ 1) * kBuf, c + ST);
+            __syncthreads();
+        };
+        for (int64_t c = c_begin; c < c_end; c += 2 * ST) {
+            step(odd, even, c, 0);
+            step(even, odd, c + ST, 1);
+        }
+    } else {
+        Staged t;
+        load(t, c_begin);
+        store(t, lds, c_begin);
+        __syncthreads();
+        int cur = 0;
+        for (int64_t c = c_begin; c < c_end; c += ST) {
+            const bool more = c + ST < c_end;
+            if (more) load(t, c + ST);
+            compute(lds + cur * kBuf, c);
+            if (more) store(t, lds + (cur ^ 1) * kBuf, c + ST);
+            __syncthreads();
+            cur ^= 1;
+        }
     }
 
     // lane l holds row p = l % 16 of each fragment and four neighbouring columns q
@@ -755,9 +777,13 @@ int launch_tiles(DenseArgs a, int64_t splits, hipStream_t s) {
     a.tiles = (int32_t)(tiles_p * a.tiles_q);
     const int64_t steps = MODE == kWgrad ? a.split : a.n_c;
     const size_t bytes = (size_t)(BP * (SPLIT ? 2 : 1) + BQ) * kRowBytes * (steps > kStage<T> ? 2 : 1);
-    auto kernel = tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, true>;
+    auto kernel = tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, true, false>;
     if constexpr (BP < 256)                                 // (the largest tiles are for aligned rows)
-        if (!a.vec) kernel = tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, false>;
+        if (!a.vec) kernel = tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, false, false>;
+    // two tiles ahead where one workgroup is all a CU holds and the contraction is long enough: weight gradient of 2^18 x 256 x 256 104 -> 90
+    // us, 65536 x 1024 x 1024 forward 226 -> 219 (dgrad has no registers left for it)
+    if constexpr (BP * BQ >= 128 * 256 && sizeof(T) == 2 && MODE != kDgrad)
+        if (a.vec && steps >= 8 * kStage<T>) kernel = tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, true, true>;
     if (int rc = allow_lds(kernel, bytes)) return rc;
     a.splits = (int32_t)splits;
     const unsigned grid = (unsigned)(ceil_div(a.tiles * splits, kNumXCD) * kNumXCD);
