@@ -724,6 +724,107 @@ __global__ __launch_bounds__(kBlock) void stream_kernel(DenseArgs a) {
     epilogue<T, kForward, VEC, NC>(a, p, col, a.n_q, z, res);
 }
 
+// ---- the weight gradient of a narrow layer in 32 bits ------------------------------------------------------------------------
+// dW[n][k] = sum_m dz[m][n] x[m][k] with n and k of up to 64.  One matrix instruction takes four rows, a lane a column of one of them: so
+// a lane loads NP (NQ) neighbouring columns of its row straight from memory, fragment f takes the f-th of them (its columns are f, NP + f,
+// 2 NP + f, ...), nothing goes through LDS, and columns are padded to 16 and not to the 64 of a tile.  Reading dy and x once bounds it.
+// The four waves of a workgroup take every fourth sixteen rows each and join their sums in LDS in order.
+template <int NP, int NQ>
+__global__ __launch_bounds__(kBlock, 2) void narrow_wgrad_kernel(DenseArgs a) {
+    constexpr int kSteps = 4;                               // four rows each, loaded together
+    struct alignas(NP * 4) PVec { float v[NP]; };
+    struct alignas(NQ * 4) QVec { float v[NQ]; };
+    struct Rows { PVec p[kSteps], s[kSteps]; uint32_t bits[kSteps]; QVec q[kSteps]; };
+    __shared__ f32x4 sums[kWavesPerBlock][NP * NQ][kWave];
+    const int lane = lane_id(), i = lane & 15, g = lane >> 4, wave = wave_in_block();
+    const int64_t stretch = blockIdx.x, begin = stretch * a.split, end = begin + a.split < a.n_c ? begin + a.split : a.n_c;
+    const int p = i * NP < a.n_p ? i * NP : 0, q = i * NQ < a.n_q ? i * NQ : 0;      // (columns that do not exist are read from one that does)
+    const bool value = a.act != NFA_ACT_NONE && !a.mask;
+    f32x4 acc[NP][NQ];
+    float db[NP];
+#pragma unroll
+    for (int f = 0; f < NP; ++f) {
+        db[f] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < NQ; ++e) acc[f][e] = f32x4{0, 0, 0, 0};
+    }
+    auto load = [&](Rows &r, int64_t row0) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            const int64_t want = row0 + k * 4 + g, row = want < end ? want : end - 1;
+            r.p[k] = *reinterpret_cast<const PVec *>(reinterpret_cast<const float *>(a.p) + row * a.ld_p + p);
+            r.q[k] = *reinterpret_cast<const QVec *>(reinterpret_cast<const float *>(a.q) + row * a.ld_q + q);
+            if (a.mask) r.bits[k] = reinterpret_cast<const uint8_t *>(a.saved)[row * a.ld_saved + (p >> 2)];
+            if (value) r.s[k] = *reinterpret_cast<const PVec *>(reinterpret_cast<const float *>(a.saved) + row * a.ld_saved + p);
+        }
+    };
+    auto add = [&](Rows &r, int64_t row0) {
+        with_act(a.act, [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int f = 0; f < NP; ++f) {
+                    float &dz = r.p[k].v[f];
+                    if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((r.bits[k] >> ((p & 3) + f)) & 1u) != 0 : r.s[k].v[f] > 0.0f) ? dz : 0.0f;
+                    else if constexpr (ACT != NFA_ACT_NONE) dz *= act_slope<ACT>(r.s[k].v[f]);
+                }
+        });
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            const bool inside = row0 + k * 4 + g < end;
+#pragma unroll
+            for (int f = 0; f < NP; ++f) db[f] += r.p[k].v[f] = inside ? r.p[k].v[f] : 0.0f;
+#pragma unroll
+            for (int e = 0; e < NQ; ++e) {
+                const float x = inside ? r.q[k].v[e] : 0.0f;
+#pragma unroll
+                for (int f = 0; f < NP; ++f) acc[f][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, r.p[k].v[f], acc[f][e], 0, 0, 0);
+            }
+        }
+    };
+    constexpr int kEach = kSteps * 4, kStride = kEach * kWavesPerBlock;
+    Rows now, next;
+    int64_t row = begin + wave * kEach;
+    load(now, row);
+    for (; row < end; row += kStride) {
+        load(next, row + kStride);
+        add(now, row);
+        now = next;
+    }
+#pragma unroll
+    for (int f = 0; f < NP; ++f)
+#pragma unroll
+        for (int e = 0; e < NQ; ++e) sums[wave][f * NQ + e][lane] = acc[f][e];
+    __syncthreads();
+    float *part = a.partial + stretch * (a.n_p * a.n_q + a.n_p);
+    for (int t = wave; t < NP * NQ; t += kWavesPerBlock) {
+        f32x4 v = sums[0][t][lane];
+#pragma unroll
+        for (int w = 1; w < kWavesPerBlock; ++w) v += sums[w][t][lane];
+        const int col = i * NP + t / NQ;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int at = (g * 4 + r) * NQ + t % NQ;
+            if (col < a.n_p && at < a.n_q) part[(int64_t)col * a.n_q + at] = v[r];
+        }
+    }
+    if (!a.want_bias) return;
+    __syncthreads();
+    float *join = reinterpret_cast<float *>(sums);          // [wave][fragment][lane]
+#pragma unroll
+    for (int f = 0; f < NP; ++f) join[(wave * NP + f) * kWave + lane] = db[f];
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c < a.n_p) {
+        float v = 0.0f;
+        for (int w = 0; w < kWavesPerBlock; ++w)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v += join[(w * NP + c % NP) * kWave + r * 16 + c / NP];
+        part[a.n_p * a.n_q + c] = v;
+    }
+}
+
 // Columns by lane, sixteen rows side by side; a column's sum is formed in the same order every time.  A workgroup sums the rows
 // [first, first + each) of its 64 columns, first = blockIdx.y * each; of many rows a first launch leaves each stretch's sum in the
 // stretch's own first row (nobody else reads it), a second one sums those.  The columns go to up to three outputs, one behind the other
@@ -817,45 +918,78 @@ int launch_resident(DenseArgs a, hipStream_t s) {
     return check_launch("resident_kernel");
 }
 
+template <class T>
+int launch_stream(DenseArgs a, hipStream_t s) {
+    a.tiles_q = (int32_t)ceil_div(a.n_q, 32);
+    NFA_REQUIRE(ceil_div(a.n_p, 16) * a.tiles_q < (1ll << 31), "linear: too many rows for one launch");
+    const auto kernel = a.vec ? stream_kernel<T, true> : stream_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(ceil_div(a.n_p, 16) * a.tiles_q)), dim3(kBlock), 0, s, a);
+    return check_launch("stream_kernel");
+}
+
 // forward or dgrad: the weight in LDS for contractions of up to 256, tiles beyond
 template <class T, int MODE, bool SPLIT>
 int launch_rows(const DenseArgs &a, hipStream_t s) {
     constexpr int step = 4 * kChunk<T>;
+    // few rows: neither a weight for every CU nor a tile, but rows, columns and the contraction over many workgroups.  In bf16 while every
+    // CU gets one (1000 x 128 x 128: 4.5 us against 4.7 with the weight in LDS, 1000 x 256 x 256, 504 workgroups, 5.6 against 6.5, but
+    // 1500 x 128 x 128, 376 of them, 5.4 against 4.7), in fp32, whose weight takes twice as long to LDS, four (1000 x 256 x 256 5.9
+    // against 10.0, 400 x 128 x 1024, 800 workgroups, 8.6 against 9.0, 1000 x 128 x 1024, 2016, 14.4 against 12.9)
+    if (MODE == kForward && ceil_div(a.n_p, 16) * ceil_div(a.n_q, 32) <= (sizeof(T) == 4 ? 4 : 1) * kNumCU) return launch_stream<T>(a, s);
+    // the weight in LDS; 2^18 x 256 x 256 bf16 forward 66 us against 88 by tiles, dgrad 62 against 81; fp32 316 against 339
     if (a.n_c <= step) return launch_resident<T, MODE, 1, SPLIT>(a, s);
     if (a.n_c <= 2 * step) return launch_resident<T, MODE, 2, SPLIT>(a, s);
     if (a.n_c <= 4 * step) return launch_resident<T, MODE, 4, SPLIT>(a, s);
     if (a.n_c <= 8 * step) return launch_resident<T, MODE, 8, SPLIT>(a, s);
+    // (dgrad in fp32 reads a number of a column at a time from LDS, here for every sixteen rows, by tiles for 64: 2^18 x 256 x 256 608 us
+    // against 439 by tiles, 2^18 x 64 x 256 220 against 144, 4096 x 256 x 256 35 against 28; 300 x 256 x 256, six tiles, 14 against 27)
     if constexpr (sizeof(T) == 4)
-        if (a.n_c <= 16 * step) return launch_resident<T, MODE, 16, SPLIT>(a, s);
-    // few tiles: rows, and the contraction, over more workgroups.  4096 x 1024 x 256, 64 tiles: fp32 49 us against 84 by tiles (whose steps
-    // are four times as long as those of 16-bit types), bf16 25 against 20
-    if (MODE == kForward && ceil_div(a.n_p, 128) * ceil_div(a.n_q, 128) < (sizeof(T) == 4 ? kNumCU : kNumCU / 4)) {
-        DenseArgs b = a;
-        b.tiles_q = (int32_t)ceil_div(a.n_q, 32);
-        const auto kernel = a.vec ? stream_kernel<T, true> : stream_kernel<T, false>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(ceil_div(a.n_p, 16) * b.tiles_q)), dim3(kBlock), 0, s, b);
-        return check_launch("stream_kernel");
-    }
+        if (a.n_c <= 16 * step && (MODE == kForward || ceil_div(a.n_p, 128) * ceil_div(a.n_q, 128) < kNumCU / 4))
+            return launch_resident<T, MODE, 16, SPLIT>(a, s);
+    // long contractions.  Few tiles: 4096 x 1024 x 256, 64 of them: fp32 49 us against 84 by tiles (whose steps are four times as long as
+    // those of 16-bit types), bf16 25 against 20.  In fp32 any number of rows too, where the 32 columns of one workgroup are all there
+    // are: 75956 x 751 x 4 61 us against 98, 75956 x 752 x 32 63 against 89; in bf16 41 against 26 and 36 against 25
+    if (MODE == kForward && ((sizeof(T) == 4 && a.n_q <= 32) ||
+                             ceil_div(a.n_p, 128) * ceil_div(a.n_q, 128) < (sizeof(T) == 4 ? kNumCU : kNumCU / 4))) return launch_stream<T>(a, s);
     // 16-bit types, aligned and large enough for every CU: 256 x 256 by eight waves, whose fragments are used often enough that the matrix
-    // units and not LDS set the pace
+    // units and not LDS set the pace (16384 x 1024 x 1024 bf16 43.9 us against 51.8 by 128 x 128, 65536 x 512 x 512 56.5 against 62.7)
     constexpr int BP = SPLIT ? 64 : 128;
     if constexpr (sizeof(T) == 2 && !SPLIT)
         if (a.vec && a.n_q > 128 && ceil_div(a.n_p, 256) * ceil_div(a.n_q, 256) >= kNumCU) return launch_tiles<T, MODE, 256, 256, 2, 4, SPLIT>(a, 1, s);
+    // (64 columns where there are no more: 65536 x 512 x 64 fp32 45 us against 79)
     return a.n_q <= 64 ? launch_tiles<T, MODE, BP, 64, 2, 2, SPLIT>(a, 1, s) : launch_tiles<T, MODE, BP, 128, 2, 2, SPLIT>(a, 1, s);
+}
+
+template <int NP>
+int launch_narrow_wgrad(DenseArgs a, int64_t splits, hipStream_t s) {
+    const auto kernel = a.n_q <= 16 ? narrow_wgrad_kernel<NP, 1> : a.n_q <= 32 ? narrow_wgrad_kernel<NP, 2> : narrow_wgrad_kernel<NP, 4>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)splits), dim3(kBlock), 0, s, a);
+    return check_launch("narrow_wgrad_kernel");
 }
 
 // rows of the long axis that one workgroup of the weight gradient sums: enough workgroups for every CU twice, and not so many that
 // their partial sums (a whole weight each) outweigh the rows read
 struct WgradPlan { int64_t split, splits, bp, bq; };
+bool narrow_layer(int64_t n, int64_t k) { return n <= 64 && k <= 64 && n % 4 == 0 && k % 4 == 0; }
 WgradPlan wgrad_plan(int64_t rows, int64_t n, int64_t k, int32_t dtype, bool two_parts) {
     const int64_t stage = dtype == NFA_DTYPE_F32 ? 32 : 64;
     WgradPlan w;
+    // large tiles read dy and x fewer times (2^18 x 256 x 256 bf16 by 64 x 64, 128 x 128, 128 x 256: 173, 130, 91 us; fp32 418, 402, 368),
+    // but in fp32, which the matrix units bound, not at the price of padding (2^18 x 129 x 32: 92 us by 64 x 64, 117 by 64 x 128),
+    auto pad = [](int64_t x, int64_t b) { return ceil_div(x, b) * b; };
+    const bool f32 = dtype == NFA_DTYPE_F32;
     w.bp = n <= 64 || two_parts ? 64 : 128;
     w.bq = k <= 64 ? 64 : k <= 128 || two_parts || w.bp == 64 ? 128 : 256;
-    const int64_t tiles = ceil_div(n, w.bp) * ceil_div(k, w.bq);
-    const int64_t per_cu = w.bq == 256 ? 1 : std::max<int64_t>(2, 256 / w.bp + 256 / w.bq - 4);      // 4 of 64 x 64, 2 of 128 x 128
-    int64_t splits = ceil_div(per_cu * kNumCU, tiles);
+    if (f32)
+        while (w.bq > 64 && pad(k, w.bq / 2) < pad(k, w.bq)) w.bq /= 2;
+    // and not where the rows are too few for a workgroup on every CU (4096 x 256 x 256 bf16 12 us by 64 x 64, 18 by 128 x 256)
     const int64_t most = ceil_div(rows, 4 * stage);
+    if (ceil_div(n, w.bp) * ceil_div(k, w.bq) * most < kNumCU) w.bp = w.bq = 64;
+    const int64_t tiles = ceil_div(n, w.bp) * ceil_div(k, w.bq);
+    // workgroups on a CU: one of 128 x 256; two otherwise (2^18 x 64 x 64 bf16 20 us, 25 with four; narrow layers 2^18 x 8 x 32 14.4, 15.5
+    // with four), but four of 64 x 64 in fp32, whose steps are short (2^18 x 129 x 32: 109 us, 129 with two)
+    const int64_t per_cu = w.bq == 256 ? 1 : f32 && w.bp == 64 && w.bq == 64 && !narrow_layer(n, k) ? 4 : 2;
+    int64_t splits = ceil_div(per_cu * kNumCU, tiles);
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
     w.split = ceil_div(ceil_div(rows, splits), stage) * stage;
@@ -990,6 +1124,12 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
             if constexpr (sizeof(T) == 2)
                 if (split) {
                     rc = w.bq == 64 ? launch_tiles<T, kWgrad, 64, 64, 2, 2, true>(e, w.splits, s) : launch_tiles<T, kWgrad, 64, 128, 2, 2, true>(e, w.splits, s);
+                    return;
+                }
+            // 2^18 x 8 x 32: 14.4 us against 33 by tiles of 64 x 64, 32 x 32 17.4 against 34, 64 x 64 39.3 against 39.7
+            if constexpr (sizeof(T) == 4)
+                if (e.vec && narrow_layer(n, k)) {
+                    rc = n <= 16 ? launch_narrow_wgrad<1>(e, w.splits, s) : n <= 32 ? launch_narrow_wgrad<2>(e, w.splits, s) : launch_narrow_wgrad<4>(e, w.splits, s);
                     return;
                 }
             if (w.bp == 64) rc = w.bq == 64 ? launch_tiles<T, kWgrad, 64, 64, 2, 2, false>(e, w.splits, s) : launch_tiles<T, kWgrad, 64, 128, 2, 2, false>(e, w.splits, s);

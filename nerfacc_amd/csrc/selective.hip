@@ -752,8 +752,12 @@ void with_shape(int32_t dtype, Shape sh, F &&f) {
     });
 }
 
-// How a call is cut: whole sequences where they give every SIMD a wave; otherwise chunks of at least 32 rows, enough for two waves per
-// SIMD.  (Cutting costs a second pass over the exponentials, so it has to more than double the waves.)
+// How a call is cut.  Cutting costs a second pass over the exponentials, so whole sequences where they give every SIMD a wave (256
+// sequences of 256 rows, 256 channels: 151 us, 215 in chunks) or would be cut in less than four (512 of 64 rows, 64 channels: 42 us, 66 in
+// chunks of 32; 256 of 128 rows: 74 us, 58 in chunks).  Otherwise chunks of at least 32 rows, for two waves per SIMD; in the forward pass
+// four (32768 rows of 1024 channels 331 -> 297 us, 64 sequences of 512 rows, 512 channels 200 -> 165), unless that makes them shorter than
+// 64 rows (two sequences of 8192 rows, 512 channels: 106 us, 116 with four) or a chain longer than 512 (131072 rows of 64 channels: 298
+// and 497).  The backward pass holds two waves per SIMD at most (its LDS).
 struct ScanPlan { Shape sh; int blocks; int64_t chunk, chunks, slots, tasks, workers; };
 ScanPlan scan_plan(int64_t n_rays, int64_t rows, int channels, int states, bool packed, bool backward) {
     ScanPlan p{};
@@ -762,17 +766,22 @@ ScanPlan scan_plan(int64_t n_rays, int64_t rows, int channels, int states, bool 
     const int64_t waves = n_rays * p.blocks, want = (int64_t)kNumCU * 8;
     p.tasks = n_rays;
     if (n_rays > 0 && waves < kNumCU * 4 && rows / n_rays >= 64) {
-        int64_t chunk = ceil_div(ceil_div(rows * p.blocks, want), kTile) * kTile;
+        const int64_t length = rows / n_rays;
+        auto chunk_for = [&](int64_t waves) { return ceil_div(ceil_div(rows * p.blocks, waves), kTile) * kTile; };
+        int64_t chunk = chunk_for(want);
+        if (!backward && chunk_for(2 * want) >= 64 && length / chunk_for(2 * want) <= 512) chunk = chunk_for(2 * want);
         if (chunk < 32) chunk = 32;
-        if (chunk < rows / n_rays) {
+        if (4 * chunk <= length) {
             p.chunk = chunk;
-            p.chunks = ceil_div(rows / n_rays, chunk);
+            p.chunks = ceil_div(length, chunk);
             p.slots = rows / chunk + 1 + n_rays;
             p.tasks = packed ? n_rays + ceil_div(rows, chunk) : n_rays * p.chunks;
         }
     }
     p.workers = p.tasks;
-    const int64_t most = ceil_div(16384, p.blocks);
+    // partial sums of the backward pass: one per sequence, so that the long ones can be dealt out first, up to 32768 waves (16384 ragged
+    // sequences, 64 channels: 1.32 ms, 1.60 with half as many waves; 65536: 1.51 with a quarter, 1.57 with all of them)
+    const int64_t most = ceil_div(32768, p.blocks);
     if (backward && p.workers > most) p.workers = most;
     return p;
 }

@@ -353,3 +353,16 @@ def test_docstring_example():
 
     x = torch.tensor([[1., 2.]], device=DEV)
     assert nerfacc.linear(x, torch.tensor([[1., 1.], [1., -1.]], device=DEV), activation="relu").tolist() == [[3.0, 0.0]]
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 4, 4), (13, 8, 32), (999, 16, 4), (700, 64, 64), (5000, 32, 12), (2100, 20, 48)])
+@pytest.mark.parametrize("act", list(ACTS))
+def test_narrow_layers(m, k, n, act):
+    """up to 64 features in and out: rows and columns that end inside a step"""
+    check(*make(m, k, n, torch.float32, seed=12), act)
+
+
+@pytest.mark.parametrize("m,k,n", [(20011, 301, 4), (9000, 256, 256), (2049, 200, 132)])
+def test_choices_of_32_bits(m, k, n):
+    """many rows with few outputs and a long contraction; a backward product that goes by tiles"""
+    check(*make(m, k, n, torch.float32, seed=14), "softplus")
