@@ -8,6 +8,9 @@
 // rows in front of it, which the caches hold).  The backward walk runs forward too: it forms z again from x, and dx[t] is finished
 // W - 1 rows later, when its last g is known.  Weight gradients stay in registers over all of a thread's pieces, are joined in LDS
 // and then in order over the workgroups: no atomics.
+//
+// On one MI355X (copies reach 5.1 TB/s): 2^18 rows of 128 channels, bf16, 4096 rays: forward 33 us (134 MB: 4.1 TB/s), backward 67 us (201
+// MB: 3.0 TB/s) + 6 to join; 32768 x 2048 fp16: forward 58-63 us (268 MB: 4.3-4.6 TB/s); one row of 256 rays of 2048 channels 5 us.
 #include "feature.hpp"
 
 #include <algorithm>
@@ -69,6 +72,7 @@ __device__ __forceinline__ void load_before(const ConvArgs &a, int64_t row, Plac
 
 constexpr int kAhead = 4;               // rows whose loads are in flight together
 
+// Three waves on a SIMD: a fourth would take the registers of the window and the rows in flight (it spilled); memory bounds it at 4.1 TB/s.
 template <class T, int W, int VC>
 __global__ __launch_bounds__(kBlock, 3) void conv_fwd_kernel(ConvArgs a) {
     const int lane = threadIdx.x % a.lanes;
@@ -138,6 +142,8 @@ __global__ __launch_bounds__(kBlock, 3) void conv_fwd_kernel(ConvArgs a) {
     }
 }
 
+// x and dy in, dx out in one walk.  3.0 TB/s: z, the activation's slope and two windows of W rows take the vector units nearly as long as
+// the rows take to come, and the W - 1 rows in front of a piece are walked twice.
 template <class T, int W, int VC>
 __global__ __launch_bounds__(kBlock, 3) void conv_bwd_kernel(ConvArgs a) {
     extern __shared__ float joined[];
@@ -334,6 +340,7 @@ __global__ __launch_bounds__(kBlock) void conv_init_grad_kernel(ConvArgs a, T *g
     }
 }
 
+// one row of every sequence: the launch bounds it (256 x 2048 bf16, 8 MB: 5.0 us)
 template <class T, int W, int VC>
 __global__ __launch_bounds__(kBlock) void conv_step_kernel(ConvArgs a, const T *state, T *y, T *next) {
     const int64_t c = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * VC;
@@ -368,7 +375,7 @@ __global__ __launch_bounds__(kBlock) void conv_step_kernel(ConvArgs a, const T *
 __global__ __launch_bounds__(kBlock) void fill_map_kernel(int32_t *ray, int32_t *pos, int64_t rows) {
     for (int64_t r = (int64_t)blockIdx.x * kBlock + threadIdx.x; r < rows; r += (int64_t)gridDim.x * kBlock) ray[r] = pos[r] = -1;
 }
-// sixteen lanes per sequence
+// sixteen lanes per sequence; 2^18 rows of 4096 sequences 3 us, the fill before it 2.3
 __global__ __launch_bounds__(kBlock) void row_map_kernel(const int64_t *__restrict__ info, int64_t n_rays, int64_t rows,
                                                          int32_t *__restrict__ row_ray, int32_t *__restrict__ row_pos) {
     const int64_t groups = (int64_t)gridDim.x * (kBlock / 16);
@@ -383,7 +390,8 @@ __global__ __launch_bounds__(kBlock) void row_map_kernel(const int64_t *__restri
 }
 
 // One workgroup: the longest length, the sequences in each of 32 classes of length, and a place for every sequence behind the longer
-// classes.  (Within a class the order is the LDS atomics'; nothing depends on it.)
+// classes.  (Within a class the order is the LDS atomics'; nothing depends on it.)  4096 sequences take 9.6 us, latency, and spare a scan of
+// them 65 us forward and 145 us backward (ragged, 2^18 rows of 64 channels).
 constexpr int kClasses = 32;
 __global__ __launch_bounds__(1024) void ray_order_kernel(const int64_t *__restrict__ info, int64_t n_rays, int64_t rows, int32_t *__restrict__ order) {
     __shared__ int longest, place[kClasses];
@@ -526,6 +534,8 @@ NFA_EXPORT int nfa_causal_conv_fwd(const nfa_causal_conv_args *a, void *outputs,
     ConvArgs d = conv_args(a);
     d.y = outputs;
     const int64_t bytes = dtype_bytes(a->dtype);
+    // sixteen bytes to a thread where rows allow it (32768 x 2048 bf16 58 us, 66 with eight bytes; 2^18 x 128 fp32 48, 81 with four), else one
+    // number
     int vec = (int)(16 / bytes);
     if (a->channels % vec || !fits(d.x, d.ld_x, bytes, vec) || !fits(outputs, 0, bytes, vec) || !fits(d.init, 0, bytes, vec)) vec = 1;
     if (a->rows > 0) {
@@ -570,7 +580,8 @@ NFA_EXPORT int nfa_causal_conv_bwd(const nfa_causal_conv_args *a, void *grad_inp
     ConvArgs d = conv_args(a);
     d.gx = grad_inputs;
     const int64_t bytes = dtype_bytes(a->dtype);
-    // four channels to a thread: with eight, the windows, sums and weights of 16-bit channels take the registers of a second wave
+    // four channels to a thread: with eight, the windows, sums and weights of 16-bit channels do not fit the registers of three waves (2^18 x
+    // 128 bf16 71 us, 433 with eight); one where rows are not aligned (fp32 111 us, 218 with one)
     int vec = 4;
     if (a->channels % vec || !fits(d.x, d.ld_x, bytes, vec) || !fits(d.gy, d.ld_gy, bytes, vec) || !fits(grad_inputs, 0, bytes, vec) ||
         !fits(d.init, 0, bytes, vec) || !fits(d.gfinal, 0, bytes, vec))

@@ -15,8 +15,13 @@
 // one such eighth, because sequences do not overlap: slot = row / 8 needs no table).  With G = dL/dh,  G[t] = C[t] dy[t] +
 // exp(step[t+1] A) G[t+1]:
 //   dC = sum_d dy h,  dB = sum_d G step u,  du = step sum_s G B + D dy,  dstep = sum_s G (A a h[t-1] + B u),  dA = sum_t G step a h[t-1].
-// The sums over channels are exchanged across lanes (halving the values at every step: 16 values over 32 lanes cost 16 + 4 moves);
-// the sums over rows stay in registers over all rows of a wave; both are joined in a fixed order.
+// The sums over channels are exchanged across lanes (halving the values at every step, as long as there are two: 16 values over 32 lanes
+// take 8 + 4 + 2 + 1 + 1 exchanges); the sums over rows stay in registers over all rows of a wave; both are joined in a fixed order.
+//
+// On one MI355X, kernels alone, 16 states: 2^18 rows of 64 channels in 4096 ragged rays, bf16: forward 147 us with the kept states (143
+// vector instructions per row and wave, 80 % of the CUs' busy cycles), backward 346 us (264 instructions, 83 %) + 18 + 10 to join; memory
+// would take 59 us for all of it.  32768 rows of 1024 channels, one sequence, bf16: 283 us in all.  Two sequences of 8192 rows of 512
+// channels, fp32: forward 40 + 17 + 57 us, backward 47 + 13 + 173 + 14.  One row of 256 rays of 1024 channels: 8.2 us (35 MB, 4.3 TB/s).
 #include "feature.hpp"
 
 #include <algorithm>
@@ -223,7 +228,9 @@ template <int NS> __device__ __forceinline__ void read_states(const float *at, f
     for (int i = 0; i < NS; ++i) v[i] = at[i];
 }
 
-// main pass (LOCAL = false): outputs, kept states, final state; first pass over chunks (LOCAL): what a chunk adds, and its steps' sum
+// main pass (LOCAL = false): outputs, kept states, final state; first pass over chunks (LOCAL): what a chunk adds, and its steps' sum.
+// The vector units bound both: 95 us over 2^18 rows of 64 channels in equal rays (2.7e8 states, 2.8e12 of them a second), 40 us the first pass
+// over 16384 rows of 512 channels.
 template <class T, int NS, int P, bool LOCAL>
 __global__ __launch_bounds__(kWave) void scan_fwd_kernel(ScanArgs a) {
     constexpr int SP = NS * P, CH = kWave / P;
@@ -314,7 +321,8 @@ __global__ __launch_bounds__(kWave) void scan_fwd_kernel(ScanArgs a) {
 }
 
 // chunk by chunk, a lane per (channel, state): ends[slot] becomes the state that the chunk starts from (REV: the gradient that
-// reaches its last row from behind), from what each chunk adds on its own
+// reaches its last row from behind), from what each chunk adds on its own.  One dependent product-sum after the other, 32 chunks' loads
+// in flight: latency bounds it, about 0.1 us a chunk (256 chunks of 1024 channels 17 us).
 template <bool REV>
 __global__ __launch_bounds__(kBlock) void scan_chain_kernel(ScanArgs a) {
     const int64_t per = (int64_t)a.channels * a.states;
@@ -346,7 +354,7 @@ __global__ __launch_bounds__(kBlock) void scan_chain_kernel(ScanArgs a) {
     }
 }
 
-// the gradient that a chunk adds at its first row, and its steps' sum
+// the gradient that a chunk adds at its first row, and its steps' sum: 47 us for 16384 rows of 512 channels, the vector units' time
 template <class T, int NS, int P>
 __global__ __launch_bounds__(kWave) void scan_bwd_local_kernel(ScanArgs a) {
     constexpr int SP = NS * P, CH = kWave / P;
@@ -408,7 +416,8 @@ __global__ __launch_bounds__(kWave) void scan_bwd_local_kernel(ScanArgs a) {
 // The backward main pass.  A tile of eight rows at a time, from the last to the first: the lanes of a channel share the rows' own
 // numbers (step and its slope, dy, ...: each lane forms them for 8 / P rows) through LDS, which also keeps h before each row; so a lane's
 // registers hold one row, the loops stay loops (the body is several hundred instructions), and LDS (20 KiB a wave with sixteen states:
-// eight waves on a CU) sets how many waves a CU holds.
+// eight waves on a CU) sets how many waves a CU holds.  The vector units bound it: 346 us for 2^18 rows of 64 channels, 264 instructions
+// per row and wave.
 template <class T, int NS, int P>
 __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
     constexpr int SP = NS * P, CH = kWave / P, PR = P < kTile ? kTile / P : 1, kStates = (kTile * SP + kWave - 1) / kWave;
@@ -623,7 +632,8 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
     }
 }
 
-// dB and dC of a row: the channel blocks' sums in order; zeros for rows of no sequence.  A thread: four neighbouring states.
+// dB and dC of a row: the channel blocks' sums in order; zeros for rows of no sequence.  A thread: four neighbouring states.  Memory: 2^18
+// rows of two blocks and 16 states, 67 MB in and 17 out, 18 us (4.7 TB/s).
 template <class T>
 __global__ __launch_bounds__(kBlock) void scan_join_bc_kernel(ScanArgs a, int log_sp, T *gB, T *gC) {
     const int64_t n = a.rows << (log_sp - 1);               // 2 sp / 4 groups in a row
@@ -645,7 +655,7 @@ __global__ __launch_bounds__(kBlock) void scan_join_bc_kernel(ScanArgs a, int lo
     }
 }
 
-// rows of no sequence
+// rows of no sequence; where there are none it reads the map of 2^18 rows in 2.2 us
 template <class T>
 __global__ __launch_bounds__(kBlock) void zero_rows_kernel(const int32_t *__restrict__ pos, int64_t rows, int32_t cols, T *p, T *q, T *r) {
     const int lane = lane_id();
@@ -666,6 +676,7 @@ __global__ __launch_bounds__(kBlock) void zero_rows_kernel(const int32_t *__rest
 
 // One row per sequence: reading and writing the state bounds it (8 bytes per state).  L lanes share a channel, each with four
 // neighbouring states (one 16-byte access); L = 0: a lane per channel and states one by one, for numbers of states that do not divide.
+// 256 x 1024 x 16, bf16: 8.2 us (4.3 TB/s), 39.5 with states one by one.
 template <class T, int L>
 __global__ __launch_bounds__(kBlock) void scan_step_kernel(ScanArgs a, const float *state, float *next) {
     constexpr int LL = L ? L : 1;
@@ -709,7 +720,8 @@ __global__ __launch_bounds__(kBlock) void scan_step_kernel(ScanArgs a, const flo
     }
 }
 
-// lanes per channel and states per lane
+// lanes per channel and states per lane: up to 16 in a lane forward (2^18 rows of 64 channels of 16: 95 us, 106 by eights), 8 backward,
+// where a wave's history in LDS decides how many waves there are (349 us, 473 by sixteens)
 struct Shape { int ns, p; };
 Shape shape_of(int states, int most) {
     Shape s{4, 1};

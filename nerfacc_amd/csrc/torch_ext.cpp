@@ -1845,7 +1845,9 @@ struct RowMap {
         else if (n_rays == 0) info = at::empty({0, 2}, opts(x, at::kLong));
         if (info) std::tie(ray, pos) = row_map(*info, x.size(0));
     }
-    // the dealing order of a scan: where whole rays are a few for each wave place of the chip, their lengths decide when the last one ends
+    // the dealing order of a scan: where whole rays are a few for each wave place of the chip, their lengths decide when the last one ends.
+    // (64 channels, without and with the order, which takes 10 us by itself: 1024 ragged rays forward 115 and 114 us, backward 232 and 190;
+    // 4096 195 and 130, 482 and 336; 16384 397 and 313; 131072 515 and 488, no longer worth one workgroup's pass over all rays)
     OptTensor order(int64_t n_rays, int64_t rows) const {
         if (!info || n_rays < 1024 || n_rays > 65536) return std::nullopt;
         return ray_order(*info, rows);
