@@ -766,7 +766,8 @@ void with_shape(int32_t dtype, Shape sh, F &&f) {
 
 // How a call is cut.  Cutting costs a second pass over the exponentials, so whole sequences where they give every SIMD a wave (256
 // sequences of 256 rows, 256 channels: 151 us, 215 in chunks) or would be cut in less than four (512 of 64 rows, 64 channels: 42 us, 66 in
-// chunks of 32; 256 of 128 rows: 74 us, 58 in chunks).  Otherwise chunks of at least 32 rows, for two waves per SIMD; in the forward pass
+// chunks of 32; 256 of 128 rows: 74 us, 58 in chunks); packed ones, of which a few may be much longer than the mean, in less than two.
+// Otherwise chunks of at least 32 rows, for two waves per SIMD; in the forward pass
 // four (32768 rows of 1024 channels 331 -> 297 us, 64 sequences of 512 rows, 512 channels 200 -> 165), unless that makes them shorter than
 // 64 rows (two sequences of 8192 rows, 512 channels: 106 us, 116 with four) or a chain longer than 512 (131072 rows of 64 channels: 298
 // and 497).  The backward pass holds two waves per SIMD at most (its LDS).
@@ -783,7 +784,7 @@ ScanPlan scan_plan(int64_t n_rays, int64_t rows, int channels, int states, bool 
         int64_t chunk = chunk_for(want);
         if (!backward && chunk_for(2 * want) >= 64 && length / chunk_for(2 * want) <= 512) chunk = chunk_for(2 * want);
         if (chunk < 32) chunk = 32;
-        if (4 * chunk <= length) {
+        if (packed ? chunk < length : 4 * chunk <= length) {
             p.chunk = chunk;
             p.chunks = ceil_div(length, chunk);
             p.slots = rows / chunk + 1 + n_rays;

@@ -1402,8 +1402,8 @@ py::tuple grid_threshold(const Tensor &occs, double occ_thre, const std::optiona
 }
 
 // ---------------------------------------------------------------------------------------------------
-// feature operators (dense.hip, conv.hip, selective.hip).  The shapes and dtypes are checked by the Python layer
-// (nerfacc_amd/dense.py, selective.py); what would be read out of bounds is checked here again.
+// feature operators (dense.hip, conv.hip, selective.hip).  These calls check what would be read out of bounds; the whole operators further
+// down, and nerfacc_amd/dense.py and selective.py for the ctypes face, check shapes and dtypes in the caller's terms.
 // ---------------------------------------------------------------------------------------------------
 inline int32_t dtype_of(const Tensor &t) {
     if (t.scalar_type() == at::kFloat) return NFA_DTYPE_F32;
@@ -1700,7 +1700,7 @@ std::vector<OptTensor> selective_scan_bwd(
     if (!none) {
         auto a = in.args(softplus);
         seq.into(a);
-    a.ray_order = ptr<int32_t>(order);
+        a.ray_order = ptr<int32_t>(order);
         a.grad_outputs = gy.data_ptr(); a.grad_outputs_stride = row_stride(gy); a.grad_final_state = ptr<float>(gfinal);
         Tensor ws = at::empty({nfa_selective_scan_workspace_bytes(n_rays, in.n, a.channels, a.states, 1)}, opts(u, at::kByte));
         nfa_selective_scan_grads gr{};

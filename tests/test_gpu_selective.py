@@ -594,3 +594,11 @@ def test_docstring_examples():
     assert y.tolist() == [[32.0]] and state.tolist() == [[[3.0]]]
     one = torch.ones(3, 1, device=DEV)
     assert nerfacc.selective_scan(one, one, torch.zeros(1, 1, device=DEV), one, one, packed_info=info).flatten().tolist() == [1.0, 2.0, 1.0]
+
+
+def test_scan_cut_into_longer_chunks():
+    """enough channels that the forward pass takes chunks of its own length, with a last one that is not whole; packed rays of which one is
+    much longer than the mean"""
+    check_scan(scan_inputs(3 * 1400, 3, 4096, 4, torch.bfloat16, seed=7), shape=(3, 1400, 4096))
+    lens = [3] * 20 + [1500] + [0, 5]
+    check_scan(scan_inputs(sum(lens), len(lens), 6, 16, torch.float32, seed=8), packed(lens))
