@@ -19,7 +19,7 @@
 // On one MI355X (copies reach 5.1 TB/s, large library products 1335 TF bf16, 153 TF fp32), kernels alone:
 //   2^18 x 256 -> 256 bf16, relu + residual: forward 99 us (410 MB: 4.1 TB/s), dgrad 94 us (276 MB), wgrad 90 us + 8 to join
 //   2^18 x 8 -> 32 fp32, relu: 15, 15 and 10 us + 4;   100003 x 63 -> 65 fp16, softplus, no row aligned: 24, 37 and 37 us + 4
-//   65536 x 1024 -> 1024 bf16, silu: 205 us, 670 TF;   1 x 256 -> 256 bf16: 4.6 us a call
+//   65536 x 1024 -> 1024 bf16, silu: 186 us, 740 TF;   1 x 256 -> 256 bf16: 4.6 us a call
 #include "feature.hpp"
 
 #include <algorithm>
@@ -425,8 +425,7 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
 
 // ---- tile by tile ------------------------------------------------------------------------------------------------------
 // LDS layouts.  c-contiguous tiles: 128-byte rows, the 16-byte chunks of row r exchanged by r / 2 & 7: sixteen rows of one chunk lie
-// in all banks.  Transposed tiles (rows along c,
-// 64 or 128 columns): the 32-byte (16-bit types) or 64-byte units of a row exchanged so that the rows that one instruction reads
+// in all banks.  DEAL: so do the sixteen rows that dealt_row() names.  Transposed tiles (rows along c, 64 or 128 columns): the 32-byte (16-bit types) or 64-byte units of a row exchanged so that the rows that one instruction reads
 // lie in different banks.
 template <class T, int COLS>
 __device__ __forceinline__ int unit_swizzle(int row) {
@@ -434,19 +433,25 @@ __device__ __forceinline__ int unit_swizzle(int row) {
     if (COLS >= 128) return (row & 3) | (((row >> 3) & 1) << 2);
     return ((row >> 1) & 1) | (((row >> 3) & 1) << 1);
 }
-template <class T, bool TR, int ROWS>
+// forward, 16-bit types: the columns (rows of the weight's tile) of a pair of fragments are dealt out so that a lane's results of both
+// are eight neighbours, one 16-byte store of the result straight from its registers
+template <class T> __device__ __forceinline__ int dealt_row(int c0, int i) { return (c0 & ~31) + column_of<T>((c0 >> 4) & 1, i >> 2, i & 3); }
+template <class T, bool TR, int ROWS, bool DEAL = false>
 __device__ __forceinline__ int stage_offset(int row, int chunk) {        // byte offset of a chunk in its tile
+    if (DEAL) return row * kRowBytes + ((chunk ^ (((row >> 1) & 1) | ((row >> 2) & 6))) << 4);
     if (!TR) return row * kRowBytes + ((chunk ^ ((row >> 1) & 7)) << 4);
     if (sizeof(T) == 4) return row * ROWS * 4 + (((chunk >> 2) ^ unit_swizzle<T, ROWS>(row)) << 6) + ((chunk & 3) << 4);
     return row * ROWS * 2 + (((chunk >> 1) ^ unit_swizzle<T, ROWS>(row)) << 5) + ((chunk & 1) << 4);
 }
 
 // the sixteen bytes that lane l feeds to the matrix units for rows (or columns) c0 .. c0 + 15 and half `ks` of the tile
-template <class T, bool TR, int ROWS>
+template <class T, bool TR, int ROWS, bool DEAL = false>
 __device__ __forceinline__ u32x4 read_frag(const char *tile, int c0, int ks, int lane) {
     const int i = lane & 15, g = lane >> 4;
     u32x4 v;
-    if (!TR) {
+    if (DEAL) {
+        v = *reinterpret_cast<const u32x4 *>(tile + stage_offset<T, false, ROWS, true>(dealt_row<T>(c0, i), ks * 4 + g));
+    } else if (!TR) {
         v = *reinterpret_cast<const u32x4 *>(tile + stage_offset<T, false, ROWS>(c0 + i, ks * 4 + g));
     } else if (sizeof(T) == 4) {
         float e[4];
@@ -469,12 +474,12 @@ __device__ __forceinline__ u32x4 read_frag(const char *tile, int c0, int ks, int
 }
 
 // WP x WQ waves, each with BP / WP x BQ / WQ of the tile.  A step is 128 bytes of the contraction: staged from registers into LDS one or
-// two steps ahead, one barrier each.  65536 x 1024 x 1024 bf16 takes 205 us (670 TF): a workgroup fills its CU, so that its first loads and
-// its epilogue (16 MB of y through LDS for each round of tiles) are not hidden behind another one's products.
+// two steps ahead, one barrier each.  65536 x 1024 x 1024 bf16 takes 186 us (740 TF): a workgroup fills its CU, so that its first loads and
+// its epilogue (the whole chip's 34 MB of y at once) are not hidden behind another one's products; without it that takes 125 to 135 us.
 template <class T, int MODE, int BP, int BQ, int WP, int WQ, bool SPLIT, bool VEC, bool DEEP>
 __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
     constexpr int TH = WP * WQ * kWave;
-    constexpr bool PT = MODE == kWgrad, QT = MODE != kForward, FUSE = MODE != kForward;
+    constexpr bool PT = MODE == kWgrad, QT = MODE != kForward, FUSE = MODE != kForward, DEAL = MODE == kForward && sizeof(T) == 2;
     constexpr int CE = kChunk<T>, ST = kStage<T>;
     constexpr int CP = BP * 8 / TH, CQ = BQ * 8 / TH;       // chunks a thread stages per tile
     constexpr int NP = BP / WP / 16, NQ = BQ / WQ / 16;     // sixteen-wide fragments of a wave
@@ -557,7 +562,7 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
             int row, chunk;
             place(QT, BQ, k, row, chunk);
             const bool inside = QT ? c + row < c_end && q0 + chunk * CE < a.n_q : q0 + row < a.n_q && c + chunk * CE < a.n_c;
-            *reinterpret_cast<u32x4 *>(buf + kBuf - BQ * kRowBytes + stage_offset<T, QT, BQ>(row, chunk)) = only_inside<VEC>(t.q[k], inside);
+            *reinterpret_cast<u32x4 *>(buf + kBuf - BQ * kRowBytes + stage_offset<T, QT, BQ, DEAL>(row, chunk)) = only_inside<VEC>(t.q[k], inside);
         }
     };
     auto compute = [&](const char *buf, int64_t c) {
@@ -566,7 +571,7 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
             if (c + ks * (ST / 2) >= c_end) break;          // a half that holds only zeros
             u32x4 fp[NP], fq[NQ];
 #pragma unroll
-            for (int j = 0; j < NQ; ++j) fq[j] = read_frag<T, QT, BQ>(buf + kBuf - BQ * kRowBytes, wq * (BQ / WQ) + j * 16, ks, lane);
+            for (int j = 0; j < NQ; ++j) fq[j] = read_frag<T, QT, BQ, DEAL>(buf + kBuf - BQ * kRowBytes, wq * (BQ / WQ) + j * 16, ks, lane);
 #pragma unroll
             for (int half = 0; half < (SPLIT ? 2 : 1); ++half) {
 #pragma unroll
@@ -644,6 +649,37 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
                 for (int k = 0; k < n; ++k) v += sum[k * BP + tid];
                 part[a.n_p * a.n_q + p0 + tid] = v;
             }
+        }
+    } else if constexpr (DEAL) {
+        // straight from the registers, sixteen rows of each wave at a time (65536 x 1024 x 1024 bf16, back to back: 164 us, through LDS
+        // as below 175; 65536 x 512 x 512 48 and 55)
+        constexpr int N = NQ / 2;                           // chunks of a lane in a row
+        const T *bias = reinterpret_cast<const T *>(a.bias);
+        int col[N];
+        float add[N][CE];
+        u32x4 res[N] = {};
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+            col[c] = q0 + wq * (BQ / WQ) + c * 32 + g * CE;
+#pragma unroll
+            for (int e = 0; e < CE; ++e) add[c][e] = bias && col[c] + e < a.n_q ? to_f(bias[col[c] + e]) : 0.0f;
+        }
+#pragma unroll 1
+        for (int pi = 0; pi < NP; ++pi) {                   // (one body for all fragments: unrolled it would not fit the instruction cache)
+            const int64_t p = p0 + wp * (BP / WP) + pi * 16 + i;
+            float z[N][CE];
+            if (a.residual)
+#pragma unroll
+                for (int c = 0; c < N; ++c) res[c] = load_chunk<T, VEC>(reinterpret_cast<const T *>(a.residual), p, a.n_p, a.ld_residual, col[c], a.n_q);
+#pragma unroll
+            for (int t = 0; t < NP; ++t) {
+                if (t != pi) continue;
+#pragma unroll
+                for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z[j >> 1][(j & 1) * 4 + r] = acc[t][j][r] + add[j >> 1][(j & 1) * 4 + r];
+            }
+            if (p < a.n_p) epilogue<T, MODE, VEC, N>(a, p, col, a.n_q, z, res);
         }
     } else {
         // through LDS, so that a thread holds whole chunks of a row: sixteen rows of each wave at a time
@@ -896,7 +932,7 @@ int launch_tiles(DenseArgs a, int64_t splits, hipStream_t s) {
     if constexpr (BP < 256)                                 // (the largest tiles are for aligned rows)
         if (!a.vec) kernel = tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, false, false>;
     // two tiles ahead where one workgroup is all a CU holds and the contraction is long enough: weight gradient of 2^18 x 256 x 256 104 -> 90
-    // us, 65536 x 1024 x 1024 forward 226 -> 219 (dgrad has no registers left for it)
+    // us, 65536 x 1024 x 1024 forward 226 -> 219 then (dgrad has no registers left for it)
     if constexpr (BP * BQ >= 128 * 256 && sizeof(T) == 2 && MODE != kDgrad)
         if (a.vec && steps >= 8 * kStage<T>) kernel = tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, true, true>;
     if (int rc = allow_lds(kernel, bytes)) return rc;
