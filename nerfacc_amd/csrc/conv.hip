@@ -540,7 +540,7 @@ NFA_EXPORT int nfa_causal_conv_fwd(const nfa_causal_conv_args *a, void *outputs,
     if (a->channels % vec || !fits(d.x, d.ld_x, bytes, vec) || !fits(outputs, 0, bytes, vec) || !fits(d.init, 0, bytes, vec)) vec = 1;
     if (a->rows > 0) {
         const ConvPlan p = conv_plan(a->rows, a->channels, vec, false);
-        NFA_REQUIRE(p.blocks_x < (1ll << 31) && p.blocks_y < 65536, "causal_conv_fwd: too large for one launch");
+        NFA_REQUIRE(p.blocks_x < kMaxThreads / kBlock && p.blocks_y < 65536, "causal_conv_fwd: too large for one launch");
         d.piece = p.piece; d.lanes = p.lanes; d.pieces = p.pieces;
         with_conv(a->dtype, a->width, vec, [&](auto t, auto w, auto vc) {
             using T = decltype(t);
@@ -588,7 +588,7 @@ NFA_EXPORT int nfa_causal_conv_bwd(const nfa_causal_conv_args *a, void *grad_inp
         vec = 1;
     if (a->rows > 0 && (grad_inputs || grad_weight || grad_bias)) {
         const ConvPlan p = conv_plan(a->rows, a->channels, vec, true);
-        NFA_REQUIRE(p.blocks_x < (1ll << 31) && p.blocks_y < 65536, "causal_conv_bwd: too large for one launch");
+        NFA_REQUIRE(p.blocks_x < kMaxThreads / kBlock && p.blocks_y < 65536, "causal_conv_bwd: too large for one launch");
         d.piece = p.piece; d.lanes = p.lanes; d.pieces = p.pieces;
         d.partial = grad_weight || grad_bias ? (float *)workspace : nullptr;
         with_conv(a->dtype, a->width, vec, [&](auto t, auto w, auto vc) {

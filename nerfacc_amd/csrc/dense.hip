@@ -924,7 +924,7 @@ template <class T, int MODE, int BP, int BQ, int WP, int WQ, bool SPLIT>
 int launch_tiles(DenseArgs a, int64_t splits, hipStream_t s) {
     const int64_t tiles_p = ceil_div(a.n_p, BP);
     a.tiles_q = (int32_t)ceil_div(a.n_q, BQ);
-    NFA_REQUIRE(tiles_p * a.tiles_q < (1 << 30), "linear: too many rows for one launch");
+    NFA_REQUIRE(tiles_p * a.tiles_q * std::max<int64_t>(splits, 1) < kMaxThreads / (WP * WQ * kWave), "linear: too many rows for one launch");
     a.tiles = (int32_t)(tiles_p * a.tiles_q);
     const int64_t steps = MODE == kWgrad ? a.split : a.n_c;
     const size_t bytes = (size_t)(BP * (SPLIT ? 2 : 1) + BQ) * kRowBytes * (steps > kStage<T> ? 2 : 1);
@@ -972,7 +972,7 @@ int launch_resident(DenseArgs a, hipStream_t s) {
 template <class T>
 int launch_stream(DenseArgs a, hipStream_t s) {
     a.tiles_q = (int32_t)ceil_div(a.n_q, 32);
-    NFA_REQUIRE(ceil_div(a.n_p, 16) * a.tiles_q < (1ll << 31), "linear: too many rows for one launch");
+    NFA_REQUIRE(ceil_div(a.n_p, 16) * a.tiles_q < kMaxThreads / kBlock, "linear: too many rows for one launch");
     const auto kernel = a.vec ? stream_kernel<T, true> : stream_kernel<T, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(ceil_div(a.n_p, 16) * a.tiles_q)), dim3(kBlock), 0, s, a);
     return check_launch("stream_kernel");
@@ -1000,7 +1000,7 @@ int launch_rows(const DenseArgs &a, hipStream_t s) {
     // long contractions.  Few tiles: 4096 x 1024 x 256, 64 of them: fp32 49 us against 84 by tiles (whose steps are four times as long as
     // those of 16-bit types), bf16 25 against 20.  In fp32 any number of rows too, where the 32 columns of one workgroup are all there
     // are: 75956 x 751 x 4 61 us against 98, 75956 x 752 x 32 63 against 89; in bf16 41 against 26 and 36 against 25
-    if (MODE == kForward && ((sizeof(T) == 4 && a.n_q <= 32) ||
+    if (MODE == kForward && ((sizeof(T) == 4 && a.n_q <= 32 && a.n_p < (1ll << 27)) ||
                              ceil_div(a.n_p, 128) * ceil_div(a.n_q, 128) < (sizeof(T) == 4 ? kNumCU : kNumCU / 4))) return launch_stream<T>(a, s);
     // 16-bit types, aligned and large enough for every CU: 256 x 256 by eight waves, whose fragments are used often enough that the matrix
     // units and not LDS set the pace (16384 x 1024 x 1024 bf16 43.9 us against 51.8 by 128 x 128, 65536 x 512 x 512 56.5 against 62.7)

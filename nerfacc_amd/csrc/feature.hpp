@@ -8,6 +8,8 @@
 
 namespace nfa {
 
+constexpr int64_t kMaxThreads = 1ll << 32;   // of a launch, along one axis of its grid
+
 using bf16 = __bf16;
 using f16 = _Float16;
 

@@ -900,7 +900,7 @@ NFA_EXPORT int nfa_selective_scan_fwd(const nfa_selective_scan_args *a, void *ou
     if (a->packed_info && a->rows > 0) launch_zero_rows(d, a->dtype, outputs, nullptr, nullptr, s);
     if (p.tasks > 0) {
         const int64_t grid = p.tasks * p.blocks;
-        NFA_REQUIRE(grid < (1ll << 31) && a->n_rays * (int64_t)(p.chunk ? 1 : 0) < 65536, "selective_scan_fwd: too large for one launch");
+        NFA_REQUIRE(grid < kMaxThreads / kWave && a->n_rays * (int64_t)(p.chunk ? 1 : 0) < 65536, "selective_scan_fwd: too large for one launch");
         with_shape<kFwdStates>(a->dtype, p.sh, [&](auto t, auto ns, auto pp) {
             using T = decltype(t);
             if (p.chunk) {
@@ -929,7 +929,7 @@ NFA_EXPORT int nfa_selective_scan_bwd(const nfa_selective_scan_args *a, const fl
     d.kept = (float *)checkpoints;
     d.gu = g->inputs; d.gdt = g->delta; d.gz = a->gate ? g->gate : nullptr; d.ginit = g->initial_state;
     const int64_t grid = p.tasks * p.blocks, main_grid = p.workers * p.blocks;
-    NFA_REQUIRE(grid < (1ll << 31) && a->n_rays * (int64_t)(p.chunk ? 1 : 0) < 65536, "selective_scan_bwd: too large for one launch");
+    NFA_REQUIRE(grid < kMaxThreads / kWave && a->n_rays * (int64_t)(p.chunk ? 1 : 0) < 65536, "selective_scan_bwd: too large for one launch");
     if (a->packed_info) launch_zero_rows(d, a->dtype, d.gu, d.gdt, d.gz, s);
     with_shape<kBwdStates>(a->dtype, p.sh, [&](auto t, auto ns, auto pp) {
         using T = decltype(t);
