@@ -909,6 +909,22 @@ __global__ __launch_bounds__(1024) void reduce_rows_kernel(float *part, int64_t 
     }
 }
 
+// the same for few rows of many columns: a thread a column, its rows in order
+template <class T>
+__global__ __launch_bounds__(kBlock) void reduce_few_rows_kernel(const float *__restrict__ part, int64_t rows, int64_t ld, Outputs o) {
+    const int64_t c = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (c >= ld) return;
+    float v = 0.0f;
+#pragma unroll 8
+    for (int64_t r = 0; r < rows; ++r) v += part[r * ld + c];
+    int64_t at = c;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        if (at >= 0 && at < o.cols[k] && o.to[k]) reinterpret_cast<T *>(o.to[k])[at] = from_f<T>(v);
+        at -= o.cols[k];
+    }
+}
+
 bool aligned(const void *p, int64_t ld, int64_t cols, int64_t bytes, int64_t to) {
     return (uintptr_t)p % to == 0 && ld * bytes % to == 0 && cols * bytes % to == 0;
 }
@@ -993,10 +1009,9 @@ int launch_rows(const DenseArgs &a, hipStream_t s) {
     if (a.n_c <= 4 * step) return launch_resident<T, MODE, 4, SPLIT>(a, s);
     if (a.n_c <= 8 * step) return launch_resident<T, MODE, 8, SPLIT>(a, s);
     // (dgrad in fp32 reads a number of a column at a time from LDS, here for every sixteen rows, by tiles for 64: 2^18 x 256 x 256 608 us
-    // against 439 by tiles, 2^18 x 64 x 256 220 against 144, 4096 x 256 x 256 35 against 28; 300 x 256 x 256, six tiles, 14 against 27)
-    if constexpr (sizeof(T) == 4)
-        if (a.n_c <= 16 * step && (MODE == kForward || ceil_div(a.n_p, 128) * ceil_div(a.n_q, 128) < kNumCU / 4))
-            return launch_resident<T, MODE, 16, SPLIT>(a, s);
+    // against 439 by tiles, 2^18 x 64 x 256 220 against 144, 4096 x 256 x 256 35 against 12)
+    if constexpr (sizeof(T) == 4 && MODE == kForward)
+        if (a.n_c <= 16 * step) return launch_resident<T, MODE, 16, SPLIT>(a, s);
     // long contractions.  Few tiles: 4096 x 1024 x 256, 64 of them: fp32 49 us against 84 by tiles (whose steps are four times as long as
     // those of 16-bit types), bf16 25 against 20.  In fp32 any number of rows too, where the 32 columns of one workgroup are all there
     // are: 75956 x 751 x 4 61 us against 98, 75956 x 752 x 32 63 against 89; in bf16 41 against 26 and 36 against 25
@@ -1007,6 +1022,10 @@ int launch_rows(const DenseArgs &a, hipStream_t s) {
     constexpr int BP = SPLIT ? 64 : 128;
     if constexpr (sizeof(T) == 2 && !SPLIT)
         if (a.vec && a.n_q > 128 && ceil_div(a.n_p, 256) * ceil_div(a.n_q, 256) >= kNumCU) return launch_tiles<T, MODE, 256, 256, 2, 4, SPLIT>(a, 1, s);
+    // dgrad of few rows: smaller tiles, so that more CUs get one (2000 x 512 x 512 fp32 22 us against 50 by 128 x 128, bf16 8.8 against 15;
+    // 588 x 908 x 804 34 against 79, 18 against 35)
+    if constexpr (MODE == kDgrad && !SPLIT)
+        if (ceil_div(a.n_p, BP) * ceil_div(a.n_q, 128) < kNumCU) return launch_tiles<T, MODE, 64, 64, 2, 2, SPLIT>(a, 1, s);
     // (64 columns where there are no more: 65536 x 512 x 64 fp32 45 us against 79)
     return a.n_q <= 64 ? launch_tiles<T, MODE, BP, 64, 2, 2, SPLIT>(a, 1, s) : launch_tiles<T, MODE, BP, 128, 2, 2, SPLIT>(a, 1, s);
 }
@@ -1064,6 +1083,13 @@ void launch_reduce_rows(float *part, int64_t rows, std::initializer_list<std::pa
         cols += p.second;
     }
     const unsigned blocks = (unsigned)ceil_div(cols, 64);
+    // few rows of many columns, a thread each: 8 rows of 2^20 columns 8 us against 37 in sixteen groups, 64 rows of 2^17 2.6 less of 52
+    if (rows <= 64 && cols >= 64 * kNumCU) {
+        with_dtype(dtype, [&](auto t) {
+            hipLaunchKernelGGL((reduce_few_rows_kernel<decltype(t)>), dim3((unsigned)ceil_div(cols, kBlock)), dim3(kBlock), 0, s, part, rows, cols, o);
+        });
+        return;
+    }
     // one launch while it fills the chip or its rows are few: 4096 rows of 1152 columns take 19 us in one, 10 in two
     int64_t step = 1;
     if (rows >= 1024 && blocks < 2 * kNumCU) {
