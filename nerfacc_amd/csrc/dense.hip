@@ -1083,7 +1083,8 @@ void launch_reduce_rows(float *part, int64_t rows, std::initializer_list<std::pa
         cols += p.second;
     }
     const unsigned blocks = (unsigned)ceil_div(cols, 64);
-    // few rows of many columns, a thread each: 8 rows of 2^20 columns 8 us against 37 in sixteen groups, 64 rows of 2^17 2.6 less of 52
+    // few rows of many columns, a thread a column: the weight gradient of 4096 x 1024 x 1024 bf16, 8 rows of 2^20 columns, takes 34 us
+    // against 63 with sixteen groups a column, that of 65536 x 256 x 512, 64 rows of 2^17, 49 against 52
     if (rows <= 64 && cols >= 64 * kNumCU) {
         with_dtype(dtype, [&](auto t) {
             hipLaunchKernelGGL((reduce_few_rows_kernel<decltype(t)>), dim3((unsigned)ceil_div(cols, kBlock)), dim3(kBlock), 0, s, part, rows, cols, o);
