@@ -186,7 +186,7 @@ __global__ __launch_bounds__(kBlock, 3) void conv_bwd_kernel(ConvArgs a) {
                         count = n < a.rows - start ? n : a.rows - start;
                     }
                     const int64_t rest = count - 1 - q.pos;
-                    if (rest < W - 1) {
+                    if (rest >= 0 && rest < W - 1) {                          // (rays that overlap leave rows behind their ray's end)
                         float f[VC];
                         load_row<T, VC>(a.gfinal, ((int64_t)q.ray * (W - 1) + (W - 2 - rest)) * a.channels + c, f);
 #pragma unroll
