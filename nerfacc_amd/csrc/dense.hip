@@ -103,6 +103,7 @@ __device__ __forceinline__ u32x4 load_saved(const DenseArgs &a, int64_t row, int
 }
 
 template <class T> struct Frag { T v[kChunk<T>]; };
+template <class T> constexpr float kLargest = std::is_same_v<T, f16> ? 65504.0f : 0x1.fep127f;
 
 // dz = dy act'(.) of N chunks, rounded to T.  SPLIT (16-bit types, smooth activations): what the rounding lost goes into `rest`, and
 // the product is taken of both parts, so that a gradient carries the rounding of its own result and of the saved number only.  relu's
@@ -121,8 +122,8 @@ __device__ __forceinline__ void form_dz(const DenseArgs &a, u32x4 (&g)[N], const
                 if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((s[k][0] >> i) & 1u) != 0 : to_f(w.v[i]) > 0.0f) ? dz : 0.0f;
                 else if constexpr (ACT != NFA_ACT_NONE) dz *= act_slope<ACT>(to_f(w.v[i]));
                 each(k, dz, i);
-                float near = dz;                            // (fp16: the largest number in place of an overflow, the rest in the second part)
-                if constexpr (SPLIT && std::is_same_v<T, f16>) near = fabsf(dz) > 65504.0f ? copysignf(65504.0f, dz) : dz;
+                float near = dz;
+                if constexpr (SPLIT) near = fabsf(dz) > kLargest<T> ? copysignf(kLargest<T>, dz) : dz;
                 if constexpr (ACT != NFA_ACT_NONE) v.v[i] = from_f<T>(near);
                 if constexpr (SPLIT) lo.v[i] = from_f<T>(dz - to_f(v.v[i]));
             }

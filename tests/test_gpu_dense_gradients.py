@@ -1,0 +1,57 @@
+"""Gradients of `nerfacc_amd.linear` in 16-bit types where act' is small, where dz = dy act' leaves the type's range and where sums cancel.
+
+What the backward pass may lose, with u = eps / 2 of the type:
+  * every result is rounded once: u |result|, and half a smallest step of fp16;
+  * act' is formed in 32 bits from z in 32 bits.  fp32 and fp16 keep 32 bits (fp32: z or the value, which lose as little); bf16 keeps act'
+    rounded once, or differentiates from its own output: u |dz| a term;
+  * None and relu multiply dy itself; the others take dz in two parts of bf16, the rest below 2^-17 |dz|, and inputs and weights of fp16 in
+    two parts whose second product with the second part of dz, 2^-18 of the term, is left out: 2^-16 |term| with room for both;
+  * sums of n terms in 32 bits: n 2^-24 sum |terms| (256 terms a lane and one more rounding per partial sum on the rows' axis).
+The error of act' in 32 bits is at most 16 (1 + |z| + z^2) 2^-24 of the sizes of its parts (an exponential of z log2 e, or of z^2 / 2, behind it), plus
+|act''| times the error of z, (k + 4) 2^-24 sum |terms| of z."""
+import math
+
+import pytest
+import torch
+
+from gpu_utils import DEV
+
+pytestmark = pytest.mark.gpu
+
+SMOOTH = ["sigmoid", "softplus", "silu", "gelu", "exp"]
+HALF = [torch.bfloat16, torch.float16]
+
+
+def parts(act, z):
+    """act'(z) in 64 bits, the sum of its parts' sizes, |act''(z)|"""
+    s, t = torch.sigmoid(z), torch.sigmoid(-z)
+    if act is None or act == "relu":
+        one = torch.ones_like(z) if act is None else (z > 0).to(z.dtype)
+        return one, one, torch.zeros_like(z)
+    if act == "exp":
+        return z.exp(), z.exp(), z.exp()
+    if act == "sigmoid":
+        return s * t, s * t, (s * t * (t - s)).abs()
+    if act == "softplus":
+        return s, s, s * t
+    if act == "silu":
+        return s * (1 + z * t), s * (1 + z.abs() * t), (s * t * (2 + z * (t - s))).abs()
+    phi, cdf = torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi), 0.5 * torch.special.erfc(-z / math.sqrt(2))
+    return cdf + z * phi, cdf + z.abs() * phi, phi * (2 - z * z).abs()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("act", SMOOTH)
+@pytest.mark.parametrize("n", [40, 300])
+def test_infinite_gradients_stay_infinite(dtype, act, n):
+    import nerfacc_amd as nerfacc
+
+    x, w, b = torch.full((5, 8), 0.25, device=DEV, dtype=dtype), torch.full((n, 8), 0.5, device=DEV, dtype=dtype), torch.zeros(n, device=DEV, dtype=dtype)
+    own = [t.requires_grad_(True) for t in (x, w, b)]
+    gy = torch.ones(5, n, device=DEV, dtype=dtype)
+    gy[1, 3], gy[2, 3], gy[4] = float("inf"), float("inf"), float("nan")
+    gx, gw, gb = torch.autograd.grad(nerfacc.linear(*own, activation=act), own, gy)
+    assert gx[1:3].isposinf().all() and gx[0].isfinite().all() and gx[3].isfinite().all() and gx[4].isnan().all()
+    gy[4] = 1.0
+    gx, gw, gb = torch.autograd.grad(nerfacc.linear(*own, activation=act), own, gy)
+    assert gw[3].isposinf().all() and gb[3].isposinf() and gw[:3].isfinite().all() and gw[4:].isfinite().all()
