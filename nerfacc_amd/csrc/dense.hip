@@ -89,64 +89,70 @@ __device__ __forceinline__ u32x4 only_inside(u32x4 v, bool inside) {
     }
     return v;
 }
-// what dz is formed from beside dy: a chunk of saved numbers, or a byte of relu's bits
-template <class T, bool VEC>
-__device__ __forceinline__ u32x4 load_saved(const DenseArgs &a, int64_t row, int64_t rows, int64_t col, int64_t cols) {
-    u32x4 v = {0, 0, 0, 0};
-    if (a.mask) {
+// of what is kept for one chunk of a smooth activation: 16-byte chunks (fp16: eight slopes in 32 bits)
+template <class T> constexpr int kKept = std::is_same_v<T, f16> ? 2 : 1;
+template <class T, bool SPLIT> constexpr int kSaved = SPLIT ? kKept<T> : 1;
+// what dz is formed from beside dy: kept numbers, or a byte of relu's bits
+template <class T, bool SPLIT, bool VEC>
+__device__ __forceinline__ void load_saved(const DenseArgs &a, int64_t row, int64_t rows, int64_t col, int64_t cols, u32x4 *v) {
+    v[0] = u32x4{0, 0, 0, 0};
+    if constexpr (kSaved<T, SPLIT> == 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v[i] = load_chunk<float, VEC>(reinterpret_cast<const float *>(a.saved), row, rows, a.ld_saved, col + 4 * i, cols);
+    } else if (a.mask) {
         const bool inside = row < rows && col < cols;
-        v[0] = reinterpret_cast<const uint8_t *>(a.saved)[inside ? row * a.ld_saved + col / kChunk<T> : 0];
+        v[0][0] = reinterpret_cast<const uint8_t *>(a.saved)[inside ? row * a.ld_saved + col / kChunk<T> : 0];
     } else if (a.act != NFA_ACT_NONE) {
-        v = load_chunk<T, VEC>(reinterpret_cast<const T *>(a.saved), row, rows, a.ld_saved, col, cols);
+        v[0] = load_chunk<T, VEC>(reinterpret_cast<const T *>(a.saved), row, rows, a.ld_saved, col, cols);
     }
-    return v;
 }
 
 template <class T> struct Frag { T v[kChunk<T>]; };
 template <class T> constexpr float kLargest = std::is_same_v<T, f16> ? 65504.0f : 0x1.fep127f;
 
 // dz = dy act'(.) of N chunks, rounded to T.  SPLIT (16-bit types, smooth activations): what the rounding lost goes into `rest`, and
-// the product is taken of both parts, so that a gradient carries the rounding of its own result and of the saved number only.  relu's
-// dz is dy or 0: nothing is lost there.  each(chunk, dz of one number in 32 bits, place in the chunk)
+// the product is taken of both parts, so that a gradient carries the rounding of its own result and, in bf16, of act' only.  relu's
+// dz is dy or 0: nothing is lost there.  What T rounds to infinity becomes T's largest number and a rest, which is infinite where dz is
+// (infinity minus infinity would be NaN).  each(chunk, dz of one number in 32 bits, place in the chunk)
 template <class T, bool SPLIT, int N, class F>
-__device__ __forceinline__ void form_dz(const DenseArgs &a, u32x4 (&g)[N], const u32x4 (&s)[N], u32x4 (&rest)[SPLIT ? N : 1], F &&each) {
+__device__ __forceinline__ void form_dz(const DenseArgs &a, u32x4 (&g)[N], const u32x4 (&s)[N * kSaved<T, SPLIT>], u32x4 (&rest)[SPLIT ? N : 1], F &&each) {
     auto with = [&](auto act) {
         constexpr int ACT = decltype(act)::value;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             Frag<T> v = __builtin_bit_cast(Frag<T>, g[k]), lo;
-            const Frag<T> w = __builtin_bit_cast(Frag<T>, s[k]);
+            float w[kChunk<T>];
+#pragma unroll
+            for (int i = 0; i < kChunk<T>; ++i) {
+                if constexpr (kSaved<T, SPLIT> == 2) w[i] = __builtin_bit_cast(Frag<float>, s[2 * k + i / 4]).v[i % 4];
+                else w[i] = to_f(__builtin_bit_cast(Frag<T>, s[k]).v[i]);
+            }
 #pragma unroll
             for (int i = 0; i < kChunk<T>; ++i) {
                 float dz = to_f(v.v[i]);
-                if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((s[k][0] >> i) & 1u) != 0 : to_f(w.v[i]) > 0.0f) ? dz : 0.0f;
-                else if constexpr (ACT != NFA_ACT_NONE) dz *= act_slope<ACT>(to_f(w.v[i]));
+                if constexpr (SPLIT) dz *= ACT == NFA_ACT_SOFTPLUS ? -expm1f(-w[i]) : w[i];          // (ACT: bf16's softplus keeps its value)
+                else if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((s[k][0] >> i) & 1u) != 0 : w[i] > 0.0f) ? dz : 0.0f;
+                else if constexpr (ACT != NFA_ACT_NONE) dz *= act_slope_of_kept<ACT>(w[i]);
                 each(k, dz, i);
                 float near = dz;
                 if constexpr (SPLIT) near = fabsf(dz) > kLargest<T> ? copysignf(kLargest<T>, dz) : dz;
-                if constexpr (ACT != NFA_ACT_NONE) v.v[i] = from_f<T>(near);
+                if constexpr (SPLIT || ACT != NFA_ACT_NONE) v.v[i] = from_f<T>(near);
                 if constexpr (SPLIT) lo.v[i] = from_f<T>(dz - to_f(v.v[i]));
             }
-            if constexpr (ACT != NFA_ACT_NONE) g[k] = __builtin_bit_cast(u32x4, v);
+            if constexpr (SPLIT || ACT != NFA_ACT_NONE) g[k] = __builtin_bit_cast(u32x4, v);
             if constexpr (SPLIT) rest[k] = __builtin_bit_cast(u32x4, lo);
         }
     };
     if constexpr (sizeof(T) == 4) {
         with_act(a.act, with);
     } else if constexpr (SPLIT) {
-        switch (a.act) {
-            case NFA_ACT_SIGMOID: with(std::integral_constant<int, NFA_ACT_SIGMOID>{}); break;
-            case NFA_ACT_SOFTPLUS: with(std::integral_constant<int, NFA_ACT_SOFTPLUS>{}); break;
-            case NFA_ACT_SILU: with(std::integral_constant<int, NFA_ACT_SILU>{}); break;
-            case NFA_ACT_GELU: with(std::integral_constant<int, NFA_ACT_GELU>{}); break;
-            default: with(std::integral_constant<int, NFA_ACT_EXP>{}); break;
-        }
+        if (std::is_same_v<T, bf16> && a.act == NFA_ACT_SOFTPLUS) with(std::integral_constant<int, NFA_ACT_SOFTPLUS>{});
+        else with(std::integral_constant<int, NFA_ACT_NONE>{});
     } else {
         if (a.act == NFA_ACT_RELU) with(std::integral_constant<int, NFA_ACT_RELU>{});
         else with(std::integral_constant<int, NFA_ACT_NONE>{});
     }
 }
-template <class T> bool splits(int32_t act) { return sizeof(T) == 2 && act != NFA_ACT_NONE && act != NFA_ACT_RELU; }
 
 // acc[q][p] += Q P over the lane's chunk.  32-bit numbers go in four steps: the contraction may run in any order as long as both
 // sides agree, so lane group g feeds chunk g and each step takes one number of it.
@@ -170,25 +176,39 @@ __device__ __forceinline__ s16x4 read_transposed(const char *at) {
 
 // y = act(z) (+ residual) of N chunks in place; `kept`: what the backward pass wants of them (bits: in the first word of a chunk)
 template <class T, int N>
-__device__ __forceinline__ void finish_chunks(const DenseArgs &a, float (&z)[N][kChunk<T>], const u32x4 (&res)[N], u32x4 (&y)[N], u32x4 (&kept)[N]) {
+__device__ __forceinline__ void finish_chunks(const DenseArgs &a, float (&z)[N][kChunk<T>], const u32x4 (&res)[N], u32x4 (&y)[N],
+                                              u32x4 (&kept)[N * kKept<T>]) {
     with_act(a.act, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
-        constexpr bool VALUE = ACT == NFA_ACT_RELU || ACT == NFA_ACT_EXP || ACT == NFA_ACT_SOFTPLUS;
+        constexpr bool SMOOTH = ACT != NFA_ACT_NONE && ACT != NFA_ACT_RELU;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             Frag<T> out, keep;
+            Frag<float> slope[2];
             const Frag<T> add = __builtin_bit_cast(Frag<T>, res[k]);
             uint32_t bits = 0;
 #pragma unroll
             for (int i = 0; i < kChunk<T>; ++i) {
                 const float v = act_fwd<ACT>(z[k][i]);
-                if constexpr (ACT == NFA_ACT_RELU) bits |= (v > 0.0f ? 1u : 0u) << i;
-                keep.v[i] = from_f<T>(VALUE ? v : z[k][i]);
                 out.v[i] = from_f<T>(a.residual ? v + to_f(add.v[i]) : v);
+                if constexpr (ACT == NFA_ACT_RELU) bits |= (v > 0.0f ? 1u : 0u) << i;
+                z[k][i] = ACT == NFA_ACT_RELU || ACT == NFA_ACT_EXP || (ACT == NFA_ACT_SOFTPLUS && kKept<T> == 1) ? v : z[k][i];
             }
             y[k] = __builtin_bit_cast(u32x4, out);
-            kept[k] = __builtin_bit_cast(u32x4, keep);
-            if (a.mask) kept[k][0] = bits;
+            if (!a.saved_out) continue;
+#pragma unroll
+            for (int i = 0; i < kChunk<T>; ++i) {           // (exp: z is its value by now)
+                if constexpr (SMOOTH && kKept<T> == 2) slope[i / 4].v[i % 4] = ACT == NFA_ACT_EXP ? z[k][i] : act_slope<ACT>(z[k][i]);
+                else if constexpr (SMOOTH && sizeof(T) == 2) keep.v[i] = from_f<T>(act_from_value(ACT) ? z[k][i] : act_slope<ACT>(z[k][i]));
+                else keep.v[i] = from_f<T>(z[k][i]);
+            }
+            if constexpr (SMOOTH && kKept<T> == 2) {
+                kept[2 * k] = __builtin_bit_cast(u32x4, slope[0]);
+                kept[2 * k + 1] = __builtin_bit_cast(u32x4, slope[1]);
+            } else {
+                kept[kKept<T> * k] = __builtin_bit_cast(u32x4, keep);
+                if (a.mask) kept[kKept<T> * k][0] = bits;
+            }
         }
     });
 }
@@ -209,7 +229,7 @@ __device__ __forceinline__ void store_chunk(T *row, int q, int n_q, u32x4 v) {
 // the epilogue of N chunks of row p (columns q[k] ..): acc in, outputs and the saved numbers out
 template <class T, int MODE, bool VEC, int N>
 __device__ __forceinline__ void epilogue(const DenseArgs &a, int64_t p, const int (&q)[N], int n_q, float (&z)[N][kChunk<T>], const u32x4 (&res)[N]) {
-    u32x4 y[N], kept[N];
+    u32x4 y[N], kept[N * kKept<T>];
     T *out = reinterpret_cast<T *>(a.out) + p * a.n_q;
     if constexpr (MODE == kForward) {
         finish_chunks<T, N>(a, z, res, y, kept);
@@ -218,9 +238,13 @@ __device__ __forceinline__ void epilogue(const DenseArgs &a, int64_t p, const in
             store_chunk<T, VEC>(out, q[k], n_q, y[k]);
             if (!a.saved_out) continue;
             if (a.mask) {
-                if (q[k] < n_q) reinterpret_cast<uint8_t *>(a.saved_out)[p * a.ld_saved + q[k] / kChunk<T>] = (uint8_t)kept[k][0];
+                if (q[k] < n_q) reinterpret_cast<uint8_t *>(a.saved_out)[p * a.ld_saved + q[k] / kChunk<T>] = (uint8_t)kept[kKept<T> * k][0];
+            } else if (kKept<T> == 2 && a.act != NFA_ACT_RELU) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    store_chunk<float, VEC>(reinterpret_cast<float *>(a.saved_out) + p * a.n_q, q[k] + 4 * i, n_q, kept[kKept<T> * k + (kKept<T> - 1) * i]);
             } else {
-                store_chunk<T, VEC>(reinterpret_cast<T *>(a.saved_out) + p * a.n_q, q[k], n_q, kept[k]);
+                store_chunk<T, VEC>(reinterpret_cast<T *>(a.saved_out) + p * a.n_q, q[k], n_q, kept[kKept<T> * k]);
             }
         }
     } else {
@@ -315,8 +339,9 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
         }
         if constexpr (MODE == kDgrad) {
             if (a.act != NFA_ACT_NONE) {
-                u32x4 s[RT * KS];
-                if (KS >= 4 && a.mask && whole && a.ld_saved % 16 == 0 && (uintptr_t)a.saved % 16 == 0) {
+                constexpr int NS = kSaved<T, SPLIT>;
+                u32x4 s[RT * KS * NS];
+                if (!SPLIT && KS >= 4 && a.mask && whole && a.ld_saved % 16 == 0 && (uintptr_t)a.saved % 16 == 0) {
                     // relu's bits, four steps of the contraction in one access: word k of a row, byte g
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
@@ -334,8 +359,11 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
-                    for (int k = 0; k < KS; ++k)
-                        s[r * KS + k] = only_inside<VEC>(load_saved<T, VEC>(a, p0 + r * 16 + i, a.n_p, (k * 4 + g) * CE, a.n_c), (k * 4 + g) * CE < a.n_c);
+                    for (int k = 0; k < KS; ++k) {
+                        load_saved<T, SPLIT, VEC>(a, p0 + r * 16 + i, a.n_p, (k * 4 + g) * CE, a.n_c, &s[(r * KS + k) * NS]);
+#pragma unroll
+                        for (int h = 0; h < NS; ++h) s[(r * KS + k) * NS + h] = only_inside<VEC>(s[(r * KS + k) * NS + h], (k * 4 + g) * CE < a.n_c);
+                    }
                 form_dz<T, SPLIT, RT * KS>(a, x, s, lo, [](int, float, int) {});
             }
         }
@@ -502,7 +530,8 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
     const int64_t c_end = MODE == kWgrad ? (c_begin + a.split < a.n_c ? c_begin + a.split : a.n_c) : a.n_c;
 
     const T *P = reinterpret_cast<const T *>(a.p), *Q = reinterpret_cast<const T *>(a.q);
-    struct Staged { u32x4 p[CP], s[FUSE ? CP : 1], q[CQ]; };
+    constexpr int NS = kSaved<T, SPLIT>;
+    struct Staged { u32x4 p[CP], s[FUSE ? CP * NS : 1], q[CQ]; };
     f32x4 acc[NP][NQ];
 #pragma unroll
     for (int i = 0; i < NP; ++i)
@@ -526,7 +555,7 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
             const int64_t r = PT ? c + row : p0 + row, col = PT ? p0 + chunk * CE : c + chunk * CE;
             const int64_t rows = PT ? c_end : a.n_p, cols = PT ? a.n_p : a.n_c;
             t.p[k] = load_chunk<T, VEC>(P, r, rows, a.ld_p, col, cols);
-            if constexpr (FUSE) t.s[k] = load_saved<T, VEC>(a, r, rows, col, cols);
+            if constexpr (FUSE) load_saved<T, SPLIT, VEC>(a, r, rows, col, cols, &t.s[k * NS]);
         }
 #pragma unroll
         for (int k = 0; k < CQ; ++k) {
@@ -545,7 +574,9 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
             place(PT, BP, k, row, chunk);
             const bool inside = PT ? c + row < c_end && p0 + chunk * CE < a.n_p : p0 + row < a.n_p && c + chunk * CE < a.n_c;
             t.p[k] = only_inside<VEC>(t.p[k], inside);
-            if constexpr (FUSE) t.s[k] = only_inside<VEC>(t.s[k], inside);
+            if constexpr (FUSE)
+#pragma unroll
+                for (int h = 0; h < NS; ++h) t.s[k * NS + h] = only_inside<VEC>(t.s[k * NS + h], inside);
         }
         if constexpr (FUSE)
             form_dz<T, SPLIT, CP>(a, t.p, t.s, lo, [&](int, float dz, int e) {
@@ -818,7 +849,7 @@ __global__ __launch_bounds__(kBlock, 2) void narrow_wgrad_kernel(DenseArgs a) {
                 for (int f = 0; f < NP; ++f) {
                     float &dz = r.p[k].v[f];
                     if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((r.bits[k] >> ((p & 3) + f)) & 1u) != 0 : r.s[k].v[f] > 0.0f) ? dz : 0.0f;
-                    else if constexpr (ACT != NFA_ACT_NONE) dz *= act_slope<ACT>(r.s[k].v[f]);
+                    else if constexpr (ACT != NFA_ACT_NONE) dz *= act_slope_of_kept<ACT>(r.s[k].v[f]);
                 }
         });
 #pragma unroll
@@ -1072,6 +1103,7 @@ bool keeps_bits(int64_t out_features, int32_t dtype, int32_t act) {
     return act == NFA_ACT_RELU && out_features % (16 / dtype_bytes(dtype)) == 0;
 }
 bool two_parts(int32_t dtype, int32_t act) { return dtype != NFA_DTYPE_F32 && act != NFA_ACT_NONE && act != NFA_ACT_RELU; }
+bool keeps_slopes(int32_t dtype, int32_t act) { return dtype == NFA_DTYPE_F16 && two_parts(dtype, act); }     // in 32 bits
 
 }  // namespace
 
@@ -1122,6 +1154,7 @@ static int check_linear(const nfa_linear_args *a, const char *who) {
 
 NFA_EXPORT int64_t nfa_linear_saved_bytes(int64_t rows, int32_t out_features, int32_t dtype, int32_t activation, int32_t has_residual) {
     if (keeps_bits(out_features, dtype, activation)) return rows * (out_features / (16 / dtype_bytes(dtype)));
+    if (keeps_slopes(dtype, activation)) return rows * out_features * 4;
     if (activation == NFA_ACT_NONE || (act_from_value(activation) && !has_residual)) return 0;
     return rows * out_features * dtype_bytes(dtype);
 }
@@ -1142,7 +1175,7 @@ NFA_EXPORT int nfa_linear_fwd(const nfa_linear_args *a, void *outputs, void *sav
     d.mask = keeps_bits(a->out_features, a->dtype, a->activation);
     d.ld_saved = d.mask ? a->out_features / (16 / bytes) : a->out_features;
     d.vec = aligned(d.p, d.ld_p, a->in_features, bytes, 16) && aligned(d.q, d.ld_q, a->in_features, bytes, 16) &&
-            aligned(outputs, d.n_q, d.n_q, bytes, 16) && (!saved || d.mask || aligned(saved, d.n_q, d.n_q, bytes, 16)) &&
+            aligned(outputs, d.n_q, d.n_q, bytes, 16) && (!saved || d.mask || aligned(saved, d.n_q, d.n_q, keeps_slopes(a->dtype, a->activation) ? 4 : bytes, 16)) &&
                 (!a->residual || aligned(a->residual, a->residual_stride, d.n_q, bytes, 16));
     int rc = NFA_OK;
     with_dtype(a->dtype, [&](auto t) { rc = launch_rows<decltype(t), kForward, false>(d, (hipStream_t)stream); });
@@ -1173,7 +1206,7 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
     d.mask = keeps_bits(n, a->dtype, a->activation);
     d.ld_saved = d.mask ? n / (16 / bytes) : n;
     const bool vec = aligned(a->grad_outputs, a->grad_outputs_stride, n, bytes, 16) &&
-              (!saved || a->activation == NFA_ACT_NONE || d.mask || aligned(saved, n, n, bytes, 16));
+              (!saved || a->activation == NFA_ACT_NONE || d.mask || aligned(saved, n, n, keeps_slopes(a->dtype, a->activation) ? 4 : bytes, 16));
     int rc = NFA_OK;
     if (grad_inputs) {
         DenseArgs e = d;

@@ -60,10 +60,12 @@ __device__ __forceinline__ float softplus_f(float x) { return softplus_from(x, f
 
 constexpr float kInvSqrt2 = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f;
 
-// What a layer keeps for its backward pass (include/nerfacc_hip.h: nfa_linear_saved_bytes): of relu one bit; exp and softplus are
-// differentiated from their own value a = act(z), which loses little by its rounding (e^z itself; 1 - e^-a with the relative error of
-// a); the others from z, whose relative rounding error is the derivative's.
-inline bool act_from_value(int32_t act) { return act == NFA_ACT_RELU || act == NFA_ACT_EXP || act == NFA_ACT_SOFTPLUS; }
+// What a layer keeps for its backward pass (include/nerfacc_hip.h: nfa_linear_saved_bytes).  relu: one bit, or its value.  The others, by type:
+//   fp32  the number that act' comes from in full: a = act(z) for exp and softplus (a itself; 1 - e^-a, as accurate as a), else z;
+//   bf16  act' rounded once, so that its relative error is bf16's at any z (z kept in bf16 would lose |z| times that where act' decays:
+//         6 % of sigmoid' at z = -16); a for exp and softplus, which round alike;
+//   fp16  act' in 32 bits: below z = -10 sigmoid', softplus' and exp' are under 2^-14, where fp16 has fewer and fewer bits.
+constexpr bool act_from_value(int32_t act) { return act == NFA_ACT_RELU || act == NFA_ACT_EXP || act == NFA_ACT_SOFTPLUS; }
 
 template <int ACT>
 __device__ __forceinline__ float act_fwd(float z) {
@@ -75,16 +77,21 @@ __device__ __forceinline__ float act_fwd(float z) {
     else if constexpr (ACT == NFA_ACT_EXP) return expf(z);
     else return z;
 }
-// the derivative, from the saved number (act_from_value)
+// the derivative of a smooth activation, from z
 template <int ACT>
-__device__ __forceinline__ float act_slope(float s) {
-    if constexpr (ACT == NFA_ACT_RELU) return s > 0.0f ? 1.0f : (s != s ? s : 0.0f);
-    else if constexpr (ACT == NFA_ACT_SIGMOID) return sigmoid_f(s) * sigmoid_f(-s);
-    else if constexpr (ACT == NFA_ACT_SOFTPLUS) return -expm1f(-s);
-    else if constexpr (ACT == NFA_ACT_SILU) return sigmoid_f(s) * fmaf(s, sigmoid_f(-s), 1.0f);
-    else if constexpr (ACT == NFA_ACT_GELU) return fmaf(s * kInvSqrt2Pi, expf(-0.5f * s * s), 0.5f * erfcf(-s * kInvSqrt2));
+__device__ __forceinline__ float act_slope(float z) {
+    if constexpr (ACT == NFA_ACT_SIGMOID) return sigmoid_f(z) * sigmoid_f(-z);
+    else if constexpr (ACT == NFA_ACT_SOFTPLUS) return sigmoid_f(z);
+    else if constexpr (ACT == NFA_ACT_SILU) return sigmoid_f(z) * fmaf(z, sigmoid_f(-z), 1.0f);
+    else if constexpr (ACT == NFA_ACT_GELU) return fmaf(z * kInvSqrt2Pi, expf(-0.5f * z * z), 0.5f * erfcf(-z * kInvSqrt2));
+    else return expf(z);
+}
+// the same from what fp32 keeps: the value of exp and softplus, z of the others
+template <int ACT>
+__device__ __forceinline__ float act_slope_of_kept(float s) {
+    if constexpr (ACT == NFA_ACT_SOFTPLUS) return -expm1f(-s);
     else if constexpr (ACT == NFA_ACT_EXP) return s;
-    else return 1.0f;
+    else return act_slope<ACT>(s);
 }
 // calls f(integral ACT): the choice is made once around a loop, not once per number (a switch inside an unrolled loop is many times
 // the instruction cache)

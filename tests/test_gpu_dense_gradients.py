@@ -40,6 +40,54 @@ def parts(act, z):
     return cdf + z * phi, cdf + z.abs() * phi, phi * (2 - z * z).abs()
 
 
+def check(x, w, b, gy, act, slope=None, only=("inputs", "weight", "bias")):
+    """gradients of linear against 64 bits; slope: act' to take in place of that of the 64-bit z (what the layer itself returned)"""
+    import nerfacc_amd as nerfacc
+
+    dt, (m, k), n = x.dtype, x.shape, w.shape[0]
+    u, tiny = torch.finfo(dt).eps / 2, 2.0**-25 if dt == torch.float16 else 0.0
+    own = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    out = nerfacc.linear(*own, activation=act)
+    got = torch.autograd.grad(out, own, gy)
+    X, W, G = x.double(), w.double(), gy.double()
+    z = X @ W.t() + b.double()
+    first, size, second = parts(act, z)
+    soft = act not in (None, "relu")
+    if slope is not None:
+        first, size, off = slope(out), torch.zeros_like(z), torch.zeros_like(z)
+    else:
+        off = 16 * (1 + z.abs() + z * z) * 2.0**-24 * size + second * (k + 4) * 2.0**-24 * (X.abs() @ W.t().abs() + b.double().abs()) if soft else 0 * z
+        if soft and dt == torch.bfloat16:
+            off = off + u * first.abs()
+    dz, off = G * first, G.abs() * off
+    two = 2.0**-16 if soft and dt != torch.float32 else 0.0
+    join = 256 + -(-m // 256)
+    for what, g, ref, mag, err, sums, lost in (("inputs", got[0], dz @ W, dz.abs() @ W.abs(), off @ W.abs(), n, two),
+                                               ("weight", got[1], dz.t() @ X, dz.abs().t() @ X.abs(), off.t() @ X.abs(), join, two),
+                                               ("bias", got[2], dz.sum(0), dz.abs().sum(0), off.sum(0), join, 0.0)):
+        if what not in only:
+            continue
+        tol = u * ref.abs() + tiny + err + (lost + (sums + 8) * 2.0**-24) * mag
+        miss = (g.double() - ref).abs()
+        over = (ref.abs() + tol > torch.finfo(dt).max) & (g.double() == ref.sign() * math.inf)      # what the type does not hold rounds to infinity
+        assert ((miss <= tol) | over).all(), (what, (miss / tol).max().item(), miss.max().item())
+
+
+def normal(*shape, seed=0):
+    return torch.randn(shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV)
+
+
+@pytest.mark.parametrize("dtype", [*HALF, torch.float32])
+@pytest.mark.parametrize("act", SMOOTH)
+@pytest.mark.parametrize("m,k,n", [(70, 24, 64), (70, 23, 63)])
+def test_slopes_far_from_the_middle(dtype, act, m, k, n):
+    """z from -20 to 8 (gelu: -6), act' down to 2e-9 under a large loss scale; the bias gradient sums dz itself"""
+    x, w = normal(m, k, seed=1).to(dtype), (normal(n, k, seed=2) * 0.1 / k**0.5).to(dtype)
+    b = torch.linspace(-6.0 if act == "gelu" else -20.0, 8.0, n, device=DEV).to(dtype)
+    gy = (normal(m, n, seed=3).abs().double() / b.double().clamp(max=0).exp().clamp(min=2.0**-14)).to(dtype)
+    check(x, w, b, gy, act, only=("bias",))
+
+
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("act", SMOOTH)
 @pytest.mark.parametrize("n", [40, 300])
