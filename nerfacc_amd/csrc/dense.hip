@@ -108,19 +108,41 @@ __device__ __forceinline__ void load_saved(const DenseArgs &a, int64_t row, int6
 }
 
 template <class T> struct Frag { T v[kChunk<T>]; };
-template <class T> constexpr float kLargest = std::is_same_v<T, f16> ? 65504.0f : 0x1.fep127f;
 
-// dz = dy act'(.) of N chunks, rounded to T.  SPLIT (16-bit types, smooth activations): what the rounding lost goes into `rest`, and
-// the product is taken of both parts, so that a gradient carries the rounding of its own result and, in bf16, of act' only.  relu's
-// dz is dy or 0: nothing is lost there.  What T rounds to infinity becomes T's largest number and a rest, which is infinite where dz is
-// (infinity minus infinity would be NaN).  each(chunk, dz of one number in 32 bits, place in the chunk)
+// Smooth activations of 16-bit types: the product is taken of dz in two parts, so that a gradient carries the rounding of its own result and,
+// in bf16, of act' only.  The parts are bf16 for fp16 too, whose own range dz leaves at both ends: the gradient of a mean over 2^18 rows
+// is below fp16's smallest step, exp' under a loss scale above its largest number.  dz = high + low to 2^-17.  The other side is exact in
+// bf16's one part, and in fp16's two (11 bits in 8 + 8); of its four products the one of both second parts, 2^-18 of the term, is left out.
+constexpr float kLargest = 0x1.fep127f;         // of bf16
+template <class T, bool SPLIT> constexpr bool kSplitBoth = SPLIT && std::is_same_v<T, f16>;
+template <class T, bool SPLIT> using Fed = std::conditional_t<SPLIT, bf16, T>;      // what the matrix units multiply
+
+// a chunk of fp16 in two parts; infinity is 1 + infinity, whose products with dz's parts are infinities of one sign
+__device__ __forceinline__ void split_chunk(u32x4 v, u32x4 &high, u32x4 &low) {
+    const Frag<f16> x = __builtin_bit_cast(Frag<f16>, v);
+    Frag<bf16> h, l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float f = to_f(x.v[i]);
+        const bool inf = fabsf(f) > 65504.0f;
+        h.v[i] = from_f<bf16>(inf ? copysignf(1.0f, f) : f);
+        l.v[i] = from_f<bf16>(inf ? f : f - to_f(h.v[i]));
+    }
+    high = __builtin_bit_cast(u32x4, h);
+    low = __builtin_bit_cast(u32x4, l);
+}
+
+// dz = dy act'(.) of N chunks, rounded to what is multiplied.  SPLIT: what the rounding lost goes into `rest`.  relu's dz is dy or 0:
+// nothing is lost there.  What rounds to infinity becomes bf16's largest number and a rest, which is infinite where dz is (infinity minus
+// infinity would be NaN).  each(chunk, dz of one number in 32 bits, place in the chunk)
 template <class T, bool SPLIT, int N, class F>
 __device__ __forceinline__ void form_dz(const DenseArgs &a, u32x4 (&g)[N], const u32x4 (&s)[N * kSaved<T, SPLIT>], u32x4 (&rest)[SPLIT ? N : 1], F &&each) {
     auto with = [&](auto act) {
         constexpr int ACT = decltype(act)::value;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            Frag<T> v = __builtin_bit_cast(Frag<T>, g[k]), lo;
+            const Frag<T> v = __builtin_bit_cast(Frag<T>, g[k]);
+            Frag<Fed<T, SPLIT>> hi, lo;
             float w[kChunk<T>];
 #pragma unroll
             for (int i = 0; i < kChunk<T>; ++i) {
@@ -134,12 +156,11 @@ __device__ __forceinline__ void form_dz(const DenseArgs &a, u32x4 (&g)[N], const
                 else if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((s[k][0] >> i) & 1u) != 0 : w[i] > 0.0f) ? dz : 0.0f;
                 else if constexpr (ACT != NFA_ACT_NONE) dz *= act_slope_of_kept<ACT>(w[i]);
                 each(k, dz, i);
-                float near = dz;
-                if constexpr (SPLIT) near = fabsf(dz) > kLargest<T> ? copysignf(kLargest<T>, dz) : dz;
-                if constexpr (SPLIT || ACT != NFA_ACT_NONE) v.v[i] = from_f<T>(near);
-                if constexpr (SPLIT) lo.v[i] = from_f<T>(dz - to_f(v.v[i]));
+                if constexpr (SPLIT) hi.v[i] = from_f<bf16>(fabsf(dz) > kLargest ? copysignf(kLargest, dz) : dz);
+                else hi.v[i] = from_f<T>(dz);
+                if constexpr (SPLIT) lo.v[i] = from_f<bf16>(dz - to_f(hi.v[i]));
             }
-            if constexpr (SPLIT || ACT != NFA_ACT_NONE) g[k] = __builtin_bit_cast(u32x4, v);
+            if constexpr (SPLIT || ACT != NFA_ACT_NONE) g[k] = __builtin_bit_cast(u32x4, hi);
             if constexpr (SPLIT) rest[k] = __builtin_bit_cast(u32x4, lo);
         }
     };
@@ -298,6 +319,9 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
     const int lane = lane_id(), i = lane & 15, g = lane >> 4;
     const int q0 = blockIdx.y * a.block_q, nq = a.n_q - q0 < a.block_q ? a.n_q - q0 : a.block_q;
     const int q_rows = (nq + 31) & ~31, pitch = a.block_q / CE;         // (dgrad: block_q is 32, 64 or a multiple of 128)
+    constexpr bool BOTH = kSplitBoth<T, SPLIT>;                         // the weight's second parts behind the first
+    using M = Fed<T, SPLIT>;
+    const int second = a.block_q * (KS * 4 * CE * (int)sizeof(T));
     const T *Q = reinterpret_cast<const T *>(a.q), *P = reinterpret_cast<const T *>(a.p);
     if (MODE == kForward) {
         for (int e = threadIdx.x; e < q_rows * KS * 4; e += blockDim.x) {
@@ -309,10 +333,12 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
         for (int e = threadIdx.x; e < KS * 4 * CE * pitch; e += blockDim.x) {
             const int n = e / pitch, chunk = e - n * pitch;
             const u32x4 v = only_inside<VEC>(load_chunk<T, VEC>(Q + q0, n, a.n_c, a.ld_q, chunk * CE, nq), n < a.n_c && chunk * CE < nq);
-            *reinterpret_cast<u32x4 *>(lds + weight_offset_t<T>(n, chunk, pitch)) = v;
+            char *at = lds + weight_offset_t<T>(n, chunk, pitch);
+            if constexpr (BOTH) split_chunk(v, *reinterpret_cast<u32x4 *>(at), *reinterpret_cast<u32x4 *>(at + second));
+            else *reinterpret_cast<u32x4 *>(at) = v;
         }
     }
-    float *bias = reinterpret_cast<float *>(lds + a.block_q * (KS * 4 * CE * (int)sizeof(T)));
+    float *bias = reinterpret_cast<float *>(lds + second);
     if (MODE == kForward)
         for (int c = threadIdx.x; c < a.block_q; c += blockDim.x) bias[c] = a.bias && c < nq ? to_f(reinterpret_cast<const T *>(a.bias)[q0 + c]) : 0.0f;
     __syncthreads();
@@ -394,7 +420,7 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 if (k * 4 * CE >= a.n_c) continue;
-                u32x4 w[2 * NG];
+                u32x4 w[2 * NG], w2[BOTH ? 2 * NG : 1];
 #pragma unroll
                 for (int j = 0; j < 2 * NG; ++j) {
                     if (j >= 2 && !both) continue;
@@ -402,13 +428,16 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
                     if constexpr (MODE == kForward) {
                         w[j] = *reinterpret_cast<const u32x4 *>(lds + weight_offset<T, KS>(qj + (j & 1) * 16 + i, k * 4 + g));
                     } else if constexpr (sizeof(T) == 2) {
-                        s16x4 h[2];
+                        s16x4 h[2], h2[2];
 #pragma unroll
                         for (int s = 0; s < 2; ++s) {
                             const int n = k * 32 + g * 8 + s * 4 + (i >> 2), c = qj + (i & 3) * 8 + (j & 1) * 4;
-                            h[s] = read_transposed(lds + weight_offset_t<T>(n, c >> 3, pitch) + (c & 7) * 2);
+                            const char *at = lds + weight_offset_t<T>(n, c >> 3, pitch) + (c & 7) * 2;
+                            h[s] = read_transposed(at);
+                            if constexpr (BOTH) h2[s] = read_transposed(at + second);
                         }
                         w[j] = __builtin_bit_cast(u32x4, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                        if constexpr (BOTH) w2[j] = __builtin_bit_cast(u32x4, __builtin_shufflevector(h2[0], h2[1], 0, 1, 2, 3, 4, 5, 6, 7));
                     } else {
                         f32x4 e;
 #pragma unroll
@@ -424,8 +453,9 @@ __global__ __launch_bounds__(512) void resident_kernel(DenseArgs a) {
 #pragma unroll
                     for (int j = 0; j < 2 * NG; ++j) {
                         if (j >= 2 && !both) continue;
-                        acc[r][j] = multiply<T>(w[j], x[r * KS + k], acc[r][j]);
-                        if constexpr (SPLIT) acc[r][j] = multiply<T>(w[j], lo[r * KS + k], acc[r][j]);
+                        acc[r][j] = multiply<M>(w[j], x[r * KS + k], acc[r][j]);
+                        if constexpr (SPLIT) acc[r][j] = multiply<M>(w[j], lo[r * KS + k], acc[r][j]);
+                        if constexpr (BOTH) acc[r][j] = multiply<M>(w2[j], x[r * KS + k], acc[r][j]);
                     }
             }
 #pragma unroll
@@ -512,7 +542,9 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
     constexpr int CE = kChunk<T>, ST = kStage<T>;
     constexpr int CP = BP * 8 / TH, CQ = BQ * 8 / TH;       // chunks a thread stages per tile
     constexpr int NP = BP / WP / 16, NQ = BQ / WQ / 16;     // sixteen-wide fragments of a wave
-    constexpr int kP = BP * kRowBytes, kBuf = kP * (SPLIT ? 2 : 1) + BQ * kRowBytes;
+    constexpr bool BOTH = kSplitBoth<T, SPLIT>;
+    constexpr int kP = BP * kRowBytes, kQ = BQ * kRowBytes, kAtQ = kP * (SPLIT ? 2 : 1), kBuf = kAtQ + kQ * (BOTH ? 2 : 1);
+    using M = Fed<T, SPLIT>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
     const int wp = wave / WQ, wq = wave % WQ;
@@ -594,16 +626,22 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
             int row, chunk;
             place(QT, BQ, k, row, chunk);
             const bool inside = QT ? c + row < c_end && q0 + chunk * CE < a.n_q : q0 + row < a.n_q && c + chunk * CE < a.n_c;
-            *reinterpret_cast<u32x4 *>(buf + kBuf - BQ * kRowBytes + stage_offset<T, QT, BQ, DEAL>(row, chunk)) = only_inside<VEC>(t.q[k], inside);
+            char *at = buf + kAtQ + stage_offset<T, QT, BQ, DEAL>(row, chunk);
+            const u32x4 v = only_inside<VEC>(t.q[k], inside);
+            if constexpr (BOTH) split_chunk(v, *reinterpret_cast<u32x4 *>(at), *reinterpret_cast<u32x4 *>(at + kQ));
+            else *reinterpret_cast<u32x4 *>(at) = v;
         }
     };
     auto compute = [&](const char *buf, int64_t c) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (c + ks * (ST / 2) >= c_end) break;          // a half that holds only zeros
-            u32x4 fp[NP], fq[NQ];
+            u32x4 fp[NP], fq[NQ], fq2[BOTH ? NQ : 1];
 #pragma unroll
-            for (int j = 0; j < NQ; ++j) fq[j] = read_frag<T, QT, BQ, DEAL>(buf + kBuf - BQ * kRowBytes, wq * (BQ / WQ) + j * 16, ks, lane);
+            for (int j = 0; j < NQ; ++j) {
+                fq[j] = read_frag<T, QT, BQ, DEAL>(buf + kAtQ, wq * (BQ / WQ) + j * 16, ks, lane);
+                if constexpr (BOTH) fq2[j] = read_frag<T, QT, BQ>(buf + kAtQ + kQ, wq * (BQ / WQ) + j * 16, ks, lane);
+            }
 #pragma unroll
             for (int half = 0; half < (SPLIT ? 2 : 1); ++half) {
 #pragma unroll
@@ -611,7 +649,11 @@ __global__ __launch_bounds__(WP * WQ * kWave, 2) void tile_kernel(DenseArgs a) {
 #pragma unroll
                 for (int i = 0; i < NP; ++i)
 #pragma unroll
-                    for (int j = 0; j < NQ; ++j) acc[i][j] = multiply<T>(fq[j], fp[i], acc[i][j]);
+                    for (int j = 0; j < NQ; ++j) {
+                        acc[i][j] = multiply<M>(fq[j], fp[i], acc[i][j]);
+                        if constexpr (BOTH)
+                            if (half == 0) acc[i][j] = multiply<M>(fq2[j], fp[i], acc[i][j]);
+                    }
             }
         }
     };
@@ -975,7 +1017,7 @@ int launch_tiles(DenseArgs a, int64_t splits, hipStream_t s) {
     NFA_REQUIRE(tiles_p * a.tiles_q * std::max<int64_t>(splits, 1) < kMaxThreads / (WP * WQ * kWave), "linear: too many rows for one launch");
     a.tiles = (int32_t)(tiles_p * a.tiles_q);
     const int64_t steps = MODE == kWgrad ? a.split : a.n_c;
-    const size_t bytes = (size_t)(BP * (SPLIT ? 2 : 1) + BQ) * kRowBytes * (steps > kStage<T> ? 2 : 1);
+    const size_t bytes = (size_t)(BP * (SPLIT ? 2 : 1) + BQ * (kSplitBoth<T, SPLIT> ? 2 : 1)) * kRowBytes * (steps > kStage<T> ? 2 : 1);
     auto kernel = tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, true, false>;
     if constexpr (BP < 256)                                 // (the largest tiles are for aligned rows)
         if (!a.vec) kernel = tile_kernel<T, MODE, BP, BQ, WP, WQ, SPLIT, false, false>;
@@ -992,7 +1034,7 @@ int launch_tiles(DenseArgs a, int64_t splits, hipStream_t s) {
 
 template <class T, int MODE, int KS, bool SPLIT>
 int launch_resident(DenseArgs a, hipStream_t s) {
-    constexpr int RT = SPLIT || KS == 16 ? 1 : 2, C = KS * 4 * kChunk<T>;
+    constexpr int RT = SPLIT || KS == 16 ? 1 : 2, C = KS * 4 * kChunk<T>, kWeight = C * (int)sizeof(T) * (kSplitBoth<T, SPLIT> ? 2 : 1);
     const int64_t tiles = ceil_div(a.n_p, 16 * RT);
     NFA_REQUIRE(tiles < (1ll << 31), "linear: too many rows for one launch");
     a.tiles = (int32_t)tiles;
@@ -1000,12 +1042,12 @@ int launch_resident(DenseArgs a, hipStream_t s) {
     // with all columns)
     auto round_q = [](int64_t q) { return q <= 32 ? 32 : q <= 64 ? 64 : ceil_div(q, 128) * 128; };
     int64_t block = round_q(a.n_q), most = 32;
-    while (round_q(most + 32) * C * (int64_t)sizeof(T) <= kResidentBytes && most < block) most = round_q(most + 32);
+    while (round_q(most + 32) * kWeight <= kResidentBytes && most < block) most = round_q(most + 32);
     if (block > most) block = most;
     while (block > 32 && tiles * ceil_div(a.n_q, block) < kNumCU * 4) block = block > 128 ? round_q(block / 2) : block / 2;
     a.block_q = (int32_t)block;
     const int64_t blocks_q = ceil_div(a.n_q, block);
-    const size_t bytes = (size_t)(block * (C * (int64_t)sizeof(T) + 4));       // and the bias in 32 bits
+    const size_t bytes = (size_t)(block * (kWeight + 4));                      // and the bias in 32 bits
     const auto kernel = a.vec ? resident_kernel<T, MODE, KS, SPLIT, true> : resident_kernel<T, MODE, KS, SPLIT, false>;
     if (int rc = allow_lds(kernel, bytes)) return rc;
     const int per_cu = bytes <= 36 * 1024 ? 4 : bytes <= 72 * 1024 ? 2 : 1, threads = std::min(512, resident_waves(KS) * kWave / per_cu);
@@ -1058,6 +1100,8 @@ int launch_rows(const DenseArgs &a, hipStream_t s) {
     // 588 x 908 x 804 34 against 79, 18 against 35)
     if constexpr (MODE == kDgrad && !SPLIT)
         if (ceil_div(a.n_p, BP) * ceil_div(a.n_q, 128) < kNumCU) return launch_tiles<T, MODE, 64, 64, 2, 2, SPLIT>(a, 1, s);
+    if constexpr (kSplitBoth<T, SPLIT>)
+        if (a.n_q > 64) return launch_tiles<T, MODE, 128, 128, 2, 4, SPLIT>(a, 1, s);
     // (64 columns where there are no more: 65536 x 512 x 64 fp32 45 us against 79)
     return a.n_q <= 64 ? launch_tiles<T, MODE, BP, 64, 2, 2, SPLIT>(a, 1, s) : launch_tiles<T, MODE, BP, 128, 2, 2, SPLIT>(a, 1, s);
 }
@@ -1080,8 +1124,10 @@ WgradPlan wgrad_plan(int64_t rows, int64_t n, int64_t k, int32_t dtype, bool two
     // but in fp32, which the matrix units bound, not at the price of padding (2^18 x 129 x 32: 92 us by 64 x 64, 117 by 64 x 128),
     auto pad = [](int64_t x, int64_t b) { return ceil_div(x, b) * b; };
     const bool f32 = dtype == NFA_DTYPE_F32;
-    w.bp = n <= 64 || two_parts ? 64 : 128;
+    const bool both = two_parts && dtype == NFA_DTYPE_F16;
+    w.bp = n <= 64 || (two_parts && !both) ? 64 : 128;
     w.bq = k <= 64 ? 64 : k <= 128 || two_parts || w.bp == 64 ? 128 : 256;
+    if (both && w.bp != w.bq) w.bp = w.bq = 64;
     if (f32)
         while (w.bq > 64 && pad(k, w.bq / 2) < pad(k, w.bq)) w.bq /= 2;
     // and not where the rows are too few for a workgroup on every CU (4096 x 256 x 256 bf16 12 us by 64 x 64, 18 by 128 x 256)
@@ -1090,7 +1136,7 @@ WgradPlan wgrad_plan(int64_t rows, int64_t n, int64_t k, int32_t dtype, bool two
     const int64_t tiles = ceil_div(n, w.bp) * ceil_div(k, w.bq);
     // workgroups on a CU: one of 128 x 256; two otherwise (2^18 x 64 x 64 bf16 20 us, 25 with four; narrow layers 2^18 x 8 x 32 14.4, 15.5
     // with four), but four of 64 x 64 in fp32, whose steps are short (2^18 x 129 x 32: 109 us, 129 with two)
-    const int64_t per_cu = w.bq == 256 ? 1 : f32 && w.bp == 64 && w.bq == 64 && !narrow_layer(n, k) ? 4 : 2;
+    const int64_t per_cu = w.bq == 256 || (both && w.bq == 128) ? 1 : f32 && w.bp == 64 && w.bq == 64 && !narrow_layer(n, k) ? 4 : 2;
     int64_t splits = ceil_div(per_cu * kNumCU, tiles);
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
@@ -1235,7 +1281,9 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
             using T = decltype(t);
             if constexpr (sizeof(T) == 2)
                 if (split) {
-                    rc = w.bq == 64 ? launch_tiles<T, kWgrad, 64, 64, 2, 2, true>(e, w.splits, s) : launch_tiles<T, kWgrad, 64, 128, 2, 2, true>(e, w.splits, s);
+                    if (w.bq == 64) rc = launch_tiles<T, kWgrad, 64, 64, 2, 2, true>(e, w.splits, s);
+                    else if constexpr (std::is_same_v<T, f16>) rc = launch_tiles<T, kWgrad, 128, 128, 2, 4, true>(e, w.splits, s);
+                    else rc = launch_tiles<T, kWgrad, 64, 128, 2, 2, true>(e, w.splits, s);
                     return;
                 }
             // 2^18 x 8 x 32: 14.4 us against 33 by tiles of 64 x 64, 32 x 32 17.4 against 34, 64 x 64 39.3 against 39.7

@@ -70,7 +70,7 @@ def check(x, w, b, gy, act, slope=None, only=("inputs", "weight", "bias")):
         tol = u * ref.abs() + tiny + err + (lost + (sums + 8) * 2.0**-24) * mag
         miss = (g.double() - ref).abs()
         over = (ref.abs() + tol > torch.finfo(dt).max) & (g.double() == ref.sign() * math.inf)      # what the type does not hold rounds to infinity
-        assert ((miss <= tol) | over).all(), (what, (miss / tol).max().item(), miss.max().item())
+        assert ((miss <= tol) | over | (ref.isnan() & g.isnan())).all(), (what, (miss / tol).max().item(), miss.max().item())
 
 
 def normal(*shape, seed=0):
@@ -86,6 +86,65 @@ def test_slopes_far_from_the_middle(dtype, act, m, k, n):
     b = torch.linspace(-6.0 if act == "gelu" else -20.0, 8.0, n, device=DEV).to(dtype)
     gy = (normal(m, n, seed=3).abs().double() / b.double().clamp(max=0).exp().clamp(min=2.0**-14)).to(dtype)
     check(x, w, b, gy, act, only=("bias",))
+
+
+SHAPES = [(70, 24, 40), (300, 96, 256), (200, 130, 300), (5000, 64, 64), (2000, 33, 65)]
+
+
+@pytest.mark.parametrize("dtype", [*HALF, torch.float32])
+@pytest.mark.parametrize("act", [None, "relu", *SMOOTH])
+@pytest.mark.parametrize("m,k,n", SHAPES)
+def test_far_from_the_middle(dtype, act, m, k, n):
+    """z from -20 to 8 (gelu: -6): act' down to 2e-9, gradients that fp16 holds"""
+    lo, hi = (-6.0, 5.0) if act == "gelu" else (-20.0, 8.0)
+    x = normal(m, k, seed=1).to(dtype)
+    w = (normal(n, k, seed=2) * 0.2 / k**0.5).to(dtype)
+    b = torch.linspace(lo, hi, n, device=DEV).to(dtype)
+    small = b.double().clamp(max=0).exp() if act not in (None, "relu") else torch.ones(n, device=DEV, dtype=torch.float64)
+    gy = (normal(m, n, seed=3).double() / small.clamp(min=2.0**-14)).to(dtype)           # (a large loss scale: up to 2^14 times a normal number)
+    check(x, w, b, gy, act)
+    if act is not None:                                                                 # one column at a time: nothing larger hides it
+        j = n // 16
+        only = torch.zeros_like(gy)
+        only[:, j] = gy[:, j]
+        check(x, w, b, only, act)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("m,k,n", [(4096, 64, 48), (4096, 130, 256), (4096, 200, 300), (4099, 61, 63)])
+def test_sums_that_cancel_see_both_parts_of_dz(dtype, m, k, n):
+    """equal rows of both signs, so that dz's roundings would all go the same way and the sum is a small part of its terms"""
+    g = torch.Generator(device=DEV).manual_seed(m + n)
+    x = torch.ones(m, k, device=DEV, dtype=dtype)
+    x[:, 1::2] = -1
+    w = (normal(n, k, seed=5) * 0.4 / k**0.5).to(dtype)
+    b = (torch.rand(n, generator=g, device=DEV) * 2 - 1).to(dtype)
+    gy = (1 + torch.rand(1, n, generator=g, device=DEV)).to(dtype).expand(m, n).contiguous()
+    gy[m // 2:] = (-(1 + 2.0**-6) * gy[m // 2:].float()).to(dtype)
+    gy[m // 2] = 0
+    # exp is differentiated from its own output in bf16: no rounding of act' is in the way
+    check(x, w, b, gy, "exp", slope=(lambda out: out.detach().double()) if dtype == torch.bfloat16 else None)
+
+
+@pytest.mark.parametrize("slope", [0.05, 0.005, 0.0005])
+def test_small_gradients_of_many_rows_in_fp16(slope):
+    """the gradient of a mean over 2^18 samples: each dz is below fp16's smallest step, their sum is not"""
+    m, k, n = 1 << 18, 8, 16
+    x, w = torch.ones(m, k, device=DEV).half(), (normal(n, k, seed=1) * 0.01).half()
+    b = torch.full((n,), math.log(slope), device=DEV).half()
+    gy = torch.full((m, n), 4e-6, device=DEV).half()
+    check(x, w, b, gy, "softplus")
+    check(torch.zeros_like(x[:3000]), (w.float() * 1e4).half(), torch.full((n,), -6.0, device=DEV).half(), gy[:3000], "sigmoid")
+
+
+@pytest.mark.parametrize("m,k,n", [(300, 24, 40), (300, 130, 300), (257, 63, 65)])
+def test_large_gradients_in_fp16(m, k, n):
+    """dz up to 10^8, whose products with small weights and inputs fit"""
+    x, w = (normal(m, k, seed=1) * 2.0**-11).half(), (normal(n, k, seed=2) * 2.0**-11).half()
+    b = torch.linspace(2.0, 9.0, n, device=DEV).half()
+    gy = (normal(m, n, seed=3) * 30).half()
+    gy[:, -1] = gy[:, -1] * 100
+    check(x, w, b, gy, "exp")
 
 
 @pytest.mark.parametrize("dtype", HALF)
