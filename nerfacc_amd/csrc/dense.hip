@@ -153,7 +153,7 @@ __device__ __forceinline__ void form_dz(const DenseArgs &a, u32x4 (&g)[N], const
             for (int i = 0; i < kChunk<T>; ++i) {
                 float dz = to_f(v.v[i]);
                 if constexpr (SPLIT) dz *= ACT == NFA_ACT_SOFTPLUS ? -expm1f(-w[i]) : w[i];          // (ACT: bf16's softplus keeps its value)
-                else if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((s[k][0] >> i) & 1u) != 0 : w[i] > 0.0f) ? dz : 0.0f;
+                else if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((s[k][0] >> i) & 1u) == 0 : w[i] <= 0.0f) ? 0.0f : dz;
                 else if constexpr (ACT != NFA_ACT_NONE) dz *= act_slope_of_kept<ACT>(w[i]);
                 each(k, dz, i);
                 if constexpr (SPLIT) hi.v[i] = from_f<bf16>(fabsf(dz) > kLargest ? copysignf(kLargest, dz) : dz);
@@ -212,7 +212,7 @@ __device__ __forceinline__ void finish_chunks(const DenseArgs &a, float (&z)[N][
             for (int i = 0; i < kChunk<T>; ++i) {
                 const float v = act_fwd<ACT>(z[k][i]);
                 out.v[i] = from_f<T>(a.residual ? v + to_f(add.v[i]) : v);
-                if constexpr (ACT == NFA_ACT_RELU) bits |= (v > 0.0f ? 1u : 0u) << i;
+                if constexpr (ACT == NFA_ACT_RELU) bits |= (v <= 0.0f ? 0u : 1u) << i;     // (NaN passes its gradient on)
                 z[k][i] = ACT == NFA_ACT_RELU || ACT == NFA_ACT_EXP || (ACT == NFA_ACT_SOFTPLUS && kKept<T> == 1) ? v : z[k][i];
             }
             y[k] = __builtin_bit_cast(u32x4, out);
@@ -890,7 +890,7 @@ __global__ __launch_bounds__(kBlock, 2) void narrow_wgrad_kernel(DenseArgs a) {
 #pragma unroll
                 for (int f = 0; f < NP; ++f) {
                     float &dz = r.p[k].v[f];
-                    if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((r.bits[k] >> ((p & 3) + f)) & 1u) != 0 : r.s[k].v[f] > 0.0f) ? dz : 0.0f;
+                    if constexpr (ACT == NFA_ACT_RELU) dz = (a.mask ? ((r.bits[k] >> ((p & 3) + f)) & 1u) == 0 : r.s[k].v[f] <= 0.0f) ? 0.0f : dz;
                     else if constexpr (ACT != NFA_ACT_NONE) dz *= act_slope_of_kept<ACT>(r.s[k].v[f]);
                 }
         });
@@ -1100,6 +1100,8 @@ int launch_rows(const DenseArgs &a, hipStream_t s) {
     // 588 x 908 x 804 34 against 79, 18 against 35)
     if constexpr (MODE == kDgrad && !SPLIT)
         if (ceil_div(a.n_p, BP) * ceil_div(a.n_q, 128) < kNumCU) return launch_tiles<T, MODE, 64, 64, 2, 2, SPLIT>(a, 1, s);
+    // both sides in two parts fill 96 KiB of LDS with 64 x 128, one wave per SIMD: eight waves by 128 x 128 (65536 x 1024 x 1024 fp16 671 us
+    // against 1091, 65536 x 512 x 512 176 against 286)
     if constexpr (kSplitBoth<T, SPLIT>)
         if (a.n_q > 64) return launch_tiles<T, MODE, 128, 128, 2, 4, SPLIT>(a, 1, s);
     // (64 columns where there are no more: 65536 x 512 x 64 fp32 45 us against 79)
@@ -1124,6 +1126,8 @@ WgradPlan wgrad_plan(int64_t rows, int64_t n, int64_t k, int32_t dtype, bool two
     // but in fp32, which the matrix units bound, not at the price of padding (2^18 x 129 x 32: 92 us by 64 x 64, 117 by 64 x 128),
     auto pad = [](int64_t x, int64_t b) { return ceil_div(x, b) * b; };
     const bool f32 = dtype == NFA_DTYPE_F32;
+    // dz in two parts: 64 rows.  fp16, x in two parts too, 128 x 128 by eight waves (2^18 x 256 x 256 184 us against 288 by 64 x 128), 64 x 64
+    // where one side is narrow (2^18 x 256 -> 64 73 us against 76 by 64 x 128, 2^18 x 65 -> 63 60 against 84)
     const bool both = two_parts && dtype == NFA_DTYPE_F16;
     w.bp = n <= 64 || (two_parts && !both) ? 64 : 128;
     w.bq = k <= 64 ? 64 : k <= 128 || two_parts || w.bp == 64 ? 128 : 256;

@@ -162,3 +162,21 @@ def test_infinite_gradients_stay_infinite(dtype, act, n):
     gy[4] = 1.0
     gx, gw, gb = torch.autograd.grad(nerfacc.linear(*own, activation=act), own, gy)
     assert gw[3].isposinf().all() and gb[3].isposinf() and gw[:3].isfinite().all() and gw[4:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, *HALF])
+@pytest.mark.parametrize("m,k,n", [(6, 8, 24), (6, 8, 25), (300, 12, 32), (400, 64, 320), (400, 30, 301)])
+def test_relu_passes_gradients_where_its_output_is_nan(dtype, m, k, n):
+    """as torch's: only z <= 0 stops them"""
+    import nerfacc_amd as nerfacc
+
+    x, w, b, gy = (normal(*s, seed=i).to(dtype) for i, s in enumerate([(m, k), (n, k), (n,), (m, n)]))
+    x[3, 2] = float("nan")
+    own = [t.requires_grad_(True) for t in (x, w, b)]
+    out = nerfacc.linear(*own, activation="relu")
+    assert out[3].isnan().all()
+    gx, _, gb = torch.autograd.grad(out, own, gy)
+    mask = (out.detach().double() > 0) | out.detach().isnan()
+    dz = gy.double() * mask
+    for got, ref, mag in ((gx, dz @ w.double(), dz.abs() @ w.double().abs()), (gb, dz.sum(0), dz.abs().sum(0))):
+        assert ((got.double() - ref).abs() <= torch.finfo(dtype).eps / 2 * ref.abs() + (m + n) * 2.0**-24 * mag + 2.0**-25).all()
