@@ -1149,9 +1149,12 @@ WgradPlan wgrad_plan(int64_t rows, int64_t n, int64_t k, int32_t dtype, bool two
     return w;
 }
 
+// relu keeps a bit of each number, a byte a chunk.  Rows that do not divide into chunks are differentiated from the value instead, but in
+// fp16, where values below 2^-25 round to 0
 bool keeps_bits(int64_t out_features, int32_t dtype, int32_t act) {
-    return act == NFA_ACT_RELU && out_features % (16 / dtype_bytes(dtype)) == 0;
+    return act == NFA_ACT_RELU && (dtype == NFA_DTYPE_F16 || out_features % (16 / dtype_bytes(dtype)) == 0);
 }
+int64_t bit_bytes(int64_t out_features, int32_t dtype) { return ceil_div(out_features, 16 / dtype_bytes(dtype)); }     // of a row
 bool two_parts(int32_t dtype, int32_t act) { return dtype != NFA_DTYPE_F32 && act != NFA_ACT_NONE && act != NFA_ACT_RELU; }
 bool keeps_slopes(int32_t dtype, int32_t act) { return dtype == NFA_DTYPE_F16 && two_parts(dtype, act); }     // in 32 bits
 
@@ -1203,7 +1206,7 @@ static int check_linear(const nfa_linear_args *a, const char *who) {
 }
 
 NFA_EXPORT int64_t nfa_linear_saved_bytes(int64_t rows, int32_t out_features, int32_t dtype, int32_t activation, int32_t has_residual) {
-    if (keeps_bits(out_features, dtype, activation)) return rows * (out_features / (16 / dtype_bytes(dtype)));
+    if (keeps_bits(out_features, dtype, activation)) return rows * bit_bytes(out_features, dtype);
     if (keeps_slopes(dtype, activation)) return rows * out_features * 4;
     if (activation == NFA_ACT_NONE || (act_from_value(activation) && !has_residual)) return 0;
     return rows * out_features * dtype_bytes(dtype);
@@ -1223,7 +1226,7 @@ NFA_EXPORT int nfa_linear_fwd(const nfa_linear_args *a, void *outputs, void *sav
     d.n_p = a->rows; d.n_q = a->out_features; d.n_c = a->in_features;
     d.act = a->activation;
     d.mask = keeps_bits(a->out_features, a->dtype, a->activation);
-    d.ld_saved = d.mask ? a->out_features / (16 / bytes) : a->out_features;
+    d.ld_saved = d.mask ? bit_bytes(a->out_features, a->dtype) : a->out_features;
     d.vec = aligned(d.p, d.ld_p, a->in_features, bytes, 16) && aligned(d.q, d.ld_q, a->in_features, bytes, 16) &&
             aligned(outputs, d.n_q, d.n_q, bytes, 16) && (!saved || d.mask || aligned(saved, d.n_q, d.n_q, keeps_slopes(a->dtype, a->activation) ? 4 : bytes, 16)) &&
                 (!a->residual || aligned(a->residual, a->residual_stride, d.n_q, bytes, 16));
@@ -1254,7 +1257,7 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
     d.saved = saved;
     d.act = a->activation;
     d.mask = keeps_bits(n, a->dtype, a->activation);
-    d.ld_saved = d.mask ? n / (16 / bytes) : n;
+    d.ld_saved = d.mask ? bit_bytes(n, a->dtype) : n;
     const bool vec = aligned(a->grad_outputs, a->grad_outputs_stride, n, bytes, 16) &&
               (!saved || a->activation == NFA_ACT_NONE || d.mask || aligned(saved, n, n, keeps_slopes(a->dtype, a->activation) ? 4 : bytes, 16));
     int rc = NFA_OK;

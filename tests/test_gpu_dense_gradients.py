@@ -180,3 +180,17 @@ def test_relu_passes_gradients_where_its_output_is_nan(dtype, m, k, n):
     dz = gy.double() * mask
     for got, ref, mag in ((gx, dz @ w.double(), dz.abs() @ w.double().abs()), (gb, dz.sum(0), dz.abs().sum(0))):
         assert ((got.double() - ref).abs() <= torch.finfo(dtype).eps / 2 * ref.abs() + (m + n) * 2.0**-24 * mag + 2.0**-25).all()
+
+
+@pytest.mark.parametrize("n", [24, 25, 5])
+@pytest.mark.parametrize("residual", [False, True])
+def test_relu_passes_gradients_where_its_fp16_output_rounds_to_zero(n, residual):
+    """z = 2^-26 is above 0, whatever the output keeps of it"""
+    import nerfacc_amd as nerfacc
+
+    x, w = torch.full((6, 4), 2.0**-14, device=DEV).half(), torch.full((n, 4), 2.0**-14, device=DEV).half()
+    own = [t.requires_grad_(True) for t in (x, w)]
+    out = nerfacc.linear(*own, activation="relu", residual=torch.zeros(6, n, device=DEV).half() if residual else None)
+    assert not out.any()
+    gx, _ = torch.autograd.grad(out, own, torch.full((6, n), 1024.0, device=DEV).half())
+    assert torch.equal(gx, torch.full_like(gx, n / 16))
