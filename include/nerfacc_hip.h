@@ -468,7 +468,7 @@ int nfa_pdf_loss_bwd(const float *g_loss, const int32_t *ids_left, const int32_t
  *                 [rows, out_features] (nullable) -> outputs [rows, out_features] contiguous.  saved (nullable unless a backward
  *                 pass follows): what nfa_linear_bwd differentiates the activation from, nfa_linear_saved_bytes(...) bytes; 0
  *                 bytes = it needs none, or (exp and softplus but in fp16, and some sizes of relu, without a residual) the outputs
- *                 themselves.
+ *                 themselves, and saved is left alone.
  * nfa_linear_bwd  grad_outputs [rows, out_features] -> grad_inputs [rows, in_features] contiguous, grad_weight, grad_bias (each
  *                 nullable); the residual's gradient is grad_outputs.  saved = the forward call's saved array, or its outputs where
  *                 nfa_linear_saved_bytes says 0 and the activation is not NONE.  workspace: nfa_linear_bwd_workspace_bytes(...). */

@@ -1218,6 +1218,7 @@ NFA_EXPORT int nfa_linear_fwd(const nfa_linear_args *a, void *outputs, void *sav
     NFA_REQUIRE(outputs, "linear_fwd: NULL pointer");
     NFA_REQUIRE(!a->residual || a->residual_stride >= a->out_features || a->rows == 1, "linear_fwd: residual_stride < out_features");
     const int64_t bytes = dtype_bytes(a->dtype);
+    if (nfa_linear_saved_bytes(a->rows, a->out_features, a->dtype, a->activation, a->residual != nullptr) == 0) saved = nullptr;
     DenseArgs d{};
     d.p = a->inputs; d.ld_p = a->inputs_stride;
     d.q = a->weight; d.ld_q = a->in_features;

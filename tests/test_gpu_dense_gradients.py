@@ -194,3 +194,22 @@ def test_relu_passes_gradients_where_its_fp16_output_rounds_to_zero(n, residual)
     assert not out.any()
     gx, _ = torch.autograd.grad(out, own, torch.full((6, n), 1024.0, device=DEV).half())
     assert torch.equal(gx, torch.full_like(gx, n / 16))
+
+
+@pytest.mark.parametrize("act,dtype", [(0, 0), (0, 2), (6, 0), (3, 1), (1, 1)])
+def test_saved_is_left_alone_where_nothing_is_kept(act, dtype):
+    """through the C ABI: an array of 0 bytes, as nfa_linear_saved_bytes asks for, is not written to"""
+    import ctypes
+
+    from nerfacc_amd.cuda import _backend
+
+    L, m, k, n = _backend.load_library(), 4, 8, 9
+    dt = [torch.float32, torch.bfloat16, torch.float16][dtype]
+    x, w, out = normal(m, k).to(dt), normal(n, k, seed=1).to(dt), torch.empty(m, n, device=DEV, dtype=dt)
+    saved = torch.full((m * n * 4,), 77, device=DEV, dtype=torch.uint8)                  # (room for whatever might be written)
+    a = _backend._STRUCTS["nfa_linear_args"](rows=m, in_features=k, out_features=n, dtype=dtype, activation=act, inputs=x.data_ptr(), inputs_stride=k,
+                                             weight=w.data_ptr())
+    assert L.nfa_linear_saved_bytes(m, n, dtype, act, 0) == 0
+    assert L.nfa_linear_fwd(ctypes.byref(a), out.data_ptr(), saved.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert saved.eq(77).all()
