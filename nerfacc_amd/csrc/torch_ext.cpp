@@ -1745,6 +1745,12 @@ void check_like(const char *op, const char *what, const Tensor &t, const Tensor 
     TORCH_CHECK_TYPE(t.scalar_type() == dtype, op, ": ", what, " must have dtype ", dtype, ", got ", t.scalar_type());
     TORCH_CHECK_VALUE(t.sizes() == shape, op, ": ", what, " must have shape ", shape, ", got ", t.sizes());
 }
+// a tangent would be dropped without a word
+void refuse_forward(const char *op, std::initializer_list<OptTensor> tensors) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (auto &t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!(t && t->defined() && t->_fw_grad(0).defined()), op, ": forward mode derivatives are not implemented");
+}
 // whether autograd records the call; refuses one whose captured backward pass would end the process
 bool records_grad(const char *op, const Tensor &x, std::initializer_list<OptTensor> tensors) {
     if (!at::GradMode::is_enabled()) return false;
@@ -1797,6 +1803,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 };
 
 Tensor linear(const Tensor &x, const Tensor &w, const OptTensor &b, const OptTensor &r, int64_t act) {
+    refuse_forward("linear", {x, w, b, r});
     TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1), "linear: inputs (..., in) and weight (out, in) expected, got ", x.sizes(),
                       " and ", w.sizes());
     const int64_t n = w.size(0), k = w.size(1);
@@ -1887,6 +1894,7 @@ int64_t check_width(const char *op, const Tensor &w, int64_t channels) {
 
 std::tuple<Tensor, OptTensor> causal_conv(const Tensor &x_, const Tensor &w, const OptTensor &b, const OptTensor &info, const OptTensor &init, int64_t act,
                                           bool want_final) {
+    refuse_forward("causal_conv", {x_, w, b, init});
     const int64_t n_rays = sequences_of("causal_conv", x_, info), d = x_.size(-1), width = check_width("causal_conv", w, d);
     check_native("causal_conv", x_);
     const auto dt = x_.scalar_type();
@@ -1934,6 +1942,7 @@ void written(const OptTensor &to) {
 }
 
 std::tuple<Tensor, Tensor> causal_conv_one(const Tensor &x, const Tensor &state, const Tensor &w, const OptTensor &b, int64_t act, const OptTensor &to_) {
+    refuse_forward("causal_conv_step", {x, state, w, b, to_});
     TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) > 0, "causal_conv_step: inputs must be (n_rays, channels)");
     const int64_t r = x.size(0), d = x.size(1), width = check_width("causal_conv_step", w, d);
     check_native("causal_conv_step", x);
@@ -2001,6 +2010,7 @@ void check_scan(const char *op, const Tensor &x, at::IntArrayRef rows, const Ten
 std::tuple<Tensor, OptTensor> selective_scan(const Tensor &x_, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const OptTensor &D,
                                              const OptTensor &z, const OptTensor &bias, bool softplus, const OptTensor &info, const OptTensor &init,
                                              bool want_final) {
+    refuse_forward("selective_scan", {x_, dt, A, B, C, D, z, bias, init});
     const int64_t n_rays = sequences_of("selective_scan", x_, info);
     check_scan("selective_scan", x_, x_.sizes().slice(0, x_.dim() - 1), dt, A, B, C, D, z, bias);
     check_like("selective_scan", "packed_info", get(info), x_, {n_rays, 2}, at::kLong);
@@ -2026,6 +2036,7 @@ std::tuple<Tensor, OptTensor> selective_scan(const Tensor &x_, const Tensor &dt,
 
 std::tuple<Tensor, Tensor> selective_scan_one(const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Tensor &state,
                                               const OptTensor &D, const OptTensor &z, const OptTensor &bias, bool softplus, const OptTensor &to_) {
+    refuse_forward("selective_scan_step", {x, dt, A, B, C, D, z, bias, state, to_});
     TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) > 0, "selective_scan_step: inputs must be (n_rays, channels)");
     check_scan("selective_scan_step", x, x.sizes().slice(0, 1), dt, A, B, C, D, z, bias);
     const int64_t r = x.size(0), d = x.size(1), s = A.size(1);

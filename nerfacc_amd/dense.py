@@ -5,6 +5,7 @@ No reference counterpart: the reference leaves fields to its examples (examples/
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
@@ -47,6 +48,12 @@ def _check_native(name: str, ref: Tensor, others) -> None:
             raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
+def _refuse_forward(name: str, *tensors) -> None:
+    """a tangent would be dropped without a word"""
+    if torch._C._is_fwd_grad_enabled() and any(isinstance(t, Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name}: forward mode derivatives are not implemented")
+
+
 def _records_grad(name: str, *tensors) -> bool:
     """whether autograd records the call; refuses one whose captured backward pass would end the process"""
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)):
@@ -75,7 +82,7 @@ def linear(inputs: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activa
         residual: (..., out_features), the same dtype, added behind the activation.
 
     Sums are held in 32 bits and the result is rounded once.  The backward pass differentiates once; its sums have a fixed order
-    (the same bits every time).
+    (the same bits every time).  Forward mode derivatives are refused.
 
         >>> x = torch.tensor([[1., 2.]], device="cuda")
         >>> linear(x, torch.tensor([[1., 1.], [1., -1.]], device="cuda"), activation="relu")
@@ -85,6 +92,7 @@ def linear(inputs: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activa
     ext = _EXT or _ext()
     if ext:
         return ext.linear(inputs, weight, bias, residual, act)
+    _refuse_forward("linear", inputs, weight, bias, residual)
     if not isinstance(inputs, Tensor) or not isinstance(weight, Tensor):
         raise TypeError("linear: inputs and weight must be torch.Tensors")
     if inputs.dim() < 1 or weight.dim() != 2 or inputs.shape[-1] != weight.shape[1]:

@@ -12,7 +12,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import cuda as _C
-from .dense import _activation_id, _check_native, _ext, _records_grad
+from .dense import _activation_id, _check_native, _ext, _records_grad, _refuse_forward
 
 _MAX_STATES = 256
 
@@ -103,6 +103,7 @@ def causal_conv(inputs: Tensor, weight: Tensor, bias: Optional[Tensor] = None, a
     if ext:
         out = ext.causal_conv(inputs, weight, bias, packed_info, initial_state, act, return_final_state)
         return out if return_final_state else out[0]
+    _refuse_forward("causal_conv", inputs, weight, bias, initial_state)
     n_rays = _sequences("causal_conv", inputs, packed_info)
     channels, dt = inputs.shape[-1], inputs.dtype
     width = _width("causal_conv", weight, channels)
@@ -158,6 +159,7 @@ def causal_conv_step(inputs: Tensor, state: Tensor, weight: Tensor, bias: Option
     ext = _ext()
     if ext:
         return ext.causal_conv_one(inputs, state, weight, bias, act, out_state)
+    _refuse_forward("causal_conv_step", inputs, state, weight, bias, out_state)
     if not isinstance(inputs, Tensor) or inputs.dim() != 2 or inputs.shape[1] == 0:
         raise ValueError("causal_conv_step: inputs must be (n_rays, channels)")
     n_rays, channels = inputs.shape
@@ -209,6 +211,7 @@ def selective_scan(inputs: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tenso
     if ext:
         out = ext.selective_scan(inputs, delta, A, B, C, D, gate, delta_bias, bool(delta_softplus), packed_info, initial_state, return_final_state)
         return out if return_final_state else out[0]
+    _refuse_forward("selective_scan", inputs, delta, A, B, C, D, gate, delta_bias, initial_state)
     n_rays = _sequences("selective_scan", inputs, packed_info)
     rows, channels = inputs.shape[:-1], inputs.shape[-1]
     _check_scan("selective_scan", inputs, rows, channels, n_rays, delta, A, B, C, D, gate, delta_bias,
@@ -265,6 +268,7 @@ def selective_scan_step(inputs: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: 
     ext = _ext()
     if ext:
         return ext.selective_scan_one(inputs, delta, A, B, C, state, D, gate, delta_bias, bool(delta_softplus), out_state)
+    _refuse_forward("selective_scan_step", inputs, delta, A, B, C, D, gate, delta_bias, state, out_state)
     if not isinstance(inputs, Tensor) or inputs.dim() != 2 or inputs.shape[1] == 0:
         raise ValueError("selective_scan_step: inputs must be (n_rays, channels)")
     if not isinstance(state, Tensor):

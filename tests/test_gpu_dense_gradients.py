@@ -213,3 +213,23 @@ def test_saved_is_left_alone_where_nothing_is_kept(act, dtype):
     assert L.nfa_linear_fwd(ctypes.byref(a), out.data_ptr(), saved.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
     torch.cuda.synchronize()
     assert saved.eq(77).all()
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_forward_mode_is_refused(python, monkeypatch):
+    import torch.autograd.forward_ad as fwd
+
+    import nerfacc_amd as nerfacc
+    from nerfacc_amd import dense
+
+    if python:
+        monkeypatch.setattr(dense, "_EXT", False)
+    x, w, b = normal(4, 8), normal(6, 8), normal(6)
+    with fwd.dual_level():
+        for i in range(3):
+            args = [fwd.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate((x, w, b))]
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                nerfacc.linear(*args)
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            nerfacc.linear(x, w, residual=fwd.make_dual(normal(4, 6), normal(4, 6)))
+        nerfacc.linear(x, w, b)

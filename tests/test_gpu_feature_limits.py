@@ -34,3 +34,33 @@ def test_conv_rays_that_overlap_leave_the_others_right(dtype):
     torch.cuda.synchronize()
     assert got.shape == x.shape
     assert torch.equal(got[100:], grad(x[100:], gy[100:], gf[3:], torch.tensor([[0, 30]], device=DEV)))
+
+
+# -------------------------------------------------------------------------------------------------------------- derivatives
+def scan_arguments(n=6, d=8, s=4):
+    return dict(inputs=normal(1, n, d), delta=normal(1, n, d, seed=1).abs(), A=-normal(d, s, seed=2).abs(), B=normal(1, n, s, seed=3), C=normal(1, n, s, seed=4),
+                D=normal(d, seed=5), gate=normal(1, n, d, seed=6), delta_bias=normal(d, seed=7), initial_state=normal(1, d, s, seed=8))
+
+
+def conv_arguments(n=6, d=8):
+    return dict(inputs=normal(1, n, d), weight=normal(d, 4, seed=1), bias=normal(d, seed=2), initial_state=normal(1, 3, d, seed=3))
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_forward_mode_is_refused(python, monkeypatch):
+    import torch.autograd.forward_ad as fwd
+
+    import nerfacc_amd as nerfacc
+    from nerfacc_amd import dense
+
+    if python:
+        monkeypatch.setattr(dense, "_EXT", False)
+    steps = [(nerfacc.causal_conv_step, {**{k: v[:, 0] if k == "inputs" else v for k, v in conv_arguments().items()}}),
+             (nerfacc.selective_scan_step, {k: v[:, 0] if k in ("inputs", "delta", "B", "C", "gate") else v for k, v in scan_arguments().items()})]
+    for _, kw in steps:
+        kw["state"] = kw.pop("initial_state")
+    for call, kw in [(nerfacc.causal_conv, conv_arguments()), (nerfacc.selective_scan, scan_arguments()), *steps]:
+        call(**kw)
+        for k in kw:
+            with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+                call(**{**kw, k: fwd.make_dual(kw[k], torch.ones_like(kw[k]))})
