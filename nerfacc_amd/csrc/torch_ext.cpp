@@ -1764,16 +1764,24 @@ bool records_grad(const char *op, const Tensor &x, std::initializer_list<OptTens
                 "eager outputs first, or call under torch.no_grad()");
     return true;
 }
-// the results of a backward pass that differentiates once: using them in another one is an error, as torch's once_differentiable does it
-variable_list once(variable_list grads, const variable_list &outer) {
+// The results of a backward pass that differentiates once.  Under create_graph those that depend on something learnt (`depends`: through the
+// tensors of the forward call; all of them where a gradient that came in requires one) are an error in another backward pass, as torch's
+// once_differentiable makes those of the second kind: a penalty on them would have no effect otherwise.
+variable_list once(variable_list grads, const variable_list &outer, std::initializer_list<bool> depends) {
+    if (!at::GradMode::is_enabled()) return grads;
     bool any = false;
     for (auto &g : outer) any |= g.defined() && g.requires_grad();
-    if (!at::GradMode::is_enabled() || !any) return grads;
-    for (auto &g : grads)
-        if (g.defined()) g = g.detach().requires_grad_(true);
-    const size_t n = grads.size();
+    variable_list held;
+    auto learnt = [&](size_t i) { return grads[i].defined() && (any || (i < depends.size() && depends.begin()[i])); };
+    for (size_t i = 0; i < grads.size(); ++i)
+        if (learnt(i)) held.push_back(grads[i].detach().requires_grad_(true));
+    if (held.empty()) return grads;
+    const size_t n = held.size();
     auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", n);
-    return (*error)(std::move(grads));
+    held = (*error)(std::move(held));
+    for (size_t i = 0, k = 0; i < grads.size(); ++i)
+        if (learnt(i)) grads[i] = held[k++];
+    return grads;
 }
 
 struct LinearFn : torch::autograd::Function<LinearFn> {
@@ -1783,6 +1791,10 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         ctx->saved_data["act"] = act;
         ctx->saved_data["bias"] = b && b->defined();
         ctx->saved_data["residual"] = r && r->defined();
+        const bool smooth = act != NFA_ACT_NONE && act != NFA_ACT_RELU;
+        ctx->saved_data["slope"] = smooth && learns;            // act' depends on something learnt
+        ctx->saved_data["x"] = x.requires_grad();
+        ctx->saved_data["w"] = w.requires_grad();
         if (learns) ctx->save_for_backward({x, w, !kept.defined() && act != NFA_ACT_NONE ? out : kept});
         return out;
     }
@@ -1798,7 +1810,8 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
             out[2] = get(std::get<2>(g));
         }
         if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(has_bias ? 3 : 2)) out[3] = grads[0];     // (counts the given tensors)
-        return once(out, grads);
+        const bool slope = ctx->saved_data["slope"].toBool();
+        return once(out, grads, {slope || ctx->saved_data["w"].toBool(), slope || ctx->saved_data["x"].toBool(), slope, false});
     }
 };
 
@@ -1882,7 +1895,9 @@ struct CausalConvFn : torch::autograd::Function<CausalConvFn> {
                                  has_b && ctx->needs_input_grad(2), has_init && ctx->needs_input_grad(has_b ? 3 : 2));
         variable_list out(10);
         out[0] = get(std::get<0>(g)); out[1] = get(std::get<1>(g)); out[2] = get(std::get<2>(g)); out[3] = get(std::get<3>(g));
-        return once(out, grads);
+        auto learns = [&](int i) { return s[i].defined() && s[i].requires_grad(); };
+        const bool slope = ctx->saved_data["act"].toInt() != NFA_ACT_NONE && (learns(0) || learns(1) || learns(2) || learns(3));
+        return once(out, grads, {slope || learns(1), slope || learns(0) || learns(3), slope, slope || learns(1)});
     }
 };
 
@@ -1984,7 +1999,11 @@ struct SelectiveScanFn : torch::autograd::Function<SelectiveScanFn> {
             if (!s[i].defined()) continue;
             if (ctx->needs_input_grad(given++)) out[i] = get(g[from[i]]);
         }
-        return once(out, grads);
+        // outputs are linear in u, B, C, D and the initial state, each by itself
+        bool any[9] = {};
+        for (int i = 0; i < 9; ++i)
+            for (int j = 0; j < 9; ++j) any[i] |= s[j].defined() && s[j].requires_grad() && (j != i || i == 1 || i == 4 || i == 5 || i == 7);
+        return once(out, grads, {any[0], any[1], any[2], any[3], any[4], any[5], any[6], any[7], any[8]});
     }
 };
 

@@ -2,12 +2,12 @@
 
 No reference counterpart: the reference leaves fields to its examples (examples/radiance_fields/mlp.py:16-107, torch layers).
 """
+import functools
 from typing import Optional
 
 import torch
 import torch.autograd.forward_ad as forward_ad
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import cuda as _C
 
@@ -112,10 +112,44 @@ def linear(inputs: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activa
     return out if inputs.dim() == 2 else out.view(shape)
 
 
+class _Once(torch.autograd.Function):
+    """passes gradients through; a backward pass over it is an error"""
+
+    @staticmethod
+    def forward(ctx, *grads):
+        return grads
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("trying to differentiate twice a function that was marked with @once_differentiable")
+
+
+def _differentiates_once(depends):
+    """A backward pass that differentiates once.  Under create_graph those of its results that depend on something learnt are an error in
+    another backward pass (a penalty on them would have no effect otherwise): all where a gradient that came in requires one, else those
+    that `depends(ctx)` names, a truth value for each."""
+    def wrap(backward):
+        @functools.wraps(backward)
+        def run(ctx, *grads):
+            with torch.no_grad():
+                outs = backward(ctx, *grads)
+            if not torch.is_grad_enabled():
+                return outs
+            outer = any(g is not None and g.requires_grad for g in grads)
+            names = depends(ctx)
+            held = [i for i, g in enumerate(outs) if g is not None and (outer or (i < len(names) and names[i]))]
+            marked = _Once.apply(*(outs[i].detach().requires_grad_(True) for i in held)) if held else ()
+            return tuple(marked[held.index(i)] if i in held else g for i, g in enumerate(outs))
+        return run
+    return wrap
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
         learns = any(ctx.needs_input_grad[:3])
+        slope = learns and act > 1                          # act' depends on something learnt
+        ctx.depends = (slope or ctx.needs_input_grad[1], slope or ctx.needs_input_grad[0], slope)
         out, saved = _C.linear_fwd(x, weight, bias, residual, act, learns)
         ctx.act, ctx.has_bias = act, bias is not None
         if learns:
@@ -123,7 +157,7 @@ class _Linear(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_differentiates_once(lambda ctx: ctx.depends)
     def backward(ctx, grad):
         gx = gw = gb = None
         need = ctx.needs_input_grad

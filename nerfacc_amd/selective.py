@@ -9,10 +9,9 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import cuda as _C
-from .dense import _activation_id, _check_native, _ext, _records_grad, _refuse_forward
+from .dense import _activation_id, _check_native, _differentiates_once, _ext, _records_grad, _refuse_forward
 
 _MAX_STATES = 256
 
@@ -132,11 +131,14 @@ class _CausalConv(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         out, final = _C.causal_conv_fwd(x, weight, bias, init, *rows, n_rays, act, want_final)
         ctx.save_for_backward(x, weight, bias, init)
+        learns = ctx.needs_input_grad[:4]
+        slope = act > 0 and any(learns)
+        ctx.depends = (slope or learns[1], slope or learns[0] or learns[3], slope, slope or learns[1])
         ctx.rows, ctx.n_rays, ctx.act = rows, n_rays, act
         return out, final
 
     @staticmethod
-    @once_differentiable
+    @_differentiates_once(lambda ctx: ctx.depends)
     def backward(ctx, gy, gfinal):
         x, weight, bias, init = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -246,11 +248,13 @@ class _SelectiveScan(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         out, final, kept = _C.selective_scan_fwd(u, delta, gate, B, C, A, D, bias, init, *rows, n_rays, softplus, want_final, True)
         ctx.save_for_backward(u, delta, gate, B, C, A, D, bias, init, kept)
+        # outputs are linear in u, B, C, D and the initial state, each by itself
+        ctx.depends = tuple(any(l and (j != i or i in (1, 2, 5, 7)) for j, l in enumerate(ctx.needs_input_grad[:9])) for i in range(9))
         ctx.rows, ctx.n_rays, ctx.softplus = rows, n_rays, softplus
         return out, final
 
     @staticmethod
-    @once_differentiable
+    @_differentiates_once(lambda ctx: ctx.depends)
     def backward(ctx, gy, gfinal):
         u, delta, gate, B, C, A, D, bias, init, kept = ctx.saved_tensors
         if gy is None:

@@ -215,6 +215,27 @@ def test_saved_is_left_alone_where_nothing_is_kept(act, dtype):
     assert saved.eq(77).all()
 
 
+@pytest.mark.parametrize("act", [None, "relu", "silu"])
+@pytest.mark.parametrize("python", [False, True])
+def test_a_penalty_on_the_gradient_is_refused(act, python, monkeypatch):
+    """it would need second derivatives, which the layer does not have: an error, never a term without effect"""
+    import nerfacc_amd as nerfacc
+    from nerfacc_amd import dense
+
+    if python:
+        monkeypatch.setattr(dense, "_EXT", False)
+    x, w, b = (normal(*s, seed=i).requires_grad_(True) for i, s in enumerate([(4, 8), (6, 8), (6,)]))
+    out = nerfacc.linear(x, w, b, activation=act)
+    gx, gw = torch.autograd.grad(out, (x, w), torch.ones_like(out), create_graph=True)
+    for g in (gx, gw):
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            (out.detach().sum() + g.square().sum()).backward(retain_graph=True)
+    # a gradient that depends on nothing that is learnt is a plain tensor, as torch's own is
+    y = nerfacc.linear(x, w.detach(), b.detach(), activation="relu")
+    assert not torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)[0].requires_grad
+
+
 @pytest.mark.parametrize("python", [False, True])
 def test_forward_mode_is_refused(python, monkeypatch):
     import torch.autograd.forward_ad as fwd

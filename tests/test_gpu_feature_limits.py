@@ -64,3 +64,21 @@ def test_forward_mode_is_refused(python, monkeypatch):
         for k in kw:
             with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
                 call(**{**kw, k: fwd.make_dual(kw[k], torch.ones_like(kw[k]))})
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_a_penalty_on_the_gradient_is_refused(python, monkeypatch):
+    import nerfacc_amd as nerfacc
+    from nerfacc_amd import dense
+
+    if python:
+        monkeypatch.setattr(dense, "_EXT", False)
+    for call, kw in ((nerfacc.causal_conv, conv_arguments()), (nerfacc.selective_scan, scan_arguments())):
+        own = {k: v.requires_grad_(True) for k, v in kw.items()}
+        out = call(**own)
+        for k, g in zip(own, torch.autograd.grad(out, list(own.values()), torch.ones_like(out), create_graph=True)):
+            if k == "bias":
+                continue                                              # (a sum of dy: it depends on nothing that is learnt)
+            assert g.requires_grad, k
+            with pytest.raises(RuntimeError, match="once_differentiable"):
+                g.square().sum().backward(retain_graph=True)
