@@ -337,19 +337,23 @@ __global__ __launch_bounds__(kBlock) void scan_chain_kernel(ScanArgs a) {
     const int64_t chunks = count > 0 ? (count + a.chunk - 1) / a.chunk : 1, first = start / a.chunk;
     constexpr int kAhead = 32;                              // chunks in flight: the chain itself is one fma each
     for (int64_t k0 = 0; k0 < chunks; k0 += kAhead) {
-        float add[kAhead], decay[kAhead];
+        // A chunk's decay may be beyond 32 bits where no row's is (growing states), and what it meets may be 0 or tiny: it is applied as two
+        // powers of two, the second 1 for all that fit one, and never to 0.
+        float add[kAhead], decay[kAhead], more[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int64_t k = k0 + i < chunks ? k0 + i : chunks - 1, slot = chunk_slot(a, ray, first, REV ? chunks - 1 - k : k);
             add[i] = a.ends[(slot * a.states + s) * a.channels + ch];
-            decay[i] = fast_exp2(a.sums[slot * a.channels + ch] * A2);
+            const float e = a.sums[slot * a.channels + ch] * A2, one = fminf(fmaxf(e, -126.0f), 126.0f);
+            decay[i] = fast_exp2(one);
+            more[i] = fast_exp2(e - one);
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             if (k0 + i >= chunks) break;
             const int64_t k = k0 + i, slot = chunk_slot(a, ray, first, REV ? chunks - 1 - k : k);
             a.ends[(slot * a.states + s) * a.channels + ch] = h;
-            h = fmaf(decay[i], h, add[i]);
+            h = h == 0.0f ? add[i] : fmaf(decay[i], h * more[i], add[i]);
         }
     }
 }

@@ -36,6 +36,37 @@ def test_conv_rays_that_overlap_leave_the_others_right(dtype):
     assert torch.equal(got[100:], grad(x[100:], gy[100:], gf[3:], torch.tensor([[0, 30]], device=DEV)))
 
 
+# ------------------------------------------------------------------------------------------------------------------ values
+@pytest.mark.parametrize("rays,n", [(1, 300), (2, 700)])
+def test_scan_of_growing_states(rays, n):
+    """positive A: a chunk's decay overflows 32 bits while there is no state yet, or a tiny one, and the sum itself is small"""
+    import nerfacc_amd as nerfacc
+
+    d, s = 6, 4
+    step, A = torch.ones(rays, n, d, device=DEV), torch.full((d, s), 3.0, device=DEV)
+    u = torch.zeros(rays, n, d, device=DEV)
+    u[:, -3:] = 1.0
+    B = C = torch.ones(rays, n, s, device=DEV)
+    own = [t.clone().requires_grad_(True) for t in (u, step)]
+    out, end = nerfacc.selective_scan(own[0], own[1], A, B, C, return_final_state=True)
+    e = torch.exp(torch.tensor(3.0)).item()
+    want = torch.tensor([1.0, 1 + e, 1 + e + e * e], device=DEV) * s
+    assert not out[:, :-3].any()
+    assert torch.allclose(out[:, -3:], want[None, :, None].expand(rays, 3, d), rtol=1e-5) and torch.allclose(end, want[-1].expand_as(end) / s, rtol=1e-5)
+    # backwards the same: a gradient that only the first rows' states could see
+    gy = torch.zeros_like(out)
+    gy[:, :2] = 1.0
+    gu, _ = torch.autograd.grad(out, own, gy)
+    assert not gu[:, 2:].any() and torch.allclose(gu[:, 1], torch.full_like(gu[:, 1], s), rtol=1e-5)
+    assert torch.allclose(gu[:, 0], torch.full_like(gu[:, 0], s * (1 + e)), rtol=1e-5)
+    # a tiny initial state that grows into an ordinary number: e^(0.15 n) 1e-25 over more rows than a chunk has
+    init = torch.full((rays, d, s), 1e-25, device=DEV)
+    A = torch.full((d, s), 70.0 / n, device=DEV)
+    out = nerfacc.selective_scan(torch.zeros_like(u), step, A, B, C, initial_state=init)
+    ref = s * 1e-25 * torch.exp(70.0 / n * torch.arange(1, n + 1, device=DEV, dtype=torch.float64))
+    assert torch.allclose(out.double(), ref[None, :, None].expand(rays, n, d), rtol=(16 + 3 * n + 70 * 4) * 2.0**-24, atol=0)
+
+
 # -------------------------------------------------------------------------------------------------------------- derivatives
 def scan_arguments(n=6, d=8, s=4):
     return dict(inputs=normal(1, n, d), delta=normal(1, n, d, seed=1).abs(), A=-normal(d, s, seed=2).abs(), B=normal(1, n, s, seed=3), C=normal(1, n, s, seed=4),
