@@ -216,6 +216,9 @@ struct Rows {
     }
 };
 
+// y + D u; without D nothing: 0 u would be NaN for an infinite u
+__device__ __forceinline__ float add_skip(const ScanArgs &a, float D, float u, float y) { return a.D ? fmaf(D, u, y) : y; }
+
 // softplus and its derivative from one exponential
 struct Step { float step, slope; };
 __device__ __forceinline__ Step softplus_step(float raw) {
@@ -294,7 +297,7 @@ __global__ __launch_bounds__(kWave) void scan_fwd_kernel(ScanArgs a) {
                 if (!LOCAL) y = fmaf(C[i], h[i], y);
             }
             if (!LOCAL) {
-                y = fmaf(D, u, sum_parts<P>(y));
+                y = add_skip(a, D, u, sum_parts<P>(y));
                 if (a.z) {
                     const float z = to_f(rows.z[j]);
                     y *= z * sigmoid_f(z);
@@ -583,9 +586,9 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
                 sB = sum_parts<P>(sB);
                 sA = sum_parts<P>(sA);
                 const float dstep = fmaf(u, sB, sA * kLn2) * slope;
-                if (a.z) y = fmaf(D, u, sum_parts<P>(y));
+                if (a.z) y = add_skip(a, D, u, sum_parts<P>(y));
                 if (part == 0) {
-                    own_rows[kU][j][col] = fmaf(step, sB, D * dy);
+                    own_rows[kU][j][col] = add_skip(a, D, dy, step * sB);
                     own_rows[kSlope][j][col] = dstep;
                     own_rows[kGate][j][col] = gate * y;
                 }
@@ -718,7 +721,7 @@ __global__ __launch_bounds__(kBlock) void scan_step_kernel(ScanArgs a, const flo
                 y = fmaf(to_f(C[s]), v, y);
             }
         }
-        y = fmaf(D, u, y);
+        y = add_skip(a, D, u, y);
         if (a.z) y *= z * sigmoid_f(z);
         if (s0 == 0) (reinterpret_cast<T *>(a.y) + ray * a.channels)[ch] = from_f<T>(y);
     }

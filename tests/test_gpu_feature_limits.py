@@ -67,6 +67,39 @@ def test_scan_of_growing_states(rays, n):
     assert torch.allclose(out.double(), ref[None, :, None].expand(rays, n, d), rtol=(16 + 3 * n + 70 * 4) * 2.0**-24, atol=0)
 
 
+def infinite_inputs(states, n, skip):
+    import nerfacc_amd as nerfacc
+
+    d = 5
+    A, one = -torch.rand(d, states, generator=generator(0), device=DEV), torch.ones(2, n, states, device=DEV)
+    u, dt = normal(2, n, d, seed=1), torch.rand(2, n, d, generator=generator(2), device=DEV) + 0.1
+    D = torch.ones(d, device=DEV) if skip else None
+    clean = nerfacc.selective_scan(u, dt, A, one, one, D=D)
+    step, _ = nerfacc.selective_scan_step(u[:, 4], dt[:, 4], A, one[:, 4], one[:, 4], torch.zeros(2, d, states, device=DEV), D=D)
+    u[1, 4, 2] = float("inf")
+    out, end = nerfacc.selective_scan(u, dt, A, one, one, D=D, return_final_state=True)
+    assert out[1, 4:, 2].isposinf().all() and end[1, 2].isposinf().all()
+    keep = torch.ones_like(out, dtype=torch.bool)
+    keep[1, 4:, 2] = False
+    assert torch.equal(out[keep], clean[keep])
+    got, _ = nerfacc.selective_scan_step(u[:, 4], dt[:, 4], A, one[:, 4], one[:, 4], torch.zeros(2, d, states, device=DEV), D=D)
+    assert got[1, 2].isposinf() and torch.equal(got[0], step[0])
+    u[1, 4, 2] = 1.0
+    own = [t.clone().requires_grad_(True) for t in (u, dt)]
+    gy = torch.ones_like(out)
+    gy[1, 10, 3] = float("inf")
+    gu, _ = torch.autograd.grad(nerfacc.selective_scan(*own, A, one, one, D=D), own, gy)
+    assert gu[1, :11, 3].isposinf().all() and gu[1, 11:].isfinite().all() and gu[0].isfinite().all()
+
+
+@pytest.mark.parametrize("states", [4, 16, 32])
+@pytest.mark.parametrize("n", [20, 400])
+@pytest.mark.parametrize("skip", [False, True])
+def test_scan_of_infinite_inputs(states, n, skip):
+    """inf is inf, and a D that is not there adds nothing"""
+    infinite_inputs(states, n, skip)
+
+
 # -------------------------------------------------------------------------------------------------------------- derivatives
 def scan_arguments(n=6, d=8, s=4):
     return dict(inputs=normal(1, n, d), delta=normal(1, n, d, seed=1).abs(), A=-normal(d, s, seed=2).abs(), B=normal(1, n, s, seed=3), C=normal(1, n, s, seed=4),
