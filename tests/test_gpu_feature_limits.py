@@ -100,6 +100,14 @@ def test_scan_of_infinite_inputs(states, n, skip):
     infinite_inputs(states, n, skip)
 
 
+@pytest.mark.parametrize("states", [1, 2, 3, 5, 9, 20])
+@pytest.mark.parametrize("n", [20, 400])
+@pytest.mark.parametrize("skip", [False, True])
+def test_scan_of_infinite_inputs_with_states_that_fill_no_power_of_two(states, n, skip):
+    """places of no state add nothing either"""
+    infinite_inputs(states, n, skip)
+
+
 # -------------------------------------------------------------------------------------------------------------- derivatives
 def scan_arguments(n=6, d=8, s=4):
     return dict(inputs=normal(1, n, d), delta=normal(1, n, d, seed=1).abs(), A=-normal(d, s, seed=2).abs(), B=normal(1, n, s, seed=3), C=normal(1, n, s, seed=4),
