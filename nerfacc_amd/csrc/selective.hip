@@ -43,11 +43,16 @@ struct ScanArgs {
     void *y, *gu, *gdt, *gz;
     float *final_state, *kept, *ginit;
     float *ends, *sums;                 // chunks: [slots][states][channels], [slots][channels]
-    float *part_bc;                     // backward: [channel blocks][rows][2][padded states]
+    float *part_bc;                     // backward: [groups of channel blocks][rows][2][padded states]
     float *part_w;                      // backward: [workers][channels * states + 2 * channels]
     int64_t rows, n_rays, length, chunk, chunks, slots, tasks, workers;
-    int32_t channels, states, softplus, blocks;
+    int32_t channels, states, softplus, blocks, groups;
 };
+// Channel blocks that a wave of the backward pass takes one after the other, summing their dB and dC in memory.  A block's channels are
+// 64 / P, so that partial sums of every block would be as large as all of h (34 GB at 32768 rows of 1024 channels of 256 states, whose
+// states kept every eight rows take 4.3): so they are as large as the kept states, at most.  8192 rows of 512 channels of 128 states: 289 MiB
+// of workspace and 1.79 ms, 1033 and 1.51 with partial sums of every block; up to 32 states every block has its own.
+constexpr int blocks_of_wave(int p) { return p > 4 ? p / 4 : 1; }
 
 // a task: a run of rows of one sequence
 struct Task { int64_t ray, start, count, first, n, slot; bool live; };      // sequence rows [start, start + count), the task's [first, first + n) of it
@@ -448,11 +453,21 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
     __shared__ __attribute__((aligned(16))) float bc[2][kTile * SP];
     __shared__ float own_rows[5][kTile][CH];                // step, u, slope, dy, dL/dy of the gate; later du, dstep, dgate
     enum { kStep, kU, kSlope, kDy, kGate };
+    constexpr int EACH = blocks_of_wave(P);
     const int lane = lane_id(), part = lane / CH, col = lane % CH;
     const int64_t id = blockIdx.x;
-    const int64_t worker = id / a.blocks;
+    const int64_t worker = id / a.groups;
     if (worker >= a.workers) return;
-    const int block = (int)(id - worker * a.blocks);
+    const int group = (int)(id - worker * a.groups);
+    // after the exchange over channels: this lane's values, their places, and whether it is the one that stores them
+    constexpr int kBits = log2_of(CH), kHalvings = kBits < log2_of(2 * NS) ? kBits : log2_of(2 * NS), kLeft = 2 * NS >> kHalvings;
+    int number = 0;
+#pragma unroll
+    for (int i = 0; i < kHalvings; ++i) number |= ((lane >> (kBits - 1 - i)) & 1) << i;
+    const bool stores = (lane & ((1 << (kBits - kHalvings)) - 1)) == 0;
+
+    for (int block = group * EACH; block < (group + 1) * EACH && block < a.blocks; ++block) {
+    const bool first_block = block == group * EACH;
     const uint32_t ch = (uint32_t)block * CH + col, last = a.channels - 1, chc = ch < last ? ch : last;
     const bool on = ch <= last;
     float A2[NS], dA[NS], dD = 0.0f, dbias = 0.0f;          // A2 = A log2(e): dstep is summed with it and scaled once
@@ -463,13 +478,6 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
         A2[i] = on && s < a.states ? a.A[ch * a.states + s] * kLog2e : 0.0f;
         dA[i] = 0.0f;
     }
-    // after the exchange over channels: this lane's values, their places, and whether it is the one that stores them
-    constexpr int kBits = log2_of(CH), kHalvings = kBits < log2_of(2 * NS) ? kBits : log2_of(2 * NS), kLeft = 2 * NS >> kHalvings;
-    int number = 0;
-#pragma unroll
-    for (int i = 0; i < kHalvings; ++i) number |= ((lane >> (kBits - 1 - i)) & 1) << i;
-    const bool stores = (lane & ((1 << (kBits - kHalvings)) - 1)) == 0;
-
     int64_t place = worker;                                 // of this worker's sums; its ray's where it has one ray: the dealing order leaves no trace
     for (int64_t task = worker; task < a.tasks; task += a.workers) {
         const Task t = find_task(a, task, lane);
@@ -579,6 +587,13 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
                 float B[NS], C[NS], before[NS], v[2 * NS], y = 0.0f, sB = 0.0f, sA = 0.0f;
                 states_at(0, j, B);
                 states_at(1, j, C);
+                float *to = a.part_bc + ((int64_t)group * a.rows + row + j) * (2 * SP), before_sum[kLeft];
+                if (EACH > 1 && !first_block)               // what the blocks before this one left, read early
+#pragma unroll
+                    for (int i = 0; i < kLeft; ++i) {
+                        const uint32_t q = i * (1 << kHalvings) + number;
+                        before_sum[i] = to[(q / NS) * SP + part * NS + q % NS];
+                    }
 #pragma unroll
                 for (int i = 0; i < NS; i += 4) {
                     f32x4 q = {h0[i], h0[i + 1], h0[i + 2], h0[i + 3]};
@@ -612,11 +627,10 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
                 dbias += dstep;
                 sum_over_lanes<2 * NS, CH / 2>(v, lane);
                 if (stores) {
-                    float *to = a.part_bc + ((int64_t)block * a.rows + row + j) * (2 * SP);
 #pragma unroll
                     for (int i = 0; i < kLeft; ++i) {
                         const uint32_t q = i * (1 << kHalvings) + number;
-                        to[(q / NS) * SP + part * NS + q % NS] = v[i];
+                        to[(q / NS) * SP + part * NS + q % NS] = EACH > 1 && !first_block ? before_sum[i] + v[i] : v[i];
                     }
                 }
             }
@@ -641,9 +655,8 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
             }
         }
     }
-    const int64_t per = (int64_t)a.channels * (a.states + 2);
-    float *to = a.part_w + place * per;
-    if (!on) return;
+    if (!on) continue;
+    float *to = a.part_w + place * ((int64_t)a.channels * (a.states + 2));
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
         const int s = part * NS + i;
@@ -653,9 +666,10 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
         to[(int64_t)a.channels * a.states + ch] = dD;
         to[(int64_t)a.channels * (a.states + 1) + ch] = dbias;
     }
+    }
 }
 
-// dB and dC of a row: the channel blocks' sums in order; zeros for rows of no sequence.  A thread: four neighbouring states.  Memory: 2^18
+// dB and dC of a row: the groups' sums in order; zeros for rows of no sequence.  A thread: four neighbouring states.  Memory: 2^18
 // rows of two blocks and 16 states, 67 MB in and 17 out, 18 us (4.7 TB/s).
 template <class T>
 __global__ __launch_bounds__(kBlock) void scan_join_bc_kernel(ScanArgs a, int log_sp, T *gB, T *gC) {
@@ -666,7 +680,7 @@ __global__ __launch_bounds__(kBlock) void scan_join_bc_kernel(ScanArgs a, int lo
         if (s >= a.states) continue;
         f32x4 v = {0, 0, 0, 0};
         if (!a.info || a.pos[row] >= 0)
-            for (int b = 0; b < a.blocks; ++b) {
+            for (int b = 0; b < a.groups; ++b) {
                 const f32x4 w = *reinterpret_cast<const f32x4 *>(a.part_bc + (((int64_t)b * a.rows + row) << (log_sp + 1)) + q);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] += w[i];
@@ -798,16 +812,17 @@ void with_shape(int32_t dtype, Shape sh, int states, F &&g) {
 // four (32768 rows of 1024 channels 331 -> 297 us, 64 sequences of 512 rows, 512 channels 200 -> 165), unless that makes them shorter than
 // 64 rows (two sequences of 8192 rows, 512 channels: 106 us, 116 with four) or a chain longer than 512 (131072 rows of 64 channels: 298
 // and 497).  The backward pass holds two waves per SIMD at most (its LDS).
-struct ScanPlan { Shape sh; int blocks; int64_t chunk, chunks, slots, tasks, workers; };
+struct ScanPlan { Shape sh; int blocks, groups; int64_t chunk, chunks, slots, tasks, workers; };
 ScanPlan scan_plan(int64_t n_rays, int64_t rows, int channels, int states, bool packed, bool backward) {
     ScanPlan p{};
     p.sh = shape_of(states, backward ? kBwdStates : kFwdStates);
     p.blocks = (int)ceil_div(channels, kWave / p.sh.p);
-    const int64_t waves = n_rays * p.blocks, want = (int64_t)kNumCU * 8;
+    p.groups = backward ? (int)ceil_div(p.blocks, blocks_of_wave(p.sh.p)) : p.blocks;      // waves side by side
+    const int64_t waves = n_rays * p.groups, want = (int64_t)kNumCU * 8;
     p.tasks = n_rays;
     if (n_rays > 0 && waves < kNumCU * 4 && rows / n_rays >= 64) {
         const int64_t length = rows / n_rays;
-        auto chunk_for = [&](int64_t waves) { return ceil_div(ceil_div(rows * p.blocks, waves), kTile) * kTile; };
+        auto chunk_for = [&](int64_t waves) { return ceil_div(ceil_div(rows * p.groups, waves), kTile) * kTile; };
         int64_t chunk = chunk_for(want);
         if (!backward && chunk_for(2 * want) >= 64 && length / chunk_for(2 * want) <= 512) chunk = chunk_for(2 * want);
         if (chunk < 32) chunk = 32;
@@ -832,7 +847,7 @@ ScanSpace scan_space(const ScanPlan &p, int64_t rows, int channels, int states, 
     s.ends = align256(p.slots * states * channels * 4);
     s.sums = align256(p.slots * channels * 4);
     if (backward) {
-        s.bc = align256((int64_t)p.blocks * rows * 2 * p.sh.ns * p.sh.p * 4);
+        s.bc = align256((int64_t)p.groups * rows * 2 * p.sh.ns * p.sh.p * 4);
         s.w = align256(p.workers * channels * (states + 2) * 4);
     }
     s.total = s.ends + s.sums + s.bc + s.w;
@@ -876,7 +891,7 @@ ScanArgs scan_args(const nfa_selective_scan_args *a) {
     return d;
 }
 void use_plan(ScanArgs &d, const ScanPlan &p, const ScanSpace &sp, void *workspace) {
-    d.chunk = p.chunk; d.chunks = p.chunks; d.slots = p.slots; d.tasks = p.tasks; d.workers = p.workers; d.blocks = p.blocks;
+    d.chunk = p.chunk; d.chunks = p.chunks; d.slots = p.slots; d.tasks = p.tasks; d.workers = p.workers; d.blocks = p.blocks; d.groups = p.groups;
     char *w = (char *)workspace;
     d.ends = (float *)w;
     d.sums = (float *)(w + sp.ends);
@@ -955,7 +970,7 @@ NFA_EXPORT int nfa_selective_scan_bwd(const nfa_selective_scan_args *a, const fl
     if (p.workers != a->n_rays || p.chunk) d.order = nullptr;
     d.kept = (float *)checkpoints;
     d.gu = g->inputs; d.gdt = g->delta; d.gz = a->gate ? g->gate : nullptr; d.ginit = g->initial_state;
-    const int64_t grid = p.tasks * p.blocks, main_grid = p.workers * p.blocks;
+    const int64_t grid = p.tasks * p.blocks, main_grid = p.workers * p.groups;
     NFA_REQUIRE(grid < kMaxThreads / kWave && a->n_rays * (int64_t)(p.chunk ? 1 : 0) < 65536, "selective_scan_bwd: too large for one launch");
     if (a->packed_info) launch_zero_rows(d, a->dtype, d.gu, d.gdt, d.gz, s);
     with_shape<kBwdStates>(a->dtype, p.sh, a->states, [&](auto t, auto ns, auto pp, auto padded) {

@@ -154,3 +154,13 @@ def test_a_penalty_on_the_gradient_is_refused(python, monkeypatch):
             assert g.requires_grad, k
             with pytest.raises(RuntimeError, match="once_differentiable"):
                 g.square().sum().backward(retain_graph=True)
+
+
+# --------------------------------------------------------------------------------------------------------------- workspaces
+@pytest.mark.parametrize("states,channels", [(100, 70), (256, 70), (256, 33), (129, 129)])
+@pytest.mark.parametrize("lens", [[9, 0, 11], [130, 1, 200]])
+def test_scan_of_many_states_and_many_channels(states, channels, lens):
+    """sums over channels that one wave takes a block of channels at a time"""
+    from test_gpu_selective import check_scan, packed, scan_inputs
+
+    check_scan(scan_inputs(sum(lens), len(lens), channels, states, torch.float32, seed=states), packed(lens))
