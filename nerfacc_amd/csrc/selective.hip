@@ -467,205 +467,205 @@ __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
     const bool stores = (lane & ((1 << (kBits - kHalvings)) - 1)) == 0;
 
     for (int block = group * EACH; block < (group + 1) * EACH && block < a.blocks; ++block) {
-    const bool first_block = block == group * EACH;
-    const uint32_t ch = (uint32_t)block * CH + col, last = a.channels - 1, chc = ch < last ? ch : last;
-    const bool on = ch <= last;
-    float A2[NS], dA[NS], dD = 0.0f, dbias = 0.0f;          // A2 = A log2(e): dstep is summed with it and scaled once
-    const float D = on && a.D ? a.D[ch] : 0.0f, bias = on && a.bias ? a.bias[ch] : 0.0f;
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        const int s = part * NS + i;
-        A2[i] = on && s < a.states ? a.A[ch * a.states + s] * kLog2e : 0.0f;
-        dA[i] = 0.0f;
-    }
-    int64_t place = worker;                                 // of this worker's sums; its ray's where it has one ray: the dealing order leaves no trace
-    for (int64_t task = worker; task < a.tasks; task += a.workers) {
-        const Task t = find_task(a, task, lane);
-        if (!t.live) continue;
-        if (a.order) place = t.ray;
-        float G[NS];                                        // dL/dh of the row behind, times its decay
+        const bool first_block = block == group * EACH;
+        const uint32_t ch = (uint32_t)block * CH + col, last = a.channels - 1, chc = ch < last ? ch : last;
+        const bool on = ch <= last;
+        float A2[NS], dA[NS], dD = 0.0f, dbias = 0.0f;          // A2 = A log2(e): dstep is summed with it and scaled once
+        const float D = on && a.D ? a.D[ch] : 0.0f, bias = on && a.bias ? a.bias[ch] : 0.0f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int s = part * NS + i;
-            const bool here = on && s < a.states;
-            G[i] = 0.0f;
-            if (here && a.chunk) G[i] = a.ends[(t.slot * a.states + s) * a.channels + ch];
-            else if (here && a.gfinal) G[i] = a.gfinal[(t.ray * a.channels + ch) * a.states + s];
+            A2[i] = on && s < a.states ? a.A[ch * a.states + s] * kLog2e : 0.0f;
+            dA[i] = 0.0f;
         }
-        const int64_t row0 = t.start + t.first, tiles = (t.n + kTile - 1) / kTile;
-        auto rows_in = [&](int64_t k) { const int64_t r = t.n - k * kTile; return (int)(r < kTile ? r : kTile); };
-
-        // what the next tile needs from memory
-        T nu[PR], ndt[PR], nz[PR], ng[PR], nb[kStates], nc[kStates];
-        float nh[NS];
-        auto load = [&](int64_t k) {
-            const int64_t row = row0 + k * kTile;
-            const int n = rows_in(k);
-#pragma unroll
-            for (int r = 0; r < PR; ++r) {
-                const int j = part * PR + r;
-                const uint32_t at = j < n ? j : n - 1;
-                nu[r] = row_at<T>(a.u, row, a.ld_u, at, chc);
-                ndt[r] = row_at<T>(a.dt, row, a.ld_dt, at, chc);
-                ng[r] = row_at<T>(a.gy, row, a.ld_gy, at, chc);
-                nz[r] = a.z ? row_at<T>(a.z, row, a.ld_z, at, chc) : T(0.0f);
-            }
-#pragma unroll
-            for (int q = 0; q < kStates; ++q) {
-                const int e = q * kWave + lane, s = e % SP;
-                const uint32_t at = e / SP < n ? e / SP : n - 1, sc = s < a.states ? s : 0;
-                nb[q] = row_at<T>(a.B, row, a.ld_B, at, sc);
-                nc[q] = row_at<T>(a.C, row, a.ld_C, at, sc);
-                if (s >= a.states) nb[q] = nc[q] = T(0.0f);
-            }
-            const bool inside = t.first + k > 0;
-            const float *from = inside ? a.kept + (row / kTile) * a.states * a.channels : a.init;
+        int64_t place = worker;                                 // of this worker's sums; its ray's where it has one ray: the dealing order leaves no trace
+        for (int64_t task = worker; task < a.tasks; task += a.workers) {
+            const Task t = find_task(a, task, lane);
+            if (!t.live) continue;
+            if (a.order) place = t.ray;
+            float G[NS];                                        // dL/dh of the row behind, times its decay
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 const int s = part * NS + i;
-                nh[i] = 0.0f;
-                if (from && on && s < a.states) nh[i] = from[inside ? (uint32_t)s * a.channels + ch : (t.ray * a.channels + ch) * a.states + s];
+                const bool here = on && s < a.states;
+                G[i] = 0.0f;
+                if (here && a.chunk) G[i] = a.ends[(t.slot * a.states + s) * a.channels + ch];
+                else if (here && a.gfinal) G[i] = a.gfinal[(t.ray * a.channels + ch) * a.states + s];
             }
-        };
-        if (tiles > 0) load(tiles - 1);
-        for (int64_t k = tiles - 1; k >= 0; --k) {
-            const int64_t row = row0 + k * kTile;
-            const int n = rows_in(k);
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int r = 0; r < PR; ++r) {
-                const int j = part * PR + r;
-                // lanes without a channel: no input and no gradient, so that they add nothing to dB and dC
-                const float raw = to_f(ndt[r]) + bias, u = on ? to_f(nu[r]) : 0.0f, gy = on ? to_f(ng[r]) : 0.0f;
-                Step st = {raw, 1.0f};
-                if (a.softplus) st = softplus_step(raw);
-                float dy = gy, gate = 0.0f;
-                if (a.z) {
-                    const float z = on ? to_f(nz[r]) : 0.0f, sig = sigmoid_f(z);
-                    dy = gy * (z * sig);
-                    gate = gy * (sig * fmaf(z, 1.0f - sig, 1.0f));
-                }
-                if (P <= kTile || j < kTile) {
-                    own_rows[kStep][j][col] = on ? st.step : 0.0f;
-                    own_rows[kU][j][col] = u;
-                    own_rows[kSlope][j][col] = st.slope;
-                    own_rows[kDy][j][col] = dy;
-                    own_rows[kGate][j][col] = gate;
-                }
-            }
-#pragma unroll
-            for (int q = 0; q < kStates; ++q) {
-                const int e = q * kWave + lane;
-                if (e < kTile * SP) {
-                    bc[0][e] = to_f(nb[q]);
-                    bc[1][e] = to_f(nc[q]);
-                }
-            }
-            float h[NS], h0[NS];
-#pragma unroll
-            for (int i = 0; i < NS; ++i) h[i] = h0[i] = nh[i];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            if (k > 0) load(k - 1);
+            const int64_t row0 = t.start + t.first, tiles = (t.n + kTile - 1) / kTile;
+            auto rows_in = [&](int64_t k) { const int64_t r = t.n - k * kTile; return (int)(r < kTile ? r : kTile); };
 
-            auto states_at = [&](int which, int j, float (&v)[NS]) { read_states<NS>(&bc[which][j * SP + part * NS], v); };
-#pragma unroll 2
-            for (int j = 0; j < n; ++j) {
-                const float step = own_rows[kStep][j][col], in = step * own_rows[kU][j][col];
-                float B[NS];
-                states_at(0, j, B);
+            // what the next tile needs from memory
+            T nu[PR], ndt[PR], nz[PR], ng[PR], nb[kStates], nc[kStates];
+            float nh[NS];
+            auto load = [&](int64_t k) {
+                const int64_t row = row0 + k * kTile;
+                const int n = rows_in(k);
 #pragma unroll
-                for (int i = 0; i < NS; ++i) h[i] = only_states<PADDED>(a, part * NS + i, fmaf(fast_exp2(step * A2[i]), h[i], in * B[i]));
-                if (j + 1 < n)
-#pragma unroll
-                    for (int i = 0; i < NS; i += 4) hist[j][i / 4][lane] = f32x4{h[i], h[i + 1], h[i + 2], h[i + 3]};
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            for (int j = n - 1; j >= 0; --j) {
-                const float step = own_rows[kStep][j][col], u = own_rows[kU][j][col], slope = own_rows[kSlope][j][col], dy = own_rows[kDy][j][col],
-                            gate = own_rows[kGate][j][col], in = step * u;
-                float B[NS], C[NS], before[NS], v[2 * NS], y = 0.0f, sB = 0.0f, sA = 0.0f;
-                states_at(0, j, B);
-                states_at(1, j, C);
-                float *to = a.part_bc + ((int64_t)group * a.rows + row + j) * (2 * SP), before_sum[kLeft];
-                if (EACH > 1 && !first_block)               // what the blocks before this one left, read early
-#pragma unroll
-                    for (int i = 0; i < kLeft; ++i) {
-                        const uint32_t q = i * (1 << kHalvings) + number;
-                        before_sum[i] = to[(q / NS) * SP + part * NS + q % NS];
-                    }
-#pragma unroll
-                for (int i = 0; i < NS; i += 4) {
-                    f32x4 q = {h0[i], h0[i + 1], h0[i + 2], h0[i + 3]};
-                    if (j > 0) q = hist[j - 1][i / 4][lane];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) before[i + r] = q[r];
+                for (int r = 0; r < PR; ++r) {
+                    const int j = part * PR + r;
+                    const uint32_t at = j < n ? j : n - 1;
+                    nu[r] = row_at<T>(a.u, row, a.ld_u, at, chc);
+                    ndt[r] = row_at<T>(a.dt, row, a.ld_dt, at, chc);
+                    ng[r] = row_at<T>(a.gy, row, a.ld_gy, at, chc);
+                    nz[r] = a.z ? row_at<T>(a.z, row, a.ld_z, at, chc) : T(0.0f);
                 }
+#pragma unroll
+                for (int q = 0; q < kStates; ++q) {
+                    const int e = q * kWave + lane, s = e % SP;
+                    const uint32_t at = e / SP < n ? e / SP : n - 1, sc = s < a.states ? s : 0;
+                    nb[q] = row_at<T>(a.B, row, a.ld_B, at, sc);
+                    nc[q] = row_at<T>(a.C, row, a.ld_C, at, sc);
+                    if (s >= a.states) nb[q] = nc[q] = T(0.0f);
+                }
+                const bool inside = t.first + k > 0;
+                const float *from = inside ? a.kept + (row / kTile) * a.states * a.channels : a.init;
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
-                    const float g = only_states<PADDED>(a, part * NS + i, fmaf(C[i], dy, G[i]));
-                    y = fmaf(C[i], h[i], y);
-                    v[i] = g * in;
-                    v[NS + i] = dy * h[i];
-                    sB = fmaf(g, B[i], sB);
-                    G[i] = only_states<PADDED>(a, part * NS + i, g * fast_exp2(step * A2[i]));
-                    const float w = G[i] * before[i];
-                    sA = fmaf(w, A2[i], sA);
-                    dA[i] = fmaf(w, step, dA[i]);
-                    h[i] = before[i];
+                    const int s = part * NS + i;
+                    nh[i] = 0.0f;
+                    if (from && on && s < a.states) nh[i] = from[inside ? (uint32_t)s * a.channels + ch : (t.ray * a.channels + ch) * a.states + s];
                 }
-                sB = sum_parts<P>(sB);
-                sA = sum_parts<P>(sA);
-                const float dstep = fmaf(u, sB, sA * kLn2) * slope;
-                if (a.z) y = add_skip(a, D, u, sum_parts<P>(y));
-                if (part == 0) {
-                    own_rows[kU][j][col] = add_skip(a, D, dy, step * sB);
-                    own_rows[kSlope][j][col] = dstep;
-                    own_rows[kGate][j][col] = gate * y;
-                }
-                dD = fmaf(dy, u, dD);
-                dbias += dstep;
-                sum_over_lanes<2 * NS, CH / 2>(v, lane);
-                if (stores) {
+            };
+            if (tiles > 0) load(tiles - 1);
+            for (int64_t k = tiles - 1; k >= 0; --k) {
+                const int64_t row = row0 + k * kTile;
+                const int n = rows_in(k);
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                    for (int i = 0; i < kLeft; ++i) {
-                        const uint32_t q = i * (1 << kHalvings) + number;
-                        to[(q / NS) * SP + part * NS + q % NS] = EACH > 1 && !first_block ? before_sum[i] + v[i] : v[i];
+                for (int r = 0; r < PR; ++r) {
+                    const int j = part * PR + r;
+                    // lanes without a channel: no input and no gradient, so that they add nothing to dB and dC
+                    const float raw = to_f(ndt[r]) + bias, u = on ? to_f(nu[r]) : 0.0f, gy = on ? to_f(ng[r]) : 0.0f;
+                    Step st = {raw, 1.0f};
+                    if (a.softplus) st = softplus_step(raw);
+                    float dy = gy, gate = 0.0f;
+                    if (a.z) {
+                        const float z = on ? to_f(nz[r]) : 0.0f, sig = sigmoid_f(z);
+                        dy = gy * (z * sig);
+                        gate = gy * (sig * fmaf(z, 1.0f - sig, 1.0f));
+                    }
+                    if (P <= kTile || j < kTile) {
+                        own_rows[kStep][j][col] = on ? st.step : 0.0f;
+                        own_rows[kU][j][col] = u;
+                        own_rows[kSlope][j][col] = st.slope;
+                        own_rows[kDy][j][col] = dy;
+                        own_rows[kGate][j][col] = gate;
                     }
                 }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int r = 0; r < PR; ++r) {
-                const int j = part * PR + r;
-                if (!on || j >= n) continue;
-                const int64_t at = row * a.channels;
-                const uint32_t to = (uint32_t)j * a.channels + ch;
-                (reinterpret_cast<T *>(a.gu) + at)[to] = from_f<T>(own_rows[kU][j][col]);
-                (reinterpret_cast<T *>(a.gdt) + at)[to] = from_f<T>(own_rows[kSlope][j][col]);
-                if (a.z) (reinterpret_cast<T *>(a.gz) + at)[to] = from_f<T>(own_rows[kGate][j][col]);
+                for (int q = 0; q < kStates; ++q) {
+                    const int e = q * kWave + lane;
+                    if (e < kTile * SP) {
+                        bc[0][e] = to_f(nb[q]);
+                        bc[1][e] = to_f(nc[q]);
+                    }
+                }
+                float h[NS], h0[NS];
+#pragma unroll
+                for (int i = 0; i < NS; ++i) h[i] = h0[i] = nh[i];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                if (k > 0) load(k - 1);
+
+                auto states_at = [&](int which, int j, float (&v)[NS]) { read_states<NS>(&bc[which][j * SP + part * NS], v); };
+#pragma unroll 2
+                for (int j = 0; j < n; ++j) {
+                    const float step = own_rows[kStep][j][col], in = step * own_rows[kU][j][col];
+                    float B[NS];
+                    states_at(0, j, B);
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) h[i] = only_states<PADDED>(a, part * NS + i, fmaf(fast_exp2(step * A2[i]), h[i], in * B[i]));
+                    if (j + 1 < n)
+#pragma unroll
+                        for (int i = 0; i < NS; i += 4) hist[j][i / 4][lane] = f32x4{h[i], h[i + 1], h[i + 2], h[i + 3]};
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                for (int j = n - 1; j >= 0; --j) {
+                    const float step = own_rows[kStep][j][col], u = own_rows[kU][j][col], slope = own_rows[kSlope][j][col], dy = own_rows[kDy][j][col],
+                                gate = own_rows[kGate][j][col], in = step * u;
+                    float B[NS], C[NS], before[NS], v[2 * NS], y = 0.0f, sB = 0.0f, sA = 0.0f;
+                    states_at(0, j, B);
+                    states_at(1, j, C);
+                    float *to = a.part_bc + ((int64_t)group * a.rows + row + j) * (2 * SP), before_sum[kLeft];
+                    if (EACH > 1 && !first_block)               // what the blocks before this one left, read early
+#pragma unroll
+                        for (int i = 0; i < kLeft; ++i) {
+                            const uint32_t q = i * (1 << kHalvings) + number;
+                            before_sum[i] = to[(q / NS) * SP + part * NS + q % NS];
+                        }
+#pragma unroll
+                    for (int i = 0; i < NS; i += 4) {
+                        f32x4 q = {h0[i], h0[i + 1], h0[i + 2], h0[i + 3]};
+                        if (j > 0) q = hist[j - 1][i / 4][lane];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) before[i + r] = q[r];
+                    }
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) {
+                        const float g = only_states<PADDED>(a, part * NS + i, fmaf(C[i], dy, G[i]));
+                        y = fmaf(C[i], h[i], y);
+                        v[i] = g * in;
+                        v[NS + i] = dy * h[i];
+                        sB = fmaf(g, B[i], sB);
+                        G[i] = only_states<PADDED>(a, part * NS + i, g * fast_exp2(step * A2[i]));
+                        const float w = G[i] * before[i];
+                        sA = fmaf(w, A2[i], sA);
+                        dA[i] = fmaf(w, step, dA[i]);
+                        h[i] = before[i];
+                    }
+                    sB = sum_parts<P>(sB);
+                    sA = sum_parts<P>(sA);
+                    const float dstep = fmaf(u, sB, sA * kLn2) * slope;
+                    if (a.z) y = add_skip(a, D, u, sum_parts<P>(y));
+                    if (part == 0) {
+                        own_rows[kU][j][col] = add_skip(a, D, dy, step * sB);
+                        own_rows[kSlope][j][col] = dstep;
+                        own_rows[kGate][j][col] = gate * y;
+                    }
+                    dD = fmaf(dy, u, dD);
+                    dbias += dstep;
+                    sum_over_lanes<2 * NS, CH / 2>(v, lane);
+                    if (stores) {
+#pragma unroll
+                        for (int i = 0; i < kLeft; ++i) {
+                            const uint32_t q = i * (1 << kHalvings) + number;
+                            to[(q / NS) * SP + part * NS + q % NS] = EACH > 1 && !first_block ? before_sum[i] + v[i] : v[i];
+                        }
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int r = 0; r < PR; ++r) {
+                    const int j = part * PR + r;
+                    if (!on || j >= n) continue;
+                    const int64_t at = row * a.channels;
+                    const uint32_t to = (uint32_t)j * a.channels + ch;
+                    (reinterpret_cast<T *>(a.gu) + at)[to] = from_f<T>(own_rows[kU][j][col]);
+                    (reinterpret_cast<T *>(a.gdt) + at)[to] = from_f<T>(own_rows[kSlope][j][col]);
+                    if (a.z) (reinterpret_cast<T *>(a.gz) + at)[to] = from_f<T>(own_rows[kGate][j][col]);
+                }
+            }
+            if (a.ginit && t.first == 0) {
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    const int s = part * NS + i;
+                    if (on && s < a.states) a.ginit[(t.ray * a.channels + ch) * a.states + s] = G[i];
+                }
             }
         }
-        if (a.ginit && t.first == 0) {
+        if (!on) continue;
+        float *to = a.part_w + place * ((int64_t)a.channels * (a.states + 2));
 #pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                const int s = part * NS + i;
-                if (on && s < a.states) a.ginit[(t.ray * a.channels + ch) * a.states + s] = G[i];
-            }
+        for (int i = 0; i < NS; ++i) {
+            const int s = part * NS + i;
+            if (s < a.states) to[ch * a.states + s] = dA[i];
         }
-    }
-    if (!on) continue;
-    float *to = a.part_w + place * ((int64_t)a.channels * (a.states + 2));
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        const int s = part * NS + i;
-        if (s < a.states) to[ch * a.states + s] = dA[i];
-    }
-    if (part == 0) {
-        to[(int64_t)a.channels * a.states + ch] = dD;
-        to[(int64_t)a.channels * (a.states + 1) + ch] = dbias;
-    }
+        if (part == 0) {
+            to[(int64_t)a.channels * a.states + ch] = dD;
+            to[(int64_t)a.channels * (a.states + 1) + ch] = dbias;
+        }
     }
 }
 
