@@ -130,21 +130,21 @@ class _CausalConv(torch.autograd.Function):
     def forward(ctx, x, weight, bias, init, rows, n_rays, act, want_final):
         ctx.set_materialize_grads(False)
         out, final = _C.causal_conv_fwd(x, weight, bias, init, *rows, n_rays, act, want_final)
-        ctx.save_for_backward(x, weight, bias, init)
+        ctx.save_for_backward(x, weight, bias, init, *rows)
         learns = ctx.needs_input_grad[:4]
         slope = act > 0 and any(learns)
         ctx.depends = (slope or learns[1], slope or learns[0] or learns[3], slope, slope or learns[1])
-        ctx.rows, ctx.n_rays, ctx.act = rows, n_rays, act
+        ctx.n_rays, ctx.act = n_rays, act
         return out, final
 
     @staticmethod
     @_differentiates_once(lambda ctx: ctx.depends)
     def backward(ctx, gy, gfinal):
-        x, weight, bias, init = ctx.saved_tensors
+        x, weight, bias, init, *rows = ctx.saved_tensors
         need = ctx.needs_input_grad
         if gy is None:
             gy = torch.zeros_like(x)
-        gx, gw, gb, gi = _C.causal_conv_bwd(gy, gfinal, x, weight, bias, init, *ctx.rows, ctx.n_rays, ctx.act, need[0], need[1],
+        gx, gw, gb, gi = _C.causal_conv_bwd(gy, gfinal, x, weight, bias, init, *rows, ctx.n_rays, ctx.act, need[0], need[1],
                                             bias is not None and need[2], init is not None and need[3])
         return gx, gw, gb, gi, None, None, None, None
 
@@ -247,19 +247,19 @@ class _SelectiveScan(torch.autograd.Function):
     def forward(ctx, u, delta, gate, B, C, A, D, bias, init, rows, n_rays, softplus, want_final):
         ctx.set_materialize_grads(False)
         out, final, kept = _C.selective_scan_fwd(u, delta, gate, B, C, A, D, bias, init, *rows, n_rays, softplus, want_final, True)
-        ctx.save_for_backward(u, delta, gate, B, C, A, D, bias, init, kept)
+        ctx.save_for_backward(u, delta, gate, B, C, A, D, bias, init, kept, *rows)
         # outputs are linear in u, B, C, D and the initial state, each by itself
         ctx.depends = tuple(any(l and (j != i or i in (1, 2, 5, 7)) for j, l in enumerate(ctx.needs_input_grad[:9])) for i in range(9))
-        ctx.rows, ctx.n_rays, ctx.softplus = rows, n_rays, softplus
+        ctx.n_rays, ctx.softplus = n_rays, softplus
         return out, final
 
     @staticmethod
     @_differentiates_once(lambda ctx: ctx.depends)
     def backward(ctx, gy, gfinal):
-        u, delta, gate, B, C, A, D, bias, init, kept = ctx.saved_tensors
+        u, delta, gate, B, C, A, D, bias, init, kept, *rows = ctx.saved_tensors
         if gy is None:
             gy = torch.zeros_like(u)
-        grads = _C.selective_scan_bwd(gy, gfinal, u, delta, gate, B, C, A, D, bias, init, kept, *ctx.rows, ctx.n_rays, ctx.softplus)
+        grads = _C.selective_scan_bwd(gy, gfinal, u, delta, gate, B, C, A, D, bias, init, kept, *rows, ctx.n_rays, ctx.softplus)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None, None)
 
 

@@ -156,6 +156,22 @@ def test_a_penalty_on_the_gradient_is_refused(python, monkeypatch):
                 g.square().sum().backward(retain_graph=True)
 
 
+@pytest.mark.parametrize("python", [False, True])
+def test_packed_info_changed_between_the_passes_is_noticed(python, monkeypatch):
+    import nerfacc_amd as nerfacc
+    from nerfacc_amd import dense
+
+    if python:
+        monkeypatch.setattr(dense, "_EXT", False)
+    for call, kw in ((nerfacc.causal_conv, conv_arguments()), (nerfacc.selective_scan, scan_arguments())):
+        kw = {k: v[0] if v.dim() == 3 and k != "initial_state" else v for k, v in kw.items()}
+        x, info = kw.pop("inputs").requires_grad_(True), torch.tensor([[0, 6]], device=DEV)
+        out = call(x, packed_info=info, **kw)
+        info[0, 1] = 3
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+
+
 # --------------------------------------------------------------------------------------------------------------- workspaces
 @pytest.mark.parametrize("states,channels", [(100, 70), (256, 70), (256, 33), (129, 129)])
 @pytest.mark.parametrize("lens", [[9, 0, 11], [130, 1, 200]])
