@@ -1933,17 +1933,27 @@ std::tuple<Tensor, OptTensor> causal_conv(const Tensor &x_, const Tensor &w, con
     return {x_.dim() == 2 ? out : out.view(x_.sizes()), last};
 }
 
-// where a step leaves its new state: `state` itself, or a buffer that shares no memory with it
-Tensor state_buffer(const char *op, const Tensor &state, const OptTensor &to_) {
+// whether two tensors share memory, by the spans between their first and last element
+bool overlaps(const Tensor &s, const Tensor &t) {
+    if (s.numel() == 0 || t.numel() == 0) return false;
+    auto span = [](const Tensor &x) {
+        int64_t reach = 1;
+        for (int64_t i = 0; i < x.dim(); ++i) reach += (x.size(i) - 1) * x.stride(i);
+        const char *at = (const char *)x.data_ptr();
+        return std::pair<const char *, const char *>(at, at + reach * x.element_size());
+    };
+    const auto a = span(s), b = span(t);
+    return a.first < b.second && b.first < a.second;
+}
+// where a step leaves its new state: `state` itself, or a buffer that shares no memory with it; nor with what the step reads beside it, in
+// whatever order its workgroups run
+Tensor state_buffer(const char *op, const Tensor &state, const OptTensor &to_, std::initializer_list<std::pair<const char *, OptTensor>> inputs) {
     const Tensor to = get(to_);
     if (!to.defined()) return at::empty(state.sizes(), state.options());
     TORCH_CHECK_VALUE(to.is_contiguous(), op, ": out_state must be contiguous");
-    if (state.numel() > 0 && !(to.data_ptr() == state.data_ptr() && state.is_contiguous())) {
-        int64_t reach = 1;
-        for (int64_t i = 0; i < state.dim(); ++i) reach += (state.size(i) - 1) * state.stride(i);
-        const char *a = (const char *)state.data_ptr(), *b = a + reach * state.element_size(), *c = (const char *)to.data_ptr(), *d = c + to.nbytes();
-        TORCH_CHECK_VALUE(!(a < d && c < b), op, ": out_state overlaps state; pass state itself to update it in place");
-    }
+    if (!(to.data_ptr() == state.data_ptr() && state.is_contiguous()))
+        TORCH_CHECK_VALUE(!overlaps(state, to), op, ": out_state overlaps state; pass state itself to update it in place");
+    for (auto &p : inputs) TORCH_CHECK_VALUE(!(p.second && p.second->defined() && overlaps(*p.second, to)), op, ": out_state overlaps ", p.first);
     return to;
 }
 void refuse_grad(const char *op, const char *other, std::initializer_list<OptTensor> tensors) {
@@ -1967,7 +1977,7 @@ std::tuple<Tensor, Tensor> causal_conv_one(const Tensor &x, const Tensor &state,
     check_like("causal_conv_step", "bias", get(b), x, {d}, dt);
     check_like("causal_conv_step", "out_state", get(to_), x, {r, width - 1, d}, dt);
     refuse_grad("causal_conv_step", "causal_conv", {x, state, w, b, to_});
-    const Tensor to = state_buffer("causal_conv_step", state, to_);
+    const Tensor to = state_buffer("causal_conv_step", state, to_, {{"inputs", x}, {"weight", w}, {"bias", b}});
     const Tensor out = causal_conv_step(x, state, w, some(get(b)), act, to);
     written(to_);
     return {out, to};
@@ -2062,7 +2072,8 @@ std::tuple<Tensor, Tensor> selective_scan_one(const Tensor &x, const Tensor &dt,
     check_like("selective_scan_step", "state", state, x, {r, d, s}, at::kFloat);
     check_like("selective_scan_step", "out_state", get(to_), x, {r, d, s}, at::kFloat);
     refuse_grad("selective_scan_step", "selective_scan", {x, dt, A, B, C, D, z, bias, state, to_});
-    const Tensor to = state_buffer("selective_scan_step", state, to_);
+    const Tensor to = state_buffer("selective_scan_step", state, to_,
+                                   {{"inputs", x}, {"delta", dt}, {"A", A}, {"B", B}, {"C", C}, {"D", D}, {"gate", z}, {"delta_bias", bias}});
     const Tensor out = selective_scan_step(x, dt, some(get(z)), B, C, A, some(get(D)), some(get(bias)), state, softplus, to);
     written(to_);
     return {out, to};

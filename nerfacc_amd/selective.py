@@ -59,17 +59,27 @@ def _flat(t: Optional[Tensor]) -> Optional[Tensor]:
     return t if t is None or t.dim() == 2 else t.reshape(-1, t.shape[-1])
 
 
-def _state_buffer(name: str, state: Tensor, out_state: Optional[Tensor]) -> Tensor:
-    """where a step leaves its new state: `state` itself, or a buffer that shares no memory with it"""
+def _overlaps(s: Tensor, t: Tensor) -> bool:
+    """whether two tensors share memory, by the spans between their first and last element"""
+    if s.numel() == 0 or t.numel() == 0:
+        return False
+    span = lambda x: (x.data_ptr(), x.data_ptr() + (1 + sum((n - 1) * k for n, k in zip(x.shape, x.stride()))) * x.element_size())  # noqa: E731
+    (a, b), (c, d) = span(s), span(t)
+    return a < d and c < b
+
+
+def _state_buffer(name: str, state: Tensor, out_state: Optional[Tensor], **inputs) -> Tensor:
+    """where a step leaves its new state: `state` itself, or a buffer that shares no memory with it; nor with what the step reads beside it, in
+    whatever order its workgroups run"""
     if out_state is None:
         return torch.empty_like(state, memory_format=torch.contiguous_format)
     if not out_state.is_contiguous():
         raise ValueError(f"{name}: out_state must be contiguous")
-    if out_state.data_ptr() != state.data_ptr() or not state.is_contiguous():
-        span = lambda t: (t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size())  # noqa: E731
-        (a, b), (c, d) = span(state), span(out_state)
-        if state.numel() and a < d and c < b:
-            raise ValueError(f"{name}: out_state overlaps state; pass state itself to update it in place")
+    if (out_state.data_ptr() != state.data_ptr() or not state.is_contiguous()) and _overlaps(state, out_state):
+        raise ValueError(f"{name}: out_state overlaps state; pass state itself to update it in place")
+    for what, t in inputs.items():
+        if t is not None and _overlaps(t, out_state):
+            raise ValueError(f"{name}: out_state overlaps {what}")
     return out_state
 
 
@@ -152,7 +162,8 @@ class _CausalConv(torch.autograd.Function):
 def causal_conv_step(inputs: Tensor, state: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None,
                      out_state: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
     """One more sample of every ray: `inputs` (n_rays, channels) and the rays' state (n_rays, width - 1, channels) -> (outputs, new
-    state).  The new state goes to `out_state` if given (`out_state=state` updates it in place).  Not differentiable.
+    state).  The new state goes to `out_state` if given (`out_state=state` updates it in place; it shares no memory with the other tensors).
+    Not differentiable.
 
         >>> causal_conv_step(torch.tensor([[3.]], device="cuda"), torch.tensor([[[2.]]], device="cuda"), torch.tensor([[1., 10.]], device="cuda"))
         (tensor([[32.]], device='cuda:0'), tensor([[[3.]]], device='cuda:0'))
@@ -172,7 +183,7 @@ def causal_conv_step(inputs: Tensor, state: Tensor, weight: Tensor, bias: Option
     _check_native("causal_conv_step", inputs, (("state", state, shape, dt), ("weight", weight, (channels, width), dt),
                                                ("bias", bias, (channels,), dt), ("out_state", out_state, shape, dt)))
     _refuse_grad("causal_conv_step", "causal_conv", inputs, state, weight, bias, out_state)
-    to = _state_buffer("causal_conv_step", state, out_state)
+    to = _state_buffer("causal_conv_step", state, out_state, inputs=inputs, weight=weight, bias=bias)
     out = _C.causal_conv_step(inputs, state, weight, bias, act, to)
     _written(out_state)
     return out, to
@@ -268,7 +279,7 @@ def selective_scan_step(inputs: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: 
                         out_state: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
     """One more sample of every ray: inputs, delta, gate (n_rays, channels), B, C (n_rays, states) and the rays' state (n_rays, channels,
     states) float32 -> (outputs, new state), as `selective_scan` of one row each.  The new state goes to `out_state` if given
-    (`out_state=state` updates it in place).  Not differentiable."""
+    (`out_state=state` updates it in place; it shares no memory with the other tensors).  Not differentiable."""
     ext = _ext()
     if ext:
         return ext.selective_scan_one(inputs, delta, A, B, C, state, D, gate, delta_bias, bool(delta_softplus), out_state)
@@ -282,7 +293,7 @@ def selective_scan_step(inputs: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: 
     _check_scan("selective_scan_step", inputs, (n_rays,), channels, n_rays, delta, A, B, C, D, gate, delta_bias,
                 (("state", state, shape, torch.float32), ("out_state", out_state, shape, torch.float32)))
     _refuse_grad("selective_scan_step", "selective_scan", inputs, delta, A, B, C, D, gate, delta_bias, state, out_state)
-    to = _state_buffer("selective_scan_step", state, out_state)
+    to = _state_buffer("selective_scan_step", state, out_state, inputs=inputs, delta=delta, A=A, B=B, C=C, D=D, gate=gate, delta_bias=delta_bias)
     out = _C.selective_scan_step(inputs, delta, gate, B, C, A, D, delta_bias, state, bool(delta_softplus), to)
     _written(out_state)
     return out, to

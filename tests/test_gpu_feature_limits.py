@@ -172,6 +172,29 @@ def test_packed_info_changed_between_the_passes_is_noticed(python, monkeypatch):
             out.sum().backward()
 
 
+# ------------------------------------------------------------------------------------------------------------------- steps
+@pytest.mark.parametrize("python", [False, True])
+def test_steps_refuse_a_state_that_would_overwrite_their_inputs(python, monkeypatch):
+    import nerfacc_amd as nerfacc
+    from nerfacc_amd import dense
+
+    if python:
+        monkeypatch.setattr(dense, "_EXT", False)
+    pool = normal(4, 3, 8)
+    with pytest.raises(ValueError, match="overlaps"):
+        nerfacc.causal_conv_step(pool[2:, 0], pool[:2].clone(), normal(8, 4), out_state=pool[2:])
+    with pytest.raises(ValueError, match="overlaps"):
+        nerfacc.causal_conv_step(normal(2, 8), pool[:2], pool.view(-1)[4:36].view(8, 4), out_state=pool[:2])
+    pool, A, bc, x = normal(6, 8, 4), normal(8, 4), normal(2, 4), normal(2, 8)
+    flat = pool.view(-1)
+    for kw in (dict(inputs=flat[8:24].view(2, 8)), dict(delta=flat[:16].view(2, 8)), dict(B=flat[60:68].view(2, 4)), dict(C=flat[:8].view(2, 4)),
+               dict(A=flat[32:64].view(8, 4)), dict(D=flat[:8]), dict(gate=flat[40:56].view(2, 8)), dict(delta_bias=flat[56:64])):
+        with pytest.raises(ValueError, match="overlaps"):
+            nerfacc.selective_scan_step(**{**dict(inputs=x, delta=x, A=A, B=bc, C=bc, state=pool[:2]), **kw}, out_state=pool[:2])
+    # neighbours that share no memory are fine
+    nerfacc.selective_scan_step(flat[64:80].view(2, 8), x, A, bc, bc, pool[:2], out_state=pool[:2])
+
+
 # --------------------------------------------------------------------------------------------------------------- workspaces
 @pytest.mark.parametrize("states,channels", [(100, 70), (256, 70), (256, 33), (129, 129)])
 @pytest.mark.parametrize("lens", [[9, 0, 11], [130, 1, 200]])
