@@ -1120,8 +1120,9 @@ class _CtypesC:
     # -- feature operators ---------------------------------------------------------------------------------------------
     @staticmethod
     def foreign_nodes(tensors) -> int:
-        """(the extension counts autograd nodes of other streams; Python cannot ask a node for its stream)"""
-        return 0
+        """how many of the tensors' autograd nodes may belong to another stream: the extension counts those that do, Python cannot ask a node
+        for its stream, so that every tensor that requires gradients counts"""
+        return sum(t is not None and t.requires_grad for t in tensors)
 
     @staticmethod
     def linear_fwd(x, w, b, r, act: int, save: bool):

@@ -54,13 +54,20 @@ def _refuse_forward(name: str, *tensors) -> None:
         raise NotImplementedError(f"{name}: forward mode derivatives are not implemented")
 
 
+def _capturing(tensors) -> bool:
+    """whether the current stream of the tensors' device is being captured into a graph"""
+    with torch.cuda.device(next(t.device for t in tensors if t is not None)):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _records_grad(name: str, *tensors) -> bool:
-    """whether autograd records the call; refuses one whose captured backward pass would end the process"""
+    """whether autograd records the call; refuses one whose captured backward pass would end the process, or (without the extension, which
+    alone can tell) might"""
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)):
         return False
-    if torch.cuda.is_current_stream_capturing() and _C.foreign_nodes(tensors):
-        raise RuntimeError(f"{name}: captured into a graph while an eager autograd graph of the same tensors lives (its backward pass "
-                           "could not be captured): drop the eager outputs first, or call under torch.no_grad()")
+    if _capturing(tensors) and _C.foreign_nodes(tensors):
+        raise RuntimeError(f"{name}: captured into a graph while an eager autograd graph of the same tensors lives, or may live without the torch "
+                           "extension to tell (its backward pass could not be captured): drop the eager outputs first, or call under torch.no_grad()")
     return True
 
 

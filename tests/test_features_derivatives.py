@@ -41,3 +41,19 @@ def test_forward_mode_is_refused(face):
                     call(**kw)                                           # without a tangent the call goes on, to the device's refusal
                 with fwd._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="no CPU kernels"):
                     call(**dual)                                         # and with tangents switched off
+
+
+def test_a_captured_training_step_needs_the_extension(monkeypatch):
+    """a capture beside an eager graph of the same leaves ends the process; the ctypes face cannot tell whether there is one"""
+    from nerfacc_amd import dense
+
+    x, w = torch.rand(2, 8), torch.rand(3, 8, requires_grad=True)
+    monkeypatch.setattr(dense._C, "foreign_nodes", _backend._CtypesC.foreign_nodes)
+    monkeypatch.setattr(dense, "_capturing", lambda tensors: True)
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        dense._records_grad("linear", x, w, None)
+    assert not dense._records_grad("linear", x, w.detach(), None)
+    with torch.no_grad():
+        assert not dense._records_grad("linear", x, w, None)
+    monkeypatch.setattr(dense, "_capturing", lambda tensors: False)
+    assert dense._records_grad("linear", x, w, None)
