@@ -449,7 +449,7 @@ int nfa_pdf_loss_bwd(const float *g_loss, const int32_t *ids_left, const int32_t
 /* ---------------------------------------------------------------------------------------
  * Feature operators: what turns samples into features between sampling and rendering.  No reference counterpart (the reference
  * leaves fields to its examples).  Element types: NFA_DTYPE_*; every sum, statistic and state is held in 32 bits, outputs are
- * rounded once.  Row strides are in elements; rows are contiguous inside.
+ * rounded once.  Row strides are in elements; rows are contiguous inside.  Gradients of calls without rows are written too: zeros.
  * ------------------------------------------------------------------------------------- */
 #define NFA_DTYPE_F32 0
 #define NFA_DTYPE_BF16 1

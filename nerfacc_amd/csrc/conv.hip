@@ -586,6 +586,11 @@ NFA_EXPORT int nfa_causal_conv_bwd(const nfa_causal_conv_args *a, void *grad_inp
     if (a->channels % vec || !fits(d.x, d.ld_x, bytes, vec) || !fits(d.gy, d.ld_gy, bytes, vec) || !fits(grad_inputs, 0, bytes, vec) ||
         !fits(d.init, 0, bytes, vec) || !fits(d.gfinal, 0, bytes, vec))
         vec = 1;
+    if (a->rows == 0) {
+        launch_zero(grad_weight, (int64_t)a->channels * a->width, a->dtype, s);
+        launch_zero(grad_bias, a->channels, a->dtype, s);
+        if (int rc = check_launch("zero_kernel")) return rc;
+    }
     if (a->rows > 0 && (grad_inputs || grad_weight || grad_bias)) {
         const ConvPlan p = conv_plan(a->rows, a->channels, vec, true);
         NFA_REQUIRE(p.blocks_x < kMaxThreads / kBlock && p.blocks_y < 65536, "causal_conv_bwd: too large for one launch");

@@ -1160,6 +1160,14 @@ bool keeps_slopes(int32_t dtype, int32_t act) { return dtype == NFA_DTYPE_F16 &&
 
 }  // namespace
 
+__global__ __launch_bounds__(kBlock) void zero_kernel(uint16_t *p, int64_t n) {
+    for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < n; e += (int64_t)gridDim.x * kBlock) p[e] = 0;
+}
+void launch_zero(void *p, int64_t n, int32_t dtype, hipStream_t s) {
+    n *= dtype_bytes(dtype) / 2;
+    if (p && n > 0) hipLaunchKernelGGL(zero_kernel, dim3(blocks_for(n)), dim3(kBlock), 0, s, (uint16_t *)p, n);
+}
+
 void launch_reduce_rows(float *part, int64_t rows, std::initializer_list<std::pair<void *, int64_t>> outputs, int32_t dtype, hipStream_t s) {
     Outputs o{};
     int64_t cols = 0, k = 0;
@@ -1246,7 +1254,11 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
                               void *workspace, void *stream) {
     if (int rc = check_linear(a, "linear_bwd")) return rc;
     hipStream_t s = (hipStream_t)stream;
-    if (a->rows == 0) return NFA_OK;
+    if (a->rows == 0) {
+        launch_zero(grad_weight, (int64_t)a->out_features * a->in_features, a->dtype, s);
+        launch_zero(grad_bias, a->out_features, a->dtype, s);
+        return check_launch("zero_kernel");
+    }
     NFA_REQUIRE(a->grad_outputs, "linear_bwd: NULL pointer");
     NFA_REQUIRE(a->grad_outputs_stride >= a->out_features || a->rows == 1, "linear_bwd: grad_outputs_stride < out_features");
     NFA_REQUIRE(saved || a->activation == NFA_ACT_NONE, "linear_bwd: the activation needs what the forward call saved");

@@ -114,4 +114,7 @@ inline bool act_ok(int32_t act) { return act >= NFA_ACT_NONE && act <= NFA_ACT_E
 // go to up to three outputs (pointer or nullptr, columns), one behind the other.  part is written to.
 void launch_reduce_rows(float *part, int64_t rows, std::initializer_list<std::pair<void *, int64_t>> outputs, int32_t dtype, hipStream_t s);
 
+// n numbers of a type (pointer or nullptr): zeros, where a gradient has no rows to be summed over
+void launch_zero(void *p, int64_t n, int32_t dtype, hipStream_t s);
+
 }  // namespace nfa

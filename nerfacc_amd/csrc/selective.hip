@@ -711,6 +711,11 @@ __global__ __launch_bounds__(kBlock) void zero_rows_kernel(const int32_t *__rest
     }
 }
 
+// a state's gradient without rows: that of the final state (nullptr: zeros)
+__global__ __launch_bounds__(kBlock) void copy_state_kernel(const float *from, float *to, int64_t n) {
+    for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < n; e += (int64_t)gridDim.x * kBlock) to[e] = from ? from[e] : 0.0f;
+}
+
 // One row per sequence: reading and writing the state bounds it (8 bytes per state).  L lanes share a channel, each with four
 // neighbouring states (one 16-byte access); L = 0: a lane per channel and states one by one, for numbers of states that do not divide.
 // 256 x 1024 x 16, bf16: 8.2 us (4.3 TB/s), 39.5 with states one by one.
@@ -958,11 +963,20 @@ NFA_EXPORT int nfa_selective_scan_fwd(const nfa_selective_scan_args *a, void *ou
 NFA_EXPORT int nfa_selective_scan_bwd(const nfa_selective_scan_args *a, const float *checkpoints, const nfa_selective_scan_grads *g,
                                       void *workspace, void *stream) {
     if (int rc = check_scan(a, "selective_scan_bwd", false)) return rc;
-    if (a->rows == 0 || a->n_rays == 0) return NFA_OK;
-    NFA_REQUIRE(g && g->inputs && g->delta && g->B && g->C && g->A && a->grad_outputs && checkpoints && workspace, "selective_scan_bwd: NULL pointer");
-    NFA_REQUIRE(!a->gate || g->gate, "selective_scan_bwd: NULL pointer");
-    NFA_REQUIRE(a->grad_outputs_stride >= a->channels || a->rows <= 1, "selective_scan_bwd: grad_outputs_stride < channels");
+    NFA_REQUIRE(g && g->A && (a->rows == 0 || (g->inputs && g->delta && g->B && g->C && (!a->gate || g->gate))), "selective_scan_bwd: NULL pointer");
     hipStream_t s = (hipStream_t)stream;
+    if (a->rows == 0 || a->n_rays == 0) {                   // no row of a sequence: zeros, and the final state's gradient as it came
+        for (void *p : {g->inputs, g->delta, g->gate}) launch_zero(p, a->rows * a->channels, a->dtype, s);
+        for (void *p : {g->B, g->C}) launch_zero(p, a->rows * a->states, a->dtype, s);
+        launch_zero(g->A, (int64_t)a->channels * a->states, NFA_DTYPE_F32, s);
+        for (float *p : {g->D, g->delta_bias}) launch_zero(p, a->channels, NFA_DTYPE_F32, s);
+        const int64_t n = a->n_rays * a->channels * a->states;
+        if (g->initial_state && n > 0)
+            hipLaunchKernelGGL(copy_state_kernel, dim3(blocks_for(n)), dim3(kBlock), 0, s, a->grad_final_state, g->initial_state, n);
+        return check_launch("copy_state_kernel");
+    }
+    NFA_REQUIRE(a->grad_outputs && checkpoints && workspace, "selective_scan_bwd: NULL pointer");
+    NFA_REQUIRE(a->grad_outputs_stride >= a->channels || a->rows <= 1, "selective_scan_bwd: grad_outputs_stride < channels");
     ScanArgs d = scan_args(a);
     const ScanPlan p = scan_plan(a->n_rays, a->rows, a->channels, a->states, a->packed_info != nullptr, true);
     const ScanSpace sp = scan_space(p, a->rows, a->channels, a->states, true);

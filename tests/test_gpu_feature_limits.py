@@ -195,6 +195,47 @@ def test_steps_refuse_a_state_that_would_overwrite_their_inputs(python, monkeypa
     nerfacc.selective_scan_step(flat[64:80].view(2, 8), x, A, bc, bc, pool[:2], out_state=pool[:2])
 
 
+# ---------------------------------------------------------------------------------------------------------------- C entries
+def test_gradients_of_calls_without_rows_are_written():
+    """zeros, and the final state's gradient for the initial one"""
+    import ctypes
+
+    from nerfacc_amd.cuda import _backend
+
+    L, S, stream = _backend.load_library(), _backend._STRUCTS, torch.cuda.current_stream().cuda_stream
+    dirty = lambda *shape, dtype=torch.float32: torch.full(shape, 7.0, device=DEV, dtype=dtype)  # noqa: E731
+    for code, dt in enumerate((torch.float32, torch.bfloat16, torch.float16)):
+        w, gw, gb = normal(5, 3).to(dt), dirty(5, 3, dtype=dt), dirty(5, dtype=dt)
+        a = S["nfa_linear_args"](rows=0, in_features=3, out_features=5, dtype=code, activation=1, weight=w.data_ptr())
+        a.grad_outputs = a.inputs = w.data_ptr()
+        assert L.nfa_linear_bwd(ctypes.byref(a), w.data_ptr(), None, gw.data_ptr(), gb.data_ptr(), w.data_ptr(), stream) == 0
+        assert not gw.any() and not gb.any()
+        w, gw, gb, gi, gf, init = normal(5, 4).to(dt), dirty(5, 4, dtype=dt), dirty(5, dtype=dt), dirty(2, 3, 5, dtype=dt), normal(2, 3, 5).to(dt), normal(2, 3, 5).to(dt)
+        a = S["nfa_causal_conv_args"](n_rays=2, rows=0, channels=5, width=4, dtype=code, weight=w.data_ptr(), initial_state=init.data_ptr(),
+                                      grad_final_state=gf.data_ptr())
+        assert L.nfa_causal_conv_bwd(ctypes.byref(a), None, gw.data_ptr(), gb.data_ptr(), gi.data_ptr(), None, stream) == 0
+        assert not gw.any() and not gb.any() and torch.equal(gi, gf)
+        for rays, rows, final in ((2, 0, True), (2, 0, False), (0, 6, False)):
+            A, init, gf, info = normal(5, 4), normal(2, 5, 4), normal(2, 5, 4), torch.zeros(1, 2, dtype=torch.int64, device=DEV)
+            x, bc, pos = normal(6, 5).to(dt), normal(6, 4).to(dt), torch.full((6,), -1, dtype=torch.int32, device=DEV)
+            g = dict(inputs=dirty(6, 5, dtype=dt), delta=dirty(6, 5, dtype=dt), gate=dirty(6, 5, dtype=dt), B=dirty(6, 4, dtype=dt), C=dirty(6, 4, dtype=dt),
+                     A=dirty(5, 4), D=dirty(5), delta_bias=dirty(5), initial_state=dirty(2, 5, 4))
+            a = S["nfa_selective_scan_args"](n_rays=rays, rows=rows, channels=5, states=4, dtype=code, A=A.data_ptr(), D=A.data_ptr(), delta_bias=A.data_ptr(),
+                                             inputs=x.data_ptr(), delta=x.data_ptr(), gate=x.data_ptr(), B=bc.data_ptr(), C=bc.data_ptr(), inputs_stride=5,
+                                             delta_stride=5, gate_stride=5, B_stride=4, C_stride=4, initial_state=init.data_ptr(), packed_info=info.data_ptr(),
+                                             row_ray=pos.data_ptr(), row_pos=pos.data_ptr(), grad_final_state=gf.data_ptr() if final else None)
+            gr = S["nfa_selective_scan_grads"](**{k: v.data_ptr() for k, v in g.items()})
+            assert L.nfa_selective_scan_bwd(ctypes.byref(a), None, ctypes.byref(gr), None, stream) == 0
+            torch.cuda.synchronize()
+            for k, v in g.items():
+                if k == "initial_state":
+                    assert torch.equal(v, gf) if final else (not v.any() if rays else v.eq(7).all())
+                elif k in ("A", "D", "delta_bias"):
+                    assert not v.any(), k
+                else:
+                    assert not v[:rows].any() and v[rows:].eq(7).all(), k
+
+
 # --------------------------------------------------------------------------------------------------------------- workspaces
 @pytest.mark.parametrize("states,channels", [(100, 70), (256, 70), (256, 33), (129, 129)])
 @pytest.mark.parametrize("lens", [[9, 0, 11], [130, 1, 200]])
