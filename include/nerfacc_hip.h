@@ -504,7 +504,7 @@ int nfa_ray_order(const int64_t *packed_info, int64_t n_rays, int64_t rows, int3
 
 /* Short causal convolution along each sequence, channel by channel:
  *   z[t] = bias + sum_j weight[:, j] x[t - width + 1 + j],  outputs = act(z);  rows before the first come from initial_state (zeros
- *   without one).  activation: NFA_ACT_NONE or NFA_ACT_SILU.  width: 2 .. 4.
+ *   without one).  activation: NFA_ACT_NONE or NFA_ACT_SILU.  width: 2 .. 4; up to 2^23 channels.
  * nfa_causal_conv_fwd   outputs [rows, channels] contiguous; final_state (nullable) [n_rays, width - 1, channels]: the last width - 1
  *                       inputs of each sequence, its initial state in front where it is shorter.
  * nfa_causal_conv_bwd   grad_outputs, grad_final_state (nullable) -> grad_inputs, grad_weight, grad_bias, grad_initial_state (each
@@ -537,7 +537,7 @@ int nfa_causal_conv_step(const nfa_causal_conv_args *args, const void *state, vo
  *   step = delta (+ delta_bias), softplus of it if delta_softplus;   h[t] = exp(step A) h[t - 1] + step B[t] u[t]    (channels x states)
  *   y[t] = C[t] . h[t] + D u[t],   outputs = y (gate == NULL) or y silu(gate)
  * h before the first row comes from initial_state (zeros without one).  inputs (u), delta, gate, B, C, outputs: dtype; A, D, delta_bias
- * and states: float.  states: 1 .. NFA_SCAN_MAX_STATES.
+ * and states: float.  states: 1 .. NFA_SCAN_MAX_STATES; up to 2^23 channels.
  * nfa_selective_scan_fwd   outputs [rows, channels] contiguous; final_state (nullable) [n_rays, channels, states]; checkpoints
  *                          (nullable unless a backward pass follows): nfa_selective_scan_checkpoint_bytes(...).
  *                          workspace: nfa_selective_scan_workspace_bytes(..., 0), may be 0 bytes.

@@ -500,7 +500,7 @@ NFA_EXPORT int nfa_ray_order(const int64_t *packed_info, int64_t n_rays, int64_t
 
 static int check_conv(const nfa_causal_conv_args *a, const char *who, bool step) {
     NFA_REQUIRE(a, "%s: NULL arguments", who);
-    NFA_REQUIRE(a->n_rays >= 0 && a->rows >= 0 && a->channels >= 1, "%s: bad size", who);
+    NFA_REQUIRE(a->n_rays >= 0 && a->rows >= 0 && a->channels >= 1 && a->channels <= (1 << 23), "%s: bad size", who);
     NFA_REQUIRE(a->width >= 2 && a->width <= 4, "%s: width must be 2, 3 or 4, got %d", who, a->width);
     NFA_REQUIRE(dtype_ok(a->dtype), "%s: bad dtype %d", who, a->dtype);
     NFA_REQUIRE(a->activation == NFA_ACT_NONE || a->activation == NFA_ACT_SILU, "%s: bad activation %d", who, a->activation);

@@ -1412,6 +1412,12 @@ inline int32_t dtype_of(const Tensor &t) {
     return NFA_DTYPE_F16;
 }
 
+// a number of features, channels or states for the C ABI, never cut off
+inline int32_t i32(int64_t v) {
+    TORCH_CHECK(v >= 0 && v < (1ll << 31), "nerfacc_amd: a size of ", v, " is over 2^31 - 1");
+    return (int32_t)v;
+}
+
 // a [rows, cols] tensor whose rows are contiguous and do not overlap, at any row stride up to 2^25; copied if it is not one
 inline Tensor as_rows(const Tensor &t, const char *name, int64_t rows, int64_t cols, const Tensor &like) {
     TORCH_CHECK(t.defined() && t.is_cuda(), name, " must be a CUDA/HIP tensor (nerfacc_amd has no CPU kernels)");
@@ -1466,10 +1472,10 @@ std::tuple<Tensor, OptTensor> linear_fwd(const Tensor &x_, const Tensor &w_, con
     if (r_ && r_->defined()) r = as_rows(*r_, "residual", m, n, x_);
     Guard g(device_of(x_));
     Tensor out = at::empty({m, n}, x_.options()), saved;
-    if (const int64_t bytes = save ? nfa_linear_saved_bytes(m, (int32_t)n, dtype_of(x), (int32_t)act, r.defined()) : 0; bytes > 0)
+    if (const int64_t bytes = save ? nfa_linear_saved_bytes(m, i32(n), dtype_of(x), (int32_t)act, r.defined()) : 0; bytes > 0)
         saved = at::empty({bytes}, opts(x, at::kByte));
     nfa_linear_args a{};
-    a.rows = m; a.in_features = (int32_t)k; a.out_features = (int32_t)n;
+    a.rows = m; a.in_features = i32(k); a.out_features = i32(n);
     a.dtype = dtype_of(x); a.activation = (int32_t)act;
     a.inputs = x.data_ptr(); a.inputs_stride = row_stride(x);
     a.weight = w.data_ptr(); a.bias = ptr<void>(b);
@@ -1487,7 +1493,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_bwd(const Tensor &g_, const T
     OptTensor saved;                            // what linear_fwd kept, or its outputs
     if (act != NFA_ACT_NONE && m > 0) {
         TORCH_CHECK(saved_ && saved_->defined() && saved_->is_cuda() && saved_->device() == x.device() && saved_->is_contiguous(), "linear: saved is missing");
-        const int64_t kept = nfa_linear_saved_bytes(m, (int32_t)n, dtype_of(x), (int32_t)act, 0);
+        const int64_t kept = nfa_linear_saved_bytes(m, i32(n), dtype_of(x), (int32_t)act, 0);
         TORCH_CHECK((int64_t)saved_->nbytes() == (kept ? kept : m * n * (int64_t)x.element_size()), "linear: saved differs in size");
         saved = saved_;
     }
@@ -1502,13 +1508,13 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_bwd(const Tensor &g_, const T
     if (need_w) gw = at::empty({n, k}, x_.options());
     if (need_b) gb = at::empty({n}, x_.options());
     nfa_linear_args a{};
-    a.rows = m; a.in_features = (int32_t)k; a.out_features = (int32_t)n;
+    a.rows = m; a.in_features = i32(k); a.out_features = i32(n);
     a.dtype = dtype_of(x); a.activation = (int32_t)act;
     a.inputs = x.data_ptr(); a.inputs_stride = row_stride(x);
     a.weight = w.data_ptr();
     a.grad_outputs = gy.data_ptr(); a.grad_outputs_stride = row_stride(gy);
     Tensor ws;
-    if (need_w || need_b) ws = at::empty({nfa_linear_bwd_workspace_bytes(m, (int32_t)k, (int32_t)n, a.dtype, a.activation)}, opts(x, at::kByte));
+    if (need_w || need_b) ws = at::empty({nfa_linear_bwd_workspace_bytes(m, i32(k), i32(n), a.dtype, a.activation)}, opts(x, at::kByte));
     check_rc(nfa_linear_bwd(&a, ptr<void>(saved), ptr<void>(gx), ptr<void>(gw), ptr<void>(gb), ptr<void>(ws), stream_of(x)));
     return {some(gx), some(gw), some(gb)};
 }
@@ -1565,7 +1571,7 @@ std::tuple<Tensor, OptTensor> causal_conv_fwd(const Tensor &x_, const Tensor &w_
     if (n_rays == 0) return {out.zero_(), some(last)};
     nfa_causal_conv_args a{};
     seq.into(a);
-    a.rows = n; a.channels = (int32_t)d; a.width = (int32_t)width; a.dtype = dtype_of(x); a.activation = (int32_t)act;
+    a.rows = n; a.channels = i32(d); a.width = i32(width); a.dtype = dtype_of(x); a.activation = (int32_t)act;
     a.inputs = x.data_ptr(); a.inputs_stride = row_stride(x);
     a.weight = w.data_ptr(); a.bias = ptr<void>(b); a.initial_state = ptr<void>(init);
     check_rc(nfa_causal_conv_fwd(&a, out.data_ptr(), ptr<void>(last), stream_of(x)));
@@ -1593,7 +1599,7 @@ std::tuple<OptTensor, OptTensor, OptTensor, OptTensor> causal_conv_bwd(
     if (n_rays == 0) return {some(gx), some(gw), some(gb), some(gi)};
     nfa_causal_conv_args a{};
     seq.into(a);
-    a.rows = n; a.channels = (int32_t)d; a.width = (int32_t)width; a.dtype = dtype_of(x); a.activation = (int32_t)act;
+    a.rows = n; a.channels = i32(d); a.width = i32(width); a.dtype = dtype_of(x); a.activation = (int32_t)act;
     a.inputs = x.data_ptr(); a.inputs_stride = row_stride(x);
     a.weight = w.data_ptr(); a.bias = ptr<void>(b); a.initial_state = ptr<void>(init);
     a.grad_outputs = gy.data_ptr(); a.grad_outputs_stride = row_stride(gy); a.grad_final_state = ptr<void>(gfinal);
@@ -1612,7 +1618,7 @@ Tensor causal_conv_step(const Tensor &x_, const Tensor &state_, const Tensor &w_
     Guard g(device_of(x_));
     Tensor out = at::empty({r, d}, x_.options());
     nfa_causal_conv_args a{};
-    a.n_rays = r; a.rows = r; a.channels = (int32_t)d; a.width = (int32_t)width; a.dtype = dtype_of(x); a.activation = (int32_t)act;
+    a.n_rays = r; a.rows = r; a.channels = i32(d); a.width = i32(width); a.dtype = dtype_of(x); a.activation = (int32_t)act;
     a.inputs = x.data_ptr(); a.inputs_stride = row_stride(x);
     a.weight = w.data_ptr(); a.bias = ptr<void>(b);
     check_rc(nfa_causal_conv_step(&a, state.data_ptr(), out.data_ptr(), to.data_ptr(), stream_of(x)));
@@ -1640,7 +1646,7 @@ struct ScanInputs {
     }
     nfa_selective_scan_args args(bool softplus) const {
         nfa_selective_scan_args a{};
-        a.rows = n; a.channels = (int32_t)d; a.states = (int32_t)s; a.dtype = dtype_of(u); a.delta_softplus = softplus;
+        a.rows = n; a.channels = i32(d); a.states = i32(s); a.dtype = dtype_of(u); a.delta_softplus = softplus;
         a.inputs = u.data_ptr(); a.inputs_stride = row_stride(u);
         a.delta = dt.data_ptr(); a.delta_stride = row_stride(dt);
         if (z.defined()) { a.gate = z.data_ptr(); a.gate_stride = row_stride(z); }
@@ -1662,8 +1668,8 @@ std::tuple<Tensor, OptTensor, OptTensor> selective_scan_fwd(
     Tensor out = at::empty({in.n, in.d}, u.options()), last, kept, ws;
     if (want_final) last = at::empty({n_rays, in.d, in.s}, opts(u, at::kFloat));
     if (n_rays == 0) out.zero_();
-    if (keep) kept = at::empty({nfa_selective_scan_checkpoint_bytes(in.n, (int32_t)in.d, (int32_t)in.s)}, opts(u, at::kByte));
-    const int64_t bytes = nfa_selective_scan_workspace_bytes(n_rays, in.n, (int32_t)in.d, (int32_t)in.s, 0);
+    if (keep) kept = at::empty({nfa_selective_scan_checkpoint_bytes(in.n, i32(in.d), i32(in.s))}, opts(u, at::kByte));
+    const int64_t bytes = nfa_selective_scan_workspace_bytes(n_rays, in.n, i32(in.d), i32(in.s), 0);
     if (bytes > 0) ws = at::empty({bytes}, opts(u, at::kByte));
     if (n_rays == 0) return {out, some(last), some(kept)};
     auto a = in.args(softplus);
@@ -1683,7 +1689,7 @@ std::vector<OptTensor> selective_scan_bwd(
     const OptTensor order = dense_of(order_, "ray_order", at::kInt, n_rays, u);
     const Tensor gy = as_rows(g_, "grad_outputs", in.n, in.d, u);
     const OptTensor gfinal = dense_of(gfinal_, "grad_final_state", at::kFloat, n_rays * in.d * in.s, u);
-    check_len(kept, "checkpoints", at::kByte, nfa_selective_scan_checkpoint_bytes(in.n, (int32_t)in.d, (int32_t)in.s), u);
+    check_len(kept, "checkpoints", at::kByte, nfa_selective_scan_checkpoint_bytes(in.n, i32(in.d), i32(in.s)), u);
     Guard g(device_of(u));
     const auto f32 = opts(u, at::kFloat);
     const bool none = in.n == 0 || n_rays == 0;
@@ -1821,6 +1827,7 @@ Tensor linear(const Tensor &x, const Tensor &w, const OptTensor &b, const OptTen
                       " and ", w.sizes());
     const int64_t n = w.size(0), k = w.size(1);
     TORCH_CHECK_VALUE(n > 0 && k > 0, "linear: in_features and out_features must be at least 1");
+    TORCH_CHECK_VALUE(n <= (1 << 20) && k <= (1 << 20), "linear: more than 2^20 features");
     check_native("linear", x);
     at::DimVector shape(x.sizes().begin(), x.sizes().end());
     shape.back() = n;
@@ -1843,6 +1850,7 @@ Tensor linear(const Tensor &x, const Tensor &w, const OptTensor &b, const OptTen
     return flat ? out : out.view(shape);
 }
 
+void check_channels(const char *op, int64_t d) { TORCH_CHECK_VALUE(d <= (1 << 23), op, ": more than 2^23 channels"); }
 // number of sequences of a batched or packed tensor
 int64_t sequences_of(const char *op, const Tensor &x, const OptTensor &info) {
     int64_t n = 0;
@@ -1855,6 +1863,7 @@ int64_t sequences_of(const char *op, const Tensor &x, const OptTensor &info) {
         n = info->size(0);
     }
     TORCH_CHECK_VALUE(x.size(-1) > 0, op, ": at least one channel expected");
+    check_channels(op, x.size(-1));
     TORCH_CHECK_VALUE(n < (1ll << 31) && x.numel() / x.size(-1) < (1ll << 31), op, ": more than 2^31 - 1 rays or samples");
     return n;
 }
@@ -1970,6 +1979,7 @@ std::tuple<Tensor, Tensor> causal_conv_one(const Tensor &x, const Tensor &state,
     refuse_forward("causal_conv_step", {x, state, w, b, to_});
     TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) > 0, "causal_conv_step: inputs must be (n_rays, channels)");
     const int64_t r = x.size(0), d = x.size(1), width = check_width("causal_conv_step", w, d);
+    check_channels("causal_conv_step", d);
     check_native("causal_conv_step", x);
     const auto dt = x.scalar_type();
     check_like("causal_conv_step", "state", state, x, {r, width - 1, d}, dt);
@@ -2067,6 +2077,7 @@ std::tuple<Tensor, Tensor> selective_scan_one(const Tensor &x, const Tensor &dt,
                                               const OptTensor &D, const OptTensor &z, const OptTensor &bias, bool softplus, const OptTensor &to_) {
     refuse_forward("selective_scan_step", {x, dt, A, B, C, D, z, bias, state, to_});
     TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) > 0, "selective_scan_step: inputs must be (n_rays, channels)");
+    check_channels("selective_scan_step", x.size(1));
     check_scan("selective_scan_step", x, x.sizes().slice(0, 1), dt, A, B, C, D, z, bias);
     const int64_t r = x.size(0), d = x.size(1), s = A.size(1);
     check_like("selective_scan_step", "state", state, x, {r, d, s}, at::kFloat);

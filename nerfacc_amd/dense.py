@@ -82,7 +82,8 @@ def linear(inputs: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activa
     """`activation(inputs @ weight.T + bias) + residual` in one kernel, differentiable in all four tensors.
 
     Args:
-        inputs: (..., in_features); rows may be strided (a slice of a wider tensor), float32, bfloat16 or float16.
+        inputs: (..., in_features); rows may be strided (a slice of a wider tensor), float32, bfloat16 or float16; up to 2^20 features in and
+            out.
         weight: (out_features, in_features), the same dtype.
         bias: (out_features,), the same dtype.
         activation: None, "relu", "sigmoid", "softplus", "silu", "gelu" (the exact form) or "exp" (a field's density).
@@ -107,6 +108,8 @@ def linear(inputs: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activa
     n, k = weight.shape
     if n == 0 or k == 0:
         raise ValueError("linear: in_features and out_features must be at least 1")
+    if max(n, k) > 1 << 20:
+        raise ValueError("linear: more than 2^20 features")
     shape = inputs.shape[:-1] + (n,)
     _check_native("linear", inputs, (("weight", weight, (n, k), inputs.dtype), ("bias", bias, (n,), inputs.dtype),
                                      ("residual", residual, shape, inputs.dtype)))

@@ -16,6 +16,11 @@ from .dense import _activation_id, _check_native, _differentiates_once, _ext, _r
 _MAX_STATES = 256
 
 
+def _check_channels(name: str, channels: int) -> None:
+    if channels > 1 << 23:
+        raise ValueError(f"{name}: more than 2^23 channels")
+
+
 def _sequences(name: str, inputs: Tensor, packed_info: Optional[Tensor]) -> int:
     """number of rays of a batched or packed tensor"""
     if not isinstance(inputs, Tensor):
@@ -32,6 +37,7 @@ def _sequences(name: str, inputs: Tensor, packed_info: Optional[Tensor]) -> int:
         n_rays = packed_info.shape[0]
     if inputs.shape[-1] == 0:
         raise ValueError(f"{name}: at least one channel expected")
+    _check_channels(name, inputs.shape[-1])
     if max(n_rays, inputs.shape[:-1].numel()) >= 2**31:
         raise ValueError(f"{name}: more than 2^31 - 1 rays or samples")
     return n_rays
@@ -177,6 +183,7 @@ def causal_conv_step(inputs: Tensor, state: Tensor, weight: Tensor, bias: Option
         raise ValueError("causal_conv_step: inputs must be (n_rays, channels)")
     n_rays, channels = inputs.shape
     width, dt = _width("causal_conv_step", weight, channels), inputs.dtype
+    _check_channels("causal_conv_step", channels)
     shape = (n_rays, width - 1, channels)
     if not isinstance(state, Tensor):
         raise TypeError("causal_conv_step: state must be a torch.Tensor")
@@ -289,6 +296,7 @@ def selective_scan_step(inputs: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: 
     if not isinstance(state, Tensor):
         raise TypeError("selective_scan_step: state must be a torch.Tensor")
     n_rays, channels = inputs.shape
+    _check_channels("selective_scan_step", channels)
     shape = (n_rays, channels, A.shape[-1] if isinstance(A, Tensor) and A.dim() else 0)
     _check_scan("selective_scan_step", inputs, (n_rays,), channels, n_rays, delta, A, B, C, D, gate, delta_bias,
                 (("state", state, shape, torch.float32), ("out_state", out_state, shape, torch.float32)))
