@@ -1263,6 +1263,8 @@ NFA_EXPORT int nfa_linear_bwd(const nfa_linear_args *a, const void *saved, void 
     NFA_REQUIRE(a->grad_outputs_stride >= a->out_features || a->rows == 1, "linear_bwd: grad_outputs_stride < out_features");
     NFA_REQUIRE(saved || a->activation == NFA_ACT_NONE, "linear_bwd: the activation needs what the forward call saved");
     NFA_REQUIRE(workspace || !(grad_weight || grad_bias), "linear_bwd: NULL workspace");
+    NFA_REQUIRE(!(grad_weight || grad_bias) || ((int64_t)a->in_features + 1) * a->out_features < kMaxThreads - kBlock,
+                "linear_bwd: too many weights for one launch");
     const int64_t bytes = dtype_bytes(a->dtype), n = a->out_features, k = a->in_features;
     const bool split = two_parts(a->dtype, a->activation);
     DenseArgs d{};

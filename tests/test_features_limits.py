@@ -27,3 +27,14 @@ def test_too_many_features_and_channels_are_refused(face, n):
                  lambda: nerfacc.selective_scan_step(wide(1, n), wide(1, n), wide(n, 1), wide(1, 1), wide(1, 1), wide(1, n, 1))):
         with pytest.raises(ValueError, match="more than 2"):
             call()
+
+
+def test_a_weight_gradient_of_more_numbers_than_one_launch_joins_is_refused():
+    """through the C ABI, before anything is launched"""
+    import ctypes
+
+    L, p = _backend.load_library(), 4096                             # (never followed)
+    a = _backend._STRUCTS["nfa_linear_args"](rows=1, in_features=1 << 16, out_features=1 << 16, dtype=1, activation=0, inputs=p, inputs_stride=1 << 16, weight=p,
+                                             grad_outputs=p, grad_outputs_stride=1 << 16)
+    assert L.nfa_linear_bwd(ctypes.byref(a), None, None, p, None, p, None) == 1
+    assert b"too many weights" in L.nfa_last_error()
