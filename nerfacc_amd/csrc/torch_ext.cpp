@@ -1791,33 +1791,30 @@ variable_list once(variable_list grads, const variable_list &outer, std::initial
 }
 
 struct LinearFn : torch::autograd::Function<LinearFn> {
+    enum : int64_t { kBias = 1 << 8, kResidual = 1 << 9, kSlope = 1 << 10, kInputs = 1 << 11, kWeight = 1 << 12 };     // beside the activation
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &b, const OptTensor &r, int64_t act, bool learns) {
         auto res = linear_fwd(x, w, b, r, act, learns);
         const Tensor out = std::get<0>(res), kept = get(std::get<1>(res));
-        ctx->saved_data["act"] = act;
-        ctx->saved_data["bias"] = b && b->defined();
-        ctx->saved_data["residual"] = r && r->defined();
-        const bool smooth = act != NFA_ACT_NONE && act != NFA_ACT_RELU;
-        ctx->saved_data["slope"] = smooth && learns;            // act' depends on something learnt
-        ctx->saved_data["x"] = x.requires_grad();
-        ctx->saved_data["w"] = w.requires_grad();
+        const bool smooth = act != NFA_ACT_NONE && act != NFA_ACT_RELU;         // (kSlope: act' depends on something learnt)
+        ctx->saved_data["call"] = act | (b && b->defined() ? kBias : 0) | (r && r->defined() ? kResidual : 0) | (smooth && learns ? kSlope : 0) |
+                                  (x.requires_grad() ? kInputs : 0) | (w.requires_grad() ? kWeight : 0);
         if (learns) ctx->save_for_backward({x, w, !kept.defined() && act != NFA_ACT_NONE ? out : kept});
         return out;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         variable_list out(6);
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
-        const bool has_bias = ctx->saved_data["bias"].toBool(), need_b = has_bias && ctx->needs_input_grad(2);
+        const int64_t call = ctx->saved_data["call"].toInt();
+        const bool has_bias = call & kBias, need_b = has_bias && ctx->needs_input_grad(2);
         if (need_x || need_w || need_b) {
             const auto saved = ctx->get_saved_variables();
-            auto g = linear_bwd(grads[0], saved[0], saved[1], some(saved[2]), ctx->saved_data["act"].toInt(), need_x, need_w, need_b);
+            auto g = linear_bwd(grads[0], saved[0], saved[1], some(saved[2]), call & 255, need_x, need_w, need_b);
             out[0] = get(std::get<0>(g));
             out[1] = get(std::get<1>(g));
             out[2] = get(std::get<2>(g));
         }
-        if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(has_bias ? 3 : 2)) out[3] = grads[0];     // (counts the given tensors)
-        const bool slope = ctx->saved_data["slope"].toBool();
-        return once(out, grads, {slope || ctx->saved_data["w"].toBool(), slope || ctx->saved_data["x"].toBool(), slope, false});
+        if ((call & kResidual) && ctx->needs_input_grad(has_bias ? 3 : 2)) out[3] = grads[0];     // (counts the given tensors)
+        return once(out, grads, {(call & (kSlope | kWeight)) != 0, (call & (kSlope | kInputs)) != 0, (call & kSlope) != 0, false});
     }
 };
 
