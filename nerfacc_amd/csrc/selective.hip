@@ -18,10 +18,11 @@
 // The sums over channels are exchanged across lanes (halving the values at every step, as long as there are two: 16 values over 32 lanes
 // take 8 + 4 + 2 + 1 + 1 exchanges); the sums over rows stay in registers over all rows of a wave; both are joined in a fixed order.
 //
-// On one MI355X, kernels alone, 16 states: 2^18 rows of 64 channels in 4096 ragged rays, bf16: forward 147 us with the kept states (143
-// vector instructions per row and wave, 80 % of the CUs' busy cycles), backward 346 us (264 instructions, 83 %) + 18 + 10 to join; memory
-// would take 59 us for all of it.  32768 rows of 1024 channels, one sequence, bf16: 283 us in all.  Two sequences of 8192 rows of 512
-// channels, fp32: forward 40 + 17 + 57 us, backward 47 + 13 + 173 + 14.  One row of 256 rays of 1024 channels: 8.2 us (35 MB, 4.3 TB/s).
+// On one MI355X, kernels alone, 16 states: 2^18 rows of 64 channels in 4096 ragged rays, bf16: forward 126 us with the kept states (144
+// vector instructions per row and wave, 91 % of the CUs' busy cycles), backward 348 us (267 instructions, 84 %) + 18 + 9 to join; memory
+// would take 49 us for all of it at 6.2 TB/s.  32768 rows of 1024 channels, one sequence, bf16: 287 us in all (124 + 37 + 156 profiled).  Two
+// sequences of 8192 rows of 512 channels, fp32: forward 39 + 20 + 53 us, backward 47 + 14 + 167 + 14.  One row of 256 rays of 1024 channels:
+// 8.3 us (35 MB, 4.3 TB/s).
 #include "feature.hpp"
 
 #include <algorithm>
@@ -249,7 +250,7 @@ template <int NS> __device__ __forceinline__ void read_states(const float *at, f
 }
 
 // main pass (LOCAL = false): outputs, kept states, final state; first pass over chunks (LOCAL): what a chunk adds, and its steps' sum.
-// The vector units bound both: 95 us over 2^18 rows of 64 channels in equal rays (2.7e8 states, 2.8e12 of them a second), 40 us the first pass
+// The vector units bound both: 89 us over 2^18 rows of 64 channels (2.7e8 states, 3.0e12 of them a second), 39 us the first pass
 // over 16384 rows of 512 channels.
 template <class T, int NS, int P, bool PADDED, bool LOCAL>
 __global__ __launch_bounds__(kWave) void scan_fwd_kernel(ScanArgs a) {
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(kWave) void scan_fwd_kernel(ScanArgs a) {
 
 // chunk by chunk, a lane per (channel, state): ends[slot] becomes the state that the chunk starts from (REV: the gradient that
 // reaches its last row from behind), from what each chunk adds on its own.  One dependent product-sum after the other, 32 chunks' loads
-// in flight: latency bounds it, about 0.1 us a chunk (256 chunks of 1024 channels 17 us).
+// in flight: latency bounds it, about 0.1 us a chunk (512 chunks of 1024 channels 37 us).
 template <bool REV>
 __global__ __launch_bounds__(kBlock) void scan_chain_kernel(ScanArgs a) {
     const int64_t per = (int64_t)a.channels * a.states;
@@ -444,7 +445,7 @@ __global__ __launch_bounds__(kWave) void scan_bwd_local_kernel(ScanArgs a) {
 // The backward main pass.  A tile of eight rows at a time, from the last to the first: the lanes of a channel share the rows' own
 // numbers (step and its slope, dy, ...: each lane forms them for 8 / P rows) through LDS, which also keeps h before each row; so a lane's
 // registers hold one row, the loops stay loops (the body is several hundred instructions), and LDS (20 KiB a wave with sixteen states:
-// eight waves on a CU) sets how many waves a CU holds.  The vector units bound it: 346 us for 2^18 rows of 64 channels, 264 instructions
+// eight waves on a CU) sets how many waves a CU holds.  The vector units bound it: 348 us for 2^18 rows of 64 channels, 267 instructions
 // per row and wave.
 template <class T, int NS, int P, bool PADDED>
 __global__ __launch_bounds__(kWave) void scan_bwd_kernel(ScanArgs a) {
@@ -813,6 +814,7 @@ void with_shape(int32_t dtype, Shape sh, int states, F &&g) {
 // How a call is cut.  Cutting costs a second pass over the exponentials, so whole sequences where they give every SIMD a wave (256
 // sequences of 256 rows, 256 channels: 151 us, 215 in chunks) or would be cut in less than four (512 of 64 rows, 64 channels: 42 us, 66 in
 // chunks of 32; 256 of 128 rows: 74 us, 58 in chunks); packed ones, of which a few may be much longer than the mean, in less than two.
+// (The mean decides: one ray that holds most rows of a thousand others is walked by one wave for each block of its channels.)
 // Otherwise chunks of at least 32 rows, for two waves per SIMD; in the forward pass
 // four (32768 rows of 1024 channels 331 -> 297 us, 64 sequences of 512 rows, 512 channels 200 -> 165), unless that makes them shorter than
 // 64 rows (two sequences of 8192 rows, 512 channels: 106 us, 116 with four) or a chain longer than 512 (131072 rows of 64 channels: 298

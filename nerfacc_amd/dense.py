@@ -90,7 +90,8 @@ def linear(inputs: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activa
         residual: (..., out_features), the same dtype, added behind the activation.
 
     Sums are held in 32 bits and the result is rounded once.  The backward pass differentiates once; its sums have a fixed order
-    (the same bits every time).  Forward mode derivatives are refused.
+    (the same bits every time).  Forward mode derivatives are refused, second ones raise.  All tensors have one dtype: autocast does not
+    cast for it.
 
         >>> x = torch.tensor([[1., 2.]], device="cuda")
         >>> linear(x, torch.tensor([[1., 1.], [1., -1.]], device="cuda"), activation="relu")

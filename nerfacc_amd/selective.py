@@ -221,7 +221,8 @@ def selective_scan(inputs: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tenso
         initial_state: (n_rays, channels, states) float32, h before each ray's first sample; zeros without it.
         return_final_state: also return h after each ray's last sample (its initial state where it has none).
 
-    States and sums are held in 32 bits; the sums of the backward pass have a fixed order (the same bits every time).
+    States and sums are held in 32 bits; the sums of the backward pass have a fixed order (the same bits every time).  It differentiates
+    once (second derivatives raise, forward mode is refused) and needs as much memory again as the states kept for it, rows / 8 of them.
 
         >>> one = torch.ones(3, 1, device="cuda")     # running sums per ray: no decay, unit steps
         >>> selective_scan(one, one, torch.zeros(1, 1, device="cuda"), one, one, packed_info=torch.tensor([[0, 2], [2, 1]], device="cuda"))
